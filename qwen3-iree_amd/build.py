@@ -3,8 +3,9 @@
   lib/q8gemv_gfx950.hsaco  hipcc --genco --offload-arch=gfx950 of csrc/q8gemv_kernels.hip
   lib/decode_gfx950.hsaco  the same for csrc/decode_kernels.hip (decode-step kernels)
   lib/prefill_gfx950.hsaco the same for csrc/prefill_kernels.hip (batched prompt ingestion)
-  lib/libq8gemv.so         g++ of csrc/q8gemv_shim.cpp and hipcc of csrc/q8gemv_noalloc.hip,
-                           linked against libamdhip64
+  lib/cache_gfx950.hsaco   the same for csrc/cache_kernels.hip (cache operators, vocabulary rows)
+  lib/libq8gemv.so         g++ of csrc/q8gemv_shim.cpp and csrc/cache_shim.cpp and hipcc of
+                           csrc/q8gemv_noalloc.hip, linked against libamdhip64
 
 Both cross-compile without a GPU.  Run as `python qwen3-iree_amd/build.py`.
 """
@@ -24,6 +25,7 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 CODE_OBJECT = LIB / "q8gemv_gfx950.hsaco"
 DECODE_OBJECT = LIB / "decode_gfx950.hsaco"
 PREFILL_OBJECT = LIB / "prefill_gfx950.hsaco"
+CACHE_OBJECT = LIB / "cache_gfx950.hsaco"
 SHIM = LIB / "libq8gemv.so"
 
 HIPCC_FLAGS = [
@@ -72,8 +74,14 @@ def build_prefill_object() -> Path:
                   ("-mllvm", "-amdgpu-mfma-vgpr-form=1"))
 
 
+def build_cache_object() -> Path:
+    # VGPR results here too: every MFMA's scores and sums go through the VALU
+    return _hsaco(CSRC / "cache_kernels.hip", CACHE_OBJECT,
+                  ("-mllvm", "-amdgpu-mfma-vgpr-form=1"))
+
+
 def build_shim() -> Path:
-    """libq8gemv.so: the host shim (g++) plus q8gemv_noalloc.hip (hipcc: host
+    """libq8gemv.so: the host shims (g++) plus q8gemv_noalloc.hip (hipcc: host
     code and the device-resident scratch array of the allocation-free entry
     point, embedded as a gfx950 fat binary)."""
     import tempfile
@@ -82,14 +90,15 @@ def build_shim() -> Path:
     tmp = SHIM.with_suffix(".so.tmp")
     inc = [f"-I{ROCM / 'include'}", f"-I{REPO / 'include'}", f"-I{CSRC}"]
     with tempfile.TemporaryDirectory() as td:
-        shim_o = Path(td) / "q8gemv_shim.o"
+        shim_o = [Path(td) / "q8gemv_shim.o", Path(td) / "cache_shim.o"]
         noalloc_o = Path(td) / "q8gemv_noalloc.o"
-        _run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-fPIC", "-c",
-              "-D__HIP_PLATFORM_AMD__", *inc, str(CSRC / "q8gemv_shim.cpp"), "-o", str(shim_o)])
+        for obj in shim_o:
+            _run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-fPIC", "-c",
+                  "-D__HIP_PLATFORM_AMD__", *inc, str(CSRC / f"{obj.stem}.cpp"), "-o", str(obj)])
         _run([str(ROCM / "bin" / "hipcc"), "--offload-arch=gfx950", "-O2", "-std=c++17", "-fPIC",
               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", *inc,
               str(CSRC / "q8gemv_noalloc.hip"), "-o", str(noalloc_o)])
-        _run(["g++", "-shared", "-fPIC", str(shim_o), str(noalloc_o),
+        _run(["g++", "-shared", "-fPIC", *map(str, shim_o), str(noalloc_o),
               f"-L{ROCM / 'lib'}", "-lamdhip64", "-ldl", f"-Wl,-rpath,{ROCM / 'lib'}",
               "-o", str(tmp)])
     os.replace(tmp, SHIM)
@@ -103,6 +112,8 @@ OBJECT_SOURCES = {
     "decode": ("decode_kernels.hip", "decode_device.h", "step_roles.h", "q8_device.h"),
     "prefill": ("prefill_kernels.hip", "prefill_rows.h", "prefill_split.h", "decode_device.h",
                 "step_roles.h", "q8_device.h"),
+    "cache": ("cache_kernels.hip", "cache_args.h", "decode_device.h", "step_roles.h",
+              "q8_device.h"),
 }
 
 
@@ -157,8 +168,9 @@ def kernel_digest(name: str, code_object: Path = CODE_OBJECT) -> str | None:
     return h.hexdigest()[:16] if found else None
 
 
-def build_all() -> tuple[Path, Path, Path, Path]:
-    return build_code_object(), build_decode_object(), build_prefill_object(), build_shim()
+def build_all() -> tuple[Path, ...]:
+    return (build_code_object(), build_decode_object(), build_prefill_object(),
+            build_cache_object(), build_shim())
 
 
 if __name__ == "__main__":

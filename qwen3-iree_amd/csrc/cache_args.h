@@ -1,0 +1,49 @@
+// Argument blocks of the kernels in cache_kernels.hip, shared with the host
+// code that fills them (cache_shim.cpp).
+#ifndef QWEN3_CACHE_ARGS_H
+#define QWEN3_CACHE_ARGS_H
+
+#include <stdint.h>
+
+constexpr int kTreeMax = 256;  // nodes of a tree, rows of a call
+
+struct AttnTreeArgs {
+  const uint16_t *k, *v;  // the layer's base, [max_seq, kv_heads, head_dim]
+  const uint16_t* q;
+  const uint32_t* mask;  // [n, mask_words] or null: rows see the rows before them
+  uint16_t* out;
+  float* lse;  // or null
+  int64_t q_stride, out_stride;
+  int32_t len, n, q_heads, kv_heads, group;
+  float scale;
+};
+
+struct WeightsArgs {
+  const uint16_t* k;
+  float* weights;
+  const uint16_t* q;
+  const float* lse;
+  const int32_t* path;  // or null
+  int64_t max_seq, q_layer_stride, q_stride, lse_layer_stride;
+  int32_t layers, kv_heads, q_heads, group, len, n, rows;
+  float scale;
+};
+
+struct SelectArgs {
+  const float* weights;
+  int32_t* keep;
+  int64_t max_seq;
+  int32_t len, budget, sinks, recent;
+};
+
+struct CompactArgs {
+  const uint16_t *k, *v;
+  const float* w;  // or null
+  uint16_t *k_to, *v_to;
+  float* w_to;
+  const int32_t* keep;
+  int64_t src_seq, dst_seq;
+  int32_t kv_heads, head_dim, per_head, base, count;
+};
+
+#endif

@@ -1,0 +1,288 @@
+// Host side of include/f16_cache.h: argument checks and launches of the
+// kernels in cache_kernels.hip.
+#include "f16_cache.h"
+#include "cache_args.h"
+#include "q8gemv.h"
+#include "shim_internal.h"
+
+#include <hip/hip_runtime_api.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+namespace {
+
+struct {
+  hipModule_t module = nullptr;
+  hipFunction_t mask = nullptr, attn[2] = {}, weights[2] = {}, select = nullptr, compact = nullptr,
+                argmax = nullptr, argmax_final = nullptr;
+} c;
+
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return q8_shim::error(code, buf);
+}
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+int check_ready() {
+  int rc = q8_shim::ready();
+  if (rc) return rc;
+  if (!c.module)
+    return fail(Q8_ERR_CODE_OBJECT, "cache_gfx950.hsaco was not found or lacks a kernel");
+  return Q8_OK;
+}
+
+int check_cache(const f16_cache* a, const char* name) {
+  if (!a) return fail(Q8_ERR_NULL_POINTER, "null %s", name);
+  if (a->max_seq < 1 || a->max_seq > (1LL << 24))
+    return fail(Q8_ERR_BAD_SHAPE, "%s: max_seq %lld outside [1, 2^24]", name, (long long)a->max_seq);
+  if (a->layers < 1 || a->layers > 1024)
+    return fail(Q8_ERR_BAD_SHAPE, "%s: %d layers outside [1, 1024]", name, a->layers);
+  if (a->kv_heads < 1 || a->kv_heads > 256)
+    return fail(Q8_ERR_BAD_SHAPE, "%s: %d kv heads outside [1, 256]", name, a->kv_heads);
+  if (a->head_dim != 64 && a->head_dim != 128)
+    return fail(Q8_ERR_BAD_SHAPE, "%s: head_dim %d is not 64 or 128", name, a->head_dim);
+  if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->weights, 4))
+    return fail(Q8_ERR_MISALIGNED, "%s: k and v 16, weights 4-byte alignment", name);
+  return Q8_OK;
+}
+
+// rows of query heads over a cache: what attention and its weights share
+int check_rows(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads, int64_t q_stride,
+               float scale) {
+  if (q_heads < 1 || q_heads > 256 || q_heads % a->kv_heads ||
+      q_heads / a->kv_heads > F16_MAX_GROUP)
+    return fail(Q8_ERR_BAD_SHAPE, "%d query heads over %d kv heads", q_heads, a->kv_heads);
+  if (n < 1 || n > F16_TREE_MAX_NODES)
+    return fail(Q8_ERR_BAD_SHAPE, "n %d outside [1, %d]", n, F16_TREE_MAX_NODES);
+  if (len < 0 || (int64_t)len + n > a->max_seq)
+    return fail(Q8_ERR_BAD_SHAPE, "slots [%d, %d + %d) outside the cache of %lld", len, len, n,
+                (long long)a->max_seq);
+  if (q_stride % 8 || q_stride < (int64_t)q_heads * a->head_dim)
+    return fail(Q8_ERR_BAD_SHAPE, "row stride %lld is no multiple of 8 of at least %d",
+                (long long)q_stride, q_heads * a->head_dim);
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(Q8_ERR_BAD_ARGUMENT, "scale %g is not finite and positive", scale);
+  return Q8_OK;
+}
+
+constexpr uint32_t kArgmaxWgsMax = 1024;
+
+}  // namespace
+
+namespace q8_shim {
+
+void cache_load(const char* path) {
+  hipModule_t m = nullptr;
+  if (hipModuleLoad(&m, path) != hipSuccess) return;
+  struct {
+    hipFunction_t* fn;
+    const char* name;
+  } names[] = {{&c.mask, "tree_mask_k"},          {&c.attn[0], "attn_tree_64"},
+               {&c.attn[1], "attn_tree_128"},     {&c.weights[0], "weights_add_64"},
+               {&c.weights[1], "weights_add_128"}, {&c.select, "cache_select_k"},
+               {&c.compact, "cache_compact_k"},   {&c.argmax, "gemm_argmax_k"},
+               {&c.argmax_final, "gemm_argmax_final"}};
+  for (auto& n : names) {
+    if (hipModuleGetFunction(n.fn, m, n.name) != hipSuccess) {
+      (void)hipModuleUnload(m);
+      return;
+    }
+  }
+  c.module = m;
+}
+
+void cache_unload() {
+  if (c.module) (void)hipModuleUnload(c.module);
+  c.module = nullptr;
+}
+
+}  // namespace q8_shim
+
+extern "C" {
+
+int f16_tree_mask(const int32_t* parents, int32_t n, uint32_t* mask, int32_t* depth,
+                  void* stream) {
+  if (!parents || !mask) return fail(Q8_ERR_NULL_POINTER, "null parents or mask");
+  if (!aligned(parents, 4) || !aligned(mask, 4) || !aligned(depth, 4))
+    return fail(Q8_ERR_MISALIGNED, "parents, mask and depth 4-byte alignment");
+  if (n < 1 || n > F16_TREE_MAX_NODES)
+    return fail(Q8_ERR_BAD_SHAPE, "n %d outside [1, %d]", n, F16_TREE_MAX_NODES);
+  int rc = check_ready();
+  if (rc) return rc;
+  void* args[] = {&parents, &n, &mask, &depth};
+  return q8_shim::launch(c.mask, 1, kTreeMax, args, static_cast<hipStream_t>(stream));
+}
+
+size_t f16_attn_tree_workspace_bytes(const f16_cache*, int32_t, int32_t, int32_t) { return 0; }
+
+int f16_attn_tree(const f16_cache* a, int32_t layer, int32_t len, const void* q, int64_t q_stride,
+                  int32_t q_heads, const uint32_t* mask, int32_t n, float scale, void* out,
+                  int64_t out_stride, float* lse, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  int rc = check_cache(a, "cache");
+  if (rc) return rc;
+  if (!a->k || !a->v || !q || !out) return fail(Q8_ERR_NULL_POINTER, "null k, v, q or out");
+  if (layer < 0 || layer >= a->layers)
+    return fail(Q8_ERR_LAYER_RANGE, "layer %d outside [0, %d)", layer, a->layers);
+  if ((rc = check_rows(a, len, n, q_heads, q_stride, scale))) return rc;
+  if (out_stride % 8 || out_stride < (int64_t)q_heads * a->head_dim)
+    return fail(Q8_ERR_BAD_SHAPE, "row stride %lld is no multiple of 8 of at least %d",
+                (long long)out_stride, q_heads * a->head_dim);
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(mask, 4) || !aligned(lse, 4))
+    return fail(Q8_ERR_MISALIGNED, "q and out 16, mask and lse 4-byte alignment");
+  (void)workspace;
+  (void)workspace_bytes;
+  if ((rc = check_ready())) return rc;
+  const int64_t base = (int64_t)layer * a->max_seq * a->kv_heads * a->head_dim;
+  AttnTreeArgs args{static_cast<const uint16_t*>(a->k) + base,
+                    static_cast<const uint16_t*>(a->v) + base,
+                    static_cast<const uint16_t*>(q),
+                    mask,
+                    static_cast<uint16_t*>(out),
+                    lse,
+                    q_stride,
+                    out_stride,
+                    len,
+                    n,
+                    q_heads,
+                    a->kv_heads,
+                    q_heads / a->kv_heads,
+                    scale};
+  void* p[] = {&args};
+  return q8_shim::launch(c.attn[a->head_dim / 64 - 1], (uint32_t)(n * q_heads), 256, p,
+                         static_cast<hipStream_t>(stream));
+}
+
+int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t q_layer_stride,
+                         int64_t q_stride, int32_t q_heads, const float* lse,
+                         int64_t lse_layer_stride, int32_t rows, const int32_t* path, int32_t n,
+                         float scale, void* stream) {
+  int rc = check_cache(a, "cache");
+  if (rc) return rc;
+  if (!a->k || !a->weights || !q || !lse)
+    return fail(Q8_ERR_NULL_POINTER, "null k, weights, q or lse");
+  if ((rc = check_rows(a, len, n, q_heads, q_stride, scale))) return rc;
+  if (rows < 1 || rows > (1 << 20))
+    return fail(Q8_ERR_BAD_SHAPE, "rows %d outside [1, 2^20]", rows);
+  if (!path && n > rows) return fail(Q8_ERR_BAD_SHAPE, "n %d exceeds the %d rows", n, rows);
+  if (a->layers > 1 && (q_layer_stride % 8 || q_layer_stride < 0 || lse_layer_stride < 0))
+    return fail(Q8_ERR_BAD_SHAPE, "layer strides %lld, %lld", (long long)q_layer_stride,
+                (long long)lse_layer_stride);
+  if (!aligned(q, 16) || !aligned(lse, 4) || !aligned(path, 4))
+    return fail(Q8_ERR_MISALIGNED, "q 16, lse and path 4-byte alignment");
+  if ((rc = check_ready())) return rc;
+  WeightsArgs args{static_cast<const uint16_t*>(a->k), a->weights,
+                   static_cast<const uint16_t*>(q),    lse,
+                   path,                               a->max_seq,
+                   q_layer_stride,                     q_stride,
+                   lse_layer_stride,                   a->layers,
+                   a->kv_heads,                        q_heads,
+                   q_heads / a->kv_heads,              len,
+                   n,                                  rows,
+                   scale};
+  void* p[] = {&args};
+  const int per_wg = 256 / (a->head_dim / 8);
+  return q8_shim::launch2(c.weights[a->head_dim / 64 - 1],
+                          (uint32_t)((len + n + per_wg - 1) / per_wg),
+                          (uint32_t)(a->layers * a->kv_heads), 256, p,
+                          static_cast<hipStream_t>(stream));
+}
+
+int f16_cache_select(const f16_cache* a, int32_t len, int32_t budget, int32_t sinks,
+                     int32_t recent, int32_t* keep, void* stream) {
+  int rc = check_cache(a, "cache");
+  if (rc) return rc;
+  if (!a->weights || !keep) return fail(Q8_ERR_NULL_POINTER, "null weights or keep");
+  if (!aligned(keep, 4)) return fail(Q8_ERR_MISALIGNED, "keep 4-byte alignment");
+  if (len > a->max_seq || budget < 1 || budget > len)
+    return fail(Q8_ERR_BAD_SHAPE, "budget %d of %d slots in a cache of %lld", budget, len,
+                (long long)a->max_seq);
+  if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+    return fail(Q8_ERR_BAD_SHAPE, "%d first and %d last slots in a budget of %d", sinks, recent,
+                budget);
+  if ((rc = check_ready())) return rc;
+  SelectArgs args{a->weights, keep, a->max_seq, len, budget, sinks, recent};
+  void* p[] = {&args};
+  return q8_shim::launch(c.select, (uint32_t)(a->layers * a->kv_heads), 1024, p,
+                         static_cast<hipStream_t>(stream));
+}
+
+int f16_cache_compact(const f16_cache* src, const f16_cache* dst, const int32_t* keep,
+                      int per_head, int32_t base, int32_t count, void* stream) {
+  int rc = check_cache(src, "src");
+  if (rc) return rc;
+  if ((rc = check_cache(dst, "dst"))) return rc;
+  if (!src->k || !src->v || !dst->k || !dst->v)
+    return fail(Q8_ERR_NULL_POINTER, "null k or v");
+  if (src->layers != dst->layers || src->kv_heads != dst->kv_heads ||
+      src->head_dim != dst->head_dim)
+    return fail(Q8_ERR_BAD_SHAPE, "the caches differ in layers, kv_heads or head_dim");
+  if (base < 0 || count < 0 || (int64_t)base + count > src->max_seq ||
+      (int64_t)base + count > dst->max_seq)
+    return fail(Q8_ERR_BAD_SHAPE, "slots [%d, %d + %d) outside a cache of %lld and one of %lld",
+                base, base, count, (long long)src->max_seq, (long long)dst->max_seq);
+  const bool weights = src->weights && dst->weights;
+  const bool same = src->k == dst->k || src->v == dst->v || (weights && src->weights == dst->weights);
+  if (same && (src->k != dst->k || src->v != dst->v || src->max_seq != dst->max_seq ||
+               (weights && src->weights != dst->weights)))
+    return fail(Q8_ERR_BAD_ARGUMENT, "src and dst share some of their buffers but not all");
+  if (count > 0 && !keep) return fail(Q8_ERR_NULL_POINTER, "null keep");
+  if (!aligned(keep, 4)) return fail(Q8_ERR_MISALIGNED, "keep 4-byte alignment");
+  if ((rc = check_ready())) return rc;
+  if (count == 0) return Q8_OK;
+  CompactArgs args{static_cast<const uint16_t*>(src->k),
+                   static_cast<const uint16_t*>(src->v),
+                   weights ? src->weights : nullptr,
+                   static_cast<uint16_t*>(dst->k),
+                   static_cast<uint16_t*>(dst->v),
+                   weights ? dst->weights : nullptr,
+                   keep,
+                   src->max_seq,
+                   dst->max_seq,
+                   src->kv_heads,
+                   src->head_dim,
+                   per_head ? 1 : 0,
+                   base,
+                   count};
+  void* p[] = {&args};
+  const int parts = 2 * (src->head_dim / 64) + (weights ? 1 : 0);
+  return q8_shim::launch(c.compact, (uint32_t)(src->layers * src->kv_heads * parts), 256, p,
+                         static_cast<hipStream_t>(stream));
+}
+
+size_t f16_gemm_argmax_workspace_bytes(int32_t n) {
+  if (n < 1 || n > F16_TREE_MAX_NODES) return 0;
+  return (size_t)n * 8 * kArgmaxWgsMax;
+}
+
+int f16_gemm_argmax(const void* w_f16, int64_t w_rows, const void* x_f16, int32_t n,
+                    void* logits_f16, int32_t* tokens, void* workspace, void* stream) {
+  if (!w_f16 || !x_f16 || !tokens || !workspace)
+    return fail(Q8_ERR_NULL_POINTER, "null w, x, tokens or workspace");
+  if (w_rows < 1 || w_rows >= (1LL << 31))
+    return fail(Q8_ERR_BAD_SHAPE, "w_rows=%lld outside [1, 2^31)", (long long)w_rows);
+  if (n < 1 || n > F16_TREE_MAX_NODES)
+    return fail(Q8_ERR_BAD_SHAPE, "n %d outside [1, %d]", n, F16_TREE_MAX_NODES);
+  if (!aligned(w_f16, 16) || !aligned(x_f16, 16) || !aligned(workspace, 16) ||
+      !aligned(logits_f16, 2) || !aligned(tokens, 4))
+    return fail(Q8_ERR_MISALIGNED, "w, x and workspace 16, logits 2, tokens 4-byte alignment");
+  int rc = check_ready();
+  if (rc) return rc;
+  int rows = (int)w_rows;
+  int wgs = (int)std::min<int64_t>(kArgmaxWgsMax, (w_rows + 3) / 4);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  void* args[] = {&w_f16, &rows, &x_f16, &n, &logits_f16, &workspace};
+  if ((rc = q8_shim::launch(c.argmax, (uint32_t)wgs, 256, args, st))) return rc;
+  void* fargs[] = {&workspace, &wgs, &n, &tokens};
+  return q8_shim::launch(c.argmax_final, (uint32_t)n, 64, fargs, st);
+}
+
+}  // extern "C"

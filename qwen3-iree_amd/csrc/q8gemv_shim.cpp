@@ -434,6 +434,22 @@ int q8gemv_init(const char* code_object_path) {
       }
     }
   }
+  // and the cache operators' kernels in a fourth
+  {
+    const size_t slash = path.rfind('/');
+    std::string dir = slash == std::string::npos ? std::string(".") : path.substr(0, slash);
+    std::string cpath = dir + "/cache_gfx950.hsaco";
+    FILE* cf = std::fopen(cpath.c_str(), "rb");
+    if (!cf) {
+      std::string lib = default_code_object();
+      cpath = lib.substr(0, lib.rfind('/')) + "/cache_gfx950.hsaco";
+      cf = std::fopen(cpath.c_str(), "rb");
+    }
+    if (cf) {
+      std::fclose(cf);
+      q8_shim::cache_load(cpath.c_str());
+    }
+  }
   int cus = 0;
   if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
     cus = 256;
@@ -504,6 +520,7 @@ void q8gemv_shutdown(void) {
       g.pf_f16_part_12k = g.pf_f16_part_44k = g.pf_expand = nullptr;
   g.vocab = g.vocab_finalize = g.argmax = g.ws_reset = g.copy = nullptr;
   g.calib_empty = g.calib_handoff = g.calib_chase = g.read = nullptr;
+  q8_shim::cache_unload();
   g.ready = false;
 }
 
@@ -747,6 +764,19 @@ namespace q8_shim {
 int error(int code, const char* msg) { return fail(code, "%s", msg); }
 
 int hip_error(hipError_t e, const char* what) { return hip_fail(e, what); }
+
+int ready() { return check_ready(); }
+
+int compute_units() { return cu_count(); }
+
+int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStream_t stream) {
+  return ::launch(fn, grid, block, args, stream);
+}
+
+int launch2(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t block, void** args,
+            hipStream_t stream) {
+  return ::launch2(fn, gx, gy, block, args, stream);
+}
 
 int noalloc_ready() {
   int rc = check_ready();

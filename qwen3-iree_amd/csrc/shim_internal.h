@@ -1,5 +1,6 @@
-// Internal interface between the C-ABI shim (q8gemv_shim.cpp) and the
-// allocation-free entry point (q8gemv_noalloc.hip); not part of the ABI.
+// Internal interface between the C-ABI shim (q8gemv_shim.cpp), the cache
+// operators (cache_shim.cpp) and the allocation-free entry point
+// (q8gemv_noalloc.hip); not part of the ABI.
 #ifndef QWEN3_SHIM_INTERNAL_H
 #define QWEN3_SHIM_INTERNAL_H
 
@@ -11,6 +12,19 @@ namespace q8_shim {
 // Sets the calling thread's error message (q8gemv_last_error) and returns code.
 int error(int code, const char* msg);
 int hip_error(hipError_t e, const char* what);
+
+// Q8_OK once q8gemv_init has run.
+int ready();
+int compute_units();
+// The launches every entry point makes (1-D and 2-D grids of 1-D workgroups).
+int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStream_t stream);
+int launch2(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t block, void** args,
+            hipStream_t stream);
+
+// Implemented in cache_shim.cpp: loads the code object at `path` (a failure
+// leaves the cache operators reporting Q8_ERR_CODE_OBJECT) and unloads it.
+void cache_load(const char* path);
+void cache_unload();
 
 // Q8_OK once q8gemv_init has run and the allocation-free scratch of its
 // device was set up; otherwise the status and message of what is missing.

@@ -185,7 +185,23 @@ _SIGNATURES = {
     "qwen3_set_prefill_tiling": [_I, _I],
     "qwen3_get_step_mode": [_P],
 }
+# include/f16_cache.h
+_CACHE_SIGNATURES = {
+    "f16_tree_mask": [_P, ctypes.c_int32, _P, _P, _P],
+    "f16_attn_tree_workspace_bytes": [_P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32],
+    "f16_attn_tree": [_P, ctypes.c_int32, ctypes.c_int32, _P, _I64, ctypes.c_int32, _P,
+                      ctypes.c_int32, ctypes.c_float, _P, _I64, _P, _P, _SZ, _P],
+    "f16_attn_weights_add": [_P, ctypes.c_int32, _P, _I64, _I64, ctypes.c_int32, _P, _I64,
+                             ctypes.c_int32, _P, ctypes.c_int32, ctypes.c_float, _P],
+    "f16_cache_select": [_P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P,
+                         _P],
+    "f16_cache_compact": [_P, _P, _P, _I, ctypes.c_int32, ctypes.c_int32, _P],
+    "f16_gemm_argmax_workspace_bytes": [ctypes.c_int32],
+    "f16_gemm_argmax": [_P, _I64, _P, ctypes.c_int32, _P, _P, _P, _P],
+}
 _RESTYPES = {
+    "f16_attn_tree_workspace_bytes": _SZ,
+    "f16_gemm_argmax_workspace_bytes": _SZ,
     "q8gemv_shutdown": None,
     "q8gemv_last_error": ctypes.c_char_p,
     "vocab_argmax_workspace_bytes": _SZ,
@@ -212,7 +228,7 @@ def load_library(path: str | Path | None = None) -> ctypes.CDLL:
         if not p.exists():
             raise Q8GemvError(Q8_ERR_CODE_OBJECT, f"{p} is not built (run qwen3-iree_amd/build.py)")
         L = ctypes.CDLL(str(p))
-        for name, argtypes in _SIGNATURES.items():
+        for name, argtypes in (*_SIGNATURES.items(), *_CACHE_SIGNATURES.items()):
             fn = getattr(L, name)
             fn.argtypes = argtypes
             fn.restype = _RESTYPES.get(name, _I)
@@ -561,6 +577,17 @@ def f16_gemv_argmax_rows_noalloc(w, n_rows: int, x, logits, token, stream=None) 
     scratch (no workspace, nothing allocated)."""
     _call("f16_gemv_argmax_rows_noalloc", _ptr(w), int(n_rows), _ptr(x), _ptr(logits),
           _ptr(token), _stream(stream))
+
+
+def gemm_argmax_workspace_bytes(n: int) -> int:
+    return int(load_library().f16_gemm_argmax_workspace_bytes(int(n)))
+
+
+def f16_gemm_argmax(w, w_rows: int, x, n: int, logits, tokens, workspace, stream=None) -> None:
+    """f16_gemv_argmax_rows for n token rows: logits f16 [n, w_rows] (or None)
+    and tokens int32 [n] (include/f16_cache.h)."""
+    _call("f16_gemm_argmax", _ptr(w), int(w_rows), _ptr(x), int(n), _ptr(logits), _ptr(tokens),
+          _ptr(workspace), _stream(stream))
 
 
 def set_batch_workgroups(n: int) -> None:
