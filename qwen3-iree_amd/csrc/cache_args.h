@@ -14,8 +14,12 @@ struct AttnTreeArgs {
   uint16_t* out;
   float* lse;  // or null
   int64_t q_stride, out_stride;
+  float* part;     // [splits, kv_heads, rows, head_dim] outputs of the splits
+  float* part_ml;  // [kv_heads, rows, 2, splits] their references and sums
   int32_t len, n, q_heads, kv_heads, group;
-  float scale;
+  uint32_t group_inv;      // ceil(2^32 / group): r / group for group > 1, r < 2^13
+  int32_t splits, blocks;  // blocks of 32 slots in a split
+  float scale;                         // with log2 e: scores in base-2 units
 };
 
 struct WeightsArgs {

@@ -4,7 +4,11 @@
 #include "cache_args.h"
 #include "decode_device.h"
 
+#include <type_traits>
+
 namespace {
+
+constexpr float kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ float half_lo(uint32_t v) { return (float)as_f16x2(v).x; }
 __device__ __forceinline__ float half_hi(uint32_t v) { return (float)as_f16x2(v).y; }
@@ -79,98 +83,532 @@ extern "C" __global__ __launch_bounds__(kTreeMax) void tree_mask_k(
 }
 
 // ------------------------------------------------------- tree attention ----
-
-// Whether row i sees slot len + a, and whether it sees anything at all.
+//
+// The rows of one kv head are its query heads' rows of all nodes, r = group
+// node + head, in tiles of 16.  A wave works transposed, one row per lane
+// column, on blocks of 32 slots:
+//   S^T = K Q^T (v_mfma_f32_16x16x32_f16: exact f16 products, f32 sums), so lane
+//     (c16, grp) holds the scores of row c16 at slots 4 grp + e and 16 + 4 grp + e;
+//   softmax in one pass: a reference m per row (base-2 units), weights
+//     2^(s - m), their sum l and the output O relative to the same m.  m is set
+//     kRefRoom below the first block's maximum and moves only when the sum of a
+//     lane's 8 weights passes kSumMax (then their maximum is 2^kRefMax above m),
+//     so most blocks look for no maximum and rescale nothing, every weight fits
+//     f16, and small ones are normal f16 numbers down to 2^-20 of the largest;
+//   O^T += V^T P^T with the weights as they stand in the lanes: the MFMA's 32 k
+//     slots mean slots 4 grp + e, 16 + 4 grp + e, and V^T is read from LDS in
+//     that order (transposing reads).  A weight goes into the product as an f16
+//     (half a step, 2^-11 of itself, at most), with one row group as the sum of two
+//     (2^-22): the bytes bound those, and the second product costs nothing.
+// K and V blocks are copied from memory straight into LDS, the next one while one
+// is computed.  RG waves share a block (RG row groups of T tiles);
+// the 4 / RG position groups of a workgroup take blocks in turn and meet in LDS.
+// With one row group no wave waits for another until the end: few rows are bound
+// by the bytes in flight, 64 KiB a CU, many rows by MFMA and exp2.
+// The slots are divided into splits of `blocks` blocks (grid: kv heads,
+// row blocks, splits; kv head fastest, so that 8 kv heads keep to an XCD each); several
+// splits leave (m, l, O) in the workspace and attn_merge combines them in order.
 namespace {
-__device__ __forceinline__ bool row_sees(const AttnTreeArgs& A, int i, int a) {
-  if (!A.mask) return a <= i;
+
+constexpr float kRefRoom = 6.0f, kRefMax = 10.0f, kSumMax = 16384.0f;
+
+// Bits of slots p0 .. p0 + 31 row i sees: those before `len` and those of its
+// mask row.
+__device__ __forceinline__ uint32_t mask_word(const AttnTreeArgs& A, int i, int w) {
   const int words = (A.n + 31) >> 5;
-  return (A.mask[i * words + (a >> 5)] >> (a & 31)) & 1;
+  if (w < 0) return ~0u;
+  if (w >= words) return 0u;
+  if (!A.mask) {
+    const int d = i - 32 * w;
+    return d >= 31 ? ~0u : (d < 0 ? 0u : (2u << d) - 1u);
+  }
+  uint32_t m = A.mask[i * words + w];
+  if (w == words - 1 && (A.n & 31)) m &= (1u << (A.n & 31)) - 1u;
+  return m;
+}
+__device__ __forceinline__ uint32_t block_bits(const AttnTreeArgs& A, int i, int p0) {
+  const int a0 = p0 - A.len;
+  const int w = a0 >> 5, sh = a0 & 31;
+  const uint32_t lo = mask_word(A, i, w);
+  return sh == 0 ? lo : (lo >> sh) | (mask_word(A, i, w + 1) << (32 - sh));
 }
 __device__ __forceinline__ bool row_empty(const AttnTreeArgs& A, int i) {
-  if (!A.mask) return false;
-  const int words = (A.n + 31) >> 5;
   uint32_t any = 0;
-  for (int w = 0; w < words; ++w) {
-    uint32_t m = A.mask[i * words + w];
-    if (w == words - 1 && (A.n & 31)) m &= (1u << (A.n & 31)) - 1u;
-    any |= m;
-  }
+  for (int w = 0; w < (A.n + 31) >> 5; ++w) any |= mask_word(A, i, w);
   return any == 0;
 }
-}  // namespace
 
-// One workgroup per (row, query head); D / 8 lanes hold a position's dims, each
-// such group of lanes keeps a running maximum, sum and output over every
-// (groups of the workgroup)th position, and the groups meet in LDS.
-template <int D>
+// The top bits of the halves that are infinities or NaN (an exponent of all ones
+// carries into its top bit, and no further).
+__device__ __forceinline__ uint32_t special_bits(uint32_t b) {
+  return ((b & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+// v with its infinities and NaN replaced by 0
+__device__ __forceinline__ f16x8 without_special(f16x8 v) {
+  u32x4 b = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t one = special_bits(b[i]) >> 15;  // bits 0 and 16, then their halves
+    b[i] &= ~((one << 16) - one);
+  }
+  return __builtin_bit_cast(f16x8, b);
+}
+
+template <int D, int RG, int T>
 __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
-  constexpr int L = D / 8, G = 256 / L;
-  __shared__ float sm[G], sl[G], so[G][D];
+  constexpr int PG = 4 / RG;
+  constexpr int kTile = 64 * D;            // bytes of a block of k or v
+  constexpr int kPieces = kTile / 1024;    // 1 KiB copies of a block
+  constexpr int kChunks = D / 8;           // 16-byte chunks of a row
+  constexpr int kRowsPerPiece = 64 / kChunks;
+  constexpr int kRows = 16 * T * RG;       // rows of a workgroup
+  constexpr bool kLow = RG == 1;           // weights as two f16 values
+  // two buffers of each position group's K and V blocks, separate arrays so
+  // that the compiler sees that reading one does not wait for copies into another
+  __shared__ __attribute__((aligned(1024))) uint8_t k0[PG * kTile], k1[PG * kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t v0[PG * kTile], v1[PG * kTile];
   const int t = threadIdx.x;
-  const int lane = t % L, grp = t / L;
-  const int i = blockIdx.x / A.q_heads, h = blockIdx.x % A.q_heads;
-  uint16_t* out = A.out + (int64_t)i * A.out_stride + h * D;
-  if (row_empty(A, i)) {
-    if (t < D) out[t] = 0;
-    if (t == 0 && A.lse) A.lse[i * A.q_heads + h] = -__builtin_inff();
-    return;
-  }
-  const int64_t row = (int64_t)A.kv_heads * D;
-  const uint16_t* kb = A.k + (h / A.group) * D + 8 * lane;
-  const uint16_t* vb = A.v + (h / A.group) * D + 8 * lane;
-  const u32x4 q = *reinterpret_cast<const u32x4*>(A.q + (int64_t)i * A.q_stride + h * D + 8 * lane);
-  float m = -__builtin_inff(), l = 0.0f, o[8];
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lane = t & 63, c16 = lane & 15, grp = lane >> 4;
+  const int rg = wave % RG, pg = wave / RG;
+  const int kvh = blockIdx.x, rb = blockIdx.y, split = blockIdx.z;
+  const int R = A.n * A.group;
+  const int row0 = rb * kRows + 16 * T * rg;  // this wave's first row
+  const int slots = A.len + A.n;
+  const int nb_all = (slots + 31) >> 5;
+  const int b_lo = split * A.blocks;
+  const int b_hi = b_lo + A.blocks < nb_all ? b_lo + A.blocks : nb_all;
+  const int64_t row_elems = (int64_t)A.kv_heads * D;
+  const uint16_t* kb = A.k + kvh * D;
+  const uint16_t* vb = A.v + kvh * D;
+
+  // Q as the B operand: column c16 is row row0 + 16 j + c16, dims 32 st + 8 grp
+  int node[T];
+  f16x8 qf[T][D / 32];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = 0.0f;
-  for (int p = grp; p < A.len + A.n; p += G) {
-    if (p >= A.len && !row_sees(A, i, p - A.len)) continue;
-    const u32x4 k = *reinterpret_cast<const u32x4*>(kb + p * row);
-    const u32x4 v = *reinterpret_cast<const u32x4*>(vb + p * row);
-    const float s = A.scale * sum_lanes<L>(dot8(q, k));
-    const float mn = fmaxf(m, s);
-    const float a = m == -__builtin_inff() ? 0.0f : expf(m - mn);
-    const float w = expf(s - mn);
-    l = l * a + w;
+  for (int j = 0; j < T; ++j) {
+    int r = row0 + 16 * j + c16;
+    r = r < R ? r : R - 1;
+    node[j] = A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv);
+    const uint16_t* q = A.q + (int64_t)node[j] * A.q_stride +
+                        (kvh * A.group + r - node[j] * A.group) * D + 8 * grp;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      o[e] = o[e] * a + w * ((e & 1) ? half_hi(v[e >> 1]) : half_lo(v[e >> 1]));
-    m = mn;
+    for (int st = 0; st < D / 32; ++st)
+      qf[j][st] = __builtin_bit_cast(f16x8, load_global(reinterpret_cast<const u32x4*>(q + 32 * st)));
   }
-  if (lane == 0) {
-    sm[grp] = m;
-    sl[grp] = l;
-  }
+  bool none[T];  // the row sees nothing
+  float m[T], l[T];
+  f32x4 o[T][D / 16];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) so[grp][8 * lane + e] = o[e];
-  __syncthreads();
-  if (t < D) {
-    float M = -__builtin_inff(), S = 0.0f, v = 0.0f;
-    for (int g = 0; g < G; ++g) M = fmaxf(M, sm[g]);
-    for (int g = 0; g < G; ++g) {
-      const float w = sm[g] == -__builtin_inff() ? 0.0f : expf(sm[g] - M);
-      S += sl[g] * w;
-      v += so[g][t] * w;
+  for (int j = 0; j < T; ++j) {
+    none[j] = A.splits == 1 && row_empty(A, node[j]);
+    m[j] = -__builtin_inff();
+    l[j] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[j][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // K chunk c of row r sits in slot c ^ (r mod kChunks) of its row, V chunk c in
+  // c ^ 2 (r mod kChunks / 2): the fragment reads below hit distinct banks
+  uint32_t k_at[kPieces / RG], v_at[kPieces / RG];  // this lane's bytes of a block
+#pragma unroll
+  for (int i = 0; i < kPieces / RG; ++i) {
+    const int row = kRowsPerPiece * (kPieces / RG * rg + i) + lane / kChunks, c = lane % kChunks;
+    k_at[i] = row * (uint32_t)(2 * row_elems) + 16 * (c ^ (row & (kChunks - 1)));
+    v_at[i] = row * (uint32_t)(2 * row_elems) + 16 * (c ^ (2 * (row & (kChunks / 2 - 1))));
+  }
+  // block b; in the last one, slots behind the last repeat it
+  auto copy = [&](auto last_t, int b, uint8_t* kt, uint8_t* vt) {
+    const uint8_t* kp = reinterpret_cast<const uint8_t*>(kb + 32 * b * row_elems);
+    const uint8_t* vp = reinterpret_cast<const uint8_t*>(vb + 32 * b * row_elems);
+    const uint32_t row_bytes = (uint32_t)(2 * row_elems);
+    auto piece = [&](const uint8_t* from, uint32_t at, uint8_t* to, int i) {
+      const int pc = kPieces / RG * rg + i;
+      if constexpr (decltype(last_t)::value) {
+        const int over = kRowsPerPiece * pc + lane / kChunks - (slots - 1 - 32 * b);
+        at -= (over > 0 ? over : 0) * row_bytes;
+      }
+      __builtin_amdgcn_global_load_lds((const GLOBAL_AS void*)(from + at),
+                                       (LDS_AS void*)(to + pg * kTile + 1024 * pc), 16, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < kPieces / RG; ++i) piece(kp, k_at[i], kt, i);
+#pragma unroll
+    for (int i = 0; i < kPieces / RG; ++i) piece(vp, v_at[i], vt, i);
+  };
+  // 4 lanes of a 16-lane group address a row each time: lane j row vrow + j / 4,
+  // dims 16 d + 4 (j mod 4); the read hands lane i V[vrow + e][16 d + i], e < 4
+  const int vrow = 4 * grp + (c16 >> 2);
+  auto v_off = [&](int row, int d) {
+    return 2 * D * row + 16 * ((2 * d + ((c16 & 3) >> 1)) ^ (2 * (row & (kChunks / 2 - 1)))) +
+           8 * (c16 & 1);
+  };
+
+  uint32_t bits[T];  // of a masked block: the lane's 8 slots
+  // between() runs once the block's fragments have been requested
+  auto block = [&](auto masked_t, const uint8_t* kt, const uint8_t* vt, auto&& between) {
+    constexpr bool kMasked = decltype(masked_t)::value;
+    kt += pg * kTile;
+    vt += pg * kTile;
+    f16x8 kf[D / 32][2], vf[D / 16];
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+        kf[st][nt] = *reinterpret_cast<const f16x8*>(
+            kt + 2 * D * (16 * nt + c16) + 16 * ((4 * st + grp) ^ (c16 & (kChunks - 1))));
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const v4i16 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4i16*)(vt + v_off(vrow, d)));
+      const v4i16 a1 =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS v4i16*)(vt + v_off(vrow + 16, d)));
+      vf[d] = __builtin_bit_cast(f16x8, (v8i16){a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w});
     }
-    out[t] = f32_to_f16_bits(v / S);
-    if (t == 0 && A.lse) A.lse[i * A.q_heads + h] = M + logf(S);
+    between();
+    f32x4 sc[T][2];
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+          sc[j][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              kf[st][nt], qf[j][st], st == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : sc[j][nt], 0, 0, 0);
+    f16x8 ph[T], pl[T];
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      float s[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = sc[j][e >> 2][e & 3];
+      if constexpr (kMasked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!((bits[j] >> (16 * (e >> 2) + (e & 3))) & 1)) s[e] = -__builtin_inff();
+      }
+      float p[8];
+      auto weigh = [&](float ref) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], A.scale, -ref));
+        return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      };
+      // The sum says whether the reference still serves: it passes the bound (or
+      // is no number) where a weight does, and in a row's first block, m = -inf.
+      float sum = weigh(m[j]);
+      if (__builtin_amdgcn_ballot_w64(!(sum <= kSumMax)) != 0) {
+        float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                         fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        mx = max_col4(mx) * A.scale;
+        const bool grow = mx > m[j] + kRefMax;
+        const float mn = grow ? mx - kRefRoom : m[j];
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m[j] - mn) : 1.0f;
+        // every score so far masked: reference 0, weights 2^-inf = 0
+        sum = weigh(mn == -__builtin_inff() ? 0.0f : mn);
+        l[j] *= alpha;
+        m[j] = mn;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[j][d] *= alpha;
+      }
+      l[j] += sum;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        typedef float f32x2_t __attribute__((ext_vector_type(2)));
+        const f16x2 hi = __builtin_convertvector((f32x2_t){p[e], p[e + 1]}, f16x2);
+        ph[j][e] = hi.x;
+        ph[j][e + 1] = hi.y;
+        if constexpr (kLow) {
+          // f16(p - hi), the difference exact, for both halves
+          uint32_t lo;
+          asm("v_fma_mixlo_f16 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]"
+              : "=v"(lo) : "v"(__builtin_bit_cast(uint32_t, hi)), "v"(p[e]));
+          asm("v_fma_mixhi_f16 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+              : "+v"(lo) : "v"(__builtin_bit_cast(uint32_t, hi)), "v"(p[e + 1]));
+          pl[j][e] = as_f16x2(lo).x;
+          pl[j][e + 1] = as_f16x2(lo).y;
+        }
+      }
+    }
+    // A masked weight of 0 times an infinity would reach every row: infinities
+    // and NaN are left out of the product.
+    bool any = false;
+    if constexpr (kMasked) {
+      uint32_t special = 0;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const u32x4 w = __builtin_bit_cast(u32x4, vf[d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) special |= special_bits(w[i]);
+      }
+      any = __builtin_amdgcn_ballot_w64(special != 0) != 0;
+      if (any) {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) vf[d] = without_special(vf[d]);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph[j], o[j][d], 0, 0, 0);
+    if constexpr (kLow) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+          o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl[j], o[j][d], 0, 0, 0);
+    }
+    // They go to the rows that see them, value by value.
+    if (any) {
+#pragma unroll 1
+      for (int x = 0; x < 32; ++x) {
+        // slot x: bit 16 (x / 16) + x mod 4 of the lanes with grp (x / 4) mod 4
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+          const bool sees = (__shfl(bits[j], c16 + 16 * ((x >> 2) & 3)) >>
+                             (16 * (x >> 4) + (x & 3))) & 1;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            const int c = 2 * d + (grp >> 1);
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(
+                vt + 2 * D * x + 16 * (c ^ (2 * (x & (kChunks / 2 - 1)))) + 8 * (grp & 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (sees && (v[e] & 0x7c00u) == 0x7c00u) o[j][d][e] += f16_bits_to_f32(v[e]);
+          }
+        }
+      }
+    }
+  };
+
+  // The split's masked blocks (from the one that holds slot len on), then the
+  // others; position group pg takes every PG-th of either.  With several row
+  // groups the waves keep in step, one barrier a round: it shows everyone's
+  // copies of this round and frees the other buffer.
+  const int b_tree = A.len >> 5;
+  const int b_mid = b_hi < b_tree ? b_hi : (b_lo > b_tree ? b_lo : b_tree);
+  const int masked = b_hi - b_mid, plain = b_mid - b_lo;
+  const int first = b_lo + ((pg - masked) & (PG - 1));  // of the plain ones
+  const std::true_type kMaskedBlock;
+  const std::false_type kPlainBlock;
+  auto masked_bits = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < T; ++j) bits[j] = block_bits(A, node[j], 32 * b) >> (4 * grp);
+  };
+  // plain round i: block first + PG i
+  auto plain_next = [&](int i) { return first + PG * i < b_mid ? first + PG * i : -1; };
+  const int plain_rounds = (plain + PG - 1) / PG;
+  // Masked blocks alternate between the buffers so that the last one is in k0 and
+  // the first plain one in k1.  One code for both buffers: the next copy is issued
+  // behind the block's own reads, or it would have to land before them.
+  const int masked_rounds = (masked + PG - 1) / PG;
+  const int b_tree0 = b_mid + pg;  // this group's first masked block
+  auto start = [&](int i) {  // the copy for masked round i
+    if (i < masked_rounds && b_tree0 + PG * i < b_hi) {
+      const bool even = ((masked_rounds - i) & 1) != 0;
+      copy(kMaskedBlock, b_tree0 + PG * i, even ? k0 : k1, even ? v0 : v1);
+    } else if (i >= masked_rounds && plain_next(0) >= 0) {
+      copy(kPlainBlock, plain_next(0), k1, v1);
+    }
+  };
+  start(0);
+  for (int i = 0; i < masked_rounds; ++i) {
+    const bool live = b_tree0 + PG * i < b_hi;
+    const bool even = ((masked_rounds - i) & 1) != 0;
+    if (live) masked_bits(b_tree0 + PG * i);
+    wait_vm<0>();
+    if constexpr (RG > 1) __syncthreads();
+    if (live)
+      block(kMaskedBlock, even ? k0 : k1, even ? v0 : v1, [&] {
+        wait_lds();
+        start(i + 1);
+      });
+    else
+      start(i + 1);
+  }
+  auto round = [&](int i, const uint8_t* kt, const uint8_t* vt, uint8_t* kn, uint8_t* vn) {
+    wait_vm<0>();
+    if constexpr (RG > 1) __syncthreads();
+    if (plain_next(i + 1) >= 0) copy(kPlainBlock, plain_next(i + 1), kn, vn);
+    if (plain_next(i) >= 0) block(kPlainBlock, kt, vt, [] {});
+    if constexpr (RG == 1) wait_lds();  // the buffer's reads are done before its next copy
+  };
+  for (int i = 0; i < plain_rounds; i += 2) {
+    round(i, k1, v1, k0, v0);
+    if (i + 1 < plain_rounds) round(i + 1, k0, v0, k1, v1);
+  }
+
+#pragma unroll
+  for (int j = 0; j < T; ++j) l[j] = sum_col4(l[j]);
+  // o[j][d][e]: dim 16 d + 4 grp + e of row row0 + 16 j + c16.  The position
+  // groups meet in LDS, (m, l) first, then O in parts that fit into k0; after
+  // that o[j][0 .. D / 16 / PG - 1] are the sums of this group's share of the dims.
+  if constexpr (PG > 1) {
+    float* const sm = reinterpret_cast<float*>(v0);  // [2][PG][kRows]
+    float* const so = reinterpret_cast<float*>(k0);  // [PG][RG][16][kPart]
+    constexpr int kPart = PG * D / 4, kParts = D / kPart;
+    // 16 bytes c of a row sit in slot c ^ (row mod 8), a row's lanes in other banks
+    auto so_at = [&](int g, int c) {
+      return so + ((g * RG + rg) * 16 + c16) * kPart + 4 * (c ^ (c16 & 7));
+    };
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const int r = 16 * (T * rg + j) + c16;
+      if (grp == 0) {
+        sm[pg * kRows + r] = m[j];
+        sm[(PG + pg) * kRows + r] = l[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const int r = 16 * (T * rg + j) + c16;
+      float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+      for (int g = 0; g < PG; ++g) M = fmaxf(M, sm[g * kRows + r]);
+      const float ref = M == -__builtin_inff() ? 0.0f : M;
+#pragma unroll
+      for (int g = 0; g < PG; ++g)
+        L += sm[(PG + g) * kRows + r] * __builtin_amdgcn_exp2f(sm[g * kRows + r] - ref);
+      const float w = __builtin_amdgcn_exp2f(m[j] - ref);
+      m[j] = M;
+      l[j] = L;
+      f32x4 sum[D / 16 / PG];
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+        for (int d = 0; d < kPart / 16; ++d)
+          *reinterpret_cast<f32x4*>(so_at(pg, 4 * d + grp)) = o[j][kPart / 16 * part + d] * w;
+        __syncthreads();
+        constexpr int kMine = kPart / 16 / PG;  // of this part's pieces
+#pragma unroll
+        for (int dd = 0; dd < kMine; ++dd) {
+          f32x4 s = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int g = 0; g < PG; ++g)
+            s += *reinterpret_cast<const f32x4*>(so_at(g, 4 * (kMine * pg + dd) + grp));
+          sum[kMine * part + dd] = s;
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16 / PG; ++d) o[j][d] = sum[d];
+    }
+  }
+  // piece d of this wave's sums: dims 16 piece(d) .. + 15
+  auto piece = [&](int d) {
+    constexpr int kPer = PG * D / 4 / 16 / PG;  // a group's pieces of one part
+    return d / kPer * (PG * D / 64) + kPer * pg + d % kPer;
+  };
+  constexpr int kDims = D / 16 / PG;  // pieces of 16 dims this wave writes
+#pragma unroll
+  for (int j = 0; j < T; ++j) {
+    const int r = row0 + 16 * j + c16;
+    if (r >= R) continue;
+    if (A.splits > 1) {
+      float* to = A.part + ((int64_t)(split * A.kv_heads + kvh) * R + r) * D + 4 * grp;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * piece(d)) = o[j][d];
+      if (grp == 0 && pg == 0) {
+        float* ml = A.part_ml + ((int64_t)kvh * R + r) * 2 * A.splits;
+        ml[split] = m[j];
+        ml[A.splits + split] = l[j];
+      }
+    } else {
+      const int h = kvh * A.group + r - node[j] * A.group;
+      const float inv = 1.0f / l[j];
+      uint16_t* to = A.out + (int64_t)node[j] * A.out_stride + h * D + 4 * grp;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        const f32x4 x = o[j][d];
+        const uint2 v = {pack_f16x2(x[0] * inv, x[1] * inv), pack_f16x2(x[2] * inv, x[3] * inv)};
+        *reinterpret_cast<uint2*>(to + 16 * piece(d)) = none[j] ? make_uint2(0, 0) : v;
+      }
+      if (grp == 0 && pg == 0 && A.lse)
+        A.lse[(int64_t)node[j] * A.q_heads + h] =
+            none[j] ? -__builtin_inff() : kLn2 * (m[j] + __builtin_amdgcn_logf(l[j]));
+    }
   }
 }
-extern "C" __global__ __launch_bounds__(256) void attn_tree_64(AttnTreeArgs A) { attn_tree<64>(A); }
-extern "C" __global__ __launch_bounds__(256) void attn_tree_128(AttnTreeArgs A) {
-  attn_tree<128>(A);
+
+}  // namespace
+
+#define ATTN_TREE(D, RG, T)                                                \
+  extern "C" __global__ __launch_bounds__(256, RG == 1 ? 1 : 2) void       \
+      attn_tree_##D##_##RG##T(AttnTreeArgs A) {                            \
+    attn_tree<D, RG, T>(A);                                                \
+  }
+ATTN_TREE(64, 1, 1)
+ATTN_TREE(64, 1, 2)
+ATTN_TREE(64, 2, 2)
+ATTN_TREE(64, 4, 2)
+ATTN_TREE(128, 1, 1)
+ATTN_TREE(128, 1, 2)
+ATTN_TREE(128, 2, 2)
+ATTN_TREE(128, 4, 2)
+
+// One wave per row: the splits' (m, l) one per lane (at most 64 splits), then
+// sum_s O_s 2^(m_s - M) in split order, each lane D / 64 dims.
+namespace {
+template <int D>
+__device__ __forceinline__ void attn_merge(const AttnTreeArgs& A) {
+  const int lane = threadIdx.x & 63;
+  const int R = A.n * A.group;
+  const int kvh = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= R) return;
+  const int64_t row = (int64_t)kvh * R + r;
+  const float* ml = A.part_ml + row * 2 * A.splits;
+  const float ms = lane < A.splits ? ml[lane] : -__builtin_inff();
+  const float ls = lane < A.splits ? ml[A.splits + lane] : 0.0f;
+  float M = ms;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+  const float ref = M == -__builtin_inff() ? 0.0f : M;
+  const float w = __builtin_amdgcn_exp2f(ms - ref);
+  const float L = wave_sum(ls * w);
+  typedef float Dims __attribute__((ext_vector_type(D / 64)));
+  Dims acc = 0.0f;
+  const int64_t step = (int64_t)A.kv_heads * R * D;
+  const float* p = A.part + row * D + D / 64 * lane;
+  constexpr int kAhead = 8;
+  for (int s0 = 0; s0 < A.splits; s0 += kAhead) {
+    Dims v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      v[k] = *reinterpret_cast<const Dims*>(p + (s0 + k < A.splits ? s0 + k : s0) * step);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (s0 + k < A.splits) acc += v[k] * __shfl(w, s0 + k);
+  }
+  const int node = A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv);
+  const int h = kvh * A.group + r - node * A.group;
+  const float inv = 1.0f / L;
+  const bool empty = row_empty(A, node);
+  uint16_t* to = A.out + (int64_t)node * A.out_stride + h * D + D / 64 * lane;
+  if constexpr (D == 128)
+    *reinterpret_cast<uint32_t*>(to) = empty ? 0u : pack_f16x2(acc[0] * inv, acc[1] * inv);
+  else
+    *to = empty ? 0 : f32_to_f16_bits(acc[0] * inv);
+  if (lane == 0 && A.lse)
+    A.lse[(int64_t)node * A.q_heads + h] = empty ? -__builtin_inff() : kLn2 * (M + __builtin_amdgcn_logf(L));
+}
+}  // namespace
+extern "C" __global__ __launch_bounds__(256) void attn_merge_64(AttnTreeArgs A) {
+  attn_merge<64>(A);
+}
+extern "C" __global__ __launch_bounds__(256) void attn_merge_128(AttnTreeArgs A) {
+  attn_merge<128>(A);
 }
 
 // ---------------------------------------------------- attention weights ----
 
-// D / 8 lanes per slot, 256 / (D / 8) slots per workgroup; grid.y = layer and
-// kv head.  Each slot's sum runs over the rows in order.
+// D / 8 lanes per slot, 256 / (D / 8) slots per workgroup; grid: slots, kv
+// heads, layers.  Each slot's sum runs over the rows in order.
 template <int D>
 __device__ __forceinline__ void weights_add(const WeightsArgs& A) {
   constexpr int L = D / 8, G = 256 / L;
   const int lane = threadIdx.x % L;
   const int p = blockIdx.x * G + threadIdx.x / L;
-  const int layer = blockIdx.y / A.kv_heads, kvh = blockIdx.y % A.kv_heads;
+  const int layer = blockIdx.z, kvh = blockIdx.y;
   if (p >= A.len + A.n) return;
   const u32x4 k = *reinterpret_cast<const u32x4*>(
       A.k + ((layer * A.max_seq + p) * A.kv_heads + kvh) * D + 8 * lane);

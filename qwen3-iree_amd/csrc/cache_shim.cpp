@@ -16,7 +16,7 @@ namespace {
 
 struct {
   hipModule_t module = nullptr;
-  hipFunction_t mask = nullptr, attn[2] = {}, weights[2] = {}, select = nullptr, compact = nullptr,
+  hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2] = {}, select = nullptr, compact = nullptr,
                 argmax = nullptr, argmax_final = nullptr;
 } c;
 
@@ -73,6 +73,50 @@ int check_rows(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads, int6
   return Q8_OK;
 }
 
+// How f16_attn_tree divides its work.
+struct AttnPlan {
+  int kernel;  // rows of a workgroup: 16, 32, 64, 128; position groups 4, 4, 2, 1
+  int row_blocks, splits, blocks;
+  int splits_max;  // before the blocks are dealt out evenly; does not shrink with len
+};
+
+constexpr int kMaxSplits = 64;  // one lane each in the merge
+
+// Splits of the nb blocks of 32 slots: each costs a partial written and merged,
+// the first one a launch, and each block of a split costs a round of its
+// workgroups, so about sqrt(nb) of them, and none up to 10 blocks.  us a layer
+// (16 query over 8 kv heads of 128), with 1 / 4 / 8 / 16 / 32 splits:
+//   1 row, 300 slots (10 blocks) 7.0 / 7.5 / 8.0, 1000 (32) 11.1 / 9.2 / 8.7 /
+//   9.2 / 10.1, 4000 (126) 46.6 / 19.2 / 13.8 / 11.8 / 12.2, 16384 (513) 97.7 /
+//   35.1 / 24.1 / 21.8 / 23.2; 61 rows, 1024 (34) 28.6 / 15.4 / 14.2 / 15.1 /
+//   16.2, 8191 (258) 184 / 55.5 / 34.3 / 24.8 / 22.9 (64: 29.7); 256 rows, 1024
+//   (40) 38.0 / 26.1 / 27.7 / 30.3 / 33.6, 16384 (520) 334 / 103 / 66.9 / 63.7 / 76.6.
+// At most one workgroup a CU where it takes the CU's LDS (up to 32 rows), else two.
+AttnPlan attn_plan(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) {
+  const int rows = n * (q_heads / a->kv_heads);
+  AttnPlan p{};
+  p.kernel = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+  const int per_wg = 16 << p.kernel;
+  p.row_blocks = (rows + per_wg - 1) / per_wg;
+  const int nb = (len + n + 31) / 32;
+  const int most = (p.kernel <= 1 ? 1 : 2) * q8_shim::compute_units() / (a->kv_heads * p.row_blocks);
+  const int want = nb <= 10 ? 1 : (int)(1.25 * std::sqrt((double)nb));
+  p.splits_max = std::max(1, std::min({want, most, kMaxSplits}));
+  p.blocks = (nb + p.splits_max - 1) / p.splits_max;
+  p.splits = (nb + p.blocks - 1) / p.blocks;
+  return p;
+}
+
+// partial outputs, then their references and sums
+size_t attn_part_floats(const f16_cache* a, int32_t n, int32_t q_heads, int splits) {
+  return (size_t)splits * n * q_heads * a->head_dim;
+}
+
+size_t attn_workspace(const f16_cache* a, const AttnPlan& p, int32_t n, int32_t q_heads) {
+  if (p.splits_max == 1) return 0;
+  return 4 * (attn_part_floats(a, n, q_heads, p.splits_max) + 2 * (size_t)n * q_heads * p.splits_max);
+}
+
 constexpr uint32_t kArgmaxWgsMax = 1024;
 
 }  // namespace
@@ -85,8 +129,12 @@ void cache_load(const char* path) {
   struct {
     hipFunction_t* fn;
     const char* name;
-  } names[] = {{&c.mask, "tree_mask_k"},          {&c.attn[0], "attn_tree_64"},
-               {&c.attn[1], "attn_tree_128"},     {&c.weights[0], "weights_add_64"},
+  } names[] = {{&c.mask, "tree_mask_k"},          {&c.attn[0][0], "attn_tree_64_11"},
+               {&c.attn[0][1], "attn_tree_64_12"}, {&c.attn[0][2], "attn_tree_64_22"},
+               {&c.attn[0][3], "attn_tree_64_42"}, {&c.attn[1][0], "attn_tree_128_11"},
+               {&c.attn[1][1], "attn_tree_128_12"}, {&c.attn[1][2], "attn_tree_128_22"},
+               {&c.attn[1][3], "attn_tree_128_42"}, {&c.merge[0], "attn_merge_64"},
+               {&c.merge[1], "attn_merge_128"},  {&c.weights[0], "weights_add_64"},
                {&c.weights[1], "weights_add_128"}, {&c.select, "cache_select_k"},
                {&c.compact, "cache_compact_k"},   {&c.argmax, "gemm_argmax_k"},
                {&c.argmax_final, "gemm_argmax_final"}};
@@ -121,7 +169,11 @@ int f16_tree_mask(const int32_t* parents, int32_t n, uint32_t* mask, int32_t* de
   return q8_shim::launch(c.mask, 1, kTreeMax, args, static_cast<hipStream_t>(stream));
 }
 
-size_t f16_attn_tree_workspace_bytes(const f16_cache*, int32_t, int32_t, int32_t) { return 0; }
+size_t f16_attn_tree_workspace_bytes(const f16_cache* a, int32_t len, int32_t n,
+                                     int32_t q_heads) {
+  if (check_cache(a, "cache") || check_rows(a, len, n, q_heads, 1 << 20, 1.0f)) return 0;
+  return attn_workspace(a, attn_plan(a, len, n, q_heads), n, q_heads);
+}
 
 int f16_attn_tree(const f16_cache* a, int32_t layer, int32_t len, const void* q, int64_t q_stride,
                   int32_t q_heads, const uint32_t* mask, int32_t n, float scale, void* out,
@@ -138,9 +190,13 @@ int f16_attn_tree(const f16_cache* a, int32_t layer, int32_t len, const void* q,
                 (long long)out_stride, q_heads * a->head_dim);
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(mask, 4) || !aligned(lse, 4))
     return fail(Q8_ERR_MISALIGNED, "q and out 16, mask and lse 4-byte alignment");
-  (void)workspace;
-  (void)workspace_bytes;
   if ((rc = check_ready())) return rc;
+  const AttnPlan plan = attn_plan(a, len, n, q_heads);
+  const size_t need = attn_workspace(a, plan, n, q_heads);
+  if (need && !workspace) return fail(Q8_ERR_NULL_POINTER, "null workspace");
+  if (!aligned(workspace, 256)) return fail(Q8_ERR_MISALIGNED, "workspace 256-byte alignment");
+  if (workspace_bytes < need)
+    return fail(Q8_ERR_BAD_SHAPE, "workspace of %zu bytes < %zu needed", workspace_bytes, need);
   const int64_t base = (int64_t)layer * a->max_seq * a->kv_heads * a->head_dim;
   AttnTreeArgs args{static_cast<const uint16_t*>(a->k) + base,
                     static_cast<const uint16_t*>(a->v) + base,
@@ -150,15 +206,27 @@ int f16_attn_tree(const f16_cache* a, int32_t layer, int32_t len, const void* q,
                     lse,
                     q_stride,
                     out_stride,
+                    static_cast<float*>(workspace),
+                    static_cast<float*>(workspace) +
+                        attn_part_floats(a, n, q_heads, plan.splits),
                     len,
                     n,
                     q_heads,
                     a->kv_heads,
                     q_heads / a->kv_heads,
-                    scale};
+                    (uint32_t)((0xffffffffull + q_heads / a->kv_heads) / (q_heads / a->kv_heads)),
+                    plan.splits,
+                    plan.blocks,
+                    scale * 1.44269504088896341f};
   void* p[] = {&args};
-  return q8_shim::launch(c.attn[a->head_dim / 64 - 1], (uint32_t)(n * q_heads), 256, p,
-                         static_cast<hipStream_t>(stream));
+  const int d = a->head_dim / 64 - 1;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint32_t heads = (uint32_t)a->kv_heads;
+  if ((rc = q8_shim::launch3(c.attn[d][plan.kernel], heads, (uint32_t)plan.row_blocks,
+                             (uint32_t)plan.splits, 256, p, st)))
+    return rc;
+  if (plan.splits == 1) return Q8_OK;
+  return q8_shim::launch3(c.merge[d], (uint32_t)((n * args.group + 3) / 4), heads, 1, 256, p, st);
 }
 
 int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t q_layer_stride,
@@ -190,9 +258,9 @@ int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t
                    scale};
   void* p[] = {&args};
   const int per_wg = 256 / (a->head_dim / 8);
-  return q8_shim::launch2(c.weights[a->head_dim / 64 - 1],
+  return q8_shim::launch3(c.weights[a->head_dim / 64 - 1],
                           (uint32_t)((len + n + per_wg - 1) / per_wg),
-                          (uint32_t)(a->layers * a->kv_heads), 256, p,
+                          (uint32_t)a->kv_heads, (uint32_t)a->layers, 256, p,
                           static_cast<hipStream_t>(stream));
 }
 

@@ -773,9 +773,11 @@ int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStre
   return ::launch(fn, grid, block, args, stream);
 }
 
-int launch2(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t block, void** args,
+int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t block, void** args,
             hipStream_t stream) {
-  return ::launch2(fn, gx, gy, block, args, stream);
+  hipError_t e = hipModuleLaunchKernel(fn, gx, gy, gz, block, 1, 1, 0, stream, args, nullptr);
+  if (e != hipSuccess) return hip_fail(e, "kernel launch");
+  return Q8_OK;
 }
 
 int noalloc_ready() {

@@ -16,9 +16,9 @@ int hip_error(hipError_t e, const char* what);
 // Q8_OK once q8gemv_init has run.
 int ready();
 int compute_units();
-// The launches every entry point makes (1-D and 2-D grids of 1-D workgroups).
+// The launches every entry point makes (1-D and 3-D grids of 1-D workgroups).
 int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStream_t stream);
-int launch2(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t block, void** args,
+int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t block, void** args,
             hipStream_t stream);
 
 // Implemented in cache_shim.cpp: loads the code object at `path` (a failure

@@ -8,8 +8,10 @@ conversion to base 2 add 4 roundings of the score itself, so
 exp and log are good to 4 ulp, and a sum of N non-negative terms in at least 16
 chains to (N / 16 + 32) 2^-24 relative.  With e = max_j e_s of the row:
   lse:    e + (N / 16 + 40) 2^-24 + 2^-23 |lse|
-  a weight, relative: 2 e + (N / 16 + 48) 2^-24, and 2^-21 where it is multiplied
-  with v as the sum of two f16 values (at most 2^-22 off) or less exactly never
+  a weight, relative: 2 e + (N / 16 + 48) 2^-24; where it is multiplied with v it
+  has been rounded to f16, at most half a step, 2^-11 of itself (the kernels keep
+  weights below 2^-14 of 2^6 or more, whose step is 2^-24, so N of them add
+  N 2^-25 / 2^6 of the row's largest)
   out:    that, times sum p |v|, and half a step of f16: 2^-11 |out| + 2^-25.
 """
 from __future__ import annotations
@@ -82,11 +84,12 @@ def attention(q, k, v, see, length, scale):
         p = w / tot
         N = len(at)
         lse_tol[i] = e + (N / 16 + 40) * EPS + 2 * EPS * np.abs(lse[i])
-        rel = 2 * e + (N / 16 + 48) * EPS + 2.0 ** -21
+        rel = 2 * e + (N / 16 + 48) * EPS + 2.0 ** -11
+        small = N * 2.0 ** -31 * p.max(-1)  # of weights that are subnormal in f16
         for h in range(qh):
             vv = v[at, h // g].astype(np.float64)
             out[i, h] = p[h] @ vv
-            out_tol[i, h] = rel[h] * (p[h] @ np.abs(vv)) + 2.0 ** -11 * np.abs(out[i, h]) + 2.0 ** -25
+            out_tol[i, h] = rel[h] * (p[h] @ np.abs(vv)) + small[h] * np.abs(vv).max(0) + 2.0 ** -11 * np.abs(out[i, h]) + 2.0 ** -25
     return out, lse, out_tol, lse_tol
 
 
