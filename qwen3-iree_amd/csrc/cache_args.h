@@ -29,8 +29,10 @@ struct WeightsArgs {
   const float* lse;
   const int32_t* path;  // or null
   int64_t max_seq, q_layer_stride, q_stride, lse_layer_stride;
-  int32_t layers, kv_heads, q_heads, group, len, n, rows;
-  float scale;
+  int32_t kv_heads, q_heads, group, len, n, rows;
+  uint32_t group_inv;  // as in AttnTreeArgs
+  int32_t blocks;      // blocks of 32 slots a wave takes
+  float scale;         // with log2 e
 };
 
 struct SelectArgs {

@@ -8,29 +8,7 @@
 
 namespace {
 
-constexpr float kLn2 = 0.693147180559945309f;
-
-__device__ __forceinline__ float half_lo(uint32_t v) { return (float)as_f16x2(v).x; }
-__device__ __forceinline__ float half_hi(uint32_t v) { return (float)as_f16x2(v).y; }
-
-// 8 products of f16 pairs, summed in f32
-__device__ __forceinline__ float dot8(const u32x4& a, const u32x4& b) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s = fmaf(half_lo(a[i]), half_lo(b[i]), s);
-    s = fmaf(half_hi(a[i]), half_hi(b[i]), s);
-  }
-  return s;
-}
-
-// the sum over L consecutive lanes (a power of two), in each of them
-template <int L>
-__device__ __forceinline__ float sum_lanes(float v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
+constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 
 }  // namespace
 
@@ -600,42 +578,224 @@ extern "C" __global__ __launch_bounds__(256) void attn_merge_128(AttnTreeArgs A)
 }
 
 // ---------------------------------------------------- attention weights ----
+//
+// The scores of 32 slots and 16 rows are S^T = K Q^T as in the attention: lane
+// (c16, grp) holds row c16's at slots 4 grp + e and 16 + 4 grp + e, adds
+// exp2(s - lse) of every row tile to 8 sums, and the 16 lanes of a DPP row meet
+// at the end.  K fragments come straight from memory (16 rows x 64 bytes a load)
+// and are read once; the sums run in one fixed order.
+namespace {
 
-// D / 8 lanes per slot, 256 / (D / 8) slots per workgroup; grid: slots, kv
-// heads, layers.  Each slot's sum runs over the rows in order.
+// One row as a lane's column: its query vector, log-sum-exp and the last slot it
+// sees (-1: none).
 template <int D>
-__device__ __forceinline__ void weights_add(const WeightsArgs& A) {
-  constexpr int L = D / 8, G = 256 / L;
-  const int lane = threadIdx.x % L;
-  const int p = blockIdx.x * G + threadIdx.x / L;
-  const int layer = blockIdx.z, kvh = blockIdx.y;
-  if (p >= A.len + A.n) return;
-  const u32x4 k = *reinterpret_cast<const u32x4*>(
-      A.k + ((layer * A.max_seq + p) * A.kv_heads + kvh) * D + 8 * lane);
-  float sum = 0.0f;
-  for (int i = p < A.len ? 0 : p - A.len; i < A.n; ++i) {
-    const int r = A.path ? A.path[i] : i;
-    if (r < 0 || r >= A.rows) continue;
-    for (int g = 0; g < A.group; ++g) {
-      const int h = kvh * A.group + g;
-      const u32x4 q = *reinterpret_cast<const u32x4*>(A.q + layer * A.q_layer_stride +
-                                                      r * A.q_stride + h * D + 8 * lane);
-      const float lse = A.lse[layer * A.lse_layer_stride + (int64_t)r * A.q_heads + h];
-      const float s = A.scale * sum_lanes<L>(dot8(q, k));
-      if (lse != -__builtin_inff()) sum += expf(s - lse);
+struct WeightRow {
+  f16x8 q[D / 32];
+  float lse;  // base 2
+  int last;
+
+  // row r of the kv head (token r / group); src: the row of q that token has
+  __device__ __forceinline__ void load(const WeightsArgs& A, int layer, int kvh, int r, int i,
+                                       int src) {
+    const int h = kvh * A.group + r - i * A.group;
+    const bool ok = r < A.n * A.group && src >= 0 && src < A.rows;
+    const int64_t at = ok ? src : 0;
+    const uint16_t* p = A.q + layer * A.q_layer_stride + at * A.q_stride + (ok ? h : 0) * D +
+                        8 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st)
+      q[st] = __builtin_bit_cast(f16x8, load_global(reinterpret_cast<const u32x4*>(p + 32 * st)));
+    const float x = A.lse[layer * A.lse_layer_stride + at * A.q_heads + (ok ? h : 0)];
+    lse = x * kLog2e;
+    last = ok && x != -__builtin_inff() ? A.len + i : -1;
+  }
+};
+
+template <int D>
+struct WeightKeys {
+  f16x8 k[D / 32][2];
+  // slots p0 .. p0 + 31; those behind `slots` repeat the last
+  __device__ __forceinline__ void load(const uint16_t* base, int64_t row, int p0, int slots) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const int p = p0 + 16 * nt + (lane & 15);
+      const uint16_t* from = base + (p < slots ? p : slots - 1) * row + 8 * (lane >> 4);
+#pragma unroll
+      for (int st = 0; st < D / 32; ++st)
+        k[st][nt] = __builtin_bit_cast(
+            f16x8, load_global(reinterpret_cast<const u32x4*>(from + 32 * st)));
     }
   }
-  if (lane == 0) {
-    float* w = A.weights + ((int64_t)layer * A.kv_heads + kvh) * A.max_seq + p;
-    *w = p < A.len ? *w + sum : sum;
+};
+
+// sum[e] += the weights of slots p0 + 16 (e / 4) + 4 grp + e mod 4
+template <int D>
+__device__ __forceinline__ void add_weights(const WeightRow<D>& R, const WeightKeys<D>& K, int p0,
+                                            float scale, bool edge, float (&sum)[8]) {
+  f32x4 sc[2];
+#pragma unroll
+  for (int st = 0; st < D / 32; ++st)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+      sc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+          K.k[st][nt], R.q[st], st == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : sc[nt], 0, 0, 0);
+  if (edge) {
+    const int p = p0 + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale, -R.lse));
+      sum[e] += p + 16 * (e >> 2) + (e & 3) <= R.last ? w : 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sum[e] += __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale, -R.lse));
   }
 }
-extern "C" __global__ __launch_bounds__(256) void weights_add_64(WeightsArgs A) {
-  weights_add<64>(A);
+
+// The lane's sums over all 16 rows; lanes c16 < 8 get that of slot
+// 16 (c16 / 4) + 4 grp + c16 mod 4.
+__device__ __forceinline__ float rows_sum(const float (&sum)[8]) {
+  const int c16 = threadIdx.x & 15;
+  float v = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float s = reduce_row16(sum[e]);
+    v = c16 == e ? s : v;
+  }
+  return v;
 }
-extern "C" __global__ __launch_bounds__(256) void weights_add_128(WeightsArgs A) {
-  weights_add<128>(A);
+__device__ __forceinline__ int sum_slot() {
+  const int lane = threadIdx.x & 63, c16 = lane & 15;
+  return 16 * (c16 >> 2) + 4 * (lane >> 4) + (c16 & 3);
 }
+
+__device__ __forceinline__ int weight_source(const WeightsArgs& A, int i) {
+  return i >= A.n ? -1 : (A.path ? A.path[i] : i);
+}
+
+// Up to 16 NT rows, whose queries stay in registers: bound by the bytes of K.
+// A wave takes A.blocks consecutive blocks, the next one's keys requested before
+// one is computed.
+template <int D, int NT>
+__device__ __forceinline__ void weights_add(const WeightsArgs& A) {
+  const int lane = threadIdx.x & 63, c16 = lane & 15;
+  const int kvh = blockIdx.y, layer = blockIdx.z;
+  const int slots = A.len + A.n, nb = (slots + 31) >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b0 = (4 * blockIdx.x + wave) * A.blocks;
+  const int b1 = b0 + A.blocks < nb ? b0 + A.blocks : nb;
+  if (b0 >= nb) return;
+  const int64_t row = (int64_t)A.kv_heads * D;
+  const uint16_t* kb = A.k + layer * A.max_seq * row + kvh * D;
+  float* wb = A.weights + ((int64_t)layer * A.kv_heads + kvh) * A.max_seq;
+  WeightKeys<D> keys[2];
+  keys[0].load(kb, row, 32 * b0, slots);
+  WeightRow<D> rows[NT];
+  bool all = true;  // every row exists and counts
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int r = 16 * j + c16;
+    const int i = A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv);
+    rows[j].load(A, layer, kvh, r, i, weight_source(A, i));
+    all = all && rows[j].last >= 0;
+  }
+  const bool some = __builtin_amdgcn_ballot_w64(!all) != 0;
+  auto block = [&](int b, const WeightKeys<D>& now, WeightKeys<D>& next) {
+    if (b + 1 < b1) next.load(kb, row, 32 * b + 32, slots);
+    const int p = 32 * b + sum_slot();
+    const bool mine = c16 < 8 && p < slots;
+    const float old = mine && p < A.len ? wb[p] : 0.0f;
+    float sum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      add_weights<D>(rows[j], now, 32 * b, A.scale, some || 32 * b + 32 > A.len, sum);
+    const float v = rows_sum(sum);
+    if (mine) wb[p] = old + v;
+  };
+  for (int b = b0; b < b1; b += 2) {
+    block(b, keys[0], keys[1]);
+    if (b + 1 < b1) block(b + 1, keys[1], keys[0]);
+  }
+}
+
+// Any number of rows: a workgroup holds the keys of 64 slots, its waves take the
+// row tiles in turn (the next one's queries requested before one is computed)
+// and meet in LDS.
+template <int D>
+__device__ __forceinline__ void weights_add_many(const WeightsArgs& A) {
+  __shared__ int source[kTreeMax];
+  __shared__ float part[4][64];
+  const int t = threadIdx.x, lane = t & 63, c16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = blockIdx.y, layer = blockIdx.z;
+  const int slots = A.len + A.n, p0 = 64 * blockIdx.x;
+  const int64_t row = (int64_t)A.kv_heads * D;
+  const uint16_t* kb = A.k + layer * A.max_seq * row + kvh * D;
+  float* wb = A.weights + ((int64_t)layer * A.kv_heads + kvh) * A.max_seq;
+  WeightKeys<D> keys[2];
+  keys[0].load(kb, row, p0, slots);
+  keys[1].load(kb, row, p0 + 32, slots);
+  source[t] = weight_source(A, t);
+  __syncthreads();
+  float sum[2][8];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[x][e] = 0.0f;
+  const int tiles = (A.n * A.group + 15) >> 4;
+  auto load = [&](int tile, WeightRow<D>& R) {
+    const int r = 16 * tile + c16;
+    const int i = A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv);
+    R.load(A, layer, kvh, r, i, i < A.n ? source[i] : -1);
+  };
+  auto use = [&](const WeightRow<D>& R) {
+    const bool edge = p0 + 64 > A.len || __builtin_amdgcn_ballot_w64(R.last < 0) != 0;
+    add_weights<D>(R, keys[0], p0, A.scale, edge, sum[0]);
+    add_weights<D>(R, keys[1], p0 + 32, A.scale, edge, sum[1]);
+  };
+  WeightRow<D> rows[2];
+  if (wave < tiles) load(wave, rows[0]);
+  for (int tile = wave; tile < tiles; tile += 8) {
+    if (tile + 4 < tiles) load(tile + 4, rows[1]);
+    use(rows[0]);
+    if (tile + 4 >= tiles) break;
+    if (tile + 8 < tiles) load(tile + 8, rows[0]);
+    use(rows[1]);
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const float v = rows_sum(sum[x]);
+    if (c16 < 8) part[wave][32 * x + sum_slot()] = v;
+  }
+  __syncthreads();
+  const int p = p0 + t;
+  if (t < 64 && p < slots) {
+    const float v = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
+    wb[p] = p < A.len ? wb[p] + v : v;
+  }
+}
+
+}  // namespace
+
+#define WEIGHTS_ADD(D)                                                                      \
+  extern "C" __global__ __launch_bounds__(256) void weights_add_##D##_1(WeightsArgs A) {    \
+    weights_add<D, 1>(A);                                                                   \
+  }                                                                                         \
+  extern "C" __global__ __launch_bounds__(256) void weights_add_##D##_2(WeightsArgs A) {    \
+    weights_add<D, 2>(A);                                                                   \
+  }                                                                                         \
+  extern "C" __global__ __launch_bounds__(256) void weights_add_##D##_4(WeightsArgs A) {    \
+    weights_add<D, 4>(A);                                                                   \
+  }                                                                                         \
+  extern "C" __global__ __launch_bounds__(256) void weights_add_##D##_many(WeightsArgs A) { \
+    weights_add_many<D>(A);                                                                 \
+  }
+WEIGHTS_ADD(64)
+WEIGHTS_ADD(128)
 
 // ------------------------------------------------------------ selection ----
 

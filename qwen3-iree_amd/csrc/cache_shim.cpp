@@ -16,7 +16,7 @@ namespace {
 
 struct {
   hipModule_t module = nullptr;
-  hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2] = {}, select = nullptr, compact = nullptr,
+  hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select = nullptr, compact = nullptr,
                 argmax = nullptr, argmax_final = nullptr;
 } c;
 
@@ -72,6 +72,11 @@ int check_rows(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads, int6
     return fail(Q8_ERR_BAD_ARGUMENT, "scale %g is not finite and positive", scale);
   return Q8_OK;
 }
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// ceil(2^32 / group), for the kernels' division of a row by it
+uint32_t group_inverse(int group) { return (uint32_t)((0xffffffffull + group) / group); }
 
 // How f16_attn_tree divides its work.
 struct AttnPlan {
@@ -134,8 +139,11 @@ void cache_load(const char* path) {
                {&c.attn[0][3], "attn_tree_64_42"}, {&c.attn[1][0], "attn_tree_128_11"},
                {&c.attn[1][1], "attn_tree_128_12"}, {&c.attn[1][2], "attn_tree_128_22"},
                {&c.attn[1][3], "attn_tree_128_42"}, {&c.merge[0], "attn_merge_64"},
-               {&c.merge[1], "attn_merge_128"},  {&c.weights[0], "weights_add_64"},
-               {&c.weights[1], "weights_add_128"}, {&c.select, "cache_select_k"},
+               {&c.merge[1], "attn_merge_128"},  {&c.weights[0][0], "weights_add_64_1"},
+               {&c.weights[0][1], "weights_add_64_2"}, {&c.weights[0][2], "weights_add_64_4"},
+               {&c.weights[0][3], "weights_add_64_many"}, {&c.weights[1][0], "weights_add_128_1"},
+               {&c.weights[1][1], "weights_add_128_2"}, {&c.weights[1][2], "weights_add_128_4"},
+               {&c.weights[1][3], "weights_add_128_many"}, {&c.select, "cache_select_k"},
                {&c.compact, "cache_compact_k"},   {&c.argmax, "gemm_argmax_k"},
                {&c.argmax_final, "gemm_argmax_final"}};
   for (auto& n : names) {
@@ -214,10 +222,10 @@ int f16_attn_tree(const f16_cache* a, int32_t layer, int32_t len, const void* q,
                     q_heads,
                     a->kv_heads,
                     q_heads / a->kv_heads,
-                    (uint32_t)((0xffffffffull + q_heads / a->kv_heads) / (q_heads / a->kv_heads)),
+                    group_inverse(q_heads / a->kv_heads),
                     plan.splits,
                     plan.blocks,
-                    scale * 1.44269504088896341f};
+                    scale * kLog2e};
   void* p[] = {&args};
   const int d = a->head_dim / 64 - 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -247,19 +255,31 @@ int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t
   if (!aligned(q, 16) || !aligned(lse, 4) || !aligned(path, 4))
     return fail(Q8_ERR_MISALIGNED, "q 16, lse and path 4-byte alignment");
   if ((rc = check_ready())) return rc;
-  WeightsArgs args{static_cast<const uint16_t*>(a->k), a->weights,
-                   static_cast<const uint16_t*>(q),    lse,
-                   path,                               a->max_seq,
-                   q_layer_stride,                     q_stride,
-                   lse_layer_stride,                   a->layers,
-                   a->kv_heads,                        q_heads,
-                   q_heads / a->kv_heads,              len,
-                   n,                                  rows,
-                   scale};
+  const int group = q_heads / a->kv_heads, tiles = (n * group + 15) / 16;
+  const int kernel = tiles <= 1 ? 0 : tiles <= 2 ? 1 : tiles <= 4 ? 2 : 3;
+  const int64_t nb = (len + n + 31) / 32, heads = (int64_t)a->layers * a->kv_heads;
+  const int64_t blocks = std::clamp<int64_t>(nb * heads / (q8_shim::compute_units() * 16), 1, 16);
+  WeightsArgs args{static_cast<const uint16_t*>(a->k),
+                   a->weights,
+                   static_cast<const uint16_t*>(q),
+                   lse,
+                   path,
+                   a->max_seq,
+                   q_layer_stride,
+                   q_stride,
+                   lse_layer_stride,
+                   a->kv_heads,
+                   q_heads,
+                   group,
+                   len,
+                   n,
+                   rows,
+                   group_inverse(group),
+                   (int32_t)blocks,
+                   scale * kLog2e};
   void* p[] = {&args};
-  const int per_wg = 256 / (a->head_dim / 8);
-  return q8_shim::launch3(c.weights[a->head_dim / 64 - 1],
-                          (uint32_t)((len + n + per_wg - 1) / per_wg),
+  const int64_t wgs = kernel == 3 ? (len + n + 63) / 64 : (nb + 4 * blocks - 1) / (4 * blocks);
+  return q8_shim::launch3(c.weights[a->head_dim / 64 - 1][kernel], (uint32_t)wgs,
                           (uint32_t)a->kv_heads, (uint32_t)a->layers, 256, p,
                           static_cast<hipStream_t>(stream));
 }
