@@ -50,6 +50,7 @@ struct CompactArgs {
   const int32_t* keep;
   int64_t src_seq, dst_seq;
   int32_t kv_heads, head_dim, per_head, base, count;
+  int32_t range;  // kept slots of one workgroup
 };
 
 #endif

@@ -809,16 +809,48 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 }
 }  // namespace
 
-// One workgroup per layer and kv head.  The weight of the last slot that still
-// fits is found digit by digit (8 bits of its order number at a time, a
-// histogram of the slots that agree in the digits before); then the slots are
-// walked in order and each thread's place comes from a prefix count, so the
-// result has no order of arrival in it.
-extern "C" __global__ __launch_bounds__(1024) void cache_select_k(SelectArgs A) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t wave_above[16], wave_equal[16];
-  __shared__ uint32_t s_prefix, s_need;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// One workgroup per layer and kv head.  The order number of the last slot that
+// still fits is found in three digits (11, 11 and 10 bits): a histogram in LDS of
+// the slots that agree in the digits before, then a count from its top down.  A
+// wave holds 64 E consecutive slots in registers, 64 at a time, so the places of
+// the kept slots come from one prefix count over the waves and ballots: nothing
+// depends on an order of arrival.  E = 0 reads the weights again for each digit.
+// Latency bound: with one layer (8 workgroups) the chain of barriers, see the
+// launch for figures.
+namespace {
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+// the sum over the lanes up to this one
+__device__ __forceinline__ uint32_t scan_u32(uint32_t v) {
+  v += dpp_u32<0x111>(v);       // row_shr 1, 2, 4, 8
+  v += dpp_u32<0x112>(v);
+  v += dpp_u32<0x114>(v);
+  v += dpp_u32<0x118>(v);
+  v += dpp_u32<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to the row behind
+  v += dpp_u32<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+  return v;
+}
+// the sum of v[0 .. wave - 1], 16 words in LDS
+__device__ __forceinline__ uint32_t waves_before(const uint32_t* v, int wave) {
+  const int lane = threadIdx.x & 63;
+  uint32_t x = lane < wave ? v[lane & 15] : 0u;
+  x += dpp_u32<0x111>(x);
+  x += dpp_u32<0x112>(x);
+  x += dpp_u32<0x114>(x);
+  x += dpp_u32<0x118>(x);
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 15);
+}
+
+template <int E>
+__device__ __forceinline__ void cache_select(const SelectArgs& A) {
+  constexpr int kBins = 2048;
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t wave_sum_[16], wave_above[16], wave_equal[16];
+  __shared__ uint32_t s_digit, s_left;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const float* w = A.weights + (int64_t)blockIdx.x * A.max_seq;
   int32_t* keep = A.keep + (int64_t)blockIdx.x * A.budget;
   const int first = A.sinks, last = A.len - A.recent;
@@ -826,85 +858,135 @@ extern "C" __global__ __launch_bounds__(1024) void cache_select_k(SelectArgs A) 
   for (int j = t; j < A.sinks; j += 1024) keep[j] = j;
   for (int j = t; j < A.recent; j += 1024) keep[A.budget - A.recent + j] = last + j;
   if (middle == 0) return;
-  if (t == 0) {
-    s_prefix = 0;
-    s_need = (uint32_t)middle;
-  }
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (t < 256) hist[t] = 0;
+  // this wave's slots: p0 + 64 e + lane, e < count
+  const int count = E ? E : (last - first + 1023) >> 10;
+  const int p0 = first + wave * 64 * count + lane;
+  uint32_t own[E ? E : 1];
+#pragma unroll
+  for (int e = 0; e < E; ++e) own[e] = p0 + 64 * e < last ? weight_order(w[p0 + 64 * e]) : 0u;
+  auto number = [&](int e) {
+    if constexpr (E != 0) return own[e];
+    else return p0 + 64 * e < last ? weight_order(w[p0 + 64 * e]) : 0u;
+  };
+  uint32_t prefix = 0, need = (uint32_t)middle;
+#pragma unroll
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+    const int bits = digit == 2 ? 10 : 11;
+    hist[t] = 0;
+    hist[1024 + t] = 0;
     __syncthreads();
-    const uint32_t prefix = s_prefix, need = s_need;
-    for (int p = first + t; p < last; p += 1024) {
-      const uint32_t o = weight_order(w[p]);
-      if (shift == 24 || (o >> (shift + 8)) == prefix >> (shift + 8))
-        atomicAdd(&hist[(o >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (t == 0) {
-      uint32_t left = need;
-      int d = 255;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      s_prefix = prefix | (uint32_t)d << shift;
-      s_need = left;
-    }
-    __syncthreads();
-  }
-  // keep every slot above the bound, and the first s_need that equal it
-  const uint32_t bound = s_prefix, ties = s_need;
-  uint32_t above0 = 0, equal0 = 0;  // among the slots before this round
-  for (int p0 = first; p0 < last; p0 += 1024) {
-    const int p = p0 + t;
-    const uint32_t o = p < last ? weight_order(w[p]) : 0u;
-    const bool above = p < last && o > bound, equal = p < last && o == bound;
-    const uint64_t ma = __ballot(above), me = __ballot(equal);
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    if (lane == 0) {
-      wave_above[wave] = (uint32_t)__popcll(ma);
-      wave_equal[wave] = (uint32_t)__popcll(me);
-    }
-    __syncthreads();
-    uint32_t a = above0, e = equal0;
-    for (int v = 0; v < 16; ++v) {
-      if (v < wave) {
-        a += wave_above[v];
-        e += wave_equal[v];
+#pragma unroll
+    for (int e = 0; e < count; ++e) {
+      const uint32_t o = number(e);
+      const bool in = p0 + 64 * e < last && (digit == 0 || (o ^ prefix) >> (shift + bits) == 0);
+      const uint32_t d = (o >> shift) & ((1u << bits) - 1);
+      // many equal weights: one addition for the wave
+      const uint64_t m = __ballot(in);
+      if (m == 0) continue;
+      const int leader = __ffsll((unsigned long long)m) - 1;
+      if (__ballot(in && d == (uint32_t)__builtin_amdgcn_readlane((int)d, leader)) == m) {
+        if (lane == leader) atomicAdd(&hist[d], (uint32_t)__popcll(m));
+      } else if (in) {
+        atomicAdd(&hist[d], 1u);
       }
-      above0 += wave_above[v];
-      equal0 += wave_equal[v];
     }
-    a += (uint32_t)__popcll(ma & below);
-    e += (uint32_t)__popcll(me & below);
-    if (above || (equal && e < ties)) keep[A.sinks + a + (e < ties ? e : ties)] = p;
     __syncthreads();
+    // thread t: bins 2047 - 2 t and 2046 - 2 t, counted from the top
+    const uint32_t c0 = hist[2047 - 2 * t], c1 = hist[2046 - 2 * t];
+    uint32_t up = scan_u32(c0 + c1);  // of the threads up to this one
+    if (lane == 63) wave_sum_[wave] = up;
+    __syncthreads();
+    up += waves_before(wave_sum_, wave);
+    const uint32_t before = up - c0 - c1;
+    if (before < need && need <= up) {
+      const bool high = need <= before + c0;
+      s_digit = high ? 2047 - 2 * t : 2046 - 2 * t;
+      s_left = need - before - (high ? 0u : c0);
+    }
+    __syncthreads();
+    prefix |= s_digit << shift;
+    need = s_left;
   }
+  // every slot above the bound, and the first `need` that equal it
+  uint32_t above = 0, equal = 0;
+#pragma unroll
+  for (int e = 0; e < count; ++e) {
+    const bool in = p0 + 64 * e < last;
+    const uint32_t o = number(e);
+    above += in && o > prefix ? 1u : 0u;
+    equal += in && o == prefix ? 1u : 0u;
+  }
+  above = scan_u32(above);
+  equal = scan_u32(equal);
+  if (lane == 63) {
+    wave_above[wave] = above;
+    wave_equal[wave] = equal;
+  }
+  __syncthreads();
+  above = waves_before(wave_above, wave);
+  equal = waves_before(wave_equal, wave);
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+  for (int e = 0; e < count; ++e) {
+    const bool in = p0 + 64 * e < last;
+    const uint32_t o = number(e);
+    const uint64_t ma = __ballot(in && o > prefix), me = __ballot(in && o == prefix);
+    const uint32_t a = above + (uint32_t)__popcll(ma & below);
+    const uint32_t q = equal + (uint32_t)__popcll(me & below);
+    if (in && (o > prefix || (o == prefix && q < need)))
+      keep[A.sinks + a + (q < need ? q : need)] = p0 + 64 * e;
+    above += (uint32_t)__popcll(ma);
+    equal += (uint32_t)__popcll(me);
+  }
+}
+}  // namespace
+extern "C" __global__ __launch_bounds__(1024) void cache_select_4(SelectArgs A) {
+  cache_select<4>(A);
+}
+extern "C" __global__ __launch_bounds__(1024) void cache_select_16(SelectArgs A) {
+  cache_select<16>(A);
+}
+extern "C" __global__ __launch_bounds__(1024) void cache_select_any(SelectArgs A) {
+  cache_select<0>(A);
 }
 
 // ----------------------------------------------------------- compaction ----
 
-// One workgroup per (layer, kv head, part): parts 0 .. head_dim / 64 - 1 move
-// 128 bytes of every k row, the next head_dim / 64 the same of v, the last one
-// the weights.  A workgroup walks the kept slots in order, 256 / 8 at a time,
-// and waits until all of them are read before it writes: with ascending slots
-// (keep[j] >= j) a write never meets a slot that is still to be read, so source
-// and destination may be one.
+// One workgroup per (layer, kv head, part) and range of the kept slots: parts 0 ..
+// head_dim / 64 - 1 move 128 bytes of every k row, the next head_dim / 64 the same
+// of v, the last one the weights.  A workgroup walks its slots in order, 256 (of
+// the weights 2048) at a time, and waits until all of them are read before it
+// writes: with ascending slots (keep[j] >= j) and one range, a write never meets a
+// slot that is still to be read, so source and destination may be one.
 extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A) {
+  constexpr int U = 8;
   const int t = threadIdx.x;
   const int halves = A.head_dim / 64;
-  const int parts = 2 * halves + (A.w ? 1 : 0);
-  const int part = blockIdx.x % parts, head = blockIdx.x / parts;
-  const int layer = head / A.kv_heads, kvh = head % A.kv_heads;
+  const int part = blockIdx.x;
+  const int kvh = blockIdx.y % A.kv_heads, layer = blockIdx.y / A.kv_heads;
+  const int head = blockIdx.y;
   const int32_t* keep = A.keep + (A.per_head ? (int64_t)head * A.count : 0);
   const int64_t src_left = A.src_seq - A.base;
+  const int j_lo = blockIdx.z * A.range;
+  const int j_hi = j_lo + A.range < A.count ? j_lo + A.range : A.count;
   if (part == 2 * halves) {
     const float* from = A.w + (int64_t)head * A.src_seq + A.base;
     float* to = A.w_to + (int64_t)head * A.dst_seq + A.base;
-    for (int j0 = 0; j0 < A.count; j0 += 256) {
-      const int j = j0 + t;
-      const int64_t p = j < A.count ? keep[j] : -1;
-      const bool ok = p >= 0 && p < src_left;
-      const float x = ok ? from[p] : 0.0f;
+    for (int j0 = j_lo; j0 < j_hi; j0 += 256 * U) {
+      float x[U];
+      bool ok[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + 256 * u + t;
+        const int p = j < j_hi ? keep[j] : -1;
+        ok[u] = p >= 0 && p < src_left;
+        if (ok[u]) x[u] = from[p];
+      }
       __syncthreads();
-      if (ok) to[j] = x;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (ok[u]) to[j0 + 256 * u + t] = x[u];
     }
     return;
   }
@@ -912,14 +994,29 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
   const int col = kvh * A.head_dim + 64 * (part % halves) + 8 * (t & 7);
   const uint16_t* from = (part < halves ? A.k : A.v) + (layer * A.src_seq + A.base) * row + col;
   uint16_t* to = (part < halves ? A.k_to : A.v_to) + (layer * A.dst_seq + A.base) * row + col;
-  for (int j0 = 0; j0 < A.count; j0 += 32) {
-    const int j = j0 + (t >> 3);
-    const int64_t p = j < A.count ? keep[j] : -1;
-    const bool ok = p >= 0 && p < src_left;
-    u32x4 x = {0, 0, 0, 0};
-    if (ok) x = *reinterpret_cast<const u32x4*>(from + p * row);
+  int next[U];
+  auto places = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + 32 * u + (t >> 3);
+      next[u] = j < j_hi ? keep[j] : -1;
+    }
+  };
+  places(j_lo);
+  for (int j0 = j_lo; j0 < j_hi; j0 += 32 * U) {
+    u32x4 x[U];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ok[u] = next[u] >= 0 && next[u] < src_left;
+      if (ok[u]) x[u] = load_global(reinterpret_cast<const u32x4*>(from + next[u] * row));
+    }
+    places(j0 + 32 * U);
     __syncthreads();
-    if (ok) *reinterpret_cast<u32x4*>(to + j * row) = x;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ok[u])
+        *reinterpret_cast<u32x4*>(to + (j0 + 32 * u + (t >> 3)) * row) = x[u];
   }
 }
 

@@ -16,7 +16,7 @@ namespace {
 
 struct {
   hipModule_t module = nullptr;
-  hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select = nullptr, compact = nullptr,
+  hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select[3] = {}, compact = nullptr,
                 argmax = nullptr, argmax_final = nullptr;
 } c;
 
@@ -143,7 +143,8 @@ void cache_load(const char* path) {
                {&c.weights[0][1], "weights_add_64_2"}, {&c.weights[0][2], "weights_add_64_4"},
                {&c.weights[0][3], "weights_add_64_many"}, {&c.weights[1][0], "weights_add_128_1"},
                {&c.weights[1][1], "weights_add_128_2"}, {&c.weights[1][2], "weights_add_128_4"},
-               {&c.weights[1][3], "weights_add_128_many"}, {&c.select, "cache_select_k"},
+               {&c.weights[1][3], "weights_add_128_many"}, {&c.select[0], "cache_select_4"},
+               {&c.select[1], "cache_select_16"}, {&c.select[2], "cache_select_any"},
                {&c.compact, "cache_compact_k"},   {&c.argmax, "gemm_argmax_k"},
                {&c.argmax_final, "gemm_argmax_final"}};
   for (auto& n : names) {
@@ -299,7 +300,8 @@ int f16_cache_select(const f16_cache* a, int32_t len, int32_t budget, int32_t si
   if ((rc = check_ready())) return rc;
   SelectArgs args{a->weights, keep, a->max_seq, len, budget, sinks, recent};
   void* p[] = {&args};
-  return q8_shim::launch(c.select, (uint32_t)(a->layers * a->kv_heads), 1024, p,
+  const int slots = len - sinks - recent;
+  return q8_shim::launch(c.select[slots <= 4096 ? 0 : slots <= 16384 ? 1 : 2], (uint32_t)(a->layers * a->kv_heads), 1024, p,
                          static_cast<hipStream_t>(stream));
 }
 
@@ -339,11 +341,20 @@ int f16_cache_compact(const f16_cache* src, const f16_cache* dst, const int32_t*
                    src->head_dim,
                    per_head ? 1 : 0,
                    base,
+                   count,
                    count};
-  void* p[] = {&args};
   const int parts = 2 * (src->head_dim / 64) + (weights ? 1 : 0);
-  return q8_shim::launch(c.compact, (uint32_t)(src->layers * src->kv_heads * parts), 256, p,
-                         static_cast<hipStream_t>(stream));
+  const int heads = src->layers * src->kv_heads;
+  int ranges = 1;
+  if (!same) {
+    // a move between caches may be cut up: four workgroups a CU, 256 slots or more each
+    ranges = std::clamp(4 * q8_shim::compute_units() / (heads * parts), 1, (count + 255) / 256);
+    args.range = ((count + ranges - 1) / ranges + 255) / 256 * 256;
+    ranges = (count + args.range - 1) / args.range;
+  }
+  void* p[] = {&args};
+  return q8_shim::launch3(c.compact, (uint32_t)parts, (uint32_t)heads, (uint32_t)ranges, 256, p,
+                          static_cast<hipStream_t>(stream));
 }
 
 size_t f16_gemm_argmax_workspace_bytes(int32_t n) {
