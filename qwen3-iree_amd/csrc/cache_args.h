@@ -53,4 +53,12 @@ struct CompactArgs {
   int32_t range;  // kept slots of one workgroup
 };
 
+struct GemmArgmaxArgs {
+  const uint16_t *w, *x;  // [rows, 1024], [n, 1024]
+  uint16_t* logits;       // [n, rows] or null
+  uint64_t* part;         // [n, workgroups] argmax keys
+  int32_t rows, n;
+  int32_t whole8;         // every row of logits starts on 8 bytes
+};
+
 #endif

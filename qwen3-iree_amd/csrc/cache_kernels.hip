@@ -1021,46 +1021,225 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
 }
 
 // ------------------------------------------------------ vocabulary rows ----
+//
+// Logits^T = W X^T, a tile of 128 vocabulary rows and all tokens (64 MS) per
+// workgroup and round, eight waves 2 (rows) x 4 (tokens) of 64 x 16 MS, one chain
+// of v_mfma_f32_16x16x32_f16 over K for every output.  The matrix is read from
+// memory once; the bound is its bytes up to about 128 tokens, its bytes and the
+// logits' beyond.  A stage is 64 k of the tile's W rows and of the X rows (those
+// out of L2), copied straight into one of NBUF LDS buffers NBUF - 1 stages ahead,
+// on into the workgroup's next tile, so that only its first tile waits for
+// memory.  Lane (c16, g) holds rows 4 g + e of token c16: 8 bytes of logits a
+// store, and the token's best row in two registers.
+namespace {
 
-// One wave per vocabulary row and round, every token row in turn; the best
-// (logit, row) of each token meets in LDS, then in the workspace.
-extern "C" __global__ __launch_bounds__(256) void gemm_argmax_k(
-    const uint16_t* __restrict__ w, int rows, const uint16_t* __restrict__ x, int n,
-    uint16_t* __restrict__ logits, uint64_t* __restrict__ part) {
-  __shared__ uint64_t best[4][kTreeMax];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (int i = lane; i < n; i += 64) best[wave][i] = 0;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)launch_wgs() * 4) {
-    const u32x4* wr = reinterpret_cast<const u32x4*>(w + r * kHidden);
-    const u32x4 w0 = wr[lane], w1 = wr[64 + lane];
-    for (int i = 0; i < n; ++i) {
-      const u32x4* xr = reinterpret_cast<const u32x4*>(x + i * kHidden);
-      const float acc = wave_sum(f16_row_dot(w1, xr[64 + lane], f16_row_dot(w0, xr[lane], 0.0f)));
-      const uint16_t h = f32_to_f16_bits(acc);
-      if (lane == 0) {
-        if (logits) logits[(int64_t)i * rows + r] = h;
-        const float v = f16_bits_to_f32(h);
-        const uint64_t key = v > -__builtin_inff() ? argmax_key(v, (int)r) : 0;
-        if (key > best[wave][i]) best[wave][i] = key;
+// byte offset of row r's 16-byte chunk c (of 8) in a stage: two rows a 256-byte
+// line, position p of the 16 in slot p ^ (line mod 16), so that neither the 16
+// rows of a fragment read nor the copies meet in a bank
+__device__ __forceinline__ int stage_off(int r, int c) {
+  const int line = r >> 1;
+  return 256 * line + 16 * ((((r & 1) << 3) | c) ^ (line & 15));
+}
+
+template <int MS, int NBUF>
+__device__ __forceinline__ void gemm_argmax(const GemmArgmaxArgs& A) {
+  constexpr int BM = 64 * MS, BN = 128, NS = 4;
+  constexpr int kStages = kHidden / 64;
+  constexpr int kBuf = (BM + BN) * 128;
+  constexpr int J = kBuf / 1024 / 8;  // copies of a wave and stage
+  static_assert(BM % 64 == 0 && kBuf % 8192 == 0, "copy pieces");
+  __shared__ __attribute__((aligned(1024))) uint8_t b0[kBuf];
+  __shared__ __attribute__((aligned(1024))) uint8_t b1[kBuf];
+  __shared__ __attribute__((aligned(1024))) uint8_t b2[kBuf];
+  __shared__ __attribute__((aligned(1024))) uint8_t b3[NBUF > 3 ? kBuf : 16];
+  // the buffer of a stage s = I (mod NBUF); a table of them would hide from the
+  // compiler which one a copy fills
+  auto buf = [&](auto i) -> uint8_t* {
+    constexpr int I = decltype(i)::value % NBUF;
+    if constexpr (I == 0) return b0;
+    else if constexpr (I == 1) return b1;
+    else if constexpr (I == 2) return b2;
+    else return b3;
+  };
+  const int t = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lane = t & 63, c16 = lane & 15, g = lane >> 4;
+  const int wr = wave & 1, wt = wave >> 1;  // rows, tokens
+  const int wgs = (int)launch_wgs();
+  const int tiles = (A.rows + BN - 1) / BN;
+  const int mine = (tiles - (int)blockIdx.x + wgs - 1) / wgs;  // tiles of this workgroup
+  const int total = mine * kStages;
+
+  // Copy j of this wave fills lines 4 (J wave + j) .. + 3 of a buffer (W rows
+  // first, then X rows); at: its lane's bytes from the tile's (X: matrix's) start.
+  uint32_t at[J];
+  int w_row[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int line = 4 * (J * wave + j) + (lane >> 4);
+    const int p = (lane & 15) ^ (line & 15);
+    const int row = 2 * line + (p >> 3);
+    w_row[j] = row;
+    int r = row;
+    if (row >= BN) r = row - BN < A.n ? row - BN : A.n - 1;
+    at[j] = (uint32_t)r * (2 * kHidden) + 16 * (p & 7);
+  }
+  // Every step copies a stage, the last ones the last stage once more: then one
+  // wait count serves them all.
+  auto issue = [&](int stage, uint8_t* to) {
+    const int s = stage < total ? stage : total - 1;
+    const int tile = (int)blockIdx.x + (s / kStages) * wgs, k = s % kStages;
+    const uint8_t* wp = reinterpret_cast<const uint8_t*>(A.w) + (int64_t)tile * BN * 2 * kHidden + 128 * k;
+    const uint8_t* xp = reinterpret_cast<const uint8_t*>(A.x) + 128 * k;
+    const int last = A.rows - 1 - tile * BN;  // of the tile's rows
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      // a piece of 8 rows is all W or all X
+      const bool is_w = 8 * (J * wave + j) < BN;
+      uint32_t o = at[j];
+      if (is_w && last < BN - 1 && w_row[j] > last) o -= (uint32_t)(w_row[j] - last) * (2 * kHidden);
+      __builtin_amdgcn_global_load_lds((const GLOBAL_AS void*)((is_w ? wp : xp) + o),
+                                       (LDS_AS void*)(to + 1024 * (J * wave + j)), 16, 0, 0);
+    }
+  };
+  // fragments: row base + c16, chunk 4 kb + g
+  int off[2][2];
+#pragma unroll
+  for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+      off[hb][kb] = stage_off(16 * hb + c16, 4 * kb + g) - 2048 * hb;
+  int off_x[2];  // MS = 1: the wave's X rows start at an odd half for odd wt
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+    off_x[kb] = stage_off(16 * (wt & 1) + c16, 4 * kb + g) - 2048 * (wt & 1);
+  f32x4 acc[NS][MS];
+  auto clear = [&] {
+#pragma unroll
+    for (int ns = 0; ns < NS; ++ns)
+#pragma unroll
+      for (int ms = 0; ms < MS; ++ms) acc[ns][ms] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  };
+  clear();
+  float best[MS];
+  int best_row[MS];
+#pragma unroll
+  for (int ms = 0; ms < MS; ++ms) {
+    best[ms] = -__builtin_inff();
+    best_row[ms] = -1;
+  }
+  auto finish = [&](int tile) {
+    const int r0 = tile * BN + 64 * wr + 4 * g;  // + 16 ns + e
+#pragma unroll
+    for (int ms = 0; ms < MS; ++ms) {
+      const int tok = 16 * (MS * wt + ms) + c16;
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        const int r = r0 + 16 * ns;
+        const uint2 v = {pack_f16x2(acc[ns][ms][0], acc[ns][ms][1]),
+                         pack_f16x2(acc[ns][ms][2], acc[ns][ms][3])};
+        const uint16_t h[4] = {(uint16_t)v.x, (uint16_t)(v.x >> 16), (uint16_t)v.y,
+                               (uint16_t)(v.y >> 16)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = f16_bits_to_f32(h[e]);
+          const bool up = x > best[ms] && r + e < A.rows;
+          best[ms] = up ? x : best[ms];
+          best_row[ms] = up ? r + e : best_row[ms];
+        }
+        if (A.logits && tok < A.n) {
+          uint16_t* to = A.logits + (int64_t)tok * A.rows + r;
+          if (A.whole8 && r + 4 <= A.rows) {
+            *reinterpret_cast<uint2*>(to) = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (r + e < A.rows) to[e] = h[e];
+          }
+        }
       }
     }
+    clear();
+  };
+  auto step = [&](int s, const uint8_t* cur, uint8_t* refill) {
+    // the copies of stage s have landed, those of the NBUF - 2 behind it may be out
+    wait_vm<J * (NBUF - 2)>();
+    wait_lds();  // this wave's reads of the buffer that is filled next
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    issue(s + NBUF - 1, refill);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f16x8 wf[NS], xf[MS];
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns)
+        wf[ns] = *reinterpret_cast<const f16x8*>(cur + (64 * wr + 16 * ns) * 128 + off[ns & 1][kb]);
+#pragma unroll
+      for (int ms = 0; ms < MS; ++ms)
+        xf[ms] = *reinterpret_cast<const f16x8*>(cur + (BN + 16 * (MS * wt + ms)) * 128 +
+                                                 (MS == 1 ? off_x[kb] : off[ms & 1][kb]));
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns)
+#pragma unroll
+        for (int ms = 0; ms < MS; ++ms)
+          acc[ns][ms] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[ns], xf[ms], acc[ns][ms], 0, 0, 0);
+    }
+    if (s % kStages == kStages - 1 && s < total) finish((int)blockIdx.x + (s / kStages) * wgs);
+  };
+  using std::integral_constant;
+  auto step_at = [&](auto i, int s) {
+    constexpr int I = decltype(i)::value;
+    step(s + I, buf(i), buf(integral_constant<int, I + NBUF - 1>{}));
+  };
+  issue(0, b0);
+  issue(1, b1);
+  if constexpr (NBUF > 3) issue(2, b2);
+  // (with three buffers up to two steps too many, whose sums nobody reads)
+  for (int s = 0; s < total; s += NBUF) {
+    step_at(integral_constant<int, 0>{}, s);
+    step_at(integral_constant<int, 1>{}, s);
+    step_at(integral_constant<int, 2>{}, s);
+    if constexpr (NBUF > 3) step_at(integral_constant<int, 3>{}, s);
   }
+  wait_vm<0>();
+
+  // a token's candidates: four lanes of each of the two row waves
   __syncthreads();
-  for (int i = t; i < n; i += 256) {
-    uint64_t key = best[0][i];
-    for (int v = 1; v < 4; ++v) key = best[v][i] > key ? best[v][i] : key;
-    part[(int64_t)blockIdx.x * n + i] = key;
+  uint64_t* const keys = reinterpret_cast<uint64_t*>(b0);  // [8][BM]
+#pragma unroll
+  for (int ms = 0; ms < MS; ++ms)
+    keys[(4 * wr + g) * BM + 16 * (MS * wt + ms) + c16] =
+        best_row[ms] >= 0 ? argmax_key(best[ms], best_row[ms]) : 0;
+  __syncthreads();
+  for (int i = t; i < A.n; i += 512) {
+    uint64_t key = 0;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) key = keys[v * BM + i] > key ? keys[v * BM + i] : key;
+    A.part[(int64_t)i * wgs + blockIdx.x] = key;
   }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(512) void gemm_argmax_64(GemmArgmaxArgs A) {
+  gemm_argmax<1, 4>(A);
+}
+extern "C" __global__ __launch_bounds__(512) void gemm_argmax_128(GemmArgmaxArgs A) {
+  gemm_argmax<2, 4>(A);
+}
+extern "C" __global__ __launch_bounds__(512) void gemm_argmax_256(GemmArgmaxArgs A) {
+  gemm_argmax<4, 3>(A);
 }
 
 // tokens[i] from the workgroups' keys (argmax_key: the larger value, then the
 // lower row; 0: none)
 extern "C" __global__ __launch_bounds__(64) void gemm_argmax_final(
-    const uint64_t* __restrict__ part, int wgs, int n, int32_t* __restrict__ tokens) {
+    const uint64_t* __restrict__ part, int wgs, int32_t* __restrict__ tokens) {
   const int i = blockIdx.x;
   uint64_t key = 0;
   for (int g = threadIdx.x; g < wgs; g += 64) {
-    const uint64_t k = part[(int64_t)g * n + i];
+    const uint64_t k = part[(int64_t)i * wgs + g];
     key = k > key ? k : key;
   }
   for (int d = 1; d < 64; d <<= 1) {

@@ -17,7 +17,7 @@ namespace {
 struct {
   hipModule_t module = nullptr;
   hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select[3] = {}, compact = nullptr,
-                argmax = nullptr, argmax_final = nullptr;
+                argmax[3] = {}, argmax_final = nullptr;
 } c;
 
 int fail(int code, const char* fmt, ...) {
@@ -122,7 +122,7 @@ size_t attn_workspace(const f16_cache* a, const AttnPlan& p, int32_t n, int32_t 
   return 4 * (attn_part_floats(a, n, q_heads, p.splits_max) + 2 * (size_t)n * q_heads * p.splits_max);
 }
 
-constexpr uint32_t kArgmaxWgsMax = 1024;
+constexpr int kArgmaxWgsMax = 512;  // keys a token has in the workspace
 
 }  // namespace
 
@@ -145,7 +145,8 @@ void cache_load(const char* path) {
                {&c.weights[1][1], "weights_add_128_2"}, {&c.weights[1][2], "weights_add_128_4"},
                {&c.weights[1][3], "weights_add_128_many"}, {&c.select[0], "cache_select_4"},
                {&c.select[1], "cache_select_16"}, {&c.select[2], "cache_select_any"},
-               {&c.compact, "cache_compact_k"},   {&c.argmax, "gemm_argmax_k"},
+               {&c.compact, "cache_compact_k"},   {&c.argmax[0], "gemm_argmax_64"},
+               {&c.argmax[1], "gemm_argmax_128"}, {&c.argmax[2], "gemm_argmax_256"},
                {&c.argmax_final, "gemm_argmax_final"}};
   for (auto& n : names) {
     if (hipModuleGetFunction(n.fn, m, n.name) != hipSuccess) {
@@ -375,12 +376,20 @@ int f16_gemm_argmax(const void* w_f16, int64_t w_rows, const void* x_f16, int32_
     return fail(Q8_ERR_MISALIGNED, "w, x and workspace 16, logits 2, tokens 4-byte alignment");
   int rc = check_ready();
   if (rc) return rc;
-  int rows = (int)w_rows;
-  int wgs = (int)std::min<int64_t>(kArgmaxWgsMax, (w_rows + 3) / 4);
+  const int64_t tiles = (w_rows + 127) / 128;
+  int wgs = (int)std::min<int64_t>({kArgmaxWgsMax, q8_shim::compute_units(), tiles});
+  GemmArgmaxArgs args{static_cast<const uint16_t*>(w_f16),
+                      static_cast<const uint16_t*>(x_f16),
+                      static_cast<uint16_t*>(logits_f16),
+                      static_cast<uint64_t*>(workspace),
+                      (int32_t)w_rows,
+                      n,
+                      w_rows % 4 == 0 && aligned(logits_f16, 8)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  void* args[] = {&w_f16, &rows, &x_f16, &n, &logits_f16, &workspace};
-  if ((rc = q8_shim::launch(c.argmax, (uint32_t)wgs, 256, args, st))) return rc;
-  void* fargs[] = {&workspace, &wgs, &n, &tokens};
+  void* p[] = {&args};
+  if ((rc = q8_shim::launch(c.argmax[n <= 64 ? 0 : n <= 128 ? 1 : 2], (uint32_t)wgs, 512, p, st)))
+    return rc;
+  void* fargs[] = {&workspace, &wgs, &tokens};
   return q8_shim::launch(c.argmax_final, (uint32_t)n, 64, fargs, st);
 }
 
