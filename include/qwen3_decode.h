@@ -270,6 +270,31 @@ int qwen3_generate(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t
                    int32_t* token, int32_t* pos, int32_t max_new, int32_t eos_id,
                    int32_t* out_tokens, int32_t* n_generated, void* scratch, void* stream);
 
+/* A tree of n drafted tokens (1 .. 256) through the whole model in one pass, over
+ * a cache whose slots 0 .. len - 1 hold the sequence so far.  tokens, parents:
+ * device int32 [n], the parents as in f16_tree_mask (f16_cache.h): -1 puts a node
+ * right behind the cache, 0 .. i - 1 behind that node, anything else marks
+ * padding.  Node i sits at RoPE position `position` + its depth (position = len
+ * unless slots have been evicted), its k and v go to slot len + i of every layer,
+ * and it attends to slots 0 .. len - 1 and its ancestors.  next_tokens (device
+ * int32 [n]): the argmax of every node's logits, what the model says follows it
+ * (of padding: unspecified); logits f16 [n, 151936], may be NULL.
+ * q_rows f16 [28, n, 2048] and lse f32 [28, n, 16] (both or neither NULL) receive
+ * each layer's queries after RoPE and log-sum-exps, what f16_attn_weights_add
+ * needs once it is known which nodes are kept; f16_cache_compact moves those
+ * nodes' slots together.  n = 1 is a decode step over such a cache.
+ * The layers' matrices are read as in qwen3_prefill_batched (w->prefill_f16, else
+ * the Q8_0 stacks); results agree with it and with qwen3_decode_step within the
+ * step's tolerance.  Only enqueues; len + n <= max_seq, position in [0, 2^24].
+ * workspace: device memory of qwen3_tree_workspace_bytes(n, max_seq) bytes (0 for
+ * arguments outside the ranges), 256-byte aligned, nothing to initialise.  No
+ * counterpart in the reference, which runs one token a step. */
+size_t qwen3_tree_workspace_bytes(int32_t n, int64_t max_seq);
+int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t max_seq,
+                    const int32_t* tokens, const int32_t* parents, int32_t n, int32_t len,
+                    int32_t position, int32_t* next_tokens, void* logits, void* q_rows, float* lse,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 /* Scratch offsets of the intermediates the last qwen3_decode_layer (or head)
  * left behind, all f16: "xn" [1024] rms_norm(h_in, attn_norm); "q" [2048],
  * "k" [1024], "v" [1024] the projections before head norm and RoPE;

@@ -60,6 +60,19 @@ extern "C" __global__ __launch_bounds__(kTreeMax) void tree_mask_k(
   if (depth) depth[i] = live ? count - 1 : -1;
 }
 
+// The RoPE table of a tree (as pf_rmsnorm writes a prompt's): row i the 64 cosines,
+// then the 64 sines at position `position` + depth[i]; padding as depth 0.
+extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __restrict__ depth,
+                                                             int position,
+                                                             float* __restrict__ table) {
+  const int i = blockIdx.x, lane = threadIdx.x;
+  const int d = depth[i];
+  float c, s;
+  rope_angle(position + (d > 0 ? d : 0), lane, c, s);
+  table[i * 128 + lane] = c;
+  table[i * 128 + 64 + lane] = s;
+}
+
 // ------------------------------------------------------- tree attention ----
 //
 // The rows of one kv head are its query heads' rows of all nodes, r = group

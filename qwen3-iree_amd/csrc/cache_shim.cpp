@@ -16,7 +16,7 @@ namespace {
 
 struct {
   hipModule_t module = nullptr;
-  hipFunction_t mask = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select[3] = {}, compact = nullptr,
+  hipFunction_t mask = nullptr, rope = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select[3] = {}, compact = nullptr,
                 argmax[3] = {}, argmax_final = nullptr;
 } c;
 
@@ -134,7 +134,8 @@ void cache_load(const char* path) {
   struct {
     hipFunction_t* fn;
     const char* name;
-  } names[] = {{&c.mask, "tree_mask_k"},          {&c.attn[0][0], "attn_tree_64_11"},
+  } names[] = {{&c.mask, "tree_mask_k"},          {&c.rope, "tree_rope_k"},
+               {&c.attn[0][0], "attn_tree_64_11"},
                {&c.attn[0][1], "attn_tree_64_12"}, {&c.attn[0][2], "attn_tree_64_22"},
                {&c.attn[0][3], "attn_tree_64_42"}, {&c.attn[1][0], "attn_tree_128_11"},
                {&c.attn[1][1], "attn_tree_128_12"}, {&c.attn[1][2], "attn_tree_128_22"},
@@ -160,6 +161,13 @@ void cache_load(const char* path) {
 void cache_unload() {
   if (c.module) (void)hipModuleUnload(c.module);
   c.module = nullptr;
+}
+
+int tree_rope(const int32_t* depth, int32_t position, int32_t n, void* table, hipStream_t stream) {
+  int rc = check_ready();
+  if (rc) return rc;
+  void* args[] = {&depth, &position, &table};
+  return launch(c.rope, (uint32_t)n, 64, args, stream);
 }
 
 }  // namespace q8_shim

@@ -4,6 +4,7 @@
 // validation and hipModuleLaunchKernel per call.  The ABI is declared in
 // include/q8gemv.h.
 #include "q8gemv.h"
+#include "f16_cache.h"
 #include "qwen3_decode.h"
 #include "prefill_split.h"
 #include "shim_internal.h"
@@ -1937,6 +1938,16 @@ int launch_rows(hipFunction_t fn, int n, int tokens, int n_tiles, int threads, v
   return launch(fn, (uint32_t)((n + tokens - 1) / tokens * n_tiles), (uint32_t)threads, args, st);
 }
 
+// The attention of a tree in place of the causal one: f16_attn_tree's arguments
+// that all layers share, and this layer's log-sum-exps (or null).
+struct TreeLayer {
+  f16_cache cache;
+  const uint32_t* mask;
+  float* lse;
+  void* workspace;
+  size_t bytes;
+};
+
 // One layer.  xn_ready: the workspace's xn already holds rms_norm(h,
 // attn_norm of this layer) (written by the previous layer's last reduce).
 // next_norm (the next layer's attn_norm, or null): if ffn_down's reduce can
@@ -1944,11 +1955,14 @@ int launch_rows(hipFunction_t fn, int n, int tokens, int n_tiles, int threads, v
 // whole_prompt: the other layers run before and after, so the attention launch
 // also brings the following weights into the caches (a layer by itself may find
 // them there: 512 tokens 62.4 us a layer over and over, 64.1 with).
+// tree: the tokens are a tree's nodes in slots p0 .. (rope_ready, positions of
+// their own).
 int launch_prefill_layer(const qwen3_weights* w, int layer, void* k_cache, void* v_cache,
                          int64_t max_seq, int32_t n, int32_t p0, int chunk_local,
                          void* const (&ws)[kPfRegions], hipStream_t st, bool xn_ready = false,
                          const void* next_norm = nullptr, bool* next_xn_ready = nullptr,
-                         bool rope_ready = false, bool whole_prompt = false) {
+                         bool rope_ready = false, bool whole_prompt = false,
+                         const TreeLayer* tree = nullptr) {
   const int64_t bpl_q = 2048LL * 1024 / 32 * 34, bpl_kv = 1024LL * 1024 / 32 * 34;
   const int64_t bpl_o = 1024LL * 2048 / 32 * 34, bpl_gu = 6144LL * 1024 / 32 * 34;
   const int64_t bpl_dn = 1024LL * 3072 / 32 * 34;
@@ -2018,7 +2032,12 @@ int launch_prefill_layer(const qwen3_weights* w, int layer, void* k_cache, void*
     void* args[] = {&q, &k, &v, &start, &qn, &kn, &rope, &qr, &kc, &vc};
     if ((rc = launch(g.pf_rope, (uint32_t)n, 256, args, st))) return rc;
   }
-  {
+  if (tree) {
+    if ((rc = f16_attn_tree(&tree->cache, layer, p0, qr, Q8_HIDDEN * 2, 16, tree->mask, n,
+                            0.0883883461356163f, attn, Q8_HIDDEN * 2, tree->lse, tree->workspace,
+                            tree->bytes, st)))
+      return rc;
+  } else {
     int start = p0, cl = chunk_local ? 1 : 0, nn = n;
     int sb = pf_attn_split_blocks(n, p0, chunk_local);
     const PfSplitGeometry G = pf_split_geometry(n, p0, cl ? p0 : 0);
@@ -2607,6 +2626,105 @@ int qwen3_prefill_batched(const qwen3_weights* w, void* k_cache, void* v_cache, 
   }
   const void* h_last = cb(ws[0]) + (size_t)(n_prompt - 1) * 2048;
   return launch_head(w, h_last, logits, token, pos, 1, max_seq, scratch, st);
+}
+
+// The tree workspace: a prompt's regions, then the nodes' masks and depths, the
+// argmax keys and the attention's partials.
+namespace {
+
+struct TreeWorkspace {
+  size_t mask, depth, keys, attn, attn_bytes, bytes;
+};
+
+f16_cache model_cache(void* k, void* v, int64_t max_seq) {
+  return f16_cache{k, v, nullptr, max_seq, kLayers, (int32_t)kKvHeads, 128};
+}
+
+TreeWorkspace tree_workspace(int32_t n, int64_t max_seq) {
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  const f16_cache c = model_cache(nullptr, nullptr, max_seq);
+  TreeWorkspace t{};
+  t.mask = pf_workspace_bytes(n);
+  t.depth = t.mask + up((size_t)n * ((n + 31) / 32) * 4);
+  t.keys = t.depth + up((size_t)n * 4);
+  t.attn = t.keys + up(f16_gemm_argmax_workspace_bytes(n));
+  t.attn_bytes = f16_attn_tree_workspace_bytes(&c, (int32_t)(max_seq - n), n, 16);
+  t.bytes = t.attn + up(t.attn_bytes);
+  return t;
+}
+
+}  // namespace
+
+size_t qwen3_tree_workspace_bytes(int32_t n, int64_t max_seq) {
+  if (n < 1 || n > F16_TREE_MAX_NODES || max_seq < n || max_seq > (1LL << 24)) return 0;
+  return tree_workspace(n, max_seq).bytes;
+}
+
+int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t max_seq,
+                    const int32_t* tokens, const int32_t* parents, int32_t n, int32_t len,
+                    int32_t position, int32_t* next_tokens, void* logits, void* q_rows, float* lse,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = validate_weights(w);
+  if (rc) return rc;
+  if ((rc = validate_cache(k_cache, v_cache, max_seq))) return rc;
+  if (!tokens || !parents || !next_tokens || !workspace)
+    return fail(Q8_ERR_NULL_POINTER, "null tokens, parents, next_tokens or workspace");
+  if (!q_rows != !lse) return fail(Q8_ERR_NULL_POINTER, "q_rows and lse go together");
+  if (!aligned(tokens, 4) || !aligned(parents, 4) || !aligned(next_tokens, 4) ||
+      !aligned(logits, 2) || !aligned(q_rows, 16) || !aligned(lse, 4) || !aligned(workspace, 256))
+    return fail(Q8_ERR_MISALIGNED,
+                "tokens, parents, next_tokens and lse 4, logits 2, q_rows 16, workspace 256-byte "
+                "alignment");
+  if (n < 1 || n > F16_TREE_MAX_NODES || len < 0 || (int64_t)len + n > max_seq)
+    return fail(Q8_ERR_BAD_SHAPE, "%d nodes at slot %d of a cache of %lld", n, len,
+                (long long)max_seq);
+  if (position < 0 || position > (1 << 24))
+    return fail(Q8_ERR_BAD_SHAPE, "position %d outside [0, 2^24]", position);
+  const TreeWorkspace t = tree_workspace(n, max_seq);
+  if (workspace_bytes < t.bytes)
+    return fail(Q8_ERR_BAD_SHAPE, "workspace of %zu bytes < %zu needed for %d nodes",
+                workspace_bytes, t.bytes, n);
+  if ((rc = check_prefill_ready())) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  void* ws[kPfRegions];
+  size_t off = 0;
+  for (int i = 0; i < kPfRegions; ++i) {
+    ws[i] = mb(workspace) + off;
+    off += pf_region_bytes(n, i);
+  }
+  uint32_t* mask = reinterpret_cast<uint32_t*>(mb(workspace) + t.mask);
+  int32_t* depth = reinterpret_cast<int32_t*>(mb(workspace) + t.depth);
+  if ((rc = f16_tree_mask(parents, n, mask, depth, stream))) return rc;
+  if ((rc = q8_shim::tree_rope(depth, position, n, ws[kPfRopeRegion], st))) return rc;
+  {
+    const void* tp = tokens;
+    const void* e = w->token_embd;
+    void* h = ws[0];
+    void* args[] = {&tp, &e, &h};
+    if ((rc = launch(g.pf_embed, (uint32_t)n, 128, args, st))) return rc;
+  }
+  TreeLayer tree{model_cache(k_cache, v_cache, max_seq), mask, nullptr, mb(workspace) + t.attn,
+                 t.attn_bytes};
+  bool xn_ready = false;
+  for (int l = 0; l < kLayers; ++l) {
+    if (q_rows) {
+      ws[6] = mb(q_rows) + (size_t)l * n * 4096;
+      tree.lse = lse + (size_t)l * n * 16;
+    }
+    const void* next_norm = l + 1 < kLayers ? cb(w->attn_norm) + (l + 1) * 2048 : nullptr;
+    if ((rc = launch_prefill_layer(w, l, k_cache, v_cache, max_seq, n, len, 0, ws, st, xn_ready,
+                                   next_norm, &xn_ready, true, false, &tree)))
+      return rc;
+  }
+  {
+    const void *h = ws[0], *on = w->output_norm;
+    void *xn = ws[2], *rope = nullptr;
+    int nn = n, start = 0;
+    void* args[] = {&h, &on, &xn, &nn, &start, &rope};
+    if ((rc = launch(g.pf_norm, (uint32_t)((n + 3) / 4), 64, args, st))) return rc;
+  }
+  return f16_gemm_argmax(w->output_w, Q8_VOCAB_ROWS, ws[2], n, logits, next_tokens,
+                         mb(workspace) + t.keys, stream);
 }
 
 }  // extern "C"

@@ -25,6 +25,8 @@ int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bl
 // leaves the cache operators reporting Q8_ERR_CODE_OBJECT) and unloads it.
 void cache_load(const char* path);
 void cache_unload();
+// The RoPE table of a tree's nodes (tree_rope_k).
+int tree_rope(const int32_t* depth, int32_t position, int32_t n, void* table, hipStream_t stream);
 
 // Q8_OK once q8gemv_init has run and the allocation-free scratch of its
 // device was set up; otherwise the status and message of what is missing.

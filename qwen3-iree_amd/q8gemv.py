@@ -179,6 +179,9 @@ _SIGNATURES = {
                               _P],
     "qwen3_prefill_layer": [_P, _I, _P, _P, _I64, ctypes.c_int32, ctypes.c_int32, _I, _P, _SZ, _P],
     "qwen3_prefill_workspace_offset": [ctypes.c_int32, ctypes.c_char_p],
+    "qwen3_tree_workspace_bytes": [ctypes.c_int32, _I64],
+    "qwen3_tree_step": [_P, _P, _P, _I64, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                        _P, _P, _P, _P, _P, _SZ, _P],
     "qwen3_set_step_mode": [_I],
     "qwen3_set_step_spin_limit": [ctypes.c_uint32],
     "qwen3_check_status": [_P, _P, _P],
@@ -200,6 +203,7 @@ _CACHE_SIGNATURES = {
     "f16_gemm_argmax": [_P, _I64, _P, ctypes.c_int32, _P, _P, _P, _P],
 }
 _RESTYPES = {
+    "qwen3_tree_workspace_bytes": _SZ,
     "f16_attn_tree_workspace_bytes": _SZ,
     "f16_gemm_argmax_workspace_bytes": _SZ,
     "q8gemv_shutdown": None,
