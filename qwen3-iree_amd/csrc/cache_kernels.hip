@@ -889,7 +889,7 @@ __device__ __forceinline__ void cache_select(const SelectArgs& A) {
     hist[t] = 0;
     hist[1024 + t] = 0;
     __syncthreads();
-#pragma unroll
+#pragma unroll(E ? E : 1)
     for (int e = 0; e < count; ++e) {
       const uint32_t o = number(e);
       const bool in = p0 + 64 * e < last && (digit == 0 || (o ^ prefix) >> (shift + bits) == 0);
@@ -923,7 +923,7 @@ __device__ __forceinline__ void cache_select(const SelectArgs& A) {
   }
   // every slot above the bound, and the first `need` that equal it
   uint32_t above = 0, equal = 0;
-#pragma unroll
+#pragma unroll(E ? E : 1)
   for (int e = 0; e < count; ++e) {
     const bool in = p0 + 64 * e < last;
     const uint32_t o = number(e);
@@ -940,7 +940,7 @@ __device__ __forceinline__ void cache_select(const SelectArgs& A) {
   above = waves_before(wave_above, wave);
   equal = waves_before(wave_equal, wave);
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-#pragma unroll
+#pragma unroll(E ? E : 1)
   for (int e = 0; e < count; ++e) {
     const bool in = p0 + 64 * e < last;
     const uint32_t o = number(e);

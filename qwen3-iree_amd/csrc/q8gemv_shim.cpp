@@ -199,18 +199,23 @@ std::string default_code_object() {
   return "q8gemv_gfx950.hsaco";
 }
 
-int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStream_t stream) {
+int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t block, void** args,
+            hipStream_t stream) {
   hipError_t e;
   if (t_start != nullptr || t_stop != nullptr) {
     hipEvent_t s = t_start, p = t_stop;
     t_start = t_stop = nullptr;
-    e = hipExtModuleLaunchKernel(fn, grid * block, 1, 1, block, 1, 1, 0, stream, args, nullptr,
-                                 s, p, 0);
+    e = hipExtModuleLaunchKernel(fn, gx * block, gy, gz, block, 1, 1, 0, stream, args, nullptr, s,
+                                 p, 0);
   } else {
-    e = hipModuleLaunchKernel(fn, grid, 1, 1, block, 1, 1, 0, stream, args, nullptr);
+    e = hipModuleLaunchKernel(fn, gx, gy, gz, block, 1, 1, 0, stream, args, nullptr);
   }
   if (e != hipSuccess) return hip_fail(e, "kernel launch");
   return Q8_OK;
+}
+
+int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStream_t stream) {
+  return launch3(fn, grid, 1, 1, block, args, stream);
 }
 
 int launch2(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t block, void** args,
@@ -776,9 +781,7 @@ int launch(hipFunction_t fn, uint32_t grid, uint32_t block, void** args, hipStre
 
 int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t block, void** args,
             hipStream_t stream) {
-  hipError_t e = hipModuleLaunchKernel(fn, gx, gy, gz, block, 1, 1, 0, stream, args, nullptr);
-  if (e != hipSuccess) return hip_fail(e, "kernel launch");
-  return Q8_OK;
+  return ::launch3(fn, gx, gy, gz, block, args, stream);
 }
 
 int noalloc_ready() {
