@@ -89,10 +89,12 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 //   O^T += V^T P^T with the weights as they stand in the lanes: the MFMA's 32 k
 //     slots mean slots 4 grp + e, 16 + 4 grp + e, and V^T is read from LDS in
 //     that order (transposing reads).  A weight goes into the product as an f16
-//     (half a step, 2^-11 of itself, at most), with one row group as the sum of two
-//     (2^-22): the bytes bound those, and the second product costs nothing.
+//     (half a step, 2^-11 of itself, at most), up to 32 rows as the sum of two (2^-22):
+//     the bytes bound those, and the second product costs nothing.
 // K and V blocks are copied from memory straight into LDS, the next one while one
-// is computed.  RG waves share a block (RG row groups of T tiles);
+// is computed.  RG waves share a block (RG row groups of T tiles,
+// T = 2 from 65 rows on: up to there the code and the registers of a second tile
+// cost more than the block's second read, 30 rows over 1024 slots 12.7 -> 10.8 us);
 // the 4 / RG position groups of a workgroup take blocks in turn and meet in LDS.
 // With one row group no wave waits for another until the end: few rows are bound
 // by the bytes in flight, 64 KiB a CU, many rows by MFMA and exp2.
@@ -103,8 +105,7 @@ namespace {
 
 constexpr float kRefRoom = 6.0f, kRefMax = 10.0f, kSumMax = 16384.0f;
 
-// Bits of slots p0 .. p0 + 31 row i sees: those before `len` and those of its
-// mask row.
+// Word w of row i's mask: all ones in front of it (the cache), zeros behind.
 __device__ __forceinline__ uint32_t mask_word(const AttnTreeArgs& A, int i, int w) {
   const int words = (A.n + 31) >> 5;
   if (w < 0) return ~0u;
@@ -116,12 +117,6 @@ __device__ __forceinline__ uint32_t mask_word(const AttnTreeArgs& A, int i, int 
   uint32_t m = A.mask[i * words + w];
   if (w == words - 1 && (A.n & 31)) m &= (1u << (A.n & 31)) - 1u;
   return m;
-}
-__device__ __forceinline__ uint32_t block_bits(const AttnTreeArgs& A, int i, int p0) {
-  const int a0 = p0 - A.len;
-  const int w = a0 >> 5, sh = a0 & 31;
-  const uint32_t lo = mask_word(A, i, w);
-  return sh == 0 ? lo : (lo >> sh) | (mask_word(A, i, w + 1) << (32 - sh));
 }
 __device__ __forceinline__ bool row_empty(const AttnTreeArgs& A, int i) {
   uint32_t any = 0;
@@ -153,11 +148,13 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
   constexpr int kChunks = D / 8;           // 16-byte chunks of a row
   constexpr int kRowsPerPiece = 64 / kChunks;
   constexpr int kRows = 16 * T * RG;       // rows of a workgroup
-  constexpr bool kLow = RG == 1;           // weights as two f16 values
+  constexpr bool kLow = T * RG <= 2;       // weights as two f16 values
   // two buffers of each position group's K and V blocks, separate arrays so
   // that the compiler sees that reading one does not wait for copies into another
   __shared__ __attribute__((aligned(1024))) uint8_t k0[PG * kTile], k1[PG * kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t v0[PG * kTile], v1[PG * kTile];
+  // mask words -1 .. words of the workgroup's rows
+  __shared__ uint32_t sees[kRows][kTreeMax / 32 + 3];
   const int t = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int lane = t & 63, c16 = lane & 15, grp = lane >> 4;
@@ -187,12 +184,10 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
     for (int st = 0; st < D / 32; ++st)
       qf[j][st] = __builtin_bit_cast(f16x8, load_global(reinterpret_cast<const u32x4*>(q + 32 * st)));
   }
-  bool none[T];  // the row sees nothing
   float m[T], l[T];
   f32x4 o[T][D / 16];
 #pragma unroll
   for (int j = 0; j < T; ++j) {
-    none[j] = A.splits == 1 && row_empty(A, node[j]);
     m[j] = -__builtin_inff();
     l[j] = 0.0f;
 #pragma unroll
@@ -382,7 +377,12 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
   const std::false_type kPlainBlock;
   auto masked_bits = [&](int b) {
 #pragma unroll
-    for (int j = 0; j < T; ++j) bits[j] = block_bits(A, node[j], 32 * b) >> (4 * grp);
+    for (int j = 0; j < T; ++j) {
+      // a block that is masked starts at most 31 slots before len
+      const int a0 = 32 * b - A.len;
+      const uint32_t* w = sees[16 * (T * rg + j) + c16] + (a0 >> 5) + 1;
+      bits[j] = (uint32_t)((((uint64_t)w[1] << 32) | w[0]) >> (a0 & 31)) >> (4 * grp);
+    }
   };
   // plain round i: block first + PG i
   auto plain_next = [&](int i) { return first + PG * i < b_mid ? first + PG * i : -1; };
@@ -401,6 +401,15 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
     }
   };
   start(0);
+  if (masked > 0 || A.splits == 1) {
+    const int words = (A.n + 31) >> 5;
+    const int row = t & (kRows - 1);
+    int rr = rb * kRows + row;
+    rr = rr < R ? rr : R - 1;
+    const int i = A.group == 1 ? rr : (int)__umulhi((uint32_t)rr, A.group_inv);
+    for (int w = t / kRows; w < words + 2; w += 256 / kRows) sees[row][w] = mask_word(A, i, w - 1);
+    __syncthreads();
+  }
   for (int i = 0; i < masked_rounds; ++i) {
     const bool live = b_tree0 + PG * i < b_hi;
     const bool even = ((masked_rounds - i) & 1) != 0;
@@ -506,17 +515,20 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
       }
     } else {
       const int h = kvh * A.group + r - node[j] * A.group;
+      uint32_t any = 0;
+      for (int w = 1; w <= (A.n + 31) >> 5; ++w) any |= sees[16 * (T * rg + j) + c16][w];
+      const bool none = any == 0;
       const float inv = 1.0f / l[j];
       uint16_t* to = A.out + (int64_t)node[j] * A.out_stride + h * D + 4 * grp;
 #pragma unroll
       for (int d = 0; d < kDims; ++d) {
         const f32x4 x = o[j][d];
         const uint2 v = {pack_f16x2(x[0] * inv, x[1] * inv), pack_f16x2(x[2] * inv, x[3] * inv)};
-        *reinterpret_cast<uint2*>(to + 16 * piece(d)) = none[j] ? make_uint2(0, 0) : v;
+        *reinterpret_cast<uint2*>(to + 16 * piece(d)) = none ? make_uint2(0, 0) : v;
       }
       if (grp == 0 && pg == 0 && A.lse)
         A.lse[(int64_t)node[j] * A.q_heads + h] =
-            none[j] ? -__builtin_inff() : kLn2 * (m[j] + __builtin_amdgcn_logf(l[j]));
+            none ? -__builtin_inff() : kLn2 * (m[j] + __builtin_amdgcn_logf(l[j]));
     }
   }
 }
@@ -529,12 +541,12 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
     attn_tree<D, RG, T>(A);                                                \
   }
 ATTN_TREE(64, 1, 1)
-ATTN_TREE(64, 1, 2)
-ATTN_TREE(64, 2, 2)
+ATTN_TREE(64, 2, 1)
+ATTN_TREE(64, 4, 1)
 ATTN_TREE(64, 4, 2)
 ATTN_TREE(128, 1, 1)
-ATTN_TREE(128, 1, 2)
-ATTN_TREE(128, 2, 2)
+ATTN_TREE(128, 2, 1)
+ATTN_TREE(128, 4, 1)
 ATTN_TREE(128, 4, 2)
 
 // One wave per row: the splits' (m, l) one per lane (at most 64 splits), then

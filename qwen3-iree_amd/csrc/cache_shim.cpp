@@ -80,7 +80,7 @@ uint32_t group_inverse(int group) { return (uint32_t)((0xffffffffull + group) / 
 
 // How f16_attn_tree divides its work.
 struct AttnPlan {
-  int kernel;  // rows of a workgroup: 16, 32, 64, 128; position groups 4, 4, 2, 1
+  int kernel;  // rows of a workgroup: 16, 32, 64, 128; position groups 4, 2, 1, 1
   int row_blocks, splits, blocks;
   int splits_max;  // before the blocks are dealt out evenly; does not shrink with len
 };
@@ -89,14 +89,17 @@ constexpr int kMaxSplits = 64;  // one lane each in the merge
 
 // Splits of the nb blocks of 32 slots: each costs a partial written and merged,
 // the first one a launch, and each block of a split costs a round of its
-// workgroups, so about sqrt(nb) of them, and none up to 10 blocks.  us a layer
-// (16 query over 8 kv heads of 128), with 1 / 4 / 8 / 16 / 32 splits:
-//   1 row, 300 slots (10 blocks) 7.0 / 7.5 / 8.0, 1000 (32) 11.1 / 9.2 / 8.7 /
-//   9.2 / 10.1, 4000 (126) 46.6 / 19.2 / 13.8 / 11.8 / 12.2, 16384 (513) 97.7 /
-//   35.1 / 24.1 / 21.8 / 23.2; 61 rows, 1024 (34) 28.6 / 15.4 / 14.2 / 15.1 /
-//   16.2, 8191 (258) 184 / 55.5 / 34.3 / 24.8 / 22.9 (64: 29.7); 256 rows, 1024
-//   (40) 38.0 / 26.1 / 27.7 / 30.3 / 33.6, 16384 (520) 334 / 103 / 66.9 / 63.7 / 76.6.
-// At most one workgroup a CU where it takes the CU's LDS (up to 32 rows), else two.
+// workgroups, so about sqrt(nb) of them (somewhat more where a round is longer:
+// several waves share a block), and none up to 10 blocks.  us a layer (16 query
+// over 8 kv heads of 128) with 1 / 4 / 8 / 16 / 32 splits:
+//   1 node, 300 slots (10 blocks) 6.8 / 7.8 / 8.2, 1000 (32) 11.1 / 9.2 / 8.5 / 9.5
+//   / 10.5, 4000 (126) 46.4 / 19.1 / 13.8 / 11.7 / 12.2, 16384 (513) 97.7 / 35.3 /
+//   24.2 / 21.6 / 23.0; 30 nodes, 1024 (33) 19.6 / 11.5 / 10.4 / 11.6 / 11.7, 8191
+//   (257) 178 / 53.1 / 32.0 / 22.4 / 19.8; 61 nodes, 1024 (34) 28.2 / 15.6 / 14.5 /
+//   15.3 / 16.5, 8191 (258) 183 / 55.3 / 34.3 / 24.8 / 22.9 (64: 28.7); 256 nodes,
+//   1024 (40) 36.1 / 25.6 / 27.2 / 29.9 / 34.1, 16384 (520) 341 / 104 / 67.1 / 60.1
+//   / 74.0.
+// At most one workgroup a CU where it takes the CU's LDS (up to 16 rows), else two.
 AttnPlan attn_plan(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) {
   const int rows = n * (q_heads / a->kv_heads);
   AttnPlan p{};
@@ -104,8 +107,9 @@ AttnPlan attn_plan(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) 
   const int per_wg = 16 << p.kernel;
   p.row_blocks = (rows + per_wg - 1) / per_wg;
   const int nb = (len + n + 31) / 32;
-  const int most = (p.kernel <= 1 ? 1 : 2) * q8_shim::compute_units() / (a->kv_heads * p.row_blocks);
-  const int want = nb <= 10 ? 1 : (int)(1.25 * std::sqrt((double)nb));
+  const int most = (p.kernel == 0 ? 1 : 2) * q8_shim::compute_units() / (a->kv_heads * p.row_blocks);
+  const double per_root = p.kernel > 0 && p.row_blocks == 1 ? 1.5 : 1.25;
+  const int want = nb <= 10 ? 1 : (int)(per_root * std::sqrt((double)nb));
   p.splits_max = std::max(1, std::min({want, most, kMaxSplits}));
   p.blocks = (nb + p.splits_max - 1) / p.splits_max;
   p.splits = (nb + p.blocks - 1) / p.blocks;
@@ -136,9 +140,9 @@ void cache_load(const char* path) {
     const char* name;
   } names[] = {{&c.mask, "tree_mask_k"},          {&c.rope, "tree_rope_k"},
                {&c.attn[0][0], "attn_tree_64_11"},
-               {&c.attn[0][1], "attn_tree_64_12"}, {&c.attn[0][2], "attn_tree_64_22"},
+               {&c.attn[0][1], "attn_tree_64_21"}, {&c.attn[0][2], "attn_tree_64_41"},
                {&c.attn[0][3], "attn_tree_64_42"}, {&c.attn[1][0], "attn_tree_128_11"},
-               {&c.attn[1][1], "attn_tree_128_12"}, {&c.attn[1][2], "attn_tree_128_22"},
+               {&c.attn[1][1], "attn_tree_128_21"}, {&c.attn[1][2], "attn_tree_128_41"},
                {&c.attn[1][3], "attn_tree_128_42"}, {&c.merge[0], "attn_merge_64"},
                {&c.merge[1], "attn_merge_128"},  {&c.weights[0][0], "weights_add_64_1"},
                {&c.weights[0][1], "weights_add_64_2"}, {&c.weights[0][2], "weights_add_64_4"},
