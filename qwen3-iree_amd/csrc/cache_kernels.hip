@@ -978,7 +978,7 @@ extern "C" __global__ __launch_bounds__(1024) void cache_select_any(SelectArgs A
 
 // ----------------------------------------------------------- compaction ----
 
-// One workgroup per (layer, kv head, part) and range of the kept slots: parts 0 ..
+// One workgroup per part and range of the kept slots, kv head and layer: parts 0 ..
 // head_dim / 64 - 1 move 128 bytes of every k row, the next head_dim / 64 the same
 // of v, the last one the weights.  A workgroup walks its slots in order, 256 (of
 // the weights 2048) at a time, and waits until all of them are read before it
@@ -988,12 +988,13 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
   constexpr int U = 8;
   const int t = threadIdx.x;
   const int halves = A.head_dim / 64;
-  const int part = blockIdx.x;
-  const int kvh = blockIdx.y % A.kv_heads, layer = blockIdx.y / A.kv_heads;
-  const int head = blockIdx.y;
+  const int parts = 2 * halves + (A.w ? 1 : 0);
+  const int part = blockIdx.x % parts, range = blockIdx.x / parts;
+  const int kvh = blockIdx.y, layer = blockIdx.z;
+  const int head = layer * A.kv_heads + kvh;
   const int32_t* keep = A.keep + (A.per_head ? (int64_t)head * A.count : 0);
   const int64_t src_left = A.src_seq - A.base;
-  const int j_lo = blockIdx.z * A.range;
+  const int j_lo = range * A.range;
   const int j_hi = j_lo + A.range < A.count ? j_lo + A.range : A.count;
   if (part == 2 * halves) {
     const float* from = A.w + (int64_t)head * A.src_seq + A.base;
@@ -1006,8 +1007,10 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
         const int j = j0 + 256 * u + t;
         const int p = j < j_hi ? keep[j] : -1;
         ok[u] = p >= 0 && p < src_left;
-        if (ok[u]) x[u] = from[p];
+        x[u] = from[ok[u] ? p : 0];  // (slot base is there: count > 0)
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) asm volatile("" : "+v"(x[u]));  // the loads are back
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -1034,9 +1037,11 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       ok[u] = next[u] >= 0 && next[u] < src_left;
-      if (ok[u]) x[u] = load_global(reinterpret_cast<const u32x4*>(from + next[u] * row));
+      x[u] = load_global(reinterpret_cast<const u32x4*>(from + (ok[u] ? next[u] : 0) * row));
     }
     places(j0 + 32 * U);
+#pragma unroll
+    for (int u = 0; u < U; ++u) asm volatile("" : "+v"(x[u]));  // the loads are back
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)

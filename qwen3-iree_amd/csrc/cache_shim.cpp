@@ -366,8 +366,8 @@ int f16_cache_compact(const f16_cache* src, const f16_cache* dst, const int32_t*
     ranges = (count + args.range - 1) / args.range;
   }
   void* p[] = {&args};
-  return q8_shim::launch3(c.compact, (uint32_t)parts, (uint32_t)heads, (uint32_t)ranges, 256, p,
-                          static_cast<hipStream_t>(stream));
+  return q8_shim::launch3(c.compact, (uint32_t)(parts * ranges), (uint32_t)src->kv_heads,
+                          (uint32_t)src->layers, 256, p, static_cast<hipStream_t>(stream));
 }
 
 size_t f16_gemm_argmax_workspace_bytes(int32_t n) {

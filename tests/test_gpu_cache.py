@@ -472,6 +472,38 @@ def test_compact_without_weights_and_nothing(gpu, C):
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
 
 
+def test_many_layers_and_heads(gpu, C):
+    """The most layers and a wide row of heads: more (layer, head) pairs than a
+    grid's second dimension holds."""
+    layers, kvh, d, seq = 1024, 80, 64, 4
+    rng = np.random.default_rng(6)
+    k, v = (normal(rng, (layers, seq, kvh, d)) for _ in range(2))
+    w = rng.random((layers, kvh, seq), dtype=np.float32)
+    dev = Dev(gpu, C, k, v, w)
+    keep = gpu.DeviceBuffer(4 * layers * kvh * 2)
+    C.cache_select(dev.c, 4, 2, 0, 0, keep)
+    C.cache_compact(dev.c, dev.c, keep, True, 0, 2)
+    gpu.synchronize()
+    want = R.select(w, 4, 2, 0, 0)
+    assert np.array_equal(keep.download(np.int32).reshape(want.shape), want)
+    li, hi = np.arange(layers)[:, None, None], np.arange(kvh)[None, :, None]
+    gk, gv, gw = dev.get()
+    assert np.array_equal(gk[:, :2], k[li, want, hi].transpose(0, 2, 1, 3))
+    assert np.array_equal(gv[:, :2], v[li, want, hi].transpose(0, 2, 1, 3))
+    assert np.array_equal(gw[:, :, :2], np.take_along_axis(w, want.astype(np.int64), 2))
+    assert np.array_equal(gk[:, 2:], k[:, 2:]) and np.array_equal(gw[:, :, 2:], w[:, :, 2:])
+    q = normal(rng, (layers, 1, kvh, d))
+    lse = np.full((layers, 1, kvh), 3.0, np.float32)
+    qb, lb = gpu.DeviceBuffer.from_array(q), gpu.DeviceBuffer.from_array(lse)
+    C.attn_weights_add(dev.c, 2, qb, kvh * d, kvh * d, kvh, lb, kvh, 1, None, 1, 0.125)
+    gpu.synchronize()
+    got = dev.get()[2]
+    for l in (0, 500, 1023):
+        ref, tol = R.weights_add(gw[l], q[l], lse[l], gk[l], [0], 2, 1, 0.125)
+        assert (np.abs(got[l] - ref) <= tol)[:, :3].all()
+        assert np.array_equal(got[l, :, 3], gw[l, :, 3])
+
+
 # ------------------------------------------------------ vocabulary rows ----
 
 def run_vocab(Q, w, x, logits=True, stream=None):
