@@ -16,7 +16,7 @@ namespace {
 
 struct {
   hipModule_t module = nullptr;
-  hipFunction_t mask = nullptr, rope = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][4] = {}, select[3] = {}, compact = nullptr,
+  hipFunction_t mask = nullptr, rope = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][5] = {}, select[3] = {}, compact = nullptr,
                 argmax[3] = {}, argmax_final = nullptr;
 } c;
 
@@ -146,7 +146,9 @@ void cache_load(const char* path) {
                {&c.attn[1][3], "attn_tree_128_42"}, {&c.merge[0], "attn_merge_64"},
                {&c.merge[1], "attn_merge_128"},  {&c.weights[0][0], "weights_add_64_1"},
                {&c.weights[0][1], "weights_add_64_2"}, {&c.weights[0][2], "weights_add_64_4"},
-               {&c.weights[0][3], "weights_add_64_many"}, {&c.weights[1][0], "weights_add_128_1"},
+               {&c.weights[0][3], "weights_add_64_many"},
+               {&c.weights[0][4], "weights_add_64_stream"},
+               {&c.weights[1][4], "weights_add_128_stream"}, {&c.weights[1][0], "weights_add_128_1"},
                {&c.weights[1][1], "weights_add_128_2"}, {&c.weights[1][2], "weights_add_128_4"},
                {&c.weights[1][3], "weights_add_128_many"}, {&c.select[0], "cache_select_4"},
                {&c.select[1], "cache_select_16"}, {&c.select[2], "cache_select_any"},
@@ -270,8 +272,13 @@ int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t
     return fail(Q8_ERR_MISALIGNED, "q 16, lse and path 4-byte alignment");
   if ((rc = check_ready())) return rc;
   const int group = q_heads / a->kv_heads, tiles = (n * group + 15) / 16;
-  const int kernel = tiles <= 1 ? 0 : tiles <= 2 ? 1 : tiles <= 4 ? 2 : 3;
   const int64_t nb = (len + n + 31) / 32, heads = (int64_t)a->layers * a->kv_heads;
+  // above 64 rows: the queries by LDS where there are workgroups enough; 256 tokens of
+  // one layer, by LDS and straight: 4096 slots (264 workgroups) 29.6 and 23.1 us, 6000
+  // (392) both 30, 16384 43.6 and 59.5; 64 tokens: 4096 slots 9.6 and 11.7, 8000 11.3
+  // and 15.7
+  const bool stream_rows = (len + n + 127) / 128 * heads >= 3 * q8_shim::compute_units() / 2;
+  const int kernel = tiles <= 1 ? 0 : tiles <= 2 ? 1 : tiles <= 4 ? 2 : stream_rows ? 4 : 3;
   const int64_t blocks = std::clamp<int64_t>(nb * heads / (q8_shim::compute_units() * 16), 1, 16);
   WeightsArgs args{static_cast<const uint16_t*>(a->k),
                    a->weights,
@@ -292,7 +299,9 @@ int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t
                    (int32_t)blocks,
                    scale * kLog2e};
   void* p[] = {&args};
-  const int64_t wgs = kernel == 3 ? (len + n + 63) / 64 : (nb + 4 * blocks - 1) / (4 * blocks);
+  const int64_t wgs = kernel == 4   ? (len + n + 127) / 128
+                      : kernel == 3 ? (len + n + 63) / 64
+                                    : (nb + 4 * blocks - 1) / (4 * blocks);
   return q8_shim::launch3(c.weights[a->head_dim / 64 - 1][kernel], (uint32_t)wgs,
                           (uint32_t)a->kv_heads, (uint32_t)a->layers, 256, p,
                           static_cast<hipStream_t>(stream));

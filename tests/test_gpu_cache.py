@@ -355,6 +355,35 @@ def test_weights_add(gpu, C, heads, n, nodes, length, layers):
         assert np.array_equal(got[l, :, S:], w[l, :, S:], equal_nan=True)
 
 
+@pytest.mark.parametrize("heads", [(16, 8, 128), (64, 2, 64), (16, 1, 128)])
+@pytest.mark.parametrize("layers,length,n", [(40, 250, 70), (2, 33, 130), (300, 100, 40)])
+def test_weights_add_many_rows_and_layers(gpu, C, heads, layers, length, n):
+    """Above 64 rows, on both sides of the number of workgroups where the kernel
+    changes; a few layers are checked."""
+    qh, kvh, d = heads
+    rng = np.random.default_rng(layers + n)
+    k, v = make(rng, kvh, d, length, n, layers=layers)
+    w = rng.random((layers, kvh, k.shape[1]), dtype=np.float32)
+    nodes = n + 5
+    q = normal(rng, (layers, nodes, qh, d), 1.5)
+    path = np.sort(rng.permutation(nodes)[:n]).astype(np.int32)
+    lse = rng.standard_normal((layers, nodes, qh), dtype=np.float32) + 6
+    path[n // 2], lse[:, path[3], 0] = nodes, -np.inf
+    dev = Dev(gpu, C, k, v, w)
+    qb, lb = gpu.DeviceBuffer.from_array(q), gpu.DeviceBuffer.from_array(lse)
+    pb = gpu.DeviceBuffer.from_array(path)
+    print(f"weights n={n} layers={layers} len={length} heads={heads}", flush=True)
+    C.attn_weights_add(dev.c, length, qb, nodes * qh * d, qh * d, qh, lb, nodes * qh, nodes, pb, n,
+                       d ** -0.5)
+    gpu.synchronize()
+    got = dev.get()[2]
+    for l in sorted({0, 1, layers // 2, layers - 1}):
+        ref, tol = R.weights_add(w[l], q[l], lse[l], k[l], path, length, n, d ** -0.5)
+        S = length + n
+        assert (np.abs(got[l, :, :S] - ref[:, :S]) <= tol[:, :S]).all()
+        assert np.array_equal(got[l, :, S:], w[l, :, S:], equal_nan=True)
+
+
 def test_weights_without_a_path_and_row_stride(gpu, C):
     rng = np.random.default_rng(2)
     n, length, qh, kvh, d = 6, 50, 4, 2, 64
