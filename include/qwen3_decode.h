@@ -278,7 +278,8 @@ int qwen3_generate(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t
  * unless slots have been evicted), its k and v go to slot len + i of every layer,
  * and it attends to slots 0 .. len - 1 and its ancestors.  next_tokens (device
  * int32 [n]): the argmax of every node's logits, what the model says follows it
- * (of padding: unspecified); logits f16 [n, 151936], may be NULL.
+ * (of padding: unspecified; a token outside the vocabulary counts as token 0);
+ * logits f16 [n, 151936], may be NULL.
  * q_rows f16 [28, n, 2048] and lse f32 [28, n, 16] (both or neither NULL) receive
  * each layer's queries after RoPE and log-sum-exps, what f16_attn_weights_add
  * needs once it is known which nodes are kept; f16_cache_compact moves those

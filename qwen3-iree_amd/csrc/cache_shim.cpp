@@ -16,8 +16,9 @@ namespace {
 
 struct {
   hipModule_t module = nullptr;
-  hipFunction_t mask = nullptr, rope = nullptr, attn[2][4] = {}, merge[2] = {}, weights[2][5] = {}, select[3] = {}, compact = nullptr,
-                argmax[3] = {}, argmax_final = nullptr;
+  hipFunction_t mask = nullptr, rope = nullptr, attn[2][4] = {}, merge[2] = {};
+  hipFunction_t weights[2][5] = {}, select[3] = {}, compact = nullptr;
+  hipFunction_t argmax[3] = {}, argmax_final = nullptr;
 } c;
 
 int fail(int code, const char* fmt, ...) {
@@ -138,22 +139,35 @@ void cache_load(const char* path) {
   struct {
     hipFunction_t* fn;
     const char* name;
-  } names[] = {{&c.mask, "tree_mask_k"},          {&c.rope, "tree_rope_k"},
+  } names[] = {{&c.mask, "tree_mask_k"},
+               {&c.rope, "tree_rope_k"},
                {&c.attn[0][0], "attn_tree_64_11"},
-               {&c.attn[0][1], "attn_tree_64_21"}, {&c.attn[0][2], "attn_tree_64_41"},
-               {&c.attn[0][3], "attn_tree_64_42"}, {&c.attn[1][0], "attn_tree_128_11"},
-               {&c.attn[1][1], "attn_tree_128_21"}, {&c.attn[1][2], "attn_tree_128_41"},
-               {&c.attn[1][3], "attn_tree_128_42"}, {&c.merge[0], "attn_merge_64"},
-               {&c.merge[1], "attn_merge_128"},  {&c.weights[0][0], "weights_add_64_1"},
-               {&c.weights[0][1], "weights_add_64_2"}, {&c.weights[0][2], "weights_add_64_4"},
+               {&c.attn[0][1], "attn_tree_64_21"},
+               {&c.attn[0][2], "attn_tree_64_41"},
+               {&c.attn[0][3], "attn_tree_64_42"},
+               {&c.attn[1][0], "attn_tree_128_11"},
+               {&c.attn[1][1], "attn_tree_128_21"},
+               {&c.attn[1][2], "attn_tree_128_41"},
+               {&c.attn[1][3], "attn_tree_128_42"},
+               {&c.merge[0], "attn_merge_64"},
+               {&c.merge[1], "attn_merge_128"},
+               {&c.weights[0][0], "weights_add_64_1"},
+               {&c.weights[0][1], "weights_add_64_2"},
+               {&c.weights[0][2], "weights_add_64_4"},
                {&c.weights[0][3], "weights_add_64_many"},
                {&c.weights[0][4], "weights_add_64_stream"},
-               {&c.weights[1][4], "weights_add_128_stream"}, {&c.weights[1][0], "weights_add_128_1"},
-               {&c.weights[1][1], "weights_add_128_2"}, {&c.weights[1][2], "weights_add_128_4"},
-               {&c.weights[1][3], "weights_add_128_many"}, {&c.select[0], "cache_select_4"},
-               {&c.select[1], "cache_select_16"}, {&c.select[2], "cache_select_any"},
-               {&c.compact, "cache_compact_k"},   {&c.argmax[0], "gemm_argmax_64"},
-               {&c.argmax[1], "gemm_argmax_128"}, {&c.argmax[2], "gemm_argmax_256"},
+               {&c.weights[1][0], "weights_add_128_1"},
+               {&c.weights[1][1], "weights_add_128_2"},
+               {&c.weights[1][2], "weights_add_128_4"},
+               {&c.weights[1][3], "weights_add_128_many"},
+               {&c.weights[1][4], "weights_add_128_stream"},
+               {&c.select[0], "cache_select_4"},
+               {&c.select[1], "cache_select_16"},
+               {&c.select[2], "cache_select_any"},
+               {&c.compact, "cache_compact_k"},
+               {&c.argmax[0], "gemm_argmax_64"},
+               {&c.argmax[1], "gemm_argmax_128"},
+               {&c.argmax[2], "gemm_argmax_256"},
                {&c.argmax_final, "gemm_argmax_final"}};
   for (auto& n : names) {
     if (hipModuleGetFunction(n.fn, m, n.name) != hipSuccess) {
@@ -323,7 +337,9 @@ int f16_cache_select(const f16_cache* a, int32_t len, int32_t budget, int32_t si
   SelectArgs args{a->weights, keep, a->max_seq, len, budget, sinks, recent};
   void* p[] = {&args};
   const int slots = len - sinks - recent;
-  return q8_shim::launch(c.select[slots <= 4096 ? 0 : slots <= 16384 ? 1 : 2], (uint32_t)(a->layers * a->kv_heads), 1024, p,
+  // a thread's 4 or 16 weights in registers where they hold all slots
+  return q8_shim::launch(c.select[slots <= 4096 ? 0 : slots <= 16384 ? 1 : 2],
+                         (uint32_t)(a->layers * a->kv_heads), 1024, p,
                          static_cast<hipStream_t>(stream));
 }
 

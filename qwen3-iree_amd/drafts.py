@@ -35,7 +35,9 @@ class DraftSession(D.DecodeSession):
     """A session whose tokens come in trees of up to max_nodes nodes.
 
     weights: keep the attention weights eviction goes by; then a prompt is read in
-    trees too (chunks of max_nodes tokens), else in one piece."""
+    trees too (chunks of max_nodes tokens), else in one piece.  The calls of a
+    DecodeSession that go by the token and position on the device are refused: they
+    know nothing of `length`."""
 
     def __init__(self, model: D.DeviceWeights, max_seq: int, max_nodes: int = 64,
                  weights: bool = True, stream: Q.Stream | None = None):
@@ -59,6 +61,11 @@ class DraftSession(D.DecodeSession):
         self.cache = C.Cache(self.k_cache, self.v_cache, self.max_seq, D.LAYERS, D.KV_HEADS,
                              D.HEAD_DIM, self._weights)
         self._tree: tuple[np.ndarray, np.ndarray] | None = None  # of the last verify
+
+    def _refused(self, *args, **kwargs):
+        raise TypeError("a session of drafted trees moves by prompt, verify and accept")
+
+    step = step_checked = capture = replay = prefill = prefill_batched = generate = _refused
 
     def _slot(self, i: int) -> int:
         return self._nodes.ptr + 4 * self.max_nodes * i
@@ -120,7 +127,7 @@ class DraftSession(D.DecodeSession):
             raise ValueError(f"{tokens.size} tokens behind {self.length} of {self.max_seq} slots")
         if self._weights is None and self.length == self.position:
             self.set_state(0, self.length)
-            self.prefill_batched(tokens)
+            super().prefill_batched(tokens)
             self.length += int(tokens.size)
             self.position = self.length
             return self.get_state()[0]

@@ -74,3 +74,14 @@ def test_session_refuses_bad_sizes(Q, D):
     for max_seq, nodes in ((100, 0), (100, 257), (10, 11)):
         with pytest.raises(ValueError):
             drafts.DraftSession(None, max_seq, nodes)
+
+
+def test_session_refuses_the_calls_by_device_words(Q, D):
+    from qwen3_iree_amd import drafts
+
+    s = object.__new__(drafts.DraftSession)
+    for name, args in (("step", ()), ("step_checked", ()), ("capture", ()), ("replay", ()),
+                       ("prefill", ([1],)), ("prefill_batched", ([1],)), ("generate", (4, 0))):
+        assert hasattr(D.DecodeSession, name)
+        with pytest.raises(TypeError):
+            getattr(s, name)(*args)
