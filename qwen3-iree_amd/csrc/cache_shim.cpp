@@ -93,13 +93,13 @@ constexpr int kMaxSplits = 64;  // one lane each in the merge
 // workgroups, so about sqrt(nb) of them (somewhat more where a round is longer:
 // several waves share a block), and none up to 10 blocks.  us a layer (16 query
 // over 8 kv heads of 128) with 1 / 4 / 8 / 16 / 32 splits:
-//   1 node, 300 slots (10 blocks) 6.8 / 7.8 / 8.2, 1000 (32) 11.1 / 9.2 / 8.5 / 9.5
-//   / 10.5, 4000 (126) 46.4 / 19.1 / 13.8 / 11.7 / 12.2, 16384 (513) 97.7 / 35.3 /
-//   24.2 / 21.6 / 23.0; 30 nodes, 1024 (33) 19.6 / 11.5 / 10.4 / 11.6 / 11.7, 8191
-//   (257) 178 / 53.1 / 32.0 / 22.4 / 19.8; 61 nodes, 1024 (34) 28.2 / 15.6 / 14.5 /
-//   15.3 / 16.5, 8191 (258) 183 / 55.3 / 34.3 / 24.8 / 22.9 (64: 28.7); 256 nodes,
-//   1024 (40) 36.1 / 25.6 / 27.2 / 29.9 / 34.1, 16384 (520) 341 / 104 / 67.1 / 60.1
-//   / 74.0.
+//   1 node, 300 slots (10 blocks) 6.8 / 7.8 / 8.1, 1000 (32) 10.7 / 9.0 / 8.4 / 8.7
+//   / 9.2, 4000 (126) 46.2 / 18.8 / 13.4 / 11.0 / 10.8, 16384 (513) 104 / 36.2 / 23.7
+//   / 20.5 / 20.5 (64: 24.2); 30 nodes, 1024 (33) 19.5 / 11.5 / 10.4 / 10.7 / 11.2; 13
+//   nodes, 8191 (257) 138 / 43.3 / 27.1 / 19.0 / 16.7; 61 nodes, 1024 (34) 28.2 / 15.5
+//   / 14.4 / 14.6 / 16.1, 8191 (258) 182 / 55.3 / 34.0 / 24.2 / 21.8 (64: 27.1); 256
+//   nodes, 1024 (40) 36.1 / 25.9 / 26.5 / 30.1 / 33.7, 16384 (520) 341 / 104 / 66.4 /
+//   60.1 / 73.2.
 // At most one workgroup a CU where it takes the CU's LDS (up to 16 rows), else two.
 AttnPlan attn_plan(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) {
   const int rows = n * (q_heads / a->kv_heads);
