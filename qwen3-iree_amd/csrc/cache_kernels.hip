@@ -948,11 +948,13 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 // One workgroup per layer and kv head.  The order number of the last slot that
 // still fits is found in three digits (11, 11 and 10 bits): a histogram in LDS of
 // the slots that agree in the digits before, then a count from its top down.  A
-// wave holds 64 E consecutive slots in registers, 64 at a time, so the places of
-// the kept slots come from one prefix count over the waves and ballots: nothing
-// depends on an order of arrival.  E = 0 reads the weights again for each digit.
-// Latency bound, the chain of barriers: 601 slots of a layer (8 workgroups) 5.6 us,
-// 2048 of 28 layers 7.2 (E = 4), 16384 of 28 layers 22.5 (E = 16).
+// wave holds consecutive slots, 64 at a time, up to E of them a lane in registers,
+// so the places of the kept slots come from one prefix count over the waves and
+// ballots: nothing depends on an order of arrival.  E = 0 reads the weights again
+// for each of the five passes.
+// Bound by the chain of barriers, then by the passes' instructions, all of a head on
+// one CU: 601 slots of a layer (8 workgroups) 4.3 us, of 28 layers 2048 5.4, 16384
+// 12.8, 30000 26.5, 48000 37.8; E = 0 by the re-reads, 60000 128, 100000 221.
 namespace {
 template <int CTRL, int ROWS = 0xF>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
@@ -979,10 +981,18 @@ __device__ __forceinline__ uint32_t waves_before(const uint32_t* v, int wave) {
   return (uint32_t)__builtin_amdgcn_readlane((int)x, 15);
 }
 
-template <int E>
+// the set bits of m below this lane, and base
+__device__ __forceinline__ uint32_t bits_below(uint64_t m, uint32_t base) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)m, base));
+}
+
+template <int E, int kCopies>
 __device__ __forceinline__ void cache_select(const SelectArgs& A) {
   constexpr int kBins = 2048;
-  __shared__ uint32_t hist[kBins];
+  constexpr int kStep = E == 4 ? 1 : E ? 4 : 16;  // slots of a thread at a time
+  // a lane counts in copy lane mod kCopies: equal weights meet in one word less often
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kCopies][kBins + 8];
   __shared__ uint32_t wave_sum_[16], wave_above[16], wave_equal[16];
   __shared__ uint32_t s_digit, s_left;
   const int t = threadIdx.x, lane = t & 63;
@@ -994,42 +1004,57 @@ __device__ __forceinline__ void cache_select(const SelectArgs& A) {
   for (int j = t; j < A.sinks; j += 1024) keep[j] = j;
   for (int j = t; j < A.recent; j += 1024) keep[A.budget - A.recent + j] = last + j;
   if (middle == 0) return;
-  // this wave's slots: p0 + 64 e + lane, e < count
-  const int count = E ? E : (last - first + 1023) >> 10;
+  // this wave's slots: p0 + 64 e + lane, e < count; behind `last` number 0, the
+  // lowest and in the last places, so that none of them is ever kept
+  const int count = (((last - first + 1023) >> 10) + kStep - 1) / kStep * kStep;
   const int p0 = first + wave * 64 * count + lane;
-  uint32_t own[E ? E : 1];
+  uint32_t own[E ? E : kStep];
 #pragma unroll
-  for (int e = 0; e < E; ++e) own[e] = p0 + 64 * e < last ? weight_order(w[p0 + 64 * e]) : 0u;
-  auto number = [&](int e) {
-    if constexpr (E != 0) return own[e];
-    else return p0 + 64 * e < last ? weight_order(w[p0 + 64 * e]) : 0u;
+  for (int e = 0; e < E; ++e)
+    own[e] = e < count && p0 + 64 * e < last ? weight_order(w[p0 + 64 * e]) : 0u;
+  // use(slot, number) for every slot of the wave in order
+  auto each = [&](auto&& use) {
+    if constexpr (E != 0) {
+#pragma unroll
+      for (int e0 = 0; e0 < E; e0 += kStep) {
+        if (e0 >= count) break;
+#pragma unroll
+        for (int e = e0; e < e0 + kStep; ++e) use(p0 + 64 * e, own[e]);
+      }
+    } else {
+      for (int e0 = 0; e0 < count; e0 += kStep) {
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {
+          const int p = p0 + 64 * (e0 + u);
+          const float x = w[p < last ? p : last - 1];
+          own[u] = p < last ? weight_order(x) : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) use(p0 + 64 * (e0 + u), own[u]);
+      }
+    }
   };
   uint32_t prefix = 0, need = (uint32_t)middle;
 #pragma unroll
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
     const int bits = digit == 2 ? 10 : 11;
-    hist[t] = 0;
-    hist[1024 + t] = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) *reinterpret_cast<uint2*>(&hist[c][2 * t]) = make_uint2(0, 0);
     __syncthreads();
-#pragma unroll(E ? E : 1)
-    for (int e = 0; e < count; ++e) {
-      const uint32_t o = number(e);
-      const bool in = p0 + 64 * e < last && (digit == 0 || (o ^ prefix) >> (shift + bits) == 0);
-      const uint32_t d = (o >> shift) & ((1u << bits) - 1);
-      // many equal weights: one addition for the wave
-      const uint64_t m = __ballot(in);
-      if (m == 0) continue;
-      const int leader = __ffsll((unsigned long long)m) - 1;
-      if (__ballot(in && d == (uint32_t)__builtin_amdgcn_readlane((int)d, leader)) == m) {
-        if (lane == leader) atomicAdd(&hist[d], (uint32_t)__popcll(m));
-      } else if (in) {
-        atomicAdd(&hist[d], 1u);
-      }
-    }
+    each([&](int p, uint32_t o) {
+      if (digit == 0 ? p < last : (o ^ prefix) >> (shift + bits) == 0)
+        atomicAdd(&hist[lane % kCopies][(o >> shift) & ((1u << bits) - 1)], 1u);
+    });
     __syncthreads();
     // thread t: bins 2047 - 2 t and 2046 - 2 t, counted from the top
-    const uint32_t c0 = hist[2047 - 2 * t], c1 = hist[2046 - 2 * t];
+    uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const uint2 two = *reinterpret_cast<const uint2*>(&hist[c][2046 - 2 * t]);
+      c0 += two.y;
+      c1 += two.x;
+    }
     uint32_t up = scan_u32(c0 + c1);  // of the threads up to this one
     if (lane == 63) wave_sum_[wave] = up;
     __syncthreads();
@@ -1046,45 +1071,37 @@ __device__ __forceinline__ void cache_select(const SelectArgs& A) {
   }
   // every slot above the bound, and the first `need` that equal it
   uint32_t above = 0, equal = 0;
-#pragma unroll(E ? E : 1)
-  for (int e = 0; e < count; ++e) {
-    const bool in = p0 + 64 * e < last;
-    const uint32_t o = number(e);
-    above += in && o > prefix ? 1u : 0u;
-    equal += in && o == prefix ? 1u : 0u;
-  }
-  above = scan_u32(above);
-  equal = scan_u32(equal);
-  if (lane == 63) {
+  each([&](int, uint32_t o) {
+    above += (uint32_t)__popcll(__ballot(o > prefix));
+    equal += (uint32_t)__popcll(__ballot(o == prefix));
+  });
+  if (lane == 0) {
     wave_above[wave] = above;
     wave_equal[wave] = equal;
   }
   __syncthreads();
   above = waves_before(wave_above, wave);
   equal = waves_before(wave_equal, wave);
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
-#pragma unroll(E ? E : 1)
-  for (int e = 0; e < count; ++e) {
-    const bool in = p0 + 64 * e < last;
-    const uint32_t o = number(e);
-    const uint64_t ma = __ballot(in && o > prefix), me = __ballot(in && o == prefix);
-    const uint32_t a = above + (uint32_t)__popcll(ma & below);
-    const uint32_t q = equal + (uint32_t)__popcll(me & below);
-    if (in && (o > prefix || (o == prefix && q < need)))
-      keep[A.sinks + a + (q < need ? q : need)] = p0 + 64 * e;
+  each([&](int p, uint32_t o) {
+    const uint64_t ma = __ballot(o > prefix), me = __ballot(o == prefix);
+    const uint32_t a = bits_below(ma, above), q = bits_below(me, equal);
+    if (o > prefix || (o == prefix && q < need)) keep[A.sinks + a + (q < need ? q : need)] = p;
     above += (uint32_t)__popcll(ma);
     equal += (uint32_t)__popcll(me);
-  }
+  });
 }
 }  // namespace
 extern "C" __global__ __launch_bounds__(1024) void cache_select_4(SelectArgs A) {
-  cache_select<4>(A);
+  cache_select<4, 1>(A);
 }
 extern "C" __global__ __launch_bounds__(1024) void cache_select_16(SelectArgs A) {
-  cache_select<16>(A);
+  cache_select<16, 4>(A);
+}
+extern "C" __global__ __launch_bounds__(1024) void cache_select_48(SelectArgs A) {
+  cache_select<48, 4>(A);
 }
 extern "C" __global__ __launch_bounds__(1024) void cache_select_any(SelectArgs A) {
-  cache_select<0>(A);
+  cache_select<0, 4>(A);
 }
 
 // ----------------------------------------------------------- compaction ----

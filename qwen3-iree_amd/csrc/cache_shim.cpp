@@ -17,7 +17,7 @@ namespace {
 struct {
   hipModule_t module = nullptr;
   hipFunction_t mask = nullptr, rope = nullptr, attn[2][4] = {}, merge[2] = {};
-  hipFunction_t weights[2][5] = {}, select[3] = {}, compact = nullptr;
+  hipFunction_t weights[2][5] = {}, select[4] = {}, compact = nullptr;
   hipFunction_t argmax[3] = {}, argmax_final = nullptr;
 } c;
 
@@ -163,7 +163,8 @@ void cache_load(const char* path) {
                {&c.weights[1][4], "weights_add_128_stream"},
                {&c.select[0], "cache_select_4"},
                {&c.select[1], "cache_select_16"},
-               {&c.select[2], "cache_select_any"},
+               {&c.select[2], "cache_select_48"},
+               {&c.select[3], "cache_select_any"},
                {&c.compact, "cache_compact_k"},
                {&c.argmax[0], "gemm_argmax_64"},
                {&c.argmax[1], "gemm_argmax_128"},
@@ -337,8 +338,9 @@ int f16_cache_select(const f16_cache* a, int32_t len, int32_t budget, int32_t si
   SelectArgs args{a->weights, keep, a->max_seq, len, budget, sinks, recent};
   void* p[] = {&args};
   const int slots = len - sinks - recent;
-  // a thread's 4 or 16 weights in registers where they hold all slots
-  return q8_shim::launch(c.select[slots <= 4096 ? 0 : slots <= 16384 ? 1 : 2],
+  // a thread's 4, 16 or 48 weights in registers where they hold all slots
+  const int kernel = slots <= 4096 ? 0 : slots <= 16384 ? 1 : slots <= 49152 ? 2 : 3;
+  return q8_shim::launch(c.select[kernel],
                          (uint32_t)(a->layers * a->kv_heads), 1024, p,
                          static_cast<hipStream_t>(stream));
 }

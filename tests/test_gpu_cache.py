@@ -431,6 +431,37 @@ def test_select(gpu, C, length, budget, sinks, recent, kind):
     assert np.array_equal(got, R.select(w, length, budget, sinks, recent))
 
 
+@pytest.mark.parametrize("slots", [1023, 1025, 4096, 4097, 16384, 16385, 20481, 49152, 49153, 70000])
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "nan", "mixed"])
+def test_select_on_both_sides_of_each_size(gpu, C, slots, kind):
+    """Slots between the first and last kept ones where the number a thread holds
+    changes; budgets of one, about a third, all but one and all of them."""
+    sinks, recent, kvh = 3, 7, 2
+    length = sinks + slots + recent
+    rng = np.random.default_rng(slots)
+    w = np.exp(2 * rng.standard_normal((1, kvh, length + 1))).astype(np.float32)
+    if kind == "ties":
+        w = rng.integers(-1, 2, w.shape).astype(np.float32)
+    elif kind == "equal":
+        w[:] = 0.25
+    elif kind == "nan":
+        w[:] = np.nan
+    elif kind == "mixed":
+        w[rng.random(w.shape) < 0.5] = np.nan
+        w[rng.random(w.shape) < 0.2] = -np.inf
+    w[:, :, length:] = np.inf
+    wb = gpu.DeviceBuffer.from_array(w)
+    c = C.Cache(None, None, length + 1, 1, kvh, 128, wb)
+    print(f"select of {slots} {kind}", flush=True)
+    for middle in (1, slots // 3, slots - 1, slots):
+        budget = sinks + middle + recent
+        keep = Guarded(gpu, 4 * kvh * budget)
+        C.cache_select(c, length, budget, sinks, recent, keep.ptr)
+        gpu.synchronize()
+        got = keep.get(np.int32).reshape(1, kvh, budget)
+        assert np.array_equal(got, R.select(w, length, budget, sinks, recent)), middle
+
+
 def move(k, v, w, k_to, v_to, w_to, keep, base):
     """numpy form of cache_compact; keep [layers, kvh, count] or [count]."""
     layers, seq, kvh, _ = k.shape
