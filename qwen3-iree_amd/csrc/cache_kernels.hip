@@ -776,42 +776,61 @@ __device__ __forceinline__ void weights_add(const WeightsArgs& A) {
 
 // Any number of rows: a workgroup holds the keys of 64 slots, its waves take the
 // row tiles in turn (the next one's queries requested before one is computed)
-// and meet in LDS.  Bound by those requests, eight tiles one behind another a wave:
-// 256 tokens, 2047 slots of a layer 15 us.
+// and meet in LDS.  Every wave needs all the keys, so they come by LDS, whole rows
+// at a time: 256 tokens, 2047 slots of a layer 13.3 us against 15.8 with each wave's
+// fragments (64 bytes of 16 rows a load) from memory, 4096 slots 18.0 against 21.8.
+// The queries stay on that way: by LDS too 14.2.
 template <int D>
 __device__ __forceinline__ void weights_add_many(const WeightsArgs& A) {
+  constexpr int kChunks = D / 8, kRowsPerPiece = 64 / kChunks, kPieces = D / 32;
   __shared__ int source[kTreeMax];
   __shared__ float part[4][64];
-  const int t = threadIdx.x, lane = t & 63, c16 = lane & 15;
+  __shared__ __attribute__((aligned(1024))) uint8_t kk[128 * D];
+  const int t = threadIdx.x, lane = t & 63, c16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = blockIdx.y, layer = blockIdx.z;
   const int slots = A.len + A.n, p0 = 64 * blockIdx.x;
   const int64_t row = (int64_t)A.kv_heads * D;
   const uint16_t* kb = A.k + layer * A.max_seq * row + kvh * D;
   float* wb = A.weights + ((int64_t)layer * A.kv_heads + kvh) * A.max_seq;
-  WeightKeys<D> keys[2];
-  keys[0].load(kb, row, p0, slots);
-  keys[1].load(kb, row, p0 + 32, slots);
+  // chunk c of slot r sits in place c ^ (r mod kChunks) of its row; slots behind the
+  // last repeat it
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int r = kRowsPerPiece * (kPieces * wave + i) + lane / kChunks, p = p0 + r;
+    const uint16_t* from = kb + (p < slots ? p : slots - 1) * row +
+                           8 * ((lane % kChunks) ^ (r & (kChunks - 1)));
+    __builtin_amdgcn_global_load_lds((const GLOBAL_AS void*)from,
+                                     (LDS_AS void*)(kk + 1024 * (kPieces * wave + i)), 16, 0, 0);
+  }
   source[t] = weight_source(A, t);
+  wait_vm<0>();
   __syncthreads();
-  float sum[2][8];
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[x][e] = 0.0f;
   const int tiles = (A.n * A.group + 15) >> 4;
   auto load = [&](int tile, WeightRow<D>& R) {
     const int r = 16 * tile + c16;
     const int i = A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv);
     R.load(A, layer, kvh, r, i, i < A.n ? source[i] : -1);
   };
+  WeightRow<D> rows[2];
+  if (wave < tiles) load(wave, rows[0]);
+  WeightKeys<D> keys[2];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int st = 0; st < D / 32; ++st)
+      keys[x >> 1].k[st][x & 1] = *reinterpret_cast<const f16x8*>(
+          kk + 2 * D * (16 * x + c16) + 16 * ((4 * st + grp) ^ (c16 & (kChunks - 1))));
+  float sum[2][8];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[x][e] = 0.0f;
   auto use = [&](const WeightRow<D>& R) {
     const bool edge = p0 + 64 > A.len || __builtin_amdgcn_ballot_w64(R.last < 0) != 0;
     add_weights<D>(R, keys[0], p0, A.scale, edge, sum[0]);
     add_weights<D>(R, keys[1], p0 + 32, A.scale, edge, sum[1]);
   };
-  WeightRow<D> rows[2];
-  if (wave < tiles) load(wave, rows[0]);
   for (int tile = wave; tile < tiles; tile += 8) {
     if (tile + 4 < tiles) load(tile + 4, rows[1]);
     use(rows[0]);
@@ -833,11 +852,10 @@ __device__ __forceinline__ void weights_add_many(const WeightsArgs& A) {
 }
 
 // The same for many slots: the four waves hold the keys of 32 slots each and share
-// the row tiles, whose queries are copied into LDS one tile ahead.  The gathered
-// loads of weights_add_many (64 bytes of 16 rows each, per 64 slots) bound that
-// one where there are workgroups enough, its shorter chain of tiles is faster
-// where there are not: 256 tokens, 2047 slots of a layer 15-16 us against 29,
-// 16384 slots 59.5 against 43.6; 64 tokens, 2047 slots of 28 layers 94 against 49.
+// the row tiles, whose queries are copied into LDS one tile ahead: a query is read
+// once per 128 slots, but the tiles come one behind another.  256 tokens, 16384 slots
+// of a layer 42.1 us against 47.1 by weights_add_many, 2047 slots 29 against 13.3;
+// 64 tokens, 2047 slots of 28 layers 46.2 against 53.8.
 template <int D>
 __device__ __forceinline__ void weights_add_stream(const WeightsArgs& A) {
   constexpr int kChunks = D / 8, kRowsPerPiece = 64 / kChunks;

@@ -288,12 +288,12 @@ int f16_attn_weights_add(const f16_cache* a, int32_t len, const void* q, int64_t
   if ((rc = check_ready())) return rc;
   const int group = q_heads / a->kv_heads, tiles = (n * group + 15) / 16;
   const int64_t nb = (len + n + 31) / 32, heads = (int64_t)a->layers * a->kv_heads;
-  // above 64 rows: the queries by LDS where there are workgroups enough; 256 tokens of
-  // one layer, by LDS and straight: 4096 slots (264 workgroups) 29.6 and 23.1 us, 6000
-  // (392) both 30, 16384 43.6 and 59.5; 64 tokens: 4096 slots 9.6 and 11.7, 8000 11.3
-  // and 15.7
-  const bool stream_rows = (len + n + 127) / 128 * heads >= 3 * q8_shim::compute_units() / 2;
-  const int kernel = tiles <= 1 ? 0 : tiles <= 2 ? 1 : tiles <= 4 ? 2 : stream_rows ? 4 : 3;
+  // above 64 rows: shared queries where there are workgroups enough.  256 tokens of one
+  // layer, with and without: 8000 slots (520 workgroups) 32.0 and 28.2 us, 12000 (768)
+  // 32.6 and 33.2, 16384 (1040) 42.1 and 47.1; 64 tokens: 8000 (504) 11.0 and 10.8,
+  // 16384 (1032) 16.2 and 17.6
+  const bool shared = (len + n + 127) / 128 * heads >= 3 * q8_shim::compute_units();
+  const int kernel = tiles <= 1 ? 0 : tiles <= 2 ? 1 : tiles <= 4 ? 2 : shared ? 4 : 3;
   const int64_t blocks = std::clamp<int64_t>(nb * heads / (q8_shim::compute_units() * 16), 1, 16);
   WeightsArgs args{static_cast<const uint16_t*>(a->k),
                    a->weights,
