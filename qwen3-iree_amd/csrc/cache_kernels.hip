@@ -104,8 +104,8 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 // row blocks, splits; kv head fastest, so that 8 kv heads keep to an XCD each); several
 // splits leave (m, l, O) in the workspace and attn_merge combines them in order.
 // 16 query heads over 8 kv heads of 128: 1 node, 300 slots 7 us (one workgroup a kv
-// head: launch, masks, four rounds); 13 nodes, 1024 slots 5.7 and 2.8 for the merge;
-// 61, 8191 13.8 and 5.6; 256, 16384 45.6 (750 TFLOP/s of both products; MFMA and
+// head: launch, masks, four rounds); 13 nodes, 1024 slots 6.4 and 2.5 for the merge;
+// 61, 8191 14.8 and 4.5; 256, 16384 46 (750 TFLOP/s of both products; MFMA and
 // VALU 39 and 38 % busy, in turn) and 8.0.
 namespace {
 
@@ -1131,8 +1131,8 @@ extern "C" __global__ __launch_bounds__(1024) void cache_select_any(SelectArgs A
 // writes: with ascending slots (keep[j] >= j) and one range, a write never meets a
 // slot that is still to be read, so source and destination may be one.
 // Bound by the bytes moved, 128 at a time from scattered slots: 28 layers, 4096 of
-// 16384 slots 191 us, 4.9 TB/s read and written; 1024 of 2048 42-52; 512 of one
-// layer 3.1 (two rounds).
+// 16384 slots 189 us, 4.95 TB/s read and written; 1024 of 2048 43-51; 512 of one
+// layer 3.3 (two rounds).
 extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A) {
   constexpr int U = 8;
   const int t = threadIdx.x;
