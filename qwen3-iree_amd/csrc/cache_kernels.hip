@@ -94,9 +94,9 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 //     (half a step, 2^-11 of itself, at most), up to 32 rows as the sum of two (2^-22):
 //     the bytes bound those, and the second product costs nothing.
 // K and V blocks are copied from memory straight into LDS, the next one while one
-// is computed.  RG waves share a block (RG row groups of T tiles,
-// T = 2 from 65 rows on: up to there the code and the registers of a second tile
-// cost more than the block's second read, 30 rows over 1024 slots 12.7 -> 10.8 us);
+// is computed.  RG waves share a block (RG row groups of T tiles:
+// T = 2 halves the reads of LDS, but one tile's rounds are shorter, so it pays only
+// where there is much to do);
 // the 4 / RG position groups of a workgroup take blocks in turn and meet in LDS.
 // With one row group no wave waits for another until the end: few rows are bound
 // by the bytes in flight, 64 KiB a CU, many rows by MFMA and exp2.

@@ -88,30 +88,41 @@ struct AttnPlan {
 
 constexpr int kMaxSplits = 64;  // one lane each in the merge
 
+// Rows of a workgroup: a wave's one tile of 16 up to 64 rows, and above them too
+// (several row blocks, whose K and V come out of L2) until every CU has 65 blocks of
+// 64 rows and 32 slots to do; then two tiles a wave.  us a layer (16 query over 8 kv
+// heads of 128), one and two tiles: 61 nodes, 1024 slots 12.0 / 14.4, 8191 22.0 / 23.1;
+// 128, 2048 16.7 / 20.6, 16384 36.4 / 41.4, 30000 66.7 / 57.4; 256, 300 18.2 / 22.1,
+// 6000 33.9 / 38.4, 8191 42.4 / 37.4, 16384 61.3 / 58.8.
+//
 // Splits of the nb blocks of 32 slots: each costs a partial written and merged,
 // the first one a launch, and each block of a split costs a round of its
-// workgroups, so about sqrt(nb) of them (somewhat more where a round is longer:
-// several waves share a block), and none up to 10 blocks.  us a layer (16 query
-// over 8 kv heads of 128) with 1 / 4 / 8 / 16 / 32 splits:
+// workgroups, so about sqrt(nb) of them (somewhat more where waves share a block),
+// and none up to 10 blocks.  With 1 / 4 / 8 / 16 / 32 splits:
 //   1 node, 300 slots (10 blocks) 6.8 / 7.8 / 8.1, 1000 (32) 10.7 / 9.0 / 8.4 / 8.7
 //   / 9.2, 4000 (126) 46.2 / 18.8 / 13.4 / 11.0 / 10.8, 16384 (513) 104 / 36.2 / 23.7
 //   / 20.5 / 20.5 (64: 24.2); 30 nodes, 1024 (33) 19.5 / 11.5 / 10.4 / 10.7 / 11.2; 13
-//   nodes, 8191 (257) 138 / 43.3 / 27.1 / 19.0 / 16.7; 61 nodes, 1024 (34) 28.2 / 15.5
-//   / 14.4 / 14.6 / 16.1, 8191 (258) 182 / 55.3 / 34.0 / 24.2 / 21.8 (64: 27.1); 256
-//   nodes, 1024 (40) 36.1 / 25.9 / 26.5 / 30.1 / 33.7, 16384 (520) 341 / 104 / 66.4 /
-//   60.1 / 73.2.
-// At most one workgroup a CU where it takes the CU's LDS (up to 16 rows), else two.
+//   nodes, 8191 (257) 138 / 43.3 / 27.1 / 19.0 / 16.7.
+// At most one workgroup a CU where it takes the CU's LDS (up to 16 rows), else two;
+// above 64 rows as many as fill every CU once, or twice where that leaves each split
+// 8 blocks: 256 nodes, 1024 slots (5 blocks at two) 21.4 at one and 23.8 at two; 128,
+// 2048 16.9 and 19.0; 4000 slots and 256 nodes (17 blocks) 35.9 and 31.4; 8191 and 61
+// (8) 22.8 and 21.5.
 AttnPlan attn_plan(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) {
-  const int rows = n * (q_heads / a->kv_heads);
+  const int rows = n * (q_heads / a->kv_heads), cus = q8_shim::compute_units();
+  const int nb = (len + n + 31) / 32;
+  const int64_t work = (int64_t)((rows + 63) / 64) * a->kv_heads * nb;
   AttnPlan p{};
-  p.kernel = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+  p.kernel = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 || work < 65 * cus ? 2 : 3;
   const int per_wg = 16 << p.kernel;
   p.row_blocks = (rows + per_wg - 1) / per_wg;
-  const int nb = (len + n + 31) / 32;
-  const int most = (p.kernel == 0 ? 1 : 2) * q8_shim::compute_units() / (a->kv_heads * p.row_blocks);
-  const double per_root = p.kernel > 0 && p.row_blocks == 1 ? 1.5 : 1.25;
-  const int want = nb <= 10 ? 1 : (int)(per_root * std::sqrt((double)nb));
-  p.splits_max = std::max(1, std::min({want, most, kMaxSplits}));
+  const int root = (int)((p.kernel > 0 && rows <= 64 ? 1.5 : 1.25) * std::sqrt((double)nb));
+  const int one = std::max(1, cus / (a->kv_heads * p.row_blocks));
+  const int two = std::max(1, 2 * cus / (a->kv_heads * p.row_blocks));
+  const int most = p.kernel == 0 || rows > 64 ? one : two;
+  if (nb <= 10) p.splits_max = 1;
+  else if (rows > 64 && nb >= 8 * two) p.splits_max = std::min(two, kMaxSplits);
+  else p.splits_max = std::min({root, most, kMaxSplits});
   p.blocks = (nb + p.splits_max - 1) / p.splits_max;
   p.splits = (nb + p.blocks - 1) / p.blocks;
   return p;

@@ -215,3 +215,12 @@ def test_reference_forms_agree_with_a_second_writing():
     assert R.pack_mask(see).tolist() == [[1], [3], [5], [13], [0]]
     w = np.array([[5, 1, 3, 3, 2, 3, 0]], np.float32)
     assert R.select(w, 7, 4, 1, 1).tolist() == [[0, 2, 3, 6]]
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(16, 8, 128), (64, 2, 64), (256, 64, 128), (32, 1, 64), (1, 1, 128)])
+def test_workspace_does_not_shrink_over_every_rule(Q, C, qh, kvh, d):
+    lengths = sorted({*range(0, 700, 13), *(2 ** i + j for i in range(9, 24) for j in (-257, 0, 31, 999))})
+    for n in (1, 2, 7, 9, 17, 31, 33, 61, 64, 65, 100, 129, 200, 256):
+        c = C.Cache(0x10000, 0x10000, 1 << 24, 1, kvh, d)
+        sizes = [C.attn_tree_workspace_bytes(c, length, n, qh) for length in lengths]
+        assert sizes == sorted(sizes), n

@@ -172,6 +172,31 @@ def test_tree_padding_and_masked_values(gpu, C, n, length):
     check_tree(got, lse, ref)
 
 
+@pytest.mark.parametrize("kvh,d,n,length,kind", [
+    (64, 128, 100, 1210, "tree"), (64, 128, 100, 1210, "padded"), (64, 64, 100, 1210, "tree"),
+    (64, 64, 100, 1210, "chain"), (128, 64, 65, 1405, "padded")])
+def test_tree_many_rows_over_many_blocks(gpu, C, kvh, d, n, length, kind):
+    """Work enough for two row tiles a wave: several row blocks, ragged at both ends."""
+    qh = 256
+    rng = np.random.default_rng(n + d)
+    k, v = make(rng, kvh, d, length, n)
+    q = normal(rng, (n, qh, d), 1.5)
+    parents = R.random_tree(rng, n, pad=n // 4 if kind == "padded" else 0)
+    see = np.tril(np.ones((n, n), bool)) if kind == "chain" else R.tree_see(parents)
+    if kind == "padded":
+        dead = ~see.any(1)
+        assert dead.any()
+        q[dead] = np.nan
+        k[0, length:length + n][dead] = np.nan
+        v[0, length:length + n][dead] = np.inf
+    got = run_tree(gpu, C, k, v, q, see, length, d ** -0.5, mask=None if kind == "chain" else "pack")
+    if kind == "padded":
+        q[dead] = 0
+        k[0, length:length + n][dead] = 0
+        v[0, length:length + n][dead] = 0
+    check_tree(*got, R.attention(q, k[0], v[0], see, length, d ** -0.5))
+
+
 @pytest.mark.parametrize("n,length", [(1, 40), (33, 200), (90, 31)])
 def test_chain_without_a_mask(gpu, C, n, length):
     rng = np.random.default_rng(n)
