@@ -104,8 +104,8 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 // row blocks, splits; kv head fastest, so that 8 kv heads keep to an XCD each); several
 // splits leave (m, l, O) in the workspace and attn_merge combines them in order.
 // 16 query heads over 8 kv heads of 128: 1 node, 300 slots 7 us (one workgroup a kv
-// head: launch, masks, four rounds); 13 nodes, 1024 slots 6.4 and 2.5 for the merge;
-// 61, 8191 14.8 and 4.5; 256, 16384 46 (750 TFLOP/s of both products; MFMA and
+// head: launch, masks, four rounds); 13 nodes, 1024 slots 5.7 and 2.5 for the merge;
+// 61, 8191 13.2 and 5.1; 256, 16384 46 (750 TFLOP/s of both products; MFMA and
 // VALU 39 and 38 % busy, in turn) and 8.0.
 namespace {
 
