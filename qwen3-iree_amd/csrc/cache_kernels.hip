@@ -90,9 +90,9 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 //     f16, and small ones are normal f16 numbers down to 2^-20 of the largest;
 //   O^T += V^T P^T with the weights as they stand in the lanes: the MFMA's 32 k
 //     slots mean slots 4 grp + e, 16 + 4 grp + e, and V^T is read from LDS in
-//     that order (transposing reads).  A weight goes into the product as an f16
-//     (half a step, 2^-11 of itself, at most), up to 32 rows as the sum of two (2^-22):
-//     the bytes bound those, and the second product costs nothing.
+//     that order (transposing reads).  A weight goes into the product as the sum of
+//     two f16 values (2^-22 of itself at most; one alone, 2^-11, would show in the
+//     outputs beside their own rounding).
 // K and V blocks are copied from memory straight into LDS, the next one while one
 // is computed.  RG waves share a block (RG row groups of T tiles:
 // T = 2 halves the reads of LDS, but one tile's rounds are shorter, so it pays only
@@ -103,10 +103,12 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 // The slots are divided into splits of `blocks` blocks (grid: kv heads,
 // row blocks, splits; kv head fastest, so that 8 kv heads keep to an XCD each); several
 // splits leave (m, l, O) in the workspace and attn_merge combines them in order.
-// 16 query heads over 8 kv heads of 128: 1 node, 300 slots 7 us (one workgroup a kv
-// head: launch, masks, four rounds); 13 nodes, 1024 slots 5.7 and 2.5 for the merge;
-// 61, 8191 13.2 and 5.1; 256, 16384 46 (750 TFLOP/s of both products; MFMA and
-// VALU 39 and 38 % busy, in turn) and 8.0.
+// 16 query heads over 8 kv heads of 128 (medians): 1 node, 300 slots 7.0 us (one
+// workgroup a kv head: launch, masks, four rounds); 13 nodes, 1024 slots 7.2 and 3.4
+// for the merge; 61, 8191 16.2 and 5.4; 256, 16384 59.9 (580 TFLOP/s of scores and
+// outputs, the weights' second halves not counted; MFMA and VALU 49 and 43 % busy, in
+// turn) and 8.7.  With one f16 a weight above 32 rows the last was 48.8, at outputs
+// 3.1e-4 relative L2 from the rounded exact ones in place of 0.3e-4.
 namespace {
 
 constexpr float kRefRoom = 6.0f, kRefMax = 10.0f, kSumMax = 16384.0f;
@@ -154,7 +156,6 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
   constexpr int kChunks = D / 8;           // 16-byte chunks of a row
   constexpr int kRowsPerPiece = 64 / kChunks;
   constexpr int kRows = 16 * T * RG;       // rows of a workgroup
-  constexpr bool kLow = T * RG <= 2;       // weights as two f16 values
   // two buffers of each position group's K and V blocks, separate arrays so
   // that the compiler sees that reading one does not wait for copies into another
   __shared__ __attribute__((aligned(1024))) uint8_t k0[PG * kTile], k1[PG * kTile];
@@ -308,16 +309,9 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
         const f16x2 hi = __builtin_convertvector((f32x2_t){p[e], p[e + 1]}, f16x2);
         ph[j][e] = hi.x;
         ph[j][e + 1] = hi.y;
-        if constexpr (kLow) {
-          // f16(p - hi), the difference exact, for both halves
-          uint32_t lo;
-          asm("v_fma_mixlo_f16 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]"
-              : "=v"(lo) : "v"(__builtin_bit_cast(uint32_t, hi)), "v"(p[e]));
-          asm("v_fma_mixhi_f16 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-              : "+v"(lo) : "v"(__builtin_bit_cast(uint32_t, hi)), "v"(p[e + 1]));
-          pl[j][e] = as_f16x2(lo).x;
-          pl[j][e + 1] = as_f16x2(lo).y;
-        }
+        const f16x2 lo = f16_rest(hi, p[e], p[e + 1]);
+        pl[j][e] = lo.x;
+        pl[j][e + 1] = lo.y;
       }
     }
     // A masked weight of 0 times an infinity would reach every row: infinities
@@ -342,13 +336,11 @@ __device__ __forceinline__ void attn_tree(const AttnTreeArgs& A) {
 #pragma unroll
       for (int j = 0; j < T; ++j)
         o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph[j], o[j][d], 0, 0, 0);
-    if constexpr (kLow) {
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d)
+    for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-        for (int j = 0; j < T; ++j)
-          o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl[j], o[j][d], 0, 0, 0);
-    }
+      for (int j = 0; j < T; ++j)
+        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl[j], o[j][d], 0, 0, 0);
     // They go to the rows that see them, value by value.
     if (any) {
 #pragma unroll 1

@@ -91,9 +91,9 @@ constexpr int kMaxSplits = 64;  // one lane each in the merge
 // Rows of a workgroup: a wave's one tile of 16 up to 64 rows, and above them too
 // (several row blocks, whose K and V come out of L2) until every CU has 65 blocks of
 // 64 rows and 32 slots to do; then two tiles a wave.  us a layer (16 query over 8 kv
-// heads of 128), one and two tiles: 61 nodes, 1024 slots 12.0 / 14.4, 8191 22.0 / 23.1;
-// 128, 2048 16.7 / 20.6, 16384 36.4 / 41.4, 30000 66.7 / 57.4; 256, 300 18.2 / 22.1,
-// 6000 33.9 / 38.4, 8191 42.4 / 37.4, 16384 61.3 / 58.8.
+// heads of 128), one and two tiles: 61 nodes, 1024 slots 12.4 / 15.0, 8191 22.8 / 23.8;
+// 128, 2048 16.8 / 20.7, 16384 43.7 / 47.7, 30000 71.6 / 67.2; 256, 300 18.6 / 22.3,
+// 6000 39.5 / 43.0, 8191 47.6 / 44.0, 16384 73.7 / 69.8.
 //
 // Splits of the nb blocks of 32 slots: each costs a partial written and merged,
 // the first one a launch, and each block of a split costs a round of its
@@ -101,13 +101,13 @@ constexpr int kMaxSplits = 64;  // one lane each in the merge
 // and none up to 10 blocks.  With 1 / 4 / 8 / 16 / 32 splits:
 //   1 node, 300 slots (10 blocks) 6.8 / 7.8 / 8.1, 1000 (32) 10.7 / 9.0 / 8.4 / 8.7
 //   / 9.2, 4000 (126) 46.2 / 18.8 / 13.4 / 11.0 / 10.8, 16384 (513) 104 / 36.2 / 23.7
-//   / 20.5 / 20.5 (64: 24.2); 30 nodes, 1024 (33) 19.5 / 11.5 / 10.4 / 10.7 / 11.2; 13
-//   nodes, 8191 (257) 138 / 43.3 / 27.1 / 19.0 / 16.7.
+//   / 20.5 / 20.5 (64: 24.2); 30 nodes, 1024 (33) 20.4 / 11.9 / 10.5 / 11.0 / 11.3; 13
+//   nodes, 8191 (257) 138 / 44.3 / 27.3 / 20.1 / 16.8.
 // At most one workgroup a CU where it takes the CU's LDS (up to 16 rows), else two;
 // above 64 rows as many as fill every CU once, or twice where that leaves each split
-// 8 blocks: 256 nodes, 1024 slots (5 blocks at two) 21.4 at one and 23.8 at two; 128,
-// 2048 16.9 and 19.0; 4000 slots and 256 nodes (17 blocks) 35.9 and 31.4; 8191 and 61
-// (8) 22.8 and 21.5.
+// 8 blocks: 256 nodes, 1024 slots (5 blocks at two) 22.0 at one and 24.9 at two; 128,
+// 2048 16.9 and 19.2; 4000 slots and 256 nodes (17 blocks) 36.5 and 34.1; 8191 and 61
+// (8) 22.7 and 22.9.
 AttnPlan attn_plan(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) {
   const int rows = n * (q_heads / a->kv_heads), cus = q8_shim::compute_units();
   const int nb = (len + n + 31) / 32;

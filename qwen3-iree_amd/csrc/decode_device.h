@@ -93,6 +93,19 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2));
 }
 
+// What the roundings hi of a and b left: f16(a - hi.x) and f16(b - hi.y), the
+// differences exact.  One v_fma_mixlo_f16 and one v_fma_mixhi_f16 (-hi times one
+// plus a, rounded once); the compiler would turn a product with a one that it can
+// see through into three instructions.  Not inline assembly: the compiler counts no
+// wait states behind that, and an MFMA may read a VALU result from the third
+// instruction behind it on.
+__device__ __forceinline__ f16x2 f16_rest(f16x2 hi, float a, float b) {
+  float one = 1.0f;
+  asm("" : "+s"(one));
+  return (f16x2){(_Float16)__builtin_fmaf(-(float)hi.x, one, a),
+                 (_Float16)__builtin_fmaf(-(float)hi.y, one, b)};
+}
+
 __device__ __forceinline__ _Float16 as_half(uint16_t b) { return __builtin_bit_cast(_Float16, b); }
 
 __device__ __forceinline__ uint2 load_global(const uint2* p) {
