@@ -1444,22 +1444,13 @@ extern "C" __global__ __launch_bounds__(256) void pf_attention(
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[d] *= alpha;
     }
-    // hi = f16(p) (pairs at a time, v_cvt_pk_f16_f32), lo = f16(p - hi): p -
-    // hi is exact in f32, so the fused -hi * 1 + p of v_fma_mixlo_f16 /
-    // v_fma_mixhi_f16 (hi's f16 half widened exactly, one rounding to f16 into
-    // the low / high half) gives the same pair as subtracting and converting
+    // hi = f16(p) (pairs at a time, v_cvt_pk_f16_f32), lo = f16(p - hi)
     f16x8 ph, pl;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       typedef float f32x2_t __attribute__((ext_vector_type(2)));
       const f16x2 h2 = __builtin_convertvector((f32x2_t){p[i], p[i + 1]}, f16x2);
-      const uint32_t hb = __builtin_bit_cast(uint32_t, h2);
-      uint32_t lb;
-      asm("v_fma_mixlo_f16 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lb) : "v"(hb), "v"(p[i]));
-      asm("v_fma_mixhi_f16 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-          : "+v"(lb)
-          : "v"(hb), "v"(p[i + 1]));
-      const f16x2 l2 = __builtin_bit_cast(f16x2, lb);
+      const f16x2 l2 = f16_rest(h2, p[i], p[i + 1]);
       ph[i] = h2.x;
       ph[i + 1] = h2.y;
       pl[i] = l2.x;
