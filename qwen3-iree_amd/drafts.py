@@ -125,6 +125,7 @@ class DraftSession(D.DecodeSession):
         tokens = np.ascontiguousarray(tokens, np.int32).reshape(-1)
         if tokens.size == 0 or self.length + tokens.size > self.max_seq:
             raise ValueError(f"{tokens.size} tokens behind {self.length} of {self.max_seq} slots")
+        self._tree = None  # the tokens go where its nodes are
         if self._weights is None and self.length == self.position:
             self.set_state(0, self.length)
             super().prefill_batched(tokens)

@@ -1,0 +1,61 @@
+"""What a DraftSession remembers between its calls, and the calls it refuses, on the CPU:
+the library's calls are recorded in place of being made."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+
+class Words:
+    """Stands for a DeviceBuffer; downloads zeros."""
+
+    ptr, nbytes = 0x10000, 1 << 20
+
+    def __int__(self):
+        return self.ptr
+
+    def upload(self, array, offset=0):
+        pass
+
+    def download(self, dtype, count, offset=0):
+        return np.zeros(count, dtype)
+
+
+@pytest.fixture
+def session(Q, monkeypatch):
+    from qwen3_iree_amd import decode, drafts
+
+    s = object.__new__(drafts.DraftSession)
+    s.model = type("Model", (), {"ref": staticmethod(lambda: None)})()
+    s.max_seq, s.max_nodes, s.length, s.position, s.stream = 100, 8, 20, 20, None
+    s.k_cache = s.v_cache = s.state = s._ws = s._nodes = s.tree_logits = Words()
+    s._q = s._lse = s._weights = s._tree = None
+    s.calls = []
+    monkeypatch.setattr(Q, "_call", lambda name, *a: s.calls.append(name))
+    monkeypatch.setattr(Q, "synchronize", lambda: None)
+    monkeypatch.setattr(decode.DecodeSession, "prefill_batched", lambda self, t: None)
+    return s
+
+
+def test_a_prompt_drops_the_verified_tree(session):
+    s = session
+    s.verify([1, 2, 3], [-1, 0, 0])
+    s.prompt([5, 6, 7, 8])
+    assert s.length == s.position == 24
+    s.calls.clear()
+    with pytest.raises(ValueError, match="no tree"):
+        s.accept([0, 1])
+    assert not s.calls and s.length == 24
+    s.verify([1], [-1])
+    s.accept([0])
+    assert s.calls[-1] == "f16_cache_compact" and s.length == 25
+
+
+def test_a_refused_prompt_keeps_the_tree(session):
+    s = session
+    s.verify([1, 2, 3], [-1, 0, 0])
+    for bad in ([], np.zeros(81)):
+        with pytest.raises(ValueError):
+            s.prompt(bad)
+    s.accept([0, 2])
+    assert s.length == 22
