@@ -51,6 +51,7 @@ struct CompactArgs {
   int64_t src_seq, dst_seq;
   int32_t kv_heads, head_dim, per_head, base, count;
   int32_t range;  // kept slots of one workgroup
+  int32_t in_place;  // source and destination are one
 };
 
 struct GemmArgmaxArgs {

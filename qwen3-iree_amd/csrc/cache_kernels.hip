@@ -1120,8 +1120,12 @@ extern "C" __global__ __launch_bounds__(1024) void cache_select_any(SelectArgs A
 // head_dim / 64 - 1 move 128 bytes of every k row, the next head_dim / 64 the same
 // of v, the last one the weights.  A workgroup walks its slots in order, 256 (of
 // the weights 2048) at a time, and waits until all of them are read before it
-// writes: with ascending slots (keep[j] >= j) and one range, a write never meets a
-// slot that is still to be read, so source and destination may be one.
+// writes.  Source and destination may be one (then with one range): keep ascends
+// strictly, so keep[j] - j never falls, and the entries that move a slot up
+// (keep[j] < j, which takes negative ones in front) come before those that do not.
+// The latter are walked upwards, where a write never meets a slot still to be read,
+// the former, if there are any, downwards; neither part reads or writes a slot of
+// the other's.
 // Bound by the bytes moved, 128 at a time from scattered slots: 28 layers, 4096 of
 // 16384 slots 189 us, 4.95 TB/s read and written; 1024 of 2048 43-51; 512 of one
 // layer 3.3 (two rounds).
@@ -1137,17 +1141,28 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
   const int64_t src_left = A.src_seq - A.base;
   const int j_lo = range * A.range;
   const int j_hi = j_lo + A.range < A.count ? j_lo + A.range : A.count;
+  const int lead = A.in_place ? keep[0] : 0;
+  // the number of entries that move a slot up
+  auto moved_up = [&] {
+    int lo = 0, hi = A.count;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (keep[mid] < mid) lo = mid + 1;
+      else hi = mid;
+    }
+    return lo;
+  };
   if (part == 2 * halves) {
     const float* from = A.w + (int64_t)head * A.src_seq + A.base;
     float* to = A.w_to + (int64_t)head * A.dst_seq + A.base;
-    for (int j0 = j_lo; j0 < j_hi; j0 += 256 * U) {
+    auto round = [&](int j0, int hi, bool up) {
       float x[U];
       bool ok[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + 256 * u + t;
-        const int p = j < j_hi ? keep[j] : -1;
-        ok[u] = p >= 0 && p < src_left;
+        const int p = j < hi ? keep[j] : -1;
+        ok[u] = p >= (A.in_place && !up ? j : 0) && p < src_left;
         x[u] = from[ok[u] ? p : 0];  // (slot base is there: count > 0)
       }
 #pragma unroll
@@ -1156,6 +1171,11 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (ok[u]) to[j0 + 256 * u + t] = x[u];
+    };
+    for (int j0 = j_lo; j0 < j_hi; j0 += 256 * U) round(j0, j_hi, false);
+    if (lead < 0) {
+      const int up = moved_up();
+      for (int j0 = (up - 1) / (256 * U) * (256 * U); j0 >= 0; j0 -= 256 * U) round(j0, up, true);
     }
     return;
   }
@@ -1163,31 +1183,40 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
   const int col = kvh * A.head_dim + 64 * (part % halves) + 8 * (t & 7);
   const uint16_t* from = (part < halves ? A.k : A.v) + (layer * A.src_seq + A.base) * row + col;
   uint16_t* to = (part < halves ? A.k_to : A.v_to) + (layer * A.dst_seq + A.base) * row + col;
-  int next[U];
-  auto places = [&](int j0) {
+  // rounds j0, j0 + step .. that start in [lo, hi)
+  auto walk = [&](int lo, int hi, int j0, int step, bool up) {
+    int next[U];
+    auto places = [&] {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + 32 * u + (t >> 3);
-      next[u] = j < j_hi ? keep[j] : -1;
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + 32 * u + (t >> 3);
+        next[u] = j >= lo && j < hi ? keep[j] : -1;
+      }
+    };
+    places();
+    while (j0 >= lo && j0 < hi) {
+      const int now = j0 + (t >> 3);
+      u32x4 x[U];
+      bool ok[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ok[u] = next[u] >= (A.in_place && !up ? now + 32 * u : 0) && next[u] < src_left;
+        x[u] = load_global(reinterpret_cast<const u32x4*>(from + (ok[u] ? next[u] : 0) * row));
+      }
+      j0 += step;
+      places();
+#pragma unroll
+      for (int u = 0; u < U; ++u) asm volatile("" : "+v"(x[u]));  // the loads are back
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (ok[u]) *reinterpret_cast<u32x4*>(to + (now + 32 * u) * row) = x[u];
     }
   };
-  places(j_lo);
-  for (int j0 = j_lo; j0 < j_hi; j0 += 32 * U) {
-    u32x4 x[U];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      ok[u] = next[u] >= 0 && next[u] < src_left;
-      x[u] = load_global(reinterpret_cast<const u32x4*>(from + (ok[u] ? next[u] : 0) * row));
-    }
-    places(j0 + 32 * U);
-#pragma unroll
-    for (int u = 0; u < U; ++u) asm volatile("" : "+v"(x[u]));  // the loads are back
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (ok[u])
-        *reinterpret_cast<u32x4*>(to + (j0 + 32 * u + (t >> 3)) * row) = x[u];
+  walk(j_lo, j_hi, j_lo, 32 * U, false);
+  if (lead < 0) {
+    const int up = moved_up();
+    walk(0, up, (up - 1) / (32 * U) * (32 * U), -32 * U, true);
   }
 }
 

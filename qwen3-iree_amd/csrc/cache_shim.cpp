@@ -393,7 +393,8 @@ int f16_cache_compact(const f16_cache* src, const f16_cache* dst, const int32_t*
                    per_head ? 1 : 0,
                    base,
                    count,
-                   count};
+                   count,
+                   same ? 1 : 0};
   const int parts = 2 * (src->head_dim / 64) + (weights ? 1 : 0);
   const int heads = src->layers * src->kv_heads;
   int ranges = 1;
