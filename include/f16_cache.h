@@ -78,8 +78,9 @@ int f16_tree_mask(const int32_t* parents, int32_t n, uint32_t* mask, int32_t* de
  * scale finite and positive.  Scores, statistics and sums are f32.
  * workspace: device memory of f16_attn_tree_workspace_bytes (256-byte aligned;
  * may be NULL where that is 0), needed only during the call, nothing to
- * initialise.  The size does not shrink as len grows, so that of max_seq - n
- * serves every call of a session.  Calls that may overlap need one each. */
+ * initialise.  The size does not shrink as len or n grows and covers every call of
+ * fewer rows over as many slots (len + n), so that of max_seq - n and n serves all
+ * calls of up to n rows of a session.  Calls that may overlap need one each. */
 size_t f16_attn_tree_workspace_bytes(const f16_cache* cache, int32_t len, int32_t n,
                                      int32_t q_heads);
 int f16_attn_tree(const f16_cache* cache, int32_t layer, int32_t len, const void* q,

@@ -288,8 +288,9 @@ int qwen3_generate(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t
  * the Q8_0 stacks); results agree with it and with qwen3_decode_step within the
  * step's tolerance.  Only enqueues; len + n <= max_seq, position in [0, 2^24].
  * workspace: device memory of qwen3_tree_workspace_bytes(n, max_seq) bytes (0 for
- * arguments outside the ranges), 256-byte aligned, nothing to initialise.  No
- * counterpart in the reference, which runs one token a step. */
+ * arguments outside the ranges), 256-byte aligned, nothing to initialise; that of
+ * the largest n serves smaller trees too.  No counterpart in the reference, which
+ * runs one token a step. */
 size_t qwen3_tree_workspace_bytes(int32_t n, int64_t max_seq);
 int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t max_seq,
                     const int32_t* tokens, const int32_t* parents, int32_t n, int32_t len,

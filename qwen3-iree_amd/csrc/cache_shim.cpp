@@ -133,6 +133,8 @@ size_t attn_part_floats(const f16_cache* a, int32_t n, int32_t q_heads, int spli
   return (size_t)splits * n * q_heads * a->head_dim;
 }
 
+// What one call needs.  It may be less for more rows: a further row block means fewer
+// splits.
 size_t attn_workspace(const f16_cache* a, const AttnPlan& p, int32_t n, int32_t q_heads) {
   if (p.splits_max == 1) return 0;
   return 4 * (attn_part_floats(a, n, q_heads, p.splits_max) + 2 * (size_t)n * q_heads * p.splits_max);
@@ -202,6 +204,10 @@ int tree_rope(const int32_t* depth, int32_t position, int32_t n, void* table, hi
   return launch(c.rope, (uint32_t)n, 64, args, stream);
 }
 
+size_t attn_tree_need(const f16_cache* a, int32_t len, int32_t n, int32_t q_heads) {
+  return attn_workspace(a, attn_plan(a, len, n, q_heads), n, q_heads);
+}
+
 }  // namespace q8_shim
 
 extern "C" {
@@ -222,7 +228,11 @@ int f16_tree_mask(const int32_t* parents, int32_t n, uint32_t* mask, int32_t* de
 size_t f16_attn_tree_workspace_bytes(const f16_cache* a, int32_t len, int32_t n,
                                      int32_t q_heads) {
   if (check_cache(a, "cache") || check_rows(a, len, n, q_heads, 1 << 20, 1.0f)) return 0;
-  return attn_workspace(a, attn_plan(a, len, n, q_heads), n, q_heads);
+  // the most that any call of up to n rows over as many slots in all needs
+  size_t most = 0;
+  for (int32_t i = 1; i <= n; ++i)
+    most = std::max(most, q8_shim::attn_tree_need(a, len + n - i, i, q_heads));
+  return most;
 }
 
 int f16_attn_tree(const f16_cache* a, int32_t layer, int32_t len, const void* q, int64_t q_stride,

@@ -2643,15 +2643,14 @@ f16_cache model_cache(void* k, void* v, int64_t max_seq) {
   return f16_cache{k, v, nullptr, max_seq, kLayers, (int32_t)kKvHeads, 128};
 }
 
-TreeWorkspace tree_workspace(int32_t n, int64_t max_seq) {
+TreeWorkspace tree_workspace(int32_t n, size_t attn_bytes) {
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  const f16_cache c = model_cache(nullptr, nullptr, max_seq);
   TreeWorkspace t{};
   t.mask = pf_workspace_bytes(n);
   t.depth = t.mask + up((size_t)n * ((n + 31) / 32) * 4);
   t.keys = t.depth + up((size_t)n * 4);
   t.attn = t.keys + up(f16_gemm_argmax_workspace_bytes(n));
-  t.attn_bytes = f16_attn_tree_workspace_bytes(&c, (int32_t)(max_seq - n), n, 16);
+  t.attn_bytes = attn_bytes;
   t.bytes = t.attn + up(t.attn_bytes);
   return t;
 }
@@ -2660,7 +2659,8 @@ TreeWorkspace tree_workspace(int32_t n, int64_t max_seq) {
 
 size_t qwen3_tree_workspace_bytes(int32_t n, int64_t max_seq) {
   if (n < 1 || n > F16_TREE_MAX_NODES || max_seq < n || max_seq > (1LL << 24)) return 0;
-  return tree_workspace(n, max_seq).bytes;
+  const f16_cache c = model_cache(nullptr, nullptr, max_seq);
+  return tree_workspace(n, f16_attn_tree_workspace_bytes(&c, (int32_t)(max_seq - n), n, 16)).bytes;
 }
 
 int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_t max_seq,
@@ -2683,7 +2683,8 @@ int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_
                 (long long)max_seq);
   if (position < 0 || position > (1 << 24))
     return fail(Q8_ERR_BAD_SHAPE, "position %d outside [0, 2^24]", position);
-  const TreeWorkspace t = tree_workspace(n, max_seq);
+  const f16_cache cache = model_cache(k_cache, v_cache, max_seq);
+  const TreeWorkspace t = tree_workspace(n, q8_shim::attn_tree_need(&cache, len, n, 16));
   if (workspace_bytes < t.bytes)
     return fail(Q8_ERR_BAD_SHAPE, "workspace of %zu bytes < %zu needed for %d nodes",
                 workspace_bytes, t.bytes, n);
@@ -2706,8 +2707,7 @@ int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_
     void* args[] = {&tp, &e, &h};
     if ((rc = launch(g.pf_embed, (uint32_t)n, 128, args, st))) return rc;
   }
-  TreeLayer tree{model_cache(k_cache, v_cache, max_seq), mask, nullptr, mb(workspace) + t.attn,
-                 t.attn_bytes};
+  TreeLayer tree{cache, mask, nullptr, mb(workspace) + t.attn, t.attn_bytes};
   bool xn_ready = false;
   for (int l = 0; l < kLayers; ++l) {
     if (q_rows) {

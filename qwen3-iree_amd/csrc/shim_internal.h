@@ -5,7 +5,10 @@
 #define QWEN3_SHIM_INTERNAL_H
 
 #include <hip/hip_runtime_api.h>
+#include <stddef.h>
 #include <stdint.h>
+
+struct f16_cache;
 
 namespace q8_shim {
 
@@ -25,6 +28,9 @@ int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bl
 // leaves the cache operators reporting Q8_ERR_CODE_OBJECT) and unloads it.
 void cache_load(const char* path);
 void cache_unload();
+// The workspace bytes of this one call of f16_attn_tree (arguments in range), at most
+// f16_attn_tree_workspace_bytes.
+size_t attn_tree_need(const f16_cache* cache, int32_t len, int32_t n, int32_t q_heads);
 // The RoPE table of a tree's nodes (tree_rope_k).
 int tree_rope(const int32_t* depth, int32_t position, int32_t n, void* table, hipStream_t stream);
 

@@ -48,8 +48,7 @@ class DraftSession(D.DecodeSession):
         self.length = self.position = 0
         n = self.max_nodes
         lib = Q.load_library()
-        self._ws = Q.DeviceBuffer(max(int(lib.qwen3_tree_workspace_bytes(i, self.max_seq))
-                                      for i in range(1, n + 1)))
+        self._ws = Q.DeviceBuffer(int(lib.qwen3_tree_workspace_bytes(n, self.max_seq)))
         self._nodes = Q.DeviceBuffer(4 * 4 * n)  # tokens, parents, next tokens, path
         self.tree_logits: Q.DeviceBuffer | None = None
         self._q = self._lse = self._weights = None
