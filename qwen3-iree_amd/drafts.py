@@ -36,8 +36,8 @@ class DraftSession(D.DecodeSession):
 
     weights: keep the attention weights eviction goes by; then a prompt is read in
     trees too (chunks of max_nodes tokens), else in one piece.  The calls of a
-    DecodeSession that go by the token and position on the device are refused: they
-    know nothing of `length`."""
+    DecodeSession that go by the token or position on the device, whole steps and
+    their parts, are refused: they know nothing of `length`."""
 
     def __init__(self, model: D.DeviceWeights, max_seq: int, max_nodes: int = 64,
                  weights: bool = True, stream: Q.Stream | None = None):
@@ -65,6 +65,7 @@ class DraftSession(D.DecodeSession):
         raise TypeError("a session of drafted trees moves by prompt, verify and accept")
 
     step = step_checked = capture = replay = prefill = prefill_batched = generate = _refused
+    embed = layer = head = _refused
 
     def _slot(self, i: int) -> int:
         return self._nodes.ptr + 4 * self.max_nodes * i

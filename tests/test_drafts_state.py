@@ -59,3 +59,11 @@ def test_a_refused_prompt_keeps_the_tree(session):
             s.prompt(bad)
     s.accept([0, 2])
     assert s.length == 22
+
+
+def test_every_call_by_the_device_words_is_refused(session):
+    """The parts of a decode step read or write the token or position word too."""
+    for name, args in (("layer", (0, Words(), Words())), ("embed", (Words(),)), ("head", (Words(),))):
+        with pytest.raises(TypeError):
+            getattr(session, name)(*args)
+    assert not session.calls
