@@ -146,7 +146,7 @@ class DraftSession(D.DecodeSession):
         out = [int(token)]
         while len(out) - 1 < max_new and self.length < self.max_seq:
             room = min(self.max_nodes, self.max_seq - self.length) - 1
-            d_tokens, d_parents = draft(out)
+            d_tokens, d_parents = draft(list(out))
             d_tokens, d_parents = list(d_tokens)[:room], list(d_parents)[:room]
             tokens = [out[-1], *d_tokens]
             parents = [-1, *(p + 1 for p in d_parents)]

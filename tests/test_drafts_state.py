@@ -67,3 +67,20 @@ def test_every_call_by_the_device_words_is_refused(session):
         with pytest.raises(TypeError):
             getattr(session, name)(*args)
     assert not session.calls
+
+
+def test_a_draft_may_keep_and_change_its_context(session, monkeypatch):
+    """The tokens so far are the draft's own copy."""
+    s = session
+    monkeypatch.setattr(type(s), "verify", lambda self, t, p: np.arange(100, 100 + len(t)))
+    monkeypatch.setattr(type(s), "accept", lambda self, path: None)
+    seen = []
+
+    def draft(context):
+        seen.append(context)
+        context += [7, 7]
+        return [], []
+
+    out = s.generate_drafted(3, 4, -1, draft)
+    assert out.tolist() == [100] * 4
+    assert seen == [[3, 7, 7], [3, 100, 7, 7], [3, 100, 100, 7, 7], [3, 100, 100, 100, 7, 7]]
