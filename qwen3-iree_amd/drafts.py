@@ -168,9 +168,9 @@ class DraftSession(D.DecodeSession):
         front in order.  Returns the kept slots int32 [28, 8, budget]."""
         if self._weights is None:
             raise ValueError("the session keeps no attention weights")
-        self._tree = None
         with Q.DeviceBuffer(4 * D.LAYERS * D.KV_HEADS * max(int(budget), 1)) as keep:
             C.cache_select(self.cache, self.length, budget, sinks, recent, keep, self.stream)
+            self._tree = None  # the slots move under it
             C.cache_compact(self.cache, self.cache, keep, True, 0, budget, self.stream)
             self.synchronize()
             self.length = int(budget)

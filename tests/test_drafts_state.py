@@ -84,3 +84,44 @@ def test_a_draft_may_keep_and_change_its_context(session, monkeypatch):
     out = s.generate_drafted(3, 4, -1, draft)
     assert out.tolist() == [100] * 4
     assert seen == [[3, 7, 7], [3, 100, 7, 7], [3, 100, 100, 7, 7], [3, 100, 100, 100, 7, 7]]
+
+
+def test_a_refused_eviction_changes_nothing(Q, session, monkeypatch):
+    """The verified tree can still be accepted behind it."""
+    from qwen3_iree_amd import cache as C
+
+    s = session
+    s._weights, s.cache = Words(), None
+
+    class Buffer(Words):
+        def __init__(self, nbytes):
+            pass
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *exc):
+            pass
+
+        def download(self, dtype, count=28 * 8 * 10, offset=0):
+            return np.zeros(count, dtype)
+
+    def select(cache, length, budget, *args):
+        if not 1 <= budget <= length:
+            raise Q.Q8GemvError(6, "budget")
+
+    monkeypatch.setattr(Q, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(C, "cache_select", select)
+    monkeypatch.setattr(C, "cache_compact", lambda *a: None)
+    monkeypatch.setattr(C, "attn_weights_add", lambda *a: None)
+    s.verify([1, 2], [-1, 0])
+    for budget in (0, 21, 10 ** 12):
+        with pytest.raises(Q.Q8GemvError):
+            s.evict(budget)
+    assert s.length == 20
+    s.accept([0])
+    assert s.length == s.position == 21
+    s.verify([1, 2], [-1, 0])
+    assert s.evict(10).shape == (28, 8, 10) and s.length == 10 and s.position == 21
+    with pytest.raises(ValueError, match="no tree"):
+        s.accept([0])
