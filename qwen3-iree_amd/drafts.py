@@ -178,6 +178,8 @@ class DraftSession(D.DecodeSession):
 
     def slot_weights(self) -> np.ndarray:
         """The attention every slot got, f32 [28, 8, length]."""
+        if self._weights is None:
+            raise ValueError("the session keeps no attention weights")
         self.synchronize()
         w = self._weights.download(np.float32).reshape(D.LAYERS, D.KV_HEADS, self.max_seq)
         return w[:, :, :self.length]

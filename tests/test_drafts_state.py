@@ -125,3 +125,10 @@ def test_a_refused_eviction_changes_nothing(Q, session, monkeypatch):
     assert s.evict(10).shape == (28, 8, 10) and s.length == 10 and s.position == 21
     with pytest.raises(ValueError, match="no tree"):
         s.accept([0])
+
+
+def test_weights_that_are_not_kept_are_refused(session):
+    with pytest.raises(ValueError, match="no attention weights"):
+        session.slot_weights()
+    with pytest.raises(ValueError, match="no attention weights"):
+        session.evict(5)
