@@ -75,7 +75,8 @@ int f16_tree_mask(const int32_t* parents, int32_t n, uint32_t* mask, int32_t* de
  * q_heads a multiple of kv_heads, at most 32 times it and at most 256; strides
  * multiples of 8 elements and at least q_heads * head_dim; q and out 16-byte,
  * mask and lse 4-byte aligned; n in [1, 256], len >= 0, len + n <= max_seq;
- * scale finite and positive.  Scores, statistics and sums are f32.
+ * scale finite and positive.  Scores, statistics and sums are f32; a weight enters
+ * its product with v to 2^-22 of itself.
  * workspace: device memory of f16_attn_tree_workspace_bytes (256-byte aligned;
  * may be NULL where that is 0), needed only during the call, nothing to
  * initialise.  The size does not shrink as len or n grows and covers every call of

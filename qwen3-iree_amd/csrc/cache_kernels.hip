@@ -18,7 +18,7 @@ constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 // round r, anc[i] holds the 2^r nearest nodes on the way up (i among them) and
 // jump[i] the node 2^r steps up (-1 behind the root, -2 once padding was met),
 // so ceil(log2 n) rounds close a chain of n nodes.  Latency only, a launch and the
-// rounds' barriers: 1.4 us for 1 node, 1.9 for 13, 3.3-4.6 for 256.
+// rounds' barriers: 1.4 us for 1 node, 1.9 for 13, 3.3-4.8 for 256.
 extern "C" __global__ __launch_bounds__(kTreeMax) void tree_mask_k(
     const int32_t* __restrict__ parents, int n, uint32_t* __restrict__ mask,
     int32_t* __restrict__ depth) {
@@ -104,10 +104,10 @@ extern "C" __global__ __launch_bounds__(64) void tree_rope_k(const int32_t* __re
 // row blocks, splits; kv head fastest, so that 8 kv heads keep to an XCD each); several
 // splits leave (m, l, O) in the workspace and attn_merge combines them in order.
 // 16 query heads over 8 kv heads of 128 (medians): 1 node, 300 slots 7.0 us (one
-// workgroup a kv head: launch, masks, four rounds); 13 nodes, 1024 slots 7.2 and 3.4
-// for the merge; 61, 8191 16.2 and 5.4; 256, 16384 59.9 (580 TFLOP/s of scores and
-// outputs, the weights' second halves not counted; MFMA and VALU 49 and 43 % busy, in
-// turn) and 8.7.  With one f16 a weight above 32 rows the last was 48.8, at outputs
+// workgroup a kv head: launch, masks, four rounds); 13 nodes, 1024 slots 7.1 and 3.5
+// for the merge; 61, 8191 16.0 and 5.6; 256, 16384 57-60 (570-600 TFLOP/s of scores
+// and outputs, the weights' second halves not counted; MFMA and VALU 49 and 43 % busy,
+// in turn) and 8.6.  With one f16 a weight above 32 rows the last was 48.8, at outputs
 // 3.1e-4 relative L2 from the rounded exact ones in place of 0.3e-4.
 namespace {
 
@@ -719,7 +719,7 @@ __device__ __forceinline__ int weight_source(const WeightsArgs& A, int i) {
 }
 
 // Up to 16 NT rows, whose queries stay in registers: bound by the bytes of K,
-// 4.9 TB/s (5 tokens, 16384 slots of 28 layers 191 us; 1 token, 1000 slots 14).
+// 5.0 TB/s (5 tokens, 16384 slots of 28 layers 194 us; 1 token, 1000 slots 15).
 // A wave takes A.blocks consecutive blocks, the next one's keys requested before
 // one is computed.
 template <int D, int NT>
@@ -963,8 +963,8 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 // ballots: nothing depends on an order of arrival.  E = 0 reads the weights again
 // for each of the five passes.
 // Bound by the chain of barriers, then by the passes' instructions, all of a head on
-// one CU: 601 slots of a layer (8 workgroups) 4.3 us, of 28 layers 2048 5.4, 16384
-// 12.8, 30000 26.5, 48000 37.8; E = 0 by the re-reads, 60000 128, 100000 221.
+// one CU: 601 slots of a layer (8 workgroups) 4.3 us, of 28 layers 2048 5.6, 16384
+// 12.8 (20 where the weights come from memory), 30000 26.5, 48000 37.8; E = 0 by the re-reads, 60000 128, 100000 221.
 namespace {
 template <int CTRL, int ROWS = 0xF>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
@@ -1127,8 +1127,8 @@ extern "C" __global__ __launch_bounds__(1024) void cache_select_any(SelectArgs A
 // the former, if there are any, downwards; neither part reads or writes a slot of
 // the other's.
 // Bound by the bytes moved, 128 at a time from scattered slots: 28 layers, 4096 of
-// 16384 slots 189 us, 4.95 TB/s read and written; 1024 of 2048 43-51; 512 of one
-// layer 3.3 (two rounds).
+// 16384 slots 192 us, 4.9 TB/s read and written, in place 199; 1024 of 2048 51, over
+// and over 43 and in place 32; 512 of one layer 3.6 (two rounds).
 extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A) {
   constexpr int U = 8;
   const int t = threadIdx.x;
@@ -1230,9 +1230,9 @@ extern "C" __global__ __launch_bounds__(256) void cache_compact_k(CompactArgs A)
 // out of L2), copied straight into one of NBUF LDS buffers NBUF - 1 stages ahead,
 // on into the workgroup's next tile, so that only its first tile waits for
 // memory.  Lane (c16, g) holds rows 4 g + e of token c16: 8 bytes of logits a
-// store, and the token's best row in two registers.  151,936 rows: 13 tokens 54.6 us
-// (6.0 TB/s), 256 tokens 117 (680 TFLOP/s; 17 of them the logits, which all
-// workgroups store at once).
+// store, and the token's best row in two registers.  151,936 rows: 13 tokens 56 us
+// (5.6 TB/s), 256 tokens 118 (675 TFLOP/s; 17 of them the logits, which all
+// workgroups store at once; 134-140 under a profiler).
 namespace {
 
 // byte offset of row r's 16-byte chunk c (of 8) in a stage: two rows a 256-byte
@@ -1435,7 +1435,7 @@ extern "C" __global__ __launch_bounds__(512) void gemm_argmax_256(GemmArgmaxArgs
 }
 
 // tokens[i] from the workgroups' keys (argmax_key: the larger value, then the
-// lower row; 0: none): a launch and one round trip, 4 us
+// lower row; 0: none): a launch and one round trip, 4-5 us
 extern "C" __global__ __launch_bounds__(64) void gemm_argmax_final(
     const uint64_t* __restrict__ part, int wgs, int32_t* __restrict__ tokens) {
   const int i = blockIdx.x;
