@@ -275,14 +275,13 @@ def _prepare_verify(s, g, rows):
     s["temperature"] = torch.where(torch.rand((seqs,), generator=g, device="cuda") < 0.1,
                                    torch.zeros_like(heat), heat)
     s["uniform"] = torch.rand((rows,), generator=g, device="cuda")
-    # the row whose distribution each drafted token was taken from: the one before it
+    # the rows with a drafted token behind them
     s["from"] = torch.nonzero(s["nth"] < s["counts"][s["seq"]] - 1)[:, 0]
     s["draft"] = None
     if c["draft"]:
-        near = x[s["from"]] + _normal(g, (s["from"].numel(), vocab), 0.7)
-        s["draft"] = torch.softmax(near, 1)
+        s["draft"] = torch.softmax(x + _normal(g, (rows, vocab), 0.7), 1)
         if s["from"].numel():
-            picked = torch.multinomial(s["draft"], 1, generator=g)[:, 0]
+            picked = torch.multinomial(s["draft"][s["from"]], 1, generator=g)[:, 0]
             s["tokens"][s["from"] + 1] = picked.int()
     elif s["from"].numel():
         # what followed in the text: mostly the likeliest token
@@ -413,7 +412,7 @@ def _plain_verify(s):
     told = s["tokens"].long()[row + 1]
     q_told = torch.ones((row.numel(),), dtype=torch.float64, device="cuda")
     if s["draft"] is not None:
-        q_told = torch.gather(s["draft"], 1, told[:, None])[:, 0].double()
+        q_told = s["draft"][row, told].double()
     yes = torch.zeros((seqs, s["most"]), dtype=torch.int64, device="cuda")
     p_told = torch.gather(p[row], 1, told[:, None])[:, 0]
     fine = s["uniform"][row].double() * q_told < p_told
@@ -426,12 +425,11 @@ def _plain_verify(s):
     last = begin[has] + n
     left = p[last]
     refused = n < s["counts"][has] - 1
-    which = torch.searchsorted(row, last).clamp(max=max(0, row.numel() - 1))
     if row.numel():
         if s["draft"] is not None:
-            taken = s["draft"][which].double()
+            taken = s["draft"][last].double()
         else:
-            taken = (at == told[which][:, None]).double()
+            taken = (at == s["tokens"].long()[(last + 1).clamp(max=rows - 1)][:, None]).double()
         rest = torch.clamp(left - taken, min=0.0)
         refused = refused & (rest.sum(1) > 0)
         left = torch.where(refused[:, None], rest, left)
@@ -690,7 +688,7 @@ def _exact_verify(s, counts):
     tokens = torch.full((c["seqs"], wide), -1, dtype=torch.int32)
     accepted = torch.zeros((c["seqs"],), dtype=torch.int32)
     logprob = torch.zeros((c["seqs"], wide), dtype=torch.float64)
-    r = drafted = 0
+    r = 0
     for i, m in enumerate(counts):
         n, done = 0, m == 0
         while not done:
@@ -707,7 +705,7 @@ def _exact_verify(s, counts):
                 q = torch.zeros_like(p)
                 q[t] = 1.0
                 if s["draft"] is not None:
-                    q = s["draft"][drafted + n].double()
+                    q = s["draft"][r + n].double()
                 if u[r + n] * float(q[t]) < float(p[t]):
                     tokens[i, n], logprob[i, n] = t, float(logp[t])
                     n += 1
@@ -722,5 +720,4 @@ def _exact_verify(s, counts):
             done = True
         accepted[i] = n
         r += m
-        drafted += max(0, m - 1)
     return {"tokens": tokens, "accepted": accepted, "logprob": logprob}
