@@ -7,12 +7,15 @@ Modules
            sessions with a KV cache, prompt ingestion, the generation loop, run.
   cache    operators over a KV cache (include/f16_cache.h): attention of drafted
            trees, attention weights, eviction.
+  pages    a paged KV cache of several sequences, f16 or 8-bit, and the verification of
+           drafted tokens (include/kv_pages.h).
   gguf     GGUF v2/v3 reader / writer and Qwen3-0.6B checkpoint ingestion into
            the device layout (no IREE).
   weights  Q8_0 quantisation / stacking (the reference's offline weight prep)
            and seeded synthetic inputs.
   build    hipcc / g++ recipe for lib/q8gemv_gfx950.hsaco, lib/decode_gfx950.hsaco,
-           lib/prefill_gfx950.hsaco, lib/cache_gfx950.hsaco and lib/libq8gemv.so.
+           lib/prefill_gfx950.hsaco, lib/cache_gfx950.hsaco, lib/pages_gfx950.hsaco and
+           lib/libq8gemv.so.
 
 The directory name is not a Python identifier; load it as a package with
 load_package() below (or put this directory on sys.path and import the

@@ -4,8 +4,10 @@
   lib/decode_gfx950.hsaco  the same for csrc/decode_kernels.hip (decode-step kernels)
   lib/prefill_gfx950.hsaco the same for csrc/prefill_kernels.hip (batched prompt ingestion)
   lib/cache_gfx950.hsaco   the same for csrc/cache_kernels.hip (cache operators, vocabulary rows)
-  lib/libq8gemv.so         g++ of csrc/q8gemv_shim.cpp and csrc/cache_shim.cpp and hipcc of
-                           csrc/q8gemv_noalloc.hip, linked against libamdhip64
+  lib/pages_gfx950.hsaco   the same for csrc/pages_kernels.hip (paged cache, draft verification)
+  lib/libq8gemv.so         g++ of csrc/q8gemv_shim.cpp, csrc/cache_shim.cpp and
+                           csrc/pages_shim.cpp and hipcc of csrc/q8gemv_noalloc.hip, linked
+                           against libamdhip64
 
 Both cross-compile without a GPU.  Run as `python qwen3-iree_amd/build.py`.
 """
@@ -26,6 +28,7 @@ CODE_OBJECT = LIB / "q8gemv_gfx950.hsaco"
 DECODE_OBJECT = LIB / "decode_gfx950.hsaco"
 PREFILL_OBJECT = LIB / "prefill_gfx950.hsaco"
 CACHE_OBJECT = LIB / "cache_gfx950.hsaco"
+PAGES_OBJECT = LIB / "pages_gfx950.hsaco"
 SHIM = LIB / "libq8gemv.so"
 
 HIPCC_FLAGS = [
@@ -80,6 +83,12 @@ def build_cache_object() -> Path:
                   ("-mllvm", "-amdgpu-mfma-vgpr-form=1"))
 
 
+def build_pages_object() -> Path:
+    # VGPR results for the same reason
+    return _hsaco(CSRC / "pages_kernels.hip", PAGES_OBJECT,
+                  ("-mllvm", "-amdgpu-mfma-vgpr-form=1"))
+
+
 def build_shim() -> Path:
     """libq8gemv.so: the host shims (g++) plus q8gemv_noalloc.hip (hipcc: host
     code and the device-resident scratch array of the allocation-free entry
@@ -90,7 +99,7 @@ def build_shim() -> Path:
     tmp = SHIM.with_suffix(".so.tmp")
     inc = [f"-I{ROCM / 'include'}", f"-I{REPO / 'include'}", f"-I{CSRC}"]
     with tempfile.TemporaryDirectory() as td:
-        shim_o = [Path(td) / "q8gemv_shim.o", Path(td) / "cache_shim.o"]
+        shim_o = [Path(td) / f"{name}_shim.o" for name in ("q8gemv", "cache", "pages")]
         noalloc_o = Path(td) / "q8gemv_noalloc.o"
         for obj in shim_o:
             _run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-fPIC", "-c",
@@ -113,6 +122,8 @@ OBJECT_SOURCES = {
     "prefill": ("prefill_kernels.hip", "prefill_rows.h", "prefill_split.h", "decode_device.h",
                 "step_roles.h", "q8_device.h"),
     "cache": ("cache_kernels.hip", "cache_args.h", "decode_device.h", "step_roles.h",
+              "q8_device.h"),
+    "pages": ("pages_kernels.hip", "pages_args.h", "decode_device.h", "step_roles.h",
               "q8_device.h"),
 }
 
@@ -170,7 +181,7 @@ def kernel_digest(name: str, code_object: Path = CODE_OBJECT) -> str | None:
 
 def build_all() -> tuple[Path, ...]:
     return (build_code_object(), build_decode_object(), build_prefill_object(),
-            build_cache_object(), build_shim())
+            build_cache_object(), build_pages_object(), build_shim())
 
 
 if __name__ == "__main__":

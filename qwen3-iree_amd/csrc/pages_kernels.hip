@@ -1,0 +1,938 @@
+// Kernels of include/kv_pages.h: rows appended to a paged KV cache, attention over
+// it, rows read back, and the verification of drafted tokens.
+#include "decode_device.h"
+#include "pages_args.h"
+
+namespace {
+
+constexpr float kLn2 = 0.693147180559945309f;
+
+// The sequence of row `row` (the wave's): the last whose start is not behind it, found
+// by counting, 64 starts a load.  lo: its first row, m: how many; -1: none's.
+__device__ __forceinline__ int seq_of_row(const PagesBatch& b, int row, int& lo, int& m) {
+  if (!b.start) {
+    lo = row;
+    m = 1;
+    return row;
+  }
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int i = lane; i - lane <= b.seqs; i += 64)
+    n += __popcll(__builtin_amdgcn_ballot_w64(i <= b.seqs && b.start[i <= b.seqs ? i : 0] <= row));
+  const int s = __builtin_amdgcn_readfirstlane(n) - 1;
+  if (s < 0 || s >= b.seqs) return -1;
+  lo = b.start[s];
+  m = rows_of(b, lo, b.start[s + 1]);
+  return row >= lo && row < lo + m ? s : -1;
+}
+
+// The row of kv head h that holds slot p of sequence s, -1 for none.
+__device__ __forceinline__ int64_t pool_row(const PagesBatch& b, int s, int64_t p, int kv_heads,
+                                            int h) {
+  if (!slot_ok(b, p)) return -1;
+  const int at = page_of_tile(b, (int)p >> 4);
+  const int page = b.table[(int64_t)s * b.table_stride + at];
+  if (!page_ok(b, page)) return -1;
+  return ((int64_t)page * kv_heads + h) * b.page_size + ((int)p - at * b.page_size);
+}
+
+__device__ __forceinline__ float half_at(u32x4 v, int j) {
+  return (float)as_half((uint16_t)(v[j >> 1] >> (16 * (j & 1))));
+}
+
+}  // namespace
+
+// --------------------------------------------------------------- append ----
+//
+// One workgroup a row; D / 8 lanes a head, 8 values each, all of the row's q, k
+// and v heads in turn.  The rotation's partners, dims i and i + D/2, are lanes half a
+// head apart.  The angles' cosines and sines are worked out once a row.
+namespace {
+
+template <int D>
+__device__ __forceinline__ double head_sum(double v) {
+#pragma unroll
+  for (int d = 1; d < D / 8; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+template <int D, bool Q8>
+__device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
+  constexpr int G = D / 8;
+  __shared__ double cs[D / 2], sn[D / 2];
+  const int t = threadIdx.x, c = t % G, row = blockIdx.x;
+  int lo, m;
+  const int s = seq_of_row(A.b, row, lo, m);
+  if (s < 0) return;
+  const int64_t slot = (int64_t)A.b.length[s] - m + (row - lo);
+  if (A.rotate) {
+    if (t < D / 2) {
+      const double turn = (double)(A.positions ? (int64_t)A.positions[row] : slot) * A.turns[t];
+      sincospi(2.0 * (turn - rint(turn)), &sn[t], &cs[t]);
+    }
+    __syncthreads();
+  }
+  const int heads = A.q_heads + 2 * A.kv_heads;
+  for (int h = t / G; h < heads; h += 256 / G) {
+    const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
+    const int hh = is_q ? h : is_v ? h - A.q_heads - A.kv_heads : h - A.q_heads;
+    const uint16_t* from = is_q   ? A.q + row * A.q_stride
+                           : is_v ? A.v + row * A.v_stride
+                                  : A.k + row * A.k_stride;
+    const u32x4 x = load_global(reinterpret_cast<const u32x4*>(from + hh * D + 8 * c));
+    double y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = (double)half_at(x, j);
+    const uint16_t* w = is_v ? nullptr : is_q ? A.q_norm : A.k_norm;
+    if (w) {
+      double ss = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
+      const double r = 1.0 / sqrt(head_sum<D>(ss) / D + A.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (double)(float)as_half(w[8 * c + j]);
+    }
+    if (A.rotate && !is_v) {
+      const bool second = c >= G / 2;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = (8 * c + j) % (D / 2);
+        const double other = __shfl_xor(y[j], G / 2);
+        y[j] = second ? y[j] * cs[i] + other * sn[i] : y[j] * cs[i] - other * sn[i];
+      }
+    }
+    auto packed = [&] {
+      u32x4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = pack_f16x2((float)y[2 * j], (float)y[2 * j + 1]);
+      return o;
+    };
+    if (is_q) {
+      *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + hh * D + 8 * c) = packed();
+      continue;
+    }
+    const int64_t to = pool_row(A.b, s, slot, A.kv_heads, hh);
+    void* pool = is_v ? A.v_to : A.k_to;
+    if constexpr (Q8) {
+      double top = 0.0;
+      bool fine = true;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        top = fmax(top, fabs(y[j]));
+        fine = fine && fabs(y[j]) < __builtin_inf();
+      }
+      if (!fine) top = __builtin_inf();
+#pragma unroll
+      for (int d = 1; d < G; d <<= 1) top = fmax(top, __shfl_xor(top, d));
+      const bool real = top < __builtin_inf();
+      const float scale = real ? (float)(top / 127.0) : __builtin_nanf("");
+      uint2 code = {0, 0};
+      if (real && scale > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          double q = rint(y[j] / (double)scale);
+          q = fmin(fmax(q, -127.0), 127.0);
+          (j < 4 ? code.x : code.y) |= ((uint32_t)(int)q & 255u) << (8 * (j & 3));
+        }
+      }
+      if (to >= 0) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + to * D + 8 * c) = code;
+        if (c == 0) (is_v ? A.v_scale : A.k_scale)[to] = scale;
+      }
+    } else {
+      if (to >= 0) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(pool) + to * D + 8 * c) = packed();
+    }
+  }
+}
+
+}  // namespace
+
+#define PAGES_APPEND(D, N, Q8)                                                   \
+  extern "C" __global__ __launch_bounds__(256) void pages_append_##D##_##N(      \
+      PagesAppendArgs A) {                                                       \
+    pages_append<D, Q8>(A);                                                      \
+  }
+PAGES_APPEND(64, f16, false)
+PAGES_APPEND(64, q8, true)
+PAGES_APPEND(128, f16, false)
+PAGES_APPEND(128, q8, true)
+
+// ------------------------------------------------------------ attention ----
+//
+// The rows of one kv head are its query heads' rows of a sequence's m new rows, r =
+// group i + head, in tiles of 16.  A wave works on blocks of 32 slots without LDS, K and
+// V straight from memory into registers:
+//   S^T = K Q^T (v_mfma_f32_16x16x32_f16: exact products, f32 sums): lane (c16, grp)
+//     holds the scores of row c16 at slots 4 grp + e and 16 + 4 grp + e, e < 4;
+//   weights 2^(s - m) against a reference m per row, which is set kRefRoom
+//     below the first block's maximum and moves only when the sum of a lane's 8
+//     weights passes kSumMax;
+//   O^T += V^T P^T with the weights as they stand in the lanes: the product's 32 k
+//     slots mean slots 4 grp + e, 16 + 4 grp + e.  A lane reads those 8 slots' dims
+//     (D/16) c16 .. + D/16 - 1 and pairs them up by byte permutes; MFMA n of the
+//     D / 16 makes the dims (D/16) i + n.
+// A weight goes into the product as the sum of two f16 values (2^-22 of itself).
+// 8-bit codes become f16 multiples of 2^-9, exact; a row's k scale multiplies its
+// score and its v scale its weight, so that the reference is that of s + log2 v_scale.
+namespace {
+
+constexpr float kRefRoom = 6.0f, kRefMax = 10.0f, kSumMax = 16384.0f;
+constexpr float kCodeUnit = 512.0f;    // codes stand in the products as code / 512
+constexpr float kLeastLogScale = -64.0f;  // values below 2^-57 leave no trace in an f16
+
+// 0x00b200b1 for two bytes, as f16 numbers u 2^-24, times 2^15 less 128 2^-9
+__device__ __forceinline__ f16x2 code_pair(uint32_t bytes) {
+  const f16x2 u = __builtin_bit_cast(f16x2, bytes);
+  const f16x2 a = {(_Float16)32768.0f, (_Float16)32768.0f}, b = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_elementwise_fma(u, a, b);
+}
+// 8 codes in order
+__device__ __forceinline__ f16x8 code8(uint32_t lo, uint32_t hi) {
+  lo ^= 0x80808080u;
+  hi ^= 0x80808080u;
+  const f16x2 a = code_pair(__builtin_amdgcn_perm(0, lo, 0x0c010c00)),
+              b = code_pair(__builtin_amdgcn_perm(0, lo, 0x0c030c02)),
+              c = code_pair(__builtin_amdgcn_perm(0, hi, 0x0c010c00)),
+              d = code_pair(__builtin_amdgcn_perm(0, hi, 0x0c030c02));
+  return (f16x8){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+__device__ __forceinline__ uint32_t special_bits(uint32_t b) {
+  return ((b & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+
+// Words of global memory, W at a time.
+template <int W>
+struct Words {
+  uint32_t w[W];
+};
+template <int W>
+__device__ __forceinline__ Words<W> load_words(const uint8_t* p) {
+  typedef uint32_t V __attribute__((ext_vector_type(W)));
+  Words<W> r;
+  if constexpr (W == 1) {
+    r.w[0] = *(const GLOBAL_AS uint32_t*)p;
+  } else {
+    const V v = *(const GLOBAL_AS V*)p;
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = v[i];
+  }
+  return r;
+}
+
+template <int D, bool Q8, int T>
+struct AttnWave {
+  static constexpr int kBytes = Q8 ? D : 2 * D;  // of a row
+  static constexpr int kK = kBytes / 64;         // 16-byte pieces of a lane's K row share
+  static constexpr int kV = kBytes / 64;         // words of a lane's V row share
+  struct Block {
+    u32x4 k[2][kK];
+    Words<kV> v[8];
+    f32x4 ks[2], vs[2];
+    int ok;  // bit nt: the 16 slots' page is one
+    int b;
+  };
+
+  const PagesAttnArgs& A;
+  const int s, kvh, lane, c16, grp;
+  f16x8 qf[T][D / 32];
+  int seen[T];
+  float m[T], l[T];
+  f32x4 o[T][D / 16];
+
+  __device__ __forceinline__ AttnWave(const PagesAttnArgs& A, int s, int kvh)
+      : A(A), s(s), kvh(kvh), lane(threadIdx.x & 63), c16(lane & 15), grp((lane >> 4) & 3) {}
+
+  // Q as the B operand: column c16 is row row0 + 16 j + c16, its dims as K's lanes
+  // hold theirs
+  __device__ __forceinline__ void start(int lo, int rows, int length, int row0) {
+    const int R = rows * A.group;
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      int r = row0 + 16 * j + c16;
+      r = r < R ? r : R - 1;
+      const int i = A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv);
+      seen[j] = slots_seen(A.b, length, rows, i);
+      const uint16_t* q = A.q + (int64_t)(lo + i) * A.q_stride +
+                          (kvh * A.group + r - i * A.group) * D;
+#pragma unroll
+      for (int st = 0; st < D / 32; ++st) {
+        const int dim = Q8 ? 64 * (st >> 1) + 16 * grp + 8 * (st & 1) : 32 * st + 8 * grp;
+        qf[j][st] =
+            __builtin_bit_cast(f16x8, load_global(reinterpret_cast<const u32x4*>(q + dim)));
+      }
+      m[j] = -__builtin_inff();
+      l[j] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[j][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+
+  // The pool row of the first of slots 16 tile .. + 15; 0 with ok = false for none.
+  __device__ __forceinline__ int64_t tile_row(int tile, bool& ok) const {
+    ok = tile < A.b.slots >> 4;
+    int page = 0, entry = 0;
+    if (ok) {
+      const int at = page_of_tile(A.b, tile);
+      page = __builtin_amdgcn_readfirstlane(A.b.table[(int64_t)s * A.b.table_stride + at]);
+      entry = 16 * (tile - at * A.b.tiles);
+      ok = page_ok(A.b, page);
+      if (!ok) page = entry = 0;
+    }
+    return ((int64_t)page * A.kv_heads + kvh) * A.b.page_size + entry;
+  }
+
+  __device__ __forceinline__ void request(Block& x, int b) const {
+    x.b = b;
+    x.ok = 0;
+    const uint8_t *kb = static_cast<const uint8_t*>(A.k), *vb = static_cast<const uint8_t*>(A.v);
+    const uint8_t* vt[2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      bool ok;
+      const int64_t row = tile_row(2 * b + nt, ok);
+      x.ok |= ok << nt;
+      const uint8_t* kt = kb + row * kBytes;
+      vt[nt] = vb + row * kBytes;
+#pragma unroll
+      for (int i = 0; i < kK; ++i)
+        x.k[nt][i] = load_global(
+            reinterpret_cast<const u32x4*>(kt + c16 * kBytes + 64 * i + 16 * grp));
+      if constexpr (Q8) {
+        x.ks[nt] = *(const GLOBAL_AS f32x4*)(A.k_scale + row + 4 * grp);
+        x.vs[nt] = *(const GLOBAL_AS f32x4*)(A.v_scale + row + 4 * grp);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x.v[e] = load_words<kV>(vt[e >> 2] + (4 * grp + (e & 3)) * kBytes + 4 * kV * c16);
+  }
+
+  // The lane's slots 4 grp + e, 16 + 4 grp + e that row j sees, bits 0 .. 7.
+  __device__ __forceinline__ int sees(const Block& x, int j) const {
+    int bits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      bits |= (32 * x.b + 16 * (e >> 2) + 4 * grp + (e & 3) < seen[j] && (x.ok >> (e >> 2) & 1)) << e;
+    return bits;
+  }
+
+  // unmasked: the slots that every row of the wave sees
+  __device__ __forceinline__ void block(Block& x, int unmasked) {
+    const bool masked = 32 * x.b + 32 > unmasked || x.ok != 3;
+    f16x8 kf[2][D / 32];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int st = 0; st < D / 32; ++st) {
+        if constexpr (Q8)
+          kf[nt][st] = code8(x.k[nt][st >> 1][2 * (st & 1)], x.k[nt][st >> 1][2 * (st & 1) + 1]);
+        else
+          kf[nt][st] = __builtin_bit_cast(f16x8, x.k[nt][st]);
+      }
+    f16x8 vf[D / 16];
+    bool any = false;
+    if constexpr (Q8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < kV; ++i) x.v[e].w[i] ^= 0x80808080u;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        f16x2 p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p[e] = code_pair(__builtin_amdgcn_perm(x.v[2 * e + 1].w[d >> 2], x.v[2 * e].w[d >> 2],
+                                                 0x0c000c00u | (4 + (d & 3)) << 16 | (d & 3)));
+        vf[d] = (f16x8){p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+      }
+    } else {
+      // A masked weight of 0 times an infinity would reach every row: infinities and
+      // NaN are left out of the product.
+      if (masked) {
+        uint32_t special = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int i = 0; i < kV; ++i) special |= special_bits(x.v[e].w[i]);
+        any = __builtin_amdgcn_ballot_w64(special != 0) != 0;
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+              const uint32_t one = special_bits(x.v[e].w[i]) >> 15;
+              x.v[e].w[i] &= ~((one << 16) - one);
+            }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        u32x4 p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p[e] = __builtin_amdgcn_perm(x.v[2 * e + 1].w[d >> 1], x.v[2 * e].w[d >> 1],
+                                       d & 1 ? 0x07060302u : 0x05040100u);
+        vf[d] = __builtin_bit_cast(f16x8, p);
+      }
+    }
+    f16x8 ph[T], pl[T];
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      f32x4 sc[2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        sc[nt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < D / 32; ++st)
+          sc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[nt][st], qf[j][st], sc[nt], 0, 0, 0);
+      }
+      float sv[8], vs[8];  // scores in base-2 units, v scales
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sv[e] = sc[e >> 2][e & 3] * A.scale;
+        vs[e] = 1.0f;
+        if constexpr (Q8) {
+          sv[e] *= x.ks[e >> 2][e & 3] * kCodeUnit;
+          vs[e] = x.vs[e >> 2][e & 3];
+        }
+      }
+      if (masked) {
+        const int bits = sees(x, j);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!(bits >> e & 1)) {
+            sv[e] = -__builtin_inff();
+            vs[e] = 0.0f;
+          }
+      }
+      // p: weights; pv: times the v scales, what goes into the product
+      float p[8], pv[8];
+      auto weigh = [&](float ref) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(sv[e] - ref);
+          pv[e] = Q8 ? p[e] * vs[e] : p[e];
+        }
+        return ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
+      };
+      float sum = weigh(m[j]);
+      if (__builtin_amdgcn_ballot_w64(!(sum <= kSumMax)) != 0) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          mx = fmaxf(mx, Q8 ? sv[e] + fmaxf(__builtin_amdgcn_logf(vs[e]), kLeastLogScale) : sv[e]);
+        mx = max_col4(mx);
+        const bool grow = mx > m[j] + kRefMax;
+        const float mn = grow ? mx - kRefRoom : m[j];
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m[j] - mn) : 1.0f;
+        // every score so far masked: reference 0, weights 2^-inf = 0
+        sum = weigh(mn == -__builtin_inff() ? 0.0f : mn);
+        l[j] *= alpha;
+        m[j] = mn;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[j][d] *= alpha;
+      }
+      if constexpr (Q8)
+        l[j] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      else
+        l[j] += sum;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        typedef float f32x2_t __attribute__((ext_vector_type(2)));
+        const f16x2 hi = __builtin_convertvector((f32x2_t){pv[e], pv[e + 1]}, f16x2);
+        ph[j][e] = hi.x;
+        ph[j][e + 1] = hi.y;
+        const f16x2 lo = f16_rest(hi, pv[e], pv[e + 1]);
+        pl[j][e] = lo.x;
+        pl[j][e + 1] = lo.y;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph[j], o[j][d], 0, 0, 0);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl[j], o[j][d], 0, 0, 0);
+    // The infinities and NaN left out go to the rows that see them, value by value.
+    if constexpr (!Q8) {
+      if (any) {
+#pragma unroll 1
+        for (int e = 0; e < 32; ++e) {
+          bool ok;
+          const int64_t row = tile_row(2 * x.b + (e >> 4), ok) + (e & 15);
+          if (!ok) continue;
+          const uint16_t* v = static_cast<const uint16_t*>(A.v) + row * D + D / 4 * grp;
+#pragma unroll
+          for (int j = 0; j < T; ++j) {
+            if (32 * x.b + e >= seen[j]) continue;
+#pragma unroll
+            for (int d = 0; d < D / 4; ++d) {
+              const uint16_t w = v[d];
+              if ((w & 0x7c00u) == 0x7c00u)
+                o[j][d % (D / 16)][d / (D / 16)] += (float)as_half(w);
+            }
+          }
+        }
+      }
+    }
+  }
+};
+
+// One workgroup: a sequence's rows 16 T rb .. of one kv head over all slots, its four
+// waves taking blocks in turn and meeting in LDS.
+template <int D, bool Q8, int T>
+__device__ __forceinline__ void pages_attn(const PagesAttnArgs& A) {
+  constexpr int kStride = D + 4;
+  __shared__ float so[4][16][kStride];
+  __shared__ float sm[4][16 * T], sl[4][16 * T];
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = blockIdx.x, rb = blockIdx.y, s = blockIdx.z;
+  const int lo = A.b.start ? A.b.start[s] : s;
+  const int rows = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
+  const int R = rows * A.group, row0 = 16 * T * rb;
+  if (row0 >= R) return;
+  const int length = A.b.length[s];
+  const int last = (row0 + 16 * T < R ? row0 + 16 * T : R) - 1;
+  auto node = [&](int r) { return A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv); };
+  const int unmasked = slots_seen(A.b, length, rows, node(row0));
+  const int nb = (slots_seen(A.b, length, rows, node(last)) + 31) >> 5;
+  typedef AttnWave<D, Q8, T> Wave;
+  Wave w(A, s, kvh);
+  typename Wave::Block x;
+  w.start(lo, rows, length, row0);
+  for (int b = wave; b < nb; b += 4) {
+    w.request(x, b);
+    w.block(x, unmasked);
+  }
+#pragma unroll
+  for (int j = 0; j < T; ++j) {
+    const float l = sum_col4(w.l[j]);
+    if (w.grp == 0) {
+      sm[wave][16 * j + w.c16] = w.m[j];
+      sl[wave][16 * j + w.c16] = l;
+    }
+  }
+  // row j of a tile and 8 (or 4) of its dims a thread
+  constexpr int kDims = D / 16;
+  const int row = t >> 4, d0 = kDims * (t & 15);
+#pragma unroll
+  for (int j = 0; j < T; ++j) {
+    if (j > 0) __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int d = 0; d < D / 16; d += 4)
+        *reinterpret_cast<f32x4*>(&so[wave][w.c16][D / 4 * w.grp + D / 16 * e + d]) =
+            (f32x4){w.o[j][d][e], w.o[j][d + 1][e], w.o[j][d + 2][e], w.o[j][d + 3][e]};
+    __syncthreads();
+    float M = -__builtin_inff(), L = 0.0f, f[4], sum[kDims];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) M = fmaxf(M, sm[g][16 * j + row]);
+    const float ref = M == -__builtin_inff() ? 0.0f : M;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f[g] = __builtin_amdgcn_exp2f(sm[g][16 * j + row] - ref);
+      L += sl[g][16 * j + row] * f[g];
+    }
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      sum[d] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) sum[d] += so[g][row][d0 + d] * f[g];
+    }
+    const int r = row0 + 16 * j + row;
+    if (r >= R) continue;
+    const int i = node(r), h = kvh * A.group + r - i * A.group;
+    const bool none = L == 0.0f;  // no slot, or none with a weight
+    const float inv = none ? 0.0f : (Q8 ? kCodeUnit : 1.0f) / L;
+    uint32_t packed[kDims / 2];
+#pragma unroll
+    for (int d = 0; d < kDims / 2; ++d)
+      packed[d] = none ? 0u : pack_f16x2(sum[2 * d] * inv, sum[2 * d + 1] * inv);
+    uint16_t* to = A.out + (int64_t)(lo + i) * A.out_stride + h * D + d0;
+    if constexpr (D == 128)
+      *reinterpret_cast<u32x4*>(to) = (u32x4){packed[0], packed[1], packed[2], packed[3]};
+    else
+      *reinterpret_cast<uint2*>(to) = make_uint2(packed[0], packed[1]);
+    if (A.lse && (t & 15) == 0)
+      A.lse[(int64_t)(lo + i) * A.q_heads + h] =
+          none ? -__builtin_inff() : kLn2 * (M + __builtin_amdgcn_logf(L));
+  }
+}
+
+}  // namespace
+
+#define PAGES_ATTN(D, N, Q8, T)                                                        \
+  extern "C" __global__ __launch_bounds__(256, T == 4 ? 1 : 2) void                    \
+      pages_attn_##D##_##N##_##T(PagesAttnArgs A) {                                    \
+    pages_attn<D, Q8, T>(A);                                                           \
+  }
+#define PAGES_ATTN_T(D, N, Q8) PAGES_ATTN(D, N, Q8, 1) PAGES_ATTN(D, N, Q8, 2) PAGES_ATTN(D, N, Q8, 4)
+PAGES_ATTN_T(64, f16, false)
+PAGES_ATTN_T(64, q8, true)
+PAGES_ATTN_T(128, f16, false)
+PAGES_ATTN_T(128, q8, true)
+
+// ------------------------------------------------------------------ read ----
+//
+// A wave a row and layer, 8 values a lane at a time: bound by memory, one read of the
+// pages and one write.
+namespace {
+
+template <int D, bool Q8>
+__device__ __forceinline__ void pages_read(const PagesReadArgs& A) {
+  const int lane = threadIdx.x & 63, layer = blockIdx.y;
+  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (row >= A.b.rows) return;
+  int lo, m;
+  const int s = seq_of_row(A.b, row, lo, m);
+  if (s < 0) return;
+  const int64_t slot = (int64_t)A.b.length[s] - m + (row - lo);
+  const int64_t rows = (int64_t)layer * A.b.pages * A.kv_heads * A.b.page_size;
+  const int64_t to = layer * A.layer_stride + row * A.row_stride;
+  for (int c = lane; c < A.kv_heads * (D / 8); c += 64) {
+    int64_t at = pool_row(A.b, s, slot, A.kv_heads, c / (D / 8));
+    const bool ok = at >= 0;
+    at += rows;
+    const int d = 8 * (c % (D / 8));
+    auto copy = [&](const void* from, const float* scale, uint16_t* out) {
+      u32x4 v = {0, 0, 0, 0};
+      if (ok) {
+        if constexpr (Q8) {
+          const uint2 code = load_global(
+              reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(from) + at * D + d));
+          const float f = scale[at];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t w = (j < 2 ? code.x : code.y) >> (16 * (j & 1));
+            v[j] = pack_f16x2((float)(int8_t)w * f, (float)(int8_t)(w >> 8) * f);
+          }
+        } else {
+          v = load_global(
+              reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(from) + at * D + d));
+        }
+      }
+      *reinterpret_cast<u32x4*>(out + to + 8 * c) = v;
+    };
+    if (A.k_out) copy(A.k, A.k_scale, A.k_out);
+    if (A.v_out) copy(A.v, A.v_scale, A.v_out);
+  }
+}
+
+}  // namespace
+
+#define PAGES_READ(D, N, Q8)                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void pages_read_##D##_##N(PagesReadArgs A) {      \
+    pages_read<D, Q8>(A);                                                                        \
+  }
+PAGES_READ(64, f16, false)
+PAGES_READ(64, q8, true)
+PAGES_READ(128, f16, false)
+PAGES_READ(128, q8, true)
+
+// ---------------------------------------------------------------- verify ----
+//
+// verify_sums_k: a chunk of one row, its maximum, the maximum's lowest index and the
+// sum of exp((x - maximum) / T).  verify_rest_k: every workgroup of a sequence joins
+// its rows' chunks, finds the row that decides and sums max(p - q, 0) and p over its
+// chunk of it.  verify_take_k: the chunk and the index whose running sum passes the
+// random number, and the outputs.  All in f64: next to a border of the running sums, one
+// in 151936, f32 sums would give other tokens.
+namespace {
+
+struct RowStat {
+  double total;
+  float top;
+  int first;
+};
+
+__device__ __forceinline__ float logit(uint16_t b) {
+  const float x = (float)as_half(b);
+  return x == x ? x : -__builtin_inff();
+}
+// exp((x - top) / T) with inv_heat = 1 / T
+__device__ __forceinline__ double weight(float x, float top, double inv_heat) {
+  return x == top ? 1.0 : exp(((double)x - (double)top) * inv_heat);
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+__device__ __forceinline__ float heat_of(const VerifyArgs& A, int s) {
+  return A.temperature ? A.temperature[s] : 1.0f;
+}
+
+// The rows of sequence s joined from their chunks into st, and how many drafted tokens
+// stand; every thread of the 256 gets that number.
+__device__ __forceinline__ int verify_join(const VerifyArgs& A, int s, int lo, int m, float heat,
+                                           RowStat* st, int* stop) {
+  const int t = threadIdx.x, lane = t & 63;
+  const double inv = 1.0 / (double)heat;
+  if (t == 0) *stop = m - 1;
+  for (int i = t >> 6; i < m; i += 4) {
+    const int64_t at = (int64_t)(lo + i) * A.chunks;
+    float top = -__builtin_inff();
+    for (int c = lane; c < A.chunks; c += 64) top = fmaxf(top, A.tops[at + c]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    double total = 0.0;
+    int first = 0x7fffffff;
+    for (int c = lane; c < A.chunks; c += 64) {
+      const float x = A.tops[at + c];
+      if (x == -__builtin_inff()) continue;
+      if (x == top && A.firsts[at + c] < first) first = A.firsts[at + c];
+      if (heat > 0.0f) total += A.sums[at + c] * weight(x, top, inv);
+    }
+    total = wave_sum64(total);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      const int other = __shfl_xor(first, d);
+      first = other < first ? other : first;
+    }
+    if (lane == 0) st[i] = {heat > 0.0f ? total : 1.0, top, first};
+  }
+  __syncthreads();
+  if (t < m - 1) {
+    const int x = A.tokens[lo + t + 1];
+    bool yes = false;
+    if (x >= 0 && x < A.vocab && st[t].top > -__builtin_inff()) {
+      const float v = logit(A.logits[(int64_t)(lo + t) * A.logits_stride + x]);
+      const double p = heat > 0.0f ? (v == -__builtin_inff() ? 0.0 : weight(v, st[t].top, inv) / st[t].total)
+                                   : (x == st[t].first ? 1.0 : 0.0);
+      double q = 1.0;
+      if (A.draft) {
+        const float d = A.draft[(int64_t)(lo + t) * A.draft_stride + x];
+        q = d > 0.0f ? (double)d : 0.0;
+      }
+      yes = (double)A.uniform[lo + t] * q < p;
+    }
+    if (!yes) atomicMin(stop, t);
+  }
+  __syncthreads();
+  return *stop;
+}
+
+// What an entry of the deciding row weighs: max(p - q, 0) and p.
+struct Decide {
+  RowStat st;
+  double inv_heat, inv_total;
+  bool greedy, refused, drafted;
+  int told;  // the refused token
+  __device__ __forceinline__ void operator()(int j, uint16_t bits, float d, double& rest,
+                                             double& p) const {
+    const float x = logit(bits);
+    if (greedy) p = j == st.first ? 1.0 : 0.0;
+    else p = x == -__builtin_inff() ? 0.0 : weight(x, st.top, inv_heat) * inv_total;
+    if (!refused) rest = 0.0;
+    else if (drafted) rest = d > 0.0f ? fmax(p - (double)d, 0.0) : p;
+    else rest = j == told ? 0.0 : p;
+  }
+};
+
+__device__ __forceinline__ Decide decide(const VerifyArgs& A, int lo, int m, int n, float heat,
+                                         const RowStat& st) {
+  Decide d;
+  d.st = st;
+  d.greedy = !(heat > 0.0f);
+  d.inv_heat = 1.0 / (double)heat;
+  d.inv_total = 1.0 / st.total;
+  d.refused = n < m - 1;
+  d.drafted = A.draft != nullptr;
+  d.told = d.refused ? A.tokens[lo + n + 1] : -1;
+  return d;
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void verify_sums_k(VerifyArgs A) {
+  __shared__ float tops[4];
+  __shared__ int firsts[4];
+  __shared__ double sums[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int chunk = blockIdx.x, row = blockIdx.y;
+  int lo, m;
+  const int s = seq_of_row(A.b, row, lo, m);
+  if (s < 0) return;
+  const float heat = heat_of(A, s);
+  const uint16_t* x = A.logits + (int64_t)row * A.logits_stride;
+  const int begin = chunk * kVerifyChunk;
+  const int end = begin + kVerifyChunk < A.vocab ? begin + kVerifyChunk : A.vocab;
+  float top = -__builtin_inff();
+  int first = 0x7fffffff;
+  for (int j = begin + t; j < end; j += 256) {
+    const float v = logit(x[j]);
+    if (v > top) {
+      top = v;
+      first = j;
+    }
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const float v = __shfl_xor(top, d);
+    const int f = __shfl_xor(first, d);
+    if (v > top || (v == top && f < first)) {
+      top = v;
+      first = f;
+    }
+  }
+  if (lane == 0) {
+    tops[wave] = top;
+    firsts[wave] = first;
+  }
+  __syncthreads();
+  top = tops[0];
+  first = firsts[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w)
+    if (tops[w] > top || (tops[w] == top && firsts[w] < first)) {
+      top = tops[w];
+      first = firsts[w];
+    }
+  double sum = 0.0;
+  if (heat > 0.0f && top > -__builtin_inff()) {
+    const double inv = 1.0 / (double)heat;
+    for (int j = begin + t; j < end; j += 256) {
+      const float v = logit(x[j]);
+      if (v > -__builtin_inff()) sum += weight(v, top, inv);
+    }
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (t == 0) {
+    const int64_t at = (int64_t)row * A.chunks + chunk;
+    A.tops[at] = top;
+    A.firsts[at] = first;
+    A.sums[at] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
+}
+
+extern "C" __global__ __launch_bounds__(256) void verify_rest_k(VerifyArgs A) {
+  __shared__ RowStat st[256];
+  __shared__ int stop;
+  __shared__ double sums[4][2];
+  const int t = threadIdx.x, chunk = blockIdx.x, s = blockIdx.y;
+  const int lo = A.b.start ? A.b.start[s] : s;
+  const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
+  if (m == 0) return;
+  const float heat = heat_of(A, s);
+  const int n = verify_join(A, s, lo, m, heat, st, &stop);
+  const Decide w = decide(A, lo, m, n, heat, st[n]);
+  const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
+  const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
+  const int begin = chunk * kVerifyChunk;
+  const int end = begin + kVerifyChunk < A.vocab ? begin + kVerifyChunk : A.vocab;
+  double rest = 0.0, all = 0.0;
+  if (w.st.top > -__builtin_inff())
+    for (int j = begin + t; j < end; j += 256) {
+      double r, p;
+      w(j, x[j], q ? q[j] : 0.0f, r, p);
+      rest += r;
+      all += p;
+    }
+  rest = wave_sum64(rest);
+  all = wave_sum64(all);
+  if ((t & 63) == 0) {
+    sums[t >> 6][0] = rest;
+    sums[t >> 6][1] = all;
+  }
+  __syncthreads();
+  if (t < 2)
+    A.rest[((int64_t)s * A.chunks + chunk) * 2 + t] =
+        (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
+}
+
+extern "C" __global__ __launch_bounds__(256) void verify_take_k(VerifyArgs A) {
+  __shared__ RowStat st[256];
+  __shared__ int stop, found, last;
+  __shared__ double run[256];
+  const int t = threadIdx.x, s = blockIdx.x;
+  const int lo = A.b.start ? A.b.start[s] : s;
+  const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
+  int n = 0, token = -1;
+  const float heat = heat_of(A, s);
+  if (m > 0) {
+    n = verify_join(A, s, lo, m, heat, st, &stop);
+    const Decide w = decide(A, lo, m, n, heat, st[n]);
+    if (w.st.top > -__builtin_inff()) {
+      const double* sums = A.rest + (int64_t)s * A.chunks * 2;
+      double total[2] = {0.0, 0.0};
+      for (int c = 0; c < A.chunks; ++c) {
+        total[0] += sums[2 * c];
+        total[1] += sums[2 * c + 1];
+      }
+      const int k = w.refused && total[0] > 0.0 ? 0 : 1;
+      const double goal = (double)A.uniform[lo + m - 1] * total[k];
+      // the chunk whose running sum passes the goal, else the last that weighs anything
+      int chunk = -1;
+      double before = 0.0, sum = 0.0;
+      for (int c = 0; c < A.chunks; ++c) {
+        const double here = sums[2 * c + k];
+        if (here > 0.0) {
+          chunk = c;
+          before = sum;
+          if (sum + here > goal) break;
+        }
+        sum += here;
+      }
+      if (chunk >= 0) {
+        const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
+        const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
+        const int begin = chunk * kVerifyChunk;
+        const int end = begin + kVerifyChunk < A.vocab ? begin + kVerifyChunk : A.vocab;
+        constexpr int kEach = kVerifyChunk / 256;
+        const int j0 = begin + t * kEach, j1 = j0 + kEach < end ? j0 + kEach : end;
+        double mine = 0.0;
+        int some = -1;
+        for (int j = j0; j < j1; ++j) {
+          double v[2];
+          w(j, x[j], q ? q[j] : 0.0f, v[0], v[1]);
+          mine += v[k];
+          if (v[k] > 0.0) some = j;
+        }
+        run[t] = mine;
+        if (t == 0) {
+          found = 0x7fffffff;
+          last = -1;
+        }
+        __syncthreads();
+        double c = before;
+        for (int i = 0; i < t; ++i) c += run[i];
+        for (int j = j0; j < j1; ++j) {
+          double v[2];
+          w(j, x[j], q ? q[j] : 0.0f, v[0], v[1]);
+          c += v[k];
+          if (v[k] > 0.0 && c > goal) {
+            atomicMin(&found, j);
+            break;
+          }
+        }
+        if (some >= 0) atomicMax(&last, some);
+        __syncthreads();
+        token = found < end ? found : last;
+      }
+    }
+  }
+  if (t == 0) A.accepted[s] = n;
+  for (int i = t; i < A.b.max_rows; i += 256) {
+    const int x = i < n ? A.tokens[lo + i + 1] : i == n ? token : -1;
+    A.out[s * A.out_stride + i] = x;
+    if (A.logprob) {
+      float lp = 0.0f;
+      if (x >= 0 && heat > 0.0f) {
+        const float v = logit(A.logits[(int64_t)(lo + i) * A.logits_stride + x]);
+        lp = (float)((v == st[i].top ? 0.0 : ((double)v - (double)st[i].top) / (double)heat) -
+                     log(st[i].total));
+      }
+      A.logprob[s * A.out_stride + i] = lp;
+    }
+  }
+}

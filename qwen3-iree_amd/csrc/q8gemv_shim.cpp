@@ -440,20 +440,25 @@ int q8gemv_init(const char* code_object_path) {
       }
     }
   }
-  // and the cache operators' kernels in a fourth
-  {
+  // and the cache operators' kernels in a fourth, the paged cache's in a fifth
+  const struct {
+    const char* name;
+    void (*load)(const char*);
+  } others[] = {{"/cache_gfx950.hsaco", q8_shim::cache_load},
+                {"/pages_gfx950.hsaco", q8_shim::pages_load}};
+  for (auto& o : others) {
     const size_t slash = path.rfind('/');
     std::string dir = slash == std::string::npos ? std::string(".") : path.substr(0, slash);
-    std::string cpath = dir + "/cache_gfx950.hsaco";
+    std::string cpath = dir + o.name;
     FILE* cf = std::fopen(cpath.c_str(), "rb");
     if (!cf) {
       std::string lib = default_code_object();
-      cpath = lib.substr(0, lib.rfind('/')) + "/cache_gfx950.hsaco";
+      cpath = lib.substr(0, lib.rfind('/')) + o.name;
       cf = std::fopen(cpath.c_str(), "rb");
     }
     if (cf) {
       std::fclose(cf);
-      q8_shim::cache_load(cpath.c_str());
+      o.load(cpath.c_str());
     }
   }
   int cus = 0;
@@ -527,6 +532,7 @@ void q8gemv_shutdown(void) {
   g.vocab = g.vocab_finalize = g.argmax = g.ws_reset = g.copy = nullptr;
   g.calib_empty = g.calib_handoff = g.calib_chase = g.read = nullptr;
   q8_shim::cache_unload();
+  q8_shim::pages_unload();
   g.ready = false;
 }
 

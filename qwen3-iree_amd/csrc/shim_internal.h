@@ -1,6 +1,6 @@
 // Internal interface between the C-ABI shim (q8gemv_shim.cpp), the cache
-// operators (cache_shim.cpp) and the allocation-free entry point
-// (q8gemv_noalloc.hip); not part of the ABI.
+// operators (cache_shim.cpp), the paged cache's (pages_shim.cpp) and the
+// allocation-free entry point (q8gemv_noalloc.hip); not part of the ABI.
 #ifndef QWEN3_SHIM_INTERNAL_H
 #define QWEN3_SHIM_INTERNAL_H
 
@@ -28,6 +28,9 @@ int launch3(hipFunction_t fn, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bl
 // leaves the cache operators reporting Q8_ERR_CODE_OBJECT) and unloads it.
 void cache_load(const char* path);
 void cache_unload();
+// The same of pages_shim.cpp and its code object.
+void pages_load(const char* path);
+void pages_unload();
 // The workspace bytes of this one call of f16_attn_tree (arguments in range), at most
 // f16_attn_tree_workspace_bytes.
 size_t attn_tree_need(const f16_cache* cache, int32_t len, int32_t n, int32_t q_heads);

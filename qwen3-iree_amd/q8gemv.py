@@ -202,7 +202,19 @@ _CACHE_SIGNATURES = {
     "f16_gemm_argmax_workspace_bytes": [ctypes.c_int32],
     "f16_gemm_argmax": [_P, _I64, _P, ctypes.c_int32, _P, _P, _P, _P],
 }
+# include/kv_pages.h
+_PAGES_SIGNATURES = {
+    "kv_pages_append": [_P, ctypes.c_int32, _P, _P, _P],
+    "kv_pages_attn_workspace_bytes": [_P, _P, ctypes.c_int32],
+    "kv_pages_attn": [_P, ctypes.c_int32, _P, _P, _I64, ctypes.c_int32, ctypes.c_float, _P, _I64,
+                      _P, _P, _SZ, _P],
+    "kv_pages_read": [_P, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _I64, _I64, _P],
+    "kv_verify_workspace_bytes": [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32],
+    "kv_verify": [_P, _P, _SZ, _P],
+}
 _RESTYPES = {
+    "kv_pages_attn_workspace_bytes": _SZ,
+    "kv_verify_workspace_bytes": _SZ,
     "qwen3_tree_workspace_bytes": _SZ,
     "f16_attn_tree_workspace_bytes": _SZ,
     "f16_gemm_argmax_workspace_bytes": _SZ,
@@ -232,7 +244,8 @@ def load_library(path: str | Path | None = None) -> ctypes.CDLL:
         if not p.exists():
             raise Q8GemvError(Q8_ERR_CODE_OBJECT, f"{p} is not built (run qwen3-iree_amd/build.py)")
         L = ctypes.CDLL(str(p))
-        for name, argtypes in (*_SIGNATURES.items(), *_CACHE_SIGNATURES.items()):
+        for name, argtypes in (*_SIGNATURES.items(), *_CACHE_SIGNATURES.items(),
+                               *_PAGES_SIGNATURES.items()):
             fn = getattr(L, name)
             fn.argtypes = argtypes
             fn.restype = _RESTYPES.get(name, _I)
