@@ -68,7 +68,11 @@ struct PagesAttnArgs {
   int64_t q_stride, out_stride;
   int32_t q_heads, kv_heads, group;
   uint32_t group_inv;  // ceil(2^32 / group): r / group for group > 1, r < 2^13
-  float scale;         // with log2 e: scores in base-2 units
+  uint32_t scale_bits; // f32: with log2 e, and with the unit of codes in the products
+  int32_t workers;     // workgroups of a kv head and row block
+  int32_t* count;      // [row blocks, kv heads, workers] parts that have arrived
+  float* part;         // [row blocks, kv heads, workers, 2, rows, head_dim]
+  float* part_ml;      // the same with 2: their references and sums
 };
 
 struct PagesReadArgs {
@@ -80,6 +84,7 @@ struct PagesReadArgs {
   int32_t kv_heads;
 };
 
+constexpr int kSeqsMax = 1024;
 constexpr int kVerifyChunk = 8192;  // logits of a workgroup
 
 struct VerifyArgs {

@@ -176,6 +176,8 @@ PAGES_APPEND(128, q8, true)
 // score and its v scale its weight, so that the reference is that of s + log2 v_scale.
 namespace {
 
+#define CONST_AS __attribute__((address_space(4)))
+
 constexpr float kRefRoom = 6.0f, kRefMax = 10.0f, kSumMax = 16384.0f;
 constexpr float kCodeUnit = 512.0f;    // codes stand in the products as code / 512
 constexpr float kLeastLogScale = -64.0f;  // values below 2^-57 leave no trace in an f16
@@ -225,23 +227,31 @@ struct AttnWave {
   static constexpr int kBytes = Q8 ? D : 2 * D;  // of a row
   static constexpr int kK = kBytes / 64;         // 16-byte pieces of a lane's K row share
   static constexpr int kV = kBytes / 64;         // words of a lane's V row share
+  // Where the two tiles of 16 slots of block b are: rows of the pool; bit nt of ok: the
+  // tile's page is one.
+  struct Place {
+    int64_t row0, row1;
+    int ok, b;
+    __device__ __forceinline__ int64_t row(int nt) const { return nt ? row1 : row0; }
+  };
   struct Block {
     u32x4 k[2][kK];
     Words<kV> v[8];
     f32x4 ks[2], vs[2];
-    int ok;  // bit nt: the 16 slots' page is one
-    int b;
   };
 
   const PagesAttnArgs& A;
-  const int s, kvh, lane, c16, grp;
+  const int kvh, lane, c16, grp;
+  const float scale;
+  const CONST_AS int32_t* table;  // the sequence's
   f16x8 qf[T][D / 32];
   int seen[T];
   float m[T], l[T];
   f32x4 o[T][D / 16];
 
-  __device__ __forceinline__ AttnWave(const PagesAttnArgs& A, int s, int kvh)
-      : A(A), s(s), kvh(kvh), lane(threadIdx.x & 63), c16(lane & 15), grp((lane >> 4) & 3) {}
+  __device__ __forceinline__ AttnWave(const PagesAttnArgs& A, int kvh)
+      : A(A), kvh(kvh), lane(threadIdx.x & 63), c16(lane & 15), grp(lane >> 4),
+        scale(__uint_as_float(A.scale_bits)) {}
 
   // Q as the B operand: column c16 is row row0 + 16 j + c16, its dims as K's lanes
   // hold theirs
@@ -268,48 +278,53 @@ struct AttnWave {
     }
   }
 
-  // The pool row of the first of slots 16 tile .. + 15; 0 with ok = false for none.
+  // The pool row of slot 16 tile; ok = false (and a row of page 0) for none.
   __device__ __forceinline__ int64_t tile_row(int tile, bool& ok) const {
     ok = tile < A.b.slots >> 4;
-    int page = 0, entry = 0;
-    if (ok) {
-      const int at = page_of_tile(A.b, tile);
-      page = __builtin_amdgcn_readfirstlane(A.b.table[(int64_t)s * A.b.table_stride + at]);
-      entry = 16 * (tile - at * A.b.tiles);
-      ok = page_ok(A.b, page);
-      if (!ok) page = entry = 0;
-    }
+    const int at = page_of_tile(A.b, ok ? tile : 0);
+    int page = table[at], entry = 16 * (tile - at * A.b.tiles);
+    ok = ok && page_ok(A.b, page);
+    if (!ok) page = entry = 0;
     return ((int64_t)page * A.kv_heads + kvh) * A.b.page_size + entry;
   }
+  __device__ __forceinline__ Place place(int b, int nb) const {  // b = -1 from block nb on
+    Place p;
+    p.b = b < nb ? b : -1;
+    b = b < nb ? b : 0;
+    bool ok0, ok1;
+    p.row0 = tile_row(2 * b, ok0);
+    p.row1 = tile_row(2 * b + 1, ok1);
+    p.ok = ok0 | ok1 << 1;
+    return p;
+  }
 
-  __device__ __forceinline__ void request(Block& x, int b) const {
-    x.b = b;
-    x.ok = 0;
-    const uint8_t *kb = static_cast<const uint8_t*>(A.k), *vb = static_cast<const uint8_t*>(A.v);
-    const uint8_t* vt[2];
+  __device__ __forceinline__ void request_k(Block& x, const Place& p) const {
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
-      bool ok;
-      const int64_t row = tile_row(2 * b + nt, ok);
-      x.ok |= ok << nt;
-      const uint8_t* kt = kb + row * kBytes;
-      vt[nt] = vb + row * kBytes;
+      const uint8_t* kt = static_cast<const uint8_t*>(A.k) + p.row(nt) * kBytes;
 #pragma unroll
       for (int i = 0; i < kK; ++i)
         x.k[nt][i] = load_global(
-            reinterpret_cast<const u32x4*>(kt + c16 * kBytes + 64 * i + 16 * grp));
-      if constexpr (Q8) {
-        x.ks[nt] = *(const GLOBAL_AS f32x4*)(A.k_scale + row + 4 * grp);
-        x.vs[nt] = *(const GLOBAL_AS f32x4*)(A.v_scale + row + 4 * grp);
-      }
+            reinterpret_cast<const u32x4*>(kt + (uint32_t)(c16 * kBytes + 64 * i + 16 * grp)));
+      if constexpr (Q8)
+        x.ks[nt] = *(const GLOBAL_AS f32x4*)(A.k_scale + p.row(nt) + (uint32_t)(4 * grp));
+    }
+  }
+  __device__ __forceinline__ void request_v(Block& x, const Place& p) const {
+    const uint8_t* vb = static_cast<const uint8_t*>(A.v);
+    if constexpr (Q8) {
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+        x.vs[nt] = *(const GLOBAL_AS f32x4*)(A.v_scale + p.row(nt) + (uint32_t)(4 * grp));
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      x.v[e] = load_words<kV>(vt[e >> 2] + (4 * grp + (e & 3)) * kBytes + 4 * kV * c16);
+      x.v[e] = load_words<kV>(vb + p.row(e >> 2) * kBytes +
+                              (uint32_t)((4 * grp + (e & 3)) * kBytes + 4 * kV * c16));
   }
 
   // The lane's slots 4 grp + e, 16 + 4 grp + e that row j sees, bits 0 .. 7.
-  __device__ __forceinline__ int sees(const Block& x, int j) const {
+  __device__ __forceinline__ int sees(const Place& x, int j) const {
     int bits = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -317,88 +332,65 @@ struct AttnWave {
     return bits;
   }
 
-  // unmasked: the slots that every row of the wave sees
-  __device__ __forceinline__ void block(Block& x, int unmasked) {
-    const bool masked = 32 * x.b + 32 > unmasked || x.ok != 3;
-    f16x8 kf[2][D / 32];
+  // V as the A operand of dims (D/16) i + d
+  __device__ __forceinline__ f16x8 v_frag(const Block& x, int d) const {
+    if constexpr (Q8) {
+      f16x2 p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        p[e] = code_pair(__builtin_amdgcn_perm(x.v[2 * e + 1].w[d >> 2], x.v[2 * e].w[d >> 2],
+                                               0x0c000c00u | (4 + (d & 3)) << 16 | (d & 3)));
+      return (f16x8){p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+    } else {
+      u32x4 p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        p[e] = __builtin_amdgcn_perm(x.v[2 * e + 1].w[d >> 1], x.v[2 * e].w[d >> 1],
+                                     d & 1 ? 0x07060302u : 0x05040100u);
+      return __builtin_bit_cast(f16x8, p);
+    }
+  }
+
+  // Block x at `here`; the registers of its K and of its V are filled again with those at
+  // `next` (if b >= 0) as soon as they have been used.  unmasked: the slots that every
+  // row of the wave sees.
+  __device__ __forceinline__ void block(Block& x, const Place& here, const Place& next,
+                                        int unmasked) {
+    const bool masked = 32 * here.b + 32 > unmasked || here.ok != 3;
+    f16x8 ph[T], pl[T];
+    f32x4 sc[T][2];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int st = 0; st < D / 32; ++st) {
+        f16x8 kf;
         if constexpr (Q8)
-          kf[nt][st] = code8(x.k[nt][st >> 1][2 * (st & 1)], x.k[nt][st >> 1][2 * (st & 1) + 1]);
+          kf = code8(x.k[nt][st >> 1][2 * (st & 1)], x.k[nt][st >> 1][2 * (st & 1) + 1]);
         else
-          kf[nt][st] = __builtin_bit_cast(f16x8, x.k[nt][st]);
-      }
-    f16x8 vf[D / 16];
-    bool any = false;
-    if constexpr (Q8) {
+          kf = __builtin_bit_cast(f16x8, x.k[nt][st]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < kV; ++i) x.v[e].w[i] ^= 0x80808080u;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        f16x2 p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          p[e] = code_pair(__builtin_amdgcn_perm(x.v[2 * e + 1].w[d >> 2], x.v[2 * e].w[d >> 2],
-                                                 0x0c000c00u | (4 + (d & 3)) << 16 | (d & 3)));
-        vf[d] = (f16x8){p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
-      }
-    } else {
-      // A masked weight of 0 times an infinity would reach every row: infinities and
-      // NaN are left out of the product.
-      if (masked) {
-        uint32_t special = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int i = 0; i < kV; ++i) special |= special_bits(x.v[e].w[i]);
-        any = __builtin_amdgcn_ballot_w64(special != 0) != 0;
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int i = 0; i < kV; ++i) {
-              const uint32_t one = special_bits(x.v[e].w[i]) >> 15;
-              x.v[e].w[i] &= ~((one << 16) - one);
-            }
-        }
+        for (int j = 0; j < T; ++j)
+          sc[j][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              kf, qf[j][st], st == 0 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : sc[j][nt], 0, 0, 0);
       }
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        u32x4 p;
+    for (int nt = 0; nt < 2; ++nt) {
+      f32x4 f = {scale, scale, scale, scale};
+      if constexpr (Q8) f *= x.ks[nt];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          p[e] = __builtin_amdgcn_perm(x.v[2 * e + 1].w[d >> 1], x.v[2 * e].w[d >> 1],
-                                       d & 1 ? 0x07060302u : 0x05040100u);
-        vf[d] = __builtin_bit_cast(f16x8, p);
-      }
+      for (int j = 0; j < T; ++j) sc[j][nt] *= f;
     }
-    f16x8 ph[T], pl[T];
+    if (next.b >= 0) request_k(x, next);
 #pragma unroll
     for (int j = 0; j < T; ++j) {
-      f32x4 sc[2];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        sc[nt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int st = 0; st < D / 32; ++st)
-          sc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[nt][st], qf[j][st], sc[nt], 0, 0, 0);
-      }
       float sv[8], vs[8];  // scores in base-2 units, v scales
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        sv[e] = sc[e >> 2][e & 3] * A.scale;
-        vs[e] = 1.0f;
-        if constexpr (Q8) {
-          sv[e] *= x.ks[e >> 2][e & 3] * kCodeUnit;
-          vs[e] = x.vs[e >> 2][e & 3];
-        }
+        sv[e] = sc[j][e >> 2][e & 3];
+        vs[e] = Q8 ? x.vs[e >> 2][e & 3] : 1.0f;
       }
       if (masked) {
-        const int bits = sees(x, j);
+        const int bits = sees(here, j);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (!(bits >> e & 1)) {
@@ -448,28 +440,60 @@ struct AttnWave {
         pl[j][e + 1] = lo.y;
       }
     }
+    bool any = false;
+    if constexpr (Q8) {
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d)
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int j = 0; j < T; ++j)
-        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph[j], o[j][d], 0, 0, 0);
+        for (int i = 0; i < kV; ++i) x.v[e].w[i] ^= 0x80808080u;
+    } else {
+      // A masked weight of 0 times an infinity would reach every row: infinities and
+      // NaN are left out of the product.
+      if (masked) {
+        uint32_t special = 0;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d)
+        for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int j = 0; j < T; ++j)
-        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pl[j], o[j][d], 0, 0, 0);
+          for (int i = 0; i < kV; ++i) special |= special_bits(x.v[e].w[i]);
+        any = __builtin_amdgcn_ballot_w64(special != 0) != 0;
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+              const uint32_t one = special_bits(x.v[e].w[i]) >> 15;
+              x.v[e].w[i] &= ~((one << 16) - one);
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; d += 2) {
+      const f16x8 v0 = v_frag(x, d), v1 = v_frag(x, d + 1);
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[j], o[j][d], 0, 0, 0);
+        o[j][d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[j], o[j][d + 1], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+        o[j][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[j], o[j][d], 0, 0, 0);
+        o[j][d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[j], o[j][d + 1], 0, 0, 0);
+      }
+    }
+    if (next.b >= 0) request_v(x, next);
     // The infinities and NaN left out go to the rows that see them, value by value.
     if constexpr (!Q8) {
       if (any) {
 #pragma unroll 1
         for (int e = 0; e < 32; ++e) {
           bool ok;
-          const int64_t row = tile_row(2 * x.b + (e >> 4), ok) + (e & 15);
+          const int64_t row = tile_row(2 * here.b + (e >> 4), ok) + (e & 15);
           if (!ok) continue;
           const uint16_t* v = static_cast<const uint16_t*>(A.v) + row * D + D / 4 * grp;
 #pragma unroll
           for (int j = 0; j < T; ++j) {
-            if (32 * x.b + e >= seen[j]) continue;
+            if (32 * here.b + e >= seen[j]) continue;
 #pragma unroll
             for (int d = 0; d < D / 4; ++d) {
               const uint16_t w = v[d];
@@ -483,77 +507,93 @@ struct AttnWave {
   }
 };
 
-// One workgroup: a sequence's rows 16 T rb .. of one kv head over all slots, its four
-// waves taking blocks in turn and meeting in LDS.
+// Partial results go between workgroups, which may sit on different XCDs: past the L2s.
+__device__ __forceinline__ void put_pair(float* p, float a, float b) {
+  const uint64_t v = __float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_pair(const float* p) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int other = __shfl_up(v, d);
+    if ((int)(threadIdx.x & 63) >= d) v += other;
+  }
+  return v;
+}
+
+// The work of a kv head and row block is the sequences' slots, in rounds of 128 (a block for
+// each of the four waves), one sequence behind the other.  The grid's `workers`
+// workgroups take equal shares of the rounds.  A sequence that lies in one share is
+// finished there; of one that is cut each part leaves its (m, l, O) in the workspace,
+// and the workgroup that comes last puts them together, in order.
 template <int D, bool Q8, int T>
 __device__ __forceinline__ void pages_attn(const PagesAttnArgs& A) {
-  constexpr int kStride = D + 4;
+  constexpr int kRows = 16 * T, kDims = D / 16, kStride = D + 4;
   __shared__ float so[4][16][kStride];
-  __shared__ float sm[4][16 * T], sl[4][16 * T];
-  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int kvh = blockIdx.x, rb = blockIdx.y, s = blockIdx.z;
-  const int lo = A.b.start ? A.b.start[s] : s;
-  const int rows = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
-  const int R = rows * A.group, row0 = 16 * T * rb;
-  if (row0 >= R) return;
-  const int length = A.b.length[s];
-  const int last = (row0 + 16 * T < R ? row0 + 16 * T : R) - 1;
-  auto node = [&](int r) { return A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv); };
-  const int unmasked = slots_seen(A.b, length, rows, node(row0));
-  const int nb = (slots_seen(A.b, length, rows, node(last)) + 31) >> 5;
-  typedef AttnWave<D, Q8, T> Wave;
-  Wave w(A, s, kvh);
-  typename Wave::Block x;
-  w.start(lo, rows, length, row0);
-  for (int b = wave; b < nb; b += 4) {
-    w.request(x, b);
-    w.block(x, unmasked);
-  }
-#pragma unroll
-  for (int j = 0; j < T; ++j) {
-    const float l = sum_col4(w.l[j]);
-    if (w.grp == 0) {
-      sm[wave][16 * j + w.c16] = w.m[j];
-      sl[wave][16 * j + w.c16] = l;
+  __shared__ float sm[4][kRows], sl[4][kRows];
+  __shared__ int ends[kSeqsMax], totals[4], arrived;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  const int kvh = blockIdx.x, rb = blockIdx.y, me = blockIdx.z;
+  const int row0 = kRows * rb;
+  auto node = [&A](int r) { return A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv); };
+  auto first_row = [&](int s) { return A.b.start ? A.b.start[s] : s; };
+  auto row_count = [&](int s, int lo) { return A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1; };
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  auto blocks = [&](int rows, int length) {  // of 32 slots that this row block sees
+    const int R = rows * A.group;
+    const int last = (row0 + kRows < R ? row0 + kRows : R) - 1;
+    return (slots_seen(A.b, length, rows, node(last)) + 31) >> 5;
+  };
+
+  // the sequences' running sums of rounds; one round at least where there are rows
+  int sum = 0;
+  for (int s0 = 0; s0 < A.b.seqs; s0 += 256) {
+    const int s = s0 + t;
+    int n = 0;
+    if (s < A.b.seqs) {
+      const int rows = row_count(s, first_row(s));
+      if (row0 < rows * A.group) {
+        n = (blocks(rows, A.b.length[s]) + 3) >> 2;
+        n = n > 0 ? n : 1;
+      }
     }
-  }
-  // row j of a tile and 8 (or 4) of its dims a thread
-  constexpr int kDims = D / 16;
-  const int row = t >> 4, d0 = kDims * (t & 15);
-#pragma unroll
-  for (int j = 0; j < T; ++j) {
-    if (j > 0) __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int d = 0; d < D / 16; d += 4)
-        *reinterpret_cast<f32x4*>(&so[wave][w.c16][D / 4 * w.grp + D / 16 * e + d]) =
-            (f32x4){w.o[j][d][e], w.o[j][d + 1][e], w.o[j][d + 2][e], w.o[j][d + 3][e]};
+    n = wave_scan(n);
+    if (lane == 63) totals[wave] = n;
     __syncthreads();
-    float M = -__builtin_inff(), L = 0.0f, f[4], sum[kDims];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) M = fmaxf(M, sm[g][16 * j + row]);
-    const float ref = M == -__builtin_inff() ? 0.0f : M;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f[g] = __builtin_amdgcn_exp2f(sm[g][16 * j + row] - ref);
-      L += sl[g][16 * j + row] * f[g];
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) n += totals[w];
     }
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) {
-      sum[d] = 0.0f;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) sum[d] += so[g][row][d0 + d] * f[g];
-    }
-    const int r = row0 + 16 * j + row;
-    if (r >= R) continue;
+    if (s < A.b.seqs) ends[s] = sum + n;
+    sum += (totals[0] + totals[1]) + (totals[2] + totals[3]);
+    __syncthreads();
+  }
+  sum = uniform(sum);
+  const int share = uniform((int)((uint32_t)(sum + A.workers - 1) / (uint32_t)A.workers));
+  const int begin = me * share, end = begin + share < sum ? begin + share : sum;
+  if (begin >= end) return;
+  int s = 0;
+  for (int i = lane; i - lane < A.b.seqs; i += 64)
+    s += __popcll(__builtin_amdgcn_ballot_w64(i < A.b.seqs && ends[i < A.b.seqs ? i : 0] <= begin));
+  s = uniform(s);
+
+  typedef AttnWave<D, Q8, T> Wave;
+  Wave w(A, kvh);
+  const int row = t >> 4, d0 = kDims * (t & 15);  // of a tile, in the sums below
+  auto write = [=, &A](int r, int lo, float M, float L, const float (&o)[kDims]) {
     const int i = node(r), h = kvh * A.group + r - i * A.group;
     const bool none = L == 0.0f;  // no slot, or none with a weight
     const float inv = none ? 0.0f : (Q8 ? kCodeUnit : 1.0f) / L;
     uint32_t packed[kDims / 2];
 #pragma unroll
     for (int d = 0; d < kDims / 2; ++d)
-      packed[d] = none ? 0u : pack_f16x2(sum[2 * d] * inv, sum[2 * d + 1] * inv);
+      packed[d] = none ? 0u : pack_f16x2(o[2 * d] * inv, o[2 * d + 1] * inv);
     uint16_t* to = A.out + (int64_t)(lo + i) * A.out_stride + h * D + d0;
     if constexpr (D == 128)
       *reinterpret_cast<u32x4*>(to) = (u32x4){packed[0], packed[1], packed[2], packed[3]};
@@ -562,6 +602,162 @@ __device__ __forceinline__ void pages_attn(const PagesAttnArgs& A) {
     if (A.lse && (t & 15) == 0)
       A.lse[(int64_t)(lo + i) * A.q_heads + h] =
           none ? -__builtin_inff() : kLn2 * (M + __builtin_amdgcn_logf(L));
+  };
+  // worker x's first or last cut sequence of this head and row block
+  const int head0 = (rb * A.kv_heads + kvh) * A.workers;
+  auto part_at = [=](int x, bool opens) { return (int64_t)(2 * (head0 + x) + (opens ? 1 : 0)) * kRows; };
+
+  for (int at = begin; at < end; ++s) {
+    const int from = s ? uniform(ends[s - 1]) : 0, to = uniform(ends[s]);
+    if (from == to) continue;
+    const int till = to < end ? to : end;
+    const int lo = uniform(first_row(s)), rows = uniform(row_count(s, lo));
+    const int length = uniform(A.b.length[s]), R = rows * A.group;
+    const int unmasked = uniform(slots_seen(A.b, length, rows, node(row0)));
+    int nb = uniform(blocks(rows, length));
+    nb = nb < 4 * (till - from) ? nb : 4 * (till - from);
+    w.table = (const CONST_AS int32_t*)(A.b.table + s * A.b.table_stride);
+    const int b0 = 4 * (at - from) + wave;
+    {
+      typename Wave::Block x;
+      typename Wave::Place here = w.place(b0, nb), next = w.place(b0 + 4, nb);
+      if (here.b >= 0) {
+        w.request_k(x, here);
+        w.request_v(x, here);
+      }
+      w.start(lo, rows, length, row0);
+      while (here.b >= 0) {
+        const typename Wave::Place after = w.place(next.b + 4, next.b >= 0 ? nb : 0);
+        w.block(x, here, next, unmasked);
+        here = next;
+        next = after;
+      }
+    }
+    const bool whole = from >= begin && to <= end;
+    if (at != begin) __syncthreads();  // the sequence before is done with LDS
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const float l = sum_col4(w.l[j]);
+      if (w.grp == 0) {
+        sm[wave][16 * j + w.c16] = w.m[j];
+        sl[wave][16 * j + w.c16] = l;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      if (j > 0) __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int d = 0; d < D / 16; d += 4)
+          *reinterpret_cast<f32x4*>(&so[wave][w.c16][D / 4 * w.grp + D / 16 * e + d]) =
+              (f32x4){w.o[j][d][e], w.o[j][d + 1][e], w.o[j][d + 2][e], w.o[j][d + 3][e]};
+      __syncthreads();
+      const int r = row0 + 16 * j + row;
+      if (r < R) {
+        float M = -__builtin_inff(), L = 0.0f, o[kDims];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) M = fmaxf(M, sm[g][16 * j + row]);
+        const float ref = M == -__builtin_inff() ? 0.0f : M;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[d] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float f = __builtin_amdgcn_exp2f(sm[g][16 * j + row] - ref);
+          L += sl[g][16 * j + row] * f;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) o[d] += so[g][row][d0 + d] * f;
+        }
+        if (whole) {
+          write(r, lo, M, L, o);
+        } else {
+          const int64_t slot = part_at(me, at == from) + 16 * j + row;
+#pragma unroll
+          for (int d = 0; d < kDims; d += 2) put_pair(A.part + slot * D + d0 + d, o[d], o[d + 1]);
+          if ((t & 15) == 0) put_pair(A.part_ml + 2 * slot, M, L);
+        }
+      }
+    }
+    at = till;
+    if (whole) continue;
+    const int x0 = from / share, parts = (to - 1) / share - x0 + 1;
+    wait_vm<0>();  // this thread's part has arrived
+    __syncthreads();
+    if (t == 0)
+      arrived = __hip_atomic_fetch_add(A.count + head0 + x0, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (uniform(arrived) != parts - 1) continue;
+    if (t == 0)
+      __hip_atomic_store(A.count + head0 + x0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The last: 16 threads a row and every `take`-th part of it, then those in order.
+    for (int j = 0; j < T; ++j) {
+      const int left = R - row0 - 16 * j;
+      if (left <= 0) break;
+      const int wide = left >= 9 ? 16 : left >= 5 ? 8 : left >= 3 ? 4 : left;  // rows, a power of two
+      const int take = 16 / wide, mine = row & (wide - 1), g = row / wide;
+      float M = -__builtin_inff(), L = 0.0f, o[kDims];
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) o[d] = 0.0f;
+      constexpr int kAhead = 4;
+      if (mine < left)
+        for (int p0 = g; p0 < parts; p0 += kAhead * take) {
+          float2 ml[kAhead], v[kAhead][kDims / 2];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int p = p0 + k * take;
+            const int64_t slot = part_at(x0 + (p < parts ? p : g), (p < parts ? p : g) == 0) + 16 * j + mine;
+            ml[k] = get_pair(A.part_ml + 2 * slot);
+#pragma unroll
+            for (int d = 0; d < kDims / 2; ++d) v[k][d] = get_pair(A.part + slot * D + d0 + 2 * d);
+            if (p >= parts) ml[k] = make_float2(-__builtin_inff(), 0.0f);
+          }
+          float top = M;
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) top = fmaxf(top, ml[k].x);
+          const float ref = top == -__builtin_inff() ? 0.0f : top;
+          const float f = __builtin_amdgcn_exp2f(M - ref);
+          L *= f;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) o[d] *= f;
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            if (p0 + k * take >= parts) continue;
+            const float fk = __builtin_amdgcn_exp2f(ml[k].x - ref);
+            L += ml[k].y * fk;
+#pragma unroll
+            for (int d = 0; d < kDims / 2; ++d) {
+              o[2 * d] += v[k][d].x * fk;
+              o[2 * d + 1] += v[k][d].y * fk;
+            }
+          }
+          M = top;
+        }
+      __syncthreads();
+      float* const all = &so[0][0][0];  // [16][kStride]
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) all[row * kStride + d0 + d] = o[d];
+      if ((t & 15) == 0) {
+        all[row * kStride + D] = M;
+        all[row * kStride + D + 1] = L;
+      }
+      __syncthreads();
+      if (g == 0 && mine < left) {
+        float top = -__builtin_inff();
+        for (int k = 0; k < take; ++k) top = fmaxf(top, all[(k * wide + mine) * kStride + D]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        float total = 0.0f, r[kDims];
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) r[d] = 0.0f;
+        for (int k = 0; k < take; ++k) {
+          const float* from_k = all + (k * wide + mine) * kStride;
+          const float f = __builtin_amdgcn_exp2f(from_k[D] - ref);
+          total += from_k[D + 1] * f;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) r[d] += from_k[d0 + d] * f;
+        }
+        write(row0 + 16 * j + mine, lo, top, total, r);
+      }
+    }
   }
 }
 

@@ -11,6 +11,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 
 namespace {
 
@@ -141,9 +142,42 @@ P* layer_at(const kv_pages* a, P* p, int32_t layer, int64_t bytes) {
   return p ? reinterpret_cast<P*>(at + (uintptr_t)(layer * layer_rows(a) * bytes)) : nullptr;
 }
 
+uint32_t float_bits(float f) {
+  uint32_t u;
+  std::memcpy(&u, &f, 4);
+  return u;
+}
+
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int32_t kAttnRowsMax = 256;
 constexpr int kVerifyRowsMax = 65535;
+
+// How kv_pages_attn divides its work.
+struct AttnPlan {
+  int tiles;       // 0, 1, 2: 1, 2, 4 tiles of 16 rows a workgroup
+  int row_blocks;
+  int workers;     // workgroups of a kv head and row block
+  size_t parts() const { return (size_t)2 * 16 * (1 << tiles); }  // rows of a workgroup's two
+};
+
+AttnPlan attn_plan(const kv_pages* a, int32_t max_rows, int32_t q_heads) {
+  const int rows = max_rows * (q_heads / a->kv_heads);
+  AttnPlan p{};
+  p.tiles = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
+  const int per_wg = 16 << p.tiles;
+  p.row_blocks = (rows + per_wg - 1) / per_wg;
+  const int wgs = (p.tiles == 2 ? 1 : 2) * q8_shim::compute_units();
+  p.workers = std::max(1, wgs / (a->kv_heads * p.row_blocks));
+  return p;
+}
+
+// Counters in front, where no layout of the parts reaches, then the parts.
+constexpr size_t kCountBytes = 1 << 16;
+
+size_t attn_workspace(const kv_pages* a, const AttnPlan& p) {
+  const size_t wgs = (size_t)a->kv_heads * p.row_blocks * p.workers;
+  return kCountBytes + wgs * p.parts() * (a->head_dim + 2) * 4;
+}
 
 int verify_chunks(int32_t vocab) { return (vocab + kVerifyChunk - 1) / kVerifyChunk; }
 
@@ -248,8 +282,13 @@ int kv_pages_append(const kv_pages* a, int32_t layer, const kv_batch* batch, con
 }
 
 size_t kv_pages_attn_workspace_bytes(const kv_pages* a, const kv_batch* batch, int32_t q_heads) {
-  if (check_pages(a) || check_batch(a, batch) || check_heads(a, q_heads)) return 0;
-  return 0;
+  if (check_pages(a) || check_batch(a, batch) || check_heads(a, q_heads) ||
+      batch->max_rows > kAttnRowsMax)
+    return 0;
+  size_t most = 0;
+  for (int32_t m = 1; m <= batch->max_rows; ++m)
+    most = std::max(most, attn_workspace(a, attn_plan(a, m, q_heads)));
+  return most;
 }
 
 int kv_pages_attn(const kv_pages* a, int32_t layer, const kv_batch* batch, const void* q,
@@ -270,14 +309,16 @@ int kv_pages_attn(const kv_pages* a, int32_t layer, const kv_batch* batch, const
   if (!(scale > 0.0f) || !std::isfinite(scale))
     return fail(Q8_ERR_BAD_ARGUMENT, "scale %g is not finite and positive", scale);
   if (!aligned(lse, 4)) return fail(Q8_ERR_MISALIGNED, "lse 4-byte alignment");
-  const size_t need = kv_pages_attn_workspace_bytes(a, batch, q_heads);
-  if (need && !workspace) return fail(Q8_ERR_NULL_POINTER, "null workspace");
+  const AttnPlan plan = attn_plan(a, batch->max_rows, q_heads);
+  const size_t need = attn_workspace(a, plan);
+  if (!workspace) return fail(Q8_ERR_NULL_POINTER, "null workspace");
   if (!aligned(workspace, 256)) return fail(Q8_ERR_MISALIGNED, "workspace 256-byte alignment");
   if (workspace_bytes < need)
     return fail(Q8_ERR_BAD_SHAPE, "workspace of %zu bytes < %zu needed", workspace_bytes, need);
   if ((rc = check_ready())) return rc;
-  const int group = q_heads / a->kv_heads, rows = batch->max_rows * group;
-  const int t = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
+  const int group = q_heads / a->kv_heads;
+  const size_t wgs = (size_t)a->kv_heads * plan.row_blocks * plan.workers;
+  char* const ws = static_cast<char*>(workspace);
   PagesAttnArgs args{batch_args(a, batch),
                      layer_at(a, static_cast<const uint8_t*>(a->k), layer, row_bytes(a)),
                      layer_at(a, static_cast<const uint8_t*>(a->v), layer, row_bytes(a)),
@@ -292,11 +333,14 @@ int kv_pages_attn(const kv_pages* a, int32_t layer, const kv_batch* batch, const
                      a->kv_heads,
                      group,
                      (uint32_t)((0xffffffffull + group) / group),
-                     scale * kLog2e};
+                     float_bits(scale * kLog2e * (a->type == KV_PAGES_Q8 ? 512.0f : 1.0f)),
+                     plan.workers,
+                     reinterpret_cast<int32_t*>(ws),
+                     reinterpret_cast<float*>(ws + kCountBytes),
+                     reinterpret_cast<float*>(ws + kCountBytes) + wgs * plan.parts() * a->head_dim};
   void* p[] = {&args};
-  const int per_wg = 16 << t;
-  return q8_shim::launch3(c.attn[dim_of(a)][a->type][t], (uint32_t)a->kv_heads,
-                          (uint32_t)((rows + per_wg - 1) / per_wg), (uint32_t)batch->seqs, 256, p,
+  return q8_shim::launch3(c.attn[dim_of(a)][a->type][plan.tiles], (uint32_t)a->kv_heads,
+                          (uint32_t)plan.row_blocks, (uint32_t)plan.workers, 256, p,
                           static_cast<hipStream_t>(stream));
 }
 
