@@ -85,7 +85,12 @@ struct PagesReadArgs {
 };
 
 constexpr int kSeqsMax = 1024;
-constexpr int kVerifyChunk = 8192;  // logits of a workgroup
+// A chunk's (or row's) maximum, its lowest index, and the sum of exp((x - top) / T).
+struct VerifyStat {
+  double sum;
+  float top;
+  int32_t first;
+};
 
 struct VerifyArgs {
   PagesBatch b;  // start, seqs, rows, max_rows
@@ -96,10 +101,9 @@ struct VerifyArgs {
   float* logprob;
   int64_t logits_stride, draft_stride, out_stride;
   int32_t vocab, chunks;
-  double* sums;   // [rows, chunks] sums of exp((x - top) / T)
-  float* tops;    // [rows, chunks] the chunk's maximum
-  int32_t* firsts;  // [rows, chunks] its lowest index
-  double* rest;   // [seqs, chunks, 2] sums of max(p - q, 0) and of p in the deciding row
+  VerifyStat* stats;  // [rows, chunks]
+  VerifyStat* rows;   // [rows]
+  double* rest;       // [seqs, chunks, 2] sums of max(p - q, 0) and of p in the deciding row
 };
 
 #endif

@@ -833,28 +833,60 @@ PAGES_READ(128, q8, true)
 
 // ---------------------------------------------------------------- verify ----
 //
-// verify_sums_k: a chunk of one row, its maximum, the maximum's lowest index and the
-// sum of exp((x - maximum) / T).  verify_rest_k: every workgroup of a sequence joins
-// its rows' chunks, finds the row that decides and sums max(p - q, 0) and p over its
-// chunk of it.  verify_take_k: the chunk and the index whose running sum passes the
+// verify_sums: a chunk of one row, its maximum, the maximum's lowest index and the
+// sum of exp((x - maximum) / T).  verify_rest: every workgroup of a sequence joins its
+// rows' chunks, finds the row that decides and sums max(p - q, 0) and p over its
+// chunk of it.  verify_take: the chunk and the index whose running sum passes the
 // random number, and the outputs.  All in f64: next to a border of the running sums, one
-// in 151936, f32 sums would give other tokens.
+// in 151936, f32 sums would give other tokens.  exp is 2^(n / 64) from a table times a
+// polynomial of degree 4 in the rest, |rest| <= ln 2 / 128: 4e-14 of it is left out, under
+// what the sums of 151936 terms lose, at a third of the instructions of a full f64 exp.
 namespace {
 
-struct RowStat {
-  double total;
-  float top;
-  int first;
+__constant__ double kExp2[64] = {  // 2^(n / 64)
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
-__device__ __forceinline__ float logit(uint16_t b) {
-  const float x = (float)as_half(b);
-  return x == x ? x : -__builtin_inff();
+__device__ __forceinline__ float logit(uint16_t b) {  // NaN counts as -inf
+  return fmaxf((float)as_half(b), -__builtin_inff());
 }
-// exp((x - top) / T) with inv_heat = 1 / T
-__device__ __forceinline__ double weight(float x, float top, double inv_heat) {
-  return x == top ? 1.0 : exp(((double)x - (double)top) * inv_heat);
-}
+
+// exp((x - top) / T).  The table lies in LDS.
+struct Exp {
+  const double* table;
+  double top, unit;  // 64 log2(e) / T
+  bool far;          // top is +inf: it alone has weight
+  __device__ __forceinline__ Exp(const double* table, float top, float heat)
+      : table(table), top((double)top), unit(92.332482616893656877 / (double)heat),
+        far(top == __builtin_inff()) {}
+  __device__ __forceinline__ double operator()(float x) const {
+    if (far) return x == __builtin_inff() ? 1.0 : 0.0;
+    const double z = fmax(((double)x - top) * unit, -70000.0);  // 2^-1093 is 0
+    const double n = rint(z), r = z - n;
+    const int i = (int)n;
+    double p = 0x1.3b2ab6fba4e77p-31;
+    p = fma(p, r, 0x1.c6b08d704a0c0p-23);
+    p = fma(p, r, 0x1.ebfbdff82c58fp-15);
+    p = fma(p, r, 0x1.62e42fefa39efp-7);
+    p = fma(p, r, 1.0);
+    return ldexp(p * table[i & 63], i >> 6);
+  }
+};
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -866,26 +898,114 @@ __device__ __forceinline__ float heat_of(const VerifyArgs& A, int s) {
   return A.temperature ? A.temperature[s] : 1.0f;
 }
 
+// 8 values from p on, the first `count` of them; rows start on any 2 (or 4) bytes.
+__device__ __forceinline__ u32x4 logits8(const uint16_t* p, int count) {
+  typedef u32x4 __attribute__((aligned(2))) Any;
+  if (count >= 8) return *(const GLOBAL_AS Any*)p;
+  u32x4 v = {0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};  // -inf
+#pragma unroll
+  for (int e = 0; e < 7; ++e)
+    if (e < count) v[e >> 1] = e & 1 ? (v[e >> 1] & 0xffffu) | (uint32_t)p[e] << 16 : 0xfc000000u | p[e];
+  return v;
+}
+__device__ __forceinline__ void probs8(const float* p, int count, float (&v)[8]) {
+  typedef f32x4 __attribute__((aligned(4))) Any;
+  if (count >= 8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 w = *(const GLOBAL_AS Any*)(p + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * h + e] = w[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < count ? p[e] : 0.0f;
+  }
+}
+__device__ __forceinline__ float value_of(u32x4 v, int e) {
+  return logit((uint16_t)(v[e >> 1] >> (16 * (e & 1))));
+}
+
+template <int V>
+__device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
+  __shared__ double table[64], sums[4];
+  __shared__ float tops[4];
+  __shared__ int firsts[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int chunk = blockIdx.x, row = blockIdx.y;
+  const int begin = chunk * 2048 * V;
+  const uint16_t* x = A.logits + (int64_t)row * A.logits_stride + begin;
+  u32x4 v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8);
+  int lo, m;
+  const int s = seq_of_row(A.b, row, lo, m);
+  if (s < 0) return;
+  const float heat = heat_of(A, s);
+  if (t < 64) table[t] = kExp2[t];
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, value_of(v[i], e));
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  int first = 0x7fffffff;
+#pragma unroll
+  for (int i = V - 1; i >= 0; --i)
+#pragma unroll
+    for (int e = 7; e >= 0; --e)
+      if (value_of(v[i], e) == top) first = begin + (i * 256 + t) * 8 + e;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const int f = __shfl_xor(first, d);
+    first = f < first ? f : first;
+  }
+  double sum = 0.0;
+  if (heat > 0.0f && top > -__builtin_inff()) {
+    const Exp weight(table, top, heat);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += weight(value_of(v[i], e));
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) {
+    sums[wave] = sum;
+    firsts[wave] = first;
+  }
+  __syncthreads();
+  if (t == 0) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w) first = firsts[w] < first ? firsts[w] : first;
+    A.stats[(int64_t)row * A.chunks + chunk] = {(sums[0] + sums[1]) + (sums[2] + sums[3]), top, first};
+  }
+}
+
 // The rows of sequence s joined from their chunks into st, and how many drafted tokens
 // stand; every thread of the 256 gets that number.
 __device__ __forceinline__ int verify_join(const VerifyArgs& A, int s, int lo, int m, float heat,
-                                           RowStat* st, int* stop) {
+                                           const double* table, VerifyStat* st, int* stop) {
   const int t = threadIdx.x, lane = t & 63;
-  const double inv = 1.0 / (double)heat;
   if (t == 0) *stop = m - 1;
+  __syncthreads();
   for (int i = t >> 6; i < m; i += 4) {
-    const int64_t at = (int64_t)(lo + i) * A.chunks;
+    const VerifyStat* stats = A.stats + (int64_t)(lo + i) * A.chunks;
     float top = -__builtin_inff();
-    for (int c = lane; c < A.chunks; c += 64) top = fmaxf(top, A.tops[at + c]);
+    for (int c = lane; c < A.chunks; c += 64) top = fmaxf(top, stats[c].top);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     double total = 0.0;
     int first = 0x7fffffff;
+    const Exp weight(table, top, heat > 0.0f ? heat : 1.0f);
     for (int c = lane; c < A.chunks; c += 64) {
-      const float x = A.tops[at + c];
-      if (x == -__builtin_inff()) continue;
-      if (x == top && A.firsts[at + c] < first) first = A.firsts[at + c];
-      if (heat > 0.0f) total += A.sums[at + c] * weight(x, top, inv);
+      const VerifyStat x = stats[c];
+      if (x.top == -__builtin_inff()) continue;
+      if (x.top == top && x.first < first) first = x.first;
+      if (heat > 0.0f) total += x.sum * weight(x.top);
     }
     total = wave_sum64(total);
 #pragma unroll
@@ -901,7 +1021,7 @@ __device__ __forceinline__ int verify_join(const VerifyArgs& A, int s, int lo, i
     bool yes = false;
     if (x >= 0 && x < A.vocab && st[t].top > -__builtin_inff()) {
       const float v = logit(A.logits[(int64_t)(lo + t) * A.logits_stride + x]);
-      const double p = heat > 0.0f ? (v == -__builtin_inff() ? 0.0 : weight(v, st[t].top, inv) / st[t].total)
+      const double p = heat > 0.0f ? Exp(table, st[t].top, heat)(v) / st[t].sum
                                    : (x == st[t].first ? 1.0 : 0.0);
       double q = 1.0;
       if (A.draft) {
@@ -918,122 +1038,61 @@ __device__ __forceinline__ int verify_join(const VerifyArgs& A, int s, int lo, i
 
 // What an entry of the deciding row weighs: max(p - q, 0) and p.
 struct Decide {
-  RowStat st;
-  double inv_heat, inv_total;
+  Exp weight;
+  double inv_total;
   bool greedy, refused, drafted;
-  int told;  // the refused token
-  __device__ __forceinline__ void operator()(int j, uint16_t bits, float d, double& rest,
-                                             double& p) const {
-    const float x = logit(bits);
-    if (greedy) p = j == st.first ? 1.0 : 0.0;
-    else p = x == -__builtin_inff() ? 0.0 : weight(x, st.top, inv_heat) * inv_total;
-    if (!refused) rest = 0.0;
-    else if (drafted) rest = d > 0.0f ? fmax(p - (double)d, 0.0) : p;
-    else rest = j == told ? 0.0 : p;
+  int first, told;  // the maximum's lowest index, the refused token
+  __device__ __forceinline__ Decide(const VerifyArgs& A, const double* table, int lo, int m, int n,
+                                    float heat, const VerifyStat& st)
+      : weight(table, st.top, heat > 0.0f ? heat : 1.0f), inv_total(1.0 / st.sum),
+        greedy(!(heat > 0.0f)), refused(n < m - 1), drafted(A.draft != nullptr), first(st.first),
+        told(refused ? A.tokens[lo + n + 1] : -1) {}
+  __device__ __forceinline__ void operator()(int j, float x, float d, double& rest, double& p) const {
+    p = greedy ? (j == first ? 1.0 : 0.0) : weight(x) * inv_total;
+    rest = !refused ? 0.0 : drafted ? (d > 0.0f ? fmax(p - (double)d, 0.0) : p) : j == told ? 0.0 : p;
   }
 };
 
-__device__ __forceinline__ Decide decide(const VerifyArgs& A, int lo, int m, int n, float heat,
-                                         const RowStat& st) {
-  Decide d;
-  d.st = st;
-  d.greedy = !(heat > 0.0f);
-  d.inv_heat = 1.0 / (double)heat;
-  d.inv_total = 1.0 / st.total;
-  d.refused = n < m - 1;
-  d.drafted = A.draft != nullptr;
-  d.told = d.refused ? A.tokens[lo + n + 1] : -1;
-  return d;
-}
-
-}  // namespace
-
-extern "C" __global__ __launch_bounds__(256) void verify_sums_k(VerifyArgs A) {
-  __shared__ float tops[4];
-  __shared__ int firsts[4];
-  __shared__ double sums[4];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int chunk = blockIdx.x, row = blockIdx.y;
-  int lo, m;
-  const int s = seq_of_row(A.b, row, lo, m);
-  if (s < 0) return;
-  const float heat = heat_of(A, s);
-  const uint16_t* x = A.logits + (int64_t)row * A.logits_stride;
-  const int begin = chunk * kVerifyChunk;
-  const int end = begin + kVerifyChunk < A.vocab ? begin + kVerifyChunk : A.vocab;
-  float top = -__builtin_inff();
-  int first = 0x7fffffff;
-  for (int j = begin + t; j < end; j += 256) {
-    const float v = logit(x[j]);
-    if (v > top) {
-      top = v;
-      first = j;
-    }
-  }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const float v = __shfl_xor(top, d);
-    const int f = __shfl_xor(first, d);
-    if (v > top || (v == top && f < first)) {
-      top = v;
-      first = f;
-    }
-  }
-  if (lane == 0) {
-    tops[wave] = top;
-    firsts[wave] = first;
-  }
-  __syncthreads();
-  top = tops[0];
-  first = firsts[0];
-#pragma unroll
-  for (int w = 1; w < 4; ++w)
-    if (tops[w] > top || (tops[w] == top && firsts[w] < first)) {
-      top = tops[w];
-      first = firsts[w];
-    }
-  double sum = 0.0;
-  if (heat > 0.0f && top > -__builtin_inff()) {
-    const double inv = 1.0 / (double)heat;
-    for (int j = begin + t; j < end; j += 256) {
-      const float v = logit(x[j]);
-      if (v > -__builtin_inff()) sum += weight(v, top, inv);
-    }
-  }
-  sum = wave_sum64(sum);
-  if (lane == 0) sums[wave] = sum;
-  __syncthreads();
-  if (t == 0) {
-    const int64_t at = (int64_t)row * A.chunks + chunk;
-    A.tops[at] = top;
-    A.firsts[at] = first;
-    A.sums[at] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  }
-}
-
-extern "C" __global__ __launch_bounds__(256) void verify_rest_k(VerifyArgs A) {
-  __shared__ RowStat st[256];
+template <int V>
+__device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
+  __shared__ double table[64], sums[4][2];
+  __shared__ VerifyStat st[256];
   __shared__ int stop;
-  __shared__ double sums[4][2];
   const int t = threadIdx.x, chunk = blockIdx.x, s = blockIdx.y;
   const int lo = A.b.start ? A.b.start[s] : s;
   const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
   if (m == 0) return;
   const float heat = heat_of(A, s);
-  const int n = verify_join(A, s, lo, m, heat, st, &stop);
-  const Decide w = decide(A, lo, m, n, heat, st[n]);
-  const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
-  const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
-  const int begin = chunk * kVerifyChunk;
-  const int end = begin + kVerifyChunk < A.vocab ? begin + kVerifyChunk : A.vocab;
+  if (t < 64) table[t] = kExp2[t];
+  const int n = verify_join(A, s, lo, m, heat, table, st, &stop);
+  if (chunk == 0) {
+    for (int i = t; i < m; i += 256) A.rows[lo + i] = st[i];
+    if (t == 0) A.accepted[s] = n;
+  }
   double rest = 0.0, all = 0.0;
-  if (w.st.top > -__builtin_inff())
-    for (int j = begin + t; j < end; j += 256) {
-      double r, p;
-      w(j, x[j], q ? q[j] : 0.0f, r, p);
-      rest += r;
-      all += p;
+  if (st[n].top > -__builtin_inff()) {
+    const Decide w(A, table, lo, m, n, heat, st[n]);
+    const int begin = chunk * 2048 * V;
+    const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride + begin;
+    const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride + begin : nullptr;
+    u32x4 v[V];
+    float d[V][8] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int j = (i * 256 + t) * 8;
+      v[i] = logits8(x + j, A.vocab - begin - j);
+      if (q) probs8(q + j, A.vocab - begin - j, d[i]);
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double r, p;
+        w(begin + (i * 256 + t) * 8 + e, value_of(v[i], e), d[i][e], r, p);
+        rest += r;
+        all += p;
+      }
+  }
   rest = wave_sum64(rest);
   all = wave_sum64(all);
   if ((t & 63) == 0) {
@@ -1046,89 +1105,145 @@ extern "C" __global__ __launch_bounds__(256) void verify_rest_k(VerifyArgs A) {
         (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
 }
 
-extern "C" __global__ __launch_bounds__(256) void verify_take_k(VerifyArgs A) {
-  __shared__ RowStat st[256];
-  __shared__ int stop, found, last;
-  __shared__ double run[256];
+// The sum of v over the threads before this one, and over all 256 (two barriers).
+__device__ __forceinline__ double block_before(double v, double* waves, double& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double c = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double other = __shfl_up(c, d);
+    if (lane >= d) c += other;
+  }
+  if (lane == 63) waves[wave] = c;
+  __syncthreads();
+  double before = 0.0;
+  total = 0.0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) before += waves[w];
+    total += waves[w];
+  }
+  __syncthreads();
+  return before + (c - v);
+}
+
+template <int V>
+__device__ __forceinline__ void verify_take(const VerifyArgs& A) {
+  __shared__ double table[64], waves[4], base;
+  __shared__ int found, last;
   const int t = threadIdx.x, s = blockIdx.x;
   const int lo = A.b.start ? A.b.start[s] : s;
   const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
-  int n = 0, token = -1;
   const float heat = heat_of(A, s);
-  if (m > 0) {
-    n = verify_join(A, s, lo, m, heat, st, &stop);
-    const Decide w = decide(A, lo, m, n, heat, st[n]);
-    if (w.st.top > -__builtin_inff()) {
-      const double* sums = A.rest + (int64_t)s * A.chunks * 2;
+  int n = 0, token = -1;
+  if (m == 0) {
+    if (t == 0) A.accepted[s] = 0;
+  } else {
+    if (t < 64) table[t] = kExp2[t];
+    n = A.accepted[s];
+    const VerifyStat st = A.rows[lo + n];
+    const double* sums = A.rest + (int64_t)s * A.chunks * 2;
+    if (st.top > -__builtin_inff()) {
+      const Decide w(A, table, lo, m, n, heat, st);
       double total[2] = {0.0, 0.0};
-      for (int c = 0; c < A.chunks; ++c) {
+      for (int c = t; c < A.chunks; c += 256) {
         total[0] += sums[2 * c];
         total[1] += sums[2 * c + 1];
       }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) (void)block_before(total[k], waves, total[k]);
       const int k = w.refused && total[0] > 0.0 ? 0 : 1;
       const double goal = (double)A.uniform[lo + m - 1] * total[k];
       // the chunk whose running sum passes the goal, else the last that weighs anything
-      int chunk = -1;
-      double before = 0.0, sum = 0.0;
-      for (int c = 0; c < A.chunks; ++c) {
-        const double here = sums[2 * c + k];
+      if (t == 0) {
+        found = 0x7fffffff;
+        last = -1;
+      }
+      double sum = 0.0;
+      for (int c0 = 0; c0 < A.chunks; c0 += 256) {
+        const int c = c0 + t;
+        const double here = c < A.chunks ? sums[2 * c + k] : 0.0;
+        double all;
+        const double before = sum + block_before(here, waves, all);
         if (here > 0.0) {
-          chunk = c;
-          before = sum;
-          if (sum + here > goal) break;
+          if (before + here > goal) atomicMin(&found, c);
+          atomicMax(&last, c);
         }
-        sum += here;
+        __syncthreads();
+        // (a chunk found in an earlier round stays)
+        if (c == (found != 0x7fffffff ? found : last)) base = before;
+        sum += all;
+        __syncthreads();
+        if (found != 0x7fffffff) break;
+      }
+      const int chunk = found != 0x7fffffff ? found : last;
+      __syncthreads();
+      if (t == 0) {
+        found = 0x7fffffff;
+        last = -1;
       }
       if (chunk >= 0) {
-        const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
-        const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
-        const int begin = chunk * kVerifyChunk;
-        const int end = begin + kVerifyChunk < A.vocab ? begin + kVerifyChunk : A.vocab;
-        constexpr int kEach = kVerifyChunk / 256;
-        const int j0 = begin + t * kEach, j1 = j0 + kEach < end ? j0 + kEach : end;
-        double mine = 0.0;
+        // 8 V values in a row a thread
+        const int begin = chunk * 2048 * V + t * 8 * V;
+        const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride + begin;
+        const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride + begin : nullptr;
+        double c[8 * V], mine = 0.0;
         int some = -1;
-        for (int j = j0; j < j1; ++j) {
-          double v[2];
-          w(j, x[j], q ? q[j] : 0.0f, v[0], v[1]);
-          mine += v[k];
-          if (v[k] > 0.0) some = j;
-        }
-        run[t] = mine;
-        if (t == 0) {
-          found = 0x7fffffff;
-          last = -1;
-        }
-        __syncthreads();
-        double c = before;
-        for (int i = 0; i < t; ++i) c += run[i];
-        for (int j = j0; j < j1; ++j) {
-          double v[2];
-          w(j, x[j], q ? q[j] : 0.0f, v[0], v[1]);
-          c += v[k];
-          if (v[k] > 0.0 && c > goal) {
-            atomicMin(&found, j);
-            break;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const u32x4 v = logits8(x + 8 * i, A.vocab - begin - 8 * i);
+          float d[8] = {};
+          if (q) probs8(q + 8 * i, A.vocab - begin - 8 * i, d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            double r, p;
+            w(begin + 8 * i + e, value_of(v, e), d[e], r, p);
+            c[8 * i + e] = k ? p : r;
+            mine += c[8 * i + e];
+            if (c[8 * i + e] > 0.0) some = begin + 8 * i + e;
           }
         }
+        double all;
+        double run = base + block_before(mine, waves, all);
+        int hit = 0x7fffffff;
+#pragma unroll
+        for (int e = 0; e < 8 * V; ++e) {
+          run += c[e];
+          if (c[e] > 0.0 && run > goal && hit == 0x7fffffff) hit = begin + e;
+        }
+        if (hit != 0x7fffffff) atomicMin(&found, hit);
         if (some >= 0) atomicMax(&last, some);
         __syncthreads();
-        token = found < end ? found : last;
+        token = found != 0x7fffffff ? found : last;
       }
     }
   }
-  if (t == 0) A.accepted[s] = n;
   for (int i = t; i < A.b.max_rows; i += 256) {
-    const int x = i < n ? A.tokens[lo + i + 1] : i == n ? token : -1;
+    const int x = m == 0 ? -1 : i < n ? A.tokens[lo + i + 1] : i == n ? token : -1;
     A.out[s * A.out_stride + i] = x;
     if (A.logprob) {
       float lp = 0.0f;
       if (x >= 0 && heat > 0.0f) {
+        const VerifyStat st = A.rows[lo + i];
         const float v = logit(A.logits[(int64_t)(lo + i) * A.logits_stride + x]);
-        lp = (float)((v == st[i].top ? 0.0 : ((double)v - (double)st[i].top) / (double)heat) -
-                     log(st[i].total));
+        lp = (float)((v == st.top ? 0.0 : ((double)v - (double)st.top) / (double)heat) - log(st.sum));
       }
       A.logprob[s * A.out_stride + i] = lp;
     }
   }
 }
+
+}  // namespace
+
+#define VERIFY(V)                                                                              \
+  extern "C" __global__ __launch_bounds__(256) void verify_sums_##V(VerifyArgs A) {            \
+    verify_sums<V>(A);                                                                         \
+  }                                                                                            \
+  extern "C" __global__ __launch_bounds__(256) void verify_rest_##V(VerifyArgs A) {            \
+    verify_rest<V>(A);                                                                         \
+  }                                                                                            \
+  extern "C" __global__ __launch_bounds__(256) void verify_take_##V(VerifyArgs A) {            \
+    verify_take<V>(A);                                                                         \
+  }
+VERIFY(1)
+VERIFY(4)

@@ -19,7 +19,7 @@ struct {
   hipModule_t module = nullptr;
   // [head_dim 64, 128][f16, q8]
   hipFunction_t append[2][2] = {}, attn[2][2][3] = {}, read[2][2] = {};
-  hipFunction_t sums = nullptr, rest = nullptr, take = nullptr;
+  hipFunction_t sums[2] = {}, rest[2] = {}, take[2] = {};  // chunks of 2048, 8192
 } c;
 
 int fail(int code, const char* fmt, ...) {
@@ -179,7 +179,10 @@ size_t attn_workspace(const kv_pages* a, const AttnPlan& p) {
   return kCountBytes + wgs * p.parts() * (a->head_dim + 2) * 4;
 }
 
-int verify_chunks(int32_t vocab) { return (vocab + kVerifyChunk - 1) / kVerifyChunk; }
+// Logits of a workgroup: 8192, or 2048 where that leaves CUs without a workgroup.
+int verify_chunk(int32_t rows, int32_t vocab) {
+  return (int64_t)rows * ((vocab + 8191) / 8192) >= q8_shim::compute_units() ? 8192 : 2048;
+}
 
 }  // namespace
 
@@ -205,9 +208,11 @@ void pages_load(const char* path) {
         get(&c.attn[d][q][t], name);
       }
     }
-  get(&c.sums, "verify_sums_k");
-  get(&c.rest, "verify_rest_k");
-  get(&c.take, "verify_take_k");
+  for (int i = 0; i < 2; ++i) {
+    get(&c.sums[i], i ? "verify_sums_4" : "verify_sums_1");
+    get(&c.rest[i], i ? "verify_rest_4" : "verify_rest_1");
+    get(&c.take[i], i ? "verify_take_4" : "verify_take_1");
+  }
   if (!ok) {
     (void)hipModuleUnload(m);
     return;
@@ -378,7 +383,8 @@ size_t kv_verify_workspace_bytes(int32_t rows, int32_t seqs, int32_t vocab) {
   if (check_rows(&rows, seqs, rows, 1, kVerifyRowsMax, kAttnRowsMax) || vocab < 1 ||
       vocab > (1 << 24))
     return 0;
-  return (size_t)verify_chunks(vocab) * (16 * ((size_t)rows + seqs));
+  const size_t chunks = (size_t)(vocab + 2047) / 2048;
+  return 16 * (chunks * ((size_t)rows + seqs) + rows);
 }
 
 int kv_verify(const kv_drafts* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -420,18 +426,17 @@ int kv_verify(const kv_drafts* d, void* workspace, size_t workspace_bytes, void*
   args.draft_stride = d->draft_stride;
   args.out_stride = d->out_stride;
   args.vocab = d->vocab;
-  args.chunks = verify_chunks(d->vocab);
-  const size_t stats = (size_t)d->rows * args.chunks;
-  args.sums = static_cast<double*>(workspace);
-  args.rest = args.sums + stats;
-  args.tops = reinterpret_cast<float*>(args.rest + 2 * (size_t)d->seqs * args.chunks);
-  args.firsts = reinterpret_cast<int32_t*>(args.tops + stats);
+  const int chunk = verify_chunk(d->rows, d->vocab), i = chunk == 8192 ? 1 : 0;
+  args.chunks = (d->vocab + chunk - 1) / chunk;
+  args.stats = static_cast<VerifyStat*>(workspace);
+  args.rows = args.stats + (size_t)d->rows * args.chunks;
+  args.rest = reinterpret_cast<double*>(args.rows + d->rows);
   void* p[] = {&args};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t chunks = (uint32_t)args.chunks;
-  if ((rc = q8_shim::launch3(c.sums, chunks, (uint32_t)d->rows, 1, 256, p, st))) return rc;
-  if ((rc = q8_shim::launch3(c.rest, chunks, (uint32_t)d->seqs, 1, 256, p, st))) return rc;
-  return q8_shim::launch(c.take, (uint32_t)d->seqs, 256, p, st);
+  if ((rc = q8_shim::launch3(c.sums[i], chunks, (uint32_t)d->rows, 1, 256, p, st))) return rc;
+  if ((rc = q8_shim::launch3(c.rest[i], chunks, (uint32_t)d->seqs, 1, 256, p, st))) return rc;
+  return q8_shim::launch(c.take[i], (uint32_t)d->seqs, 256, p, st);
 }
 
 }  // extern "C"
