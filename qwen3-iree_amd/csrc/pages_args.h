@@ -102,8 +102,8 @@ struct VerifyArgs {
   int64_t logits_stride, draft_stride, out_stride;
   int32_t vocab, chunks;
   VerifyStat* stats;  // [rows, chunks]
-  VerifyStat* rows;   // [rows]
   double* rest;       // [seqs, chunks, 2] sums of max(p - q, 0) and of p in the deciding row
+  int32_t* count;     // [seqs] workgroups that have left theirs
 };
 
 #endif

@@ -3,6 +3,8 @@
 #include "decode_device.h"
 #include "pages_args.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr float kLn2 = 0.693147180559945309f;
@@ -36,6 +38,12 @@ __device__ __forceinline__ int64_t pool_row(const PagesBatch& b, int s, int64_t 
   return ((int64_t)page * kv_heads + h) * b.page_size + ((int)p - at * b.page_size);
 }
 
+// 8 halves that start on any 2 bytes
+__device__ __forceinline__ u32x4 load_words4(const uint16_t* p) {
+  typedef u32x4 __attribute__((aligned(2))) Any;
+  return *(const GLOBAL_AS Any*)p;
+}
+
 __device__ __forceinline__ float half_at(u32x4 v, int j) {
   return (float)as_half((uint16_t)(v[j >> 1] >> (16 * (j & 1))));
 }
@@ -46,111 +54,170 @@ __device__ __forceinline__ float half_at(u32x4 v, int j) {
 //
 // One workgroup a row; D / 8 lanes a head, 8 values each, all of the row's q, k
 // and v heads in turn.  The rotation's partners, dims i and i + D/2, are lanes half a
-// head apart.  The angles' cosines and sines are worked out once a row.
+// head apart.  The angles' cosines and sines are worked out once a row.  In f64: the rounding
+// to codes must not depend on an order of sums.
 namespace {
 
-template <int D>
-__device__ __forceinline__ double head_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < D / 8; d <<= 1) v += __shfl_xor(v, d);
+template <int kCtrl>
+__device__ __forceinline__ double lane_of(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)b, kCtrl, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(b >> 32), kCtrl, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, lo | (uint64_t)hi << 32);
+}
+
+// f over a head's D / 8 lanes, in every one: lanes xor 1, xor 2, then the halves of 8 and of
+// 16 mirrored (whose quads and eights hold one value by then).
+template <int D, class F>
+__device__ __forceinline__ double over_head(double v, F f) {
+  v = f(v, lane_of<0xb1>(v));
+  v = f(v, lane_of<0x4e>(v));
+  v = f(v, lane_of<0x141>(v));
+  if constexpr (D == 128) v = f(v, lane_of<0x140>(v));
   return v;
+}
+
+// The value half a head away: lane xor 8 of 16, xor 4 of 8.
+template <int D>
+__device__ __forceinline__ double other_half(double v) {
+  if constexpr (D == 128) return lane_of<0x128>(v);
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_ds_swizzle((uint32_t)b, 0x101f);
+  const uint32_t hi = __builtin_amdgcn_ds_swizzle((uint32_t)(b >> 32), 0x101f);
+  return __builtin_bit_cast(double, lo | (uint64_t)hi << 32);
+}
+
+// Norm (w not null) and rotation (by turn[i] = (cos, sin)) of a head's lane c.
+template <int D>
+__device__ __forceinline__ void turn_head(double (&y)[8], int c, const uint16_t* w, double eps,
+                                          bool rotate, const double2* turn) {
+  if (w) {
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
+    ss = over_head<D>(ss, [](double a, double b) { return a + b; });
+    const double r = rsqrt(ss / D + eps);
+    const u32x4 wv = load_words4(w + 8 * c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (double)half_at(wv, j);
+  }
+  if (rotate) {
+    const bool second = c >= D / 16;
+    const int i = (8 * c) % (D / 2);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double2 a = turn[i + j];
+      const double o = other_half<D>(y[j]);
+      y[j] = y[j] * a.x + o * (second ? a.y : -a.y);
+    }
+  }
+}
+
+__device__ __forceinline__ u32x4 packed8(const double (&y)[8]) {
+  u32x4 o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = pack_f16x2((float)y[2 * j], (float)y[2 * j + 1]);
+  return o;
+}
+
+// The 8 codes of a lane and their head's scale.  y / scale is y times 1 / scale, rounded to
+// a multiple of 2^-36: a quotient that lies on a border exactly (a v of 11 bits by a
+// scale of 24 can; the next ones are 2^-25 away) is on it again, and the sum with
+// 1.5 2^52 leaves the nearest integer, ties to even, in the low bits.
+template <int D>
+__device__ __forceinline__ uint2 codes8(const double (&y)[8], float& scale) {
+  double top = 0.0;
+  bool fine = true;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    top = fmax(top, fabs(y[j]));
+    fine = fine && fabs(y[j]) < __builtin_inf();
+  }
+  if (!fine) top = __builtin_inf();
+  top = over_head<D>(top, [](double a, double b) { return fmax(a, b); });
+  const bool real = top < __builtin_inf();
+  scale = real ? (float)(top / 127.0) : __builtin_nanf("");
+  uint2 code = {0, 0};
+  if (!real || scale == 0.0f) return code;
+  const double inv = 1.0 / (double)scale;
+  uint32_t low[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    double q = y[j] * inv;
+    if (scale < 1.17549435e-38f) q = fmin(fmax(q, -127.0), 127.0);  // a scale of few bits
+    q = (q + 98304.0) - 98304.0;
+    low[j] = (uint32_t)__builtin_bit_cast(uint64_t, q + 6755399441055744.0);
+  }
+  const uint32_t pairs[4] = {__builtin_amdgcn_perm(low[1], low[0], 0x0c0c0400),
+                             __builtin_amdgcn_perm(low[3], low[2], 0x0c0c0400),
+                             __builtin_amdgcn_perm(low[5], low[4], 0x0c0c0400),
+                             __builtin_amdgcn_perm(low[7], low[6], 0x0c0c0400)};
+  code.x = pairs[0] | pairs[1] << 16;
+  code.y = pairs[2] | pairs[3] << 16;
+  return code;
 }
 
 template <int D, bool Q8>
 __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
   constexpr int G = D / 8;
-  __shared__ double cs[D / 2], sn[D / 2];
+  __shared__ double2 turn[D / 2];
   const int t = threadIdx.x, c = t % G, row = blockIdx.x;
+  const int heads = A.q_heads + 2 * A.kv_heads;
+  auto request = [&](int h) {
+    const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
+    const uint16_t* from = is_q   ? A.q + row * A.q_stride + h * D
+                           : is_v ? A.v + row * A.v_stride + (h - A.q_heads - A.kv_heads) * D
+                                  : A.k + row * A.k_stride + (h - A.q_heads) * D;
+    return load_global(reinterpret_cast<const u32x4*>(from + 8 * c));
+  };
+  int h = t / G;
+  u32x4 x = {};
+  if (h < heads) x = request(h);
   int lo, m;
   const int s = seq_of_row(A.b, row, lo, m);
   if (s < 0) return;
   const int64_t slot = (int64_t)A.b.length[s] - m + (row - lo);
   if (A.rotate) {
     if (t < D / 2) {
-      const double turn = (double)(A.positions ? (int64_t)A.positions[row] : slot) * A.turns[t];
-      sincospi(2.0 * (turn - rint(turn)), &sn[t], &cs[t]);
+      const double by = (double)(A.positions ? (int64_t)A.positions[row] : slot) * A.turns[t];
+      double2 a;
+      sincospi(2.0 * (by - rint(by)), &a.y, &a.x);
+      turn[t] = a;
     }
     __syncthreads();
   }
-  const int heads = A.q_heads + 2 * A.kv_heads;
-  for (int h = t / G; h < heads; h += 256 / G) {
+  const int64_t to = pool_row(A.b, s, slot, A.kv_heads, 0);  // of head 0
+  for (; h < heads; h += 256 / G) {
+    const u32x4 here = x;
+    if (h + 256 / G < heads) x = request(h + 256 / G);
     const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
-    const int hh = is_q ? h : is_v ? h - A.q_heads - A.kv_heads : h - A.q_heads;
-    const uint16_t* from = is_q   ? A.q + row * A.q_stride
-                           : is_v ? A.v + row * A.v_stride
-                                  : A.k + row * A.k_stride;
-    const u32x4 x = load_global(reinterpret_cast<const u32x4*>(from + hh * D + 8 * c));
+    const int64_t at = to + (int64_t)(h - A.q_heads - (is_v ? A.kv_heads : 0)) * A.b.page_size;
+    void* pool = is_v ? A.v_to : A.k_to;
     double y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (double)half_at(x, j);
-    const uint16_t* w = is_v ? nullptr : is_q ? A.q_norm : A.k_norm;
-    if (w) {
-      double ss = 0.0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
-      const double r = 1.0 / sqrt(head_sum<D>(ss) / D + A.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (double)(float)as_half(w[8 * c + j]);
-    }
-    if (A.rotate && !is_v) {
-      const bool second = c >= G / 2;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = (8 * c + j) % (D / 2);
-        const double other = __shfl_xor(y[j], G / 2);
-        y[j] = second ? y[j] * cs[i] + other * sn[i] : y[j] * cs[i] - other * sn[i];
-      }
-    }
-    auto packed = [&] {
-      u32x4 o;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = pack_f16x2((float)y[2 * j], (float)y[2 * j + 1]);
-      return o;
-    };
+    for (int j = 0; j < 8; ++j) y[j] = (double)half_at(here, j);
+    if (!is_v) turn_head<D>(y, c, is_q ? A.q_norm : A.k_norm, A.eps, A.rotate, turn);
     if (is_q) {
-      *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + hh * D + 8 * c) = packed();
-      continue;
-    }
-    const int64_t to = pool_row(A.b, s, slot, A.kv_heads, hh);
-    void* pool = is_v ? A.v_to : A.k_to;
-    if constexpr (Q8) {
-      double top = 0.0;
-      bool fine = true;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        top = fmax(top, fabs(y[j]));
-        fine = fine && fabs(y[j]) < __builtin_inf();
-      }
-      if (!fine) top = __builtin_inf();
-#pragma unroll
-      for (int d = 1; d < G; d <<= 1) top = fmax(top, __shfl_xor(top, d));
-      const bool real = top < __builtin_inf();
-      const float scale = real ? (float)(top / 127.0) : __builtin_nanf("");
-      uint2 code = {0, 0};
-      if (real && scale > 0.0f) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          double q = rint(y[j] / (double)scale);
-          q = fmin(fmax(q, -127.0), 127.0);
-          (j < 4 ? code.x : code.y) |= ((uint32_t)(int)q & 255u) << (8 * (j & 3));
-        }
-      }
+      *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + h * D + 8 * c) = packed8(y);
+    } else if constexpr (Q8) {
+      float scale;
+      const uint2 code = codes8<D>(y, scale);
       if (to >= 0) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + to * D + 8 * c) = code;
-        if (c == 0) (is_v ? A.v_scale : A.k_scale)[to] = scale;
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at * D + 8 * c) = code;
+        if (c == 0) (is_v ? A.v_scale : A.k_scale)[at] = scale;
       }
-    } else {
-      if (to >= 0) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(pool) + to * D + 8 * c) = packed();
+    } else if (to >= 0) {
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(pool) + at * D + 8 * c) =
+          is_v ? here : packed8(y);
     }
   }
 }
 
 }  // namespace
 
-#define PAGES_APPEND(D, N, Q8)                                                   \
-  extern "C" __global__ __launch_bounds__(256) void pages_append_##D##_##N(      \
-      PagesAppendArgs A) {                                                       \
-    pages_append<D, Q8>(A);                                                      \
+#define PAGES_APPEND(D, N, Q8)                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void pages_append_##D##_##N(PagesAppendArgs A) {   \
+    pages_append<D, Q8>(A);                                                                       \
   }
 PAGES_APPEND(64, f16, false)
 PAGES_APPEND(64, q8, true)
@@ -836,61 +903,85 @@ PAGES_READ(128, q8, true)
 // verify_sums: a chunk of one row, its maximum, the maximum's lowest index and the
 // sum of exp((x - maximum) / T).  verify_rest: every workgroup of a sequence joins its
 // rows' chunks, finds the row that decides and sums max(p - q, 0) and p over its
-// chunk of it.  verify_take: the chunk and the index whose running sum passes the
-// random number, and the outputs.  All in f64: next to a border of the running sums, one
-// in 151936, f32 sums would give other tokens.  exp is 2^(n / 64) from a table times a
-// polynomial of degree 4 in the rest, |rest| <= ln 2 / 128: 4e-14 of it is left out, under
-// what the sums of 151936 terms lose, at a third of the instructions of a full f64 exp.
+// chunk of it; the last of them finds the chunk and the index whose running sum passes
+// the random number, and writes the outputs.  All in f64: next to a border of the running sums, one
+// in 151936, f32 sums would give other tokens.  exp is 2^(n / 16) from a table (16
+// doubles: no two in one LDS bank) times a polynomial of degree 5 in the rest, |rest| <=
+// ln 2 / 32: 1.5e-13 of it is left out, for a third of the instructions of a full f64 exp.
 namespace {
 
-__constant__ double kExp2[64] = {  // 2^(n / 64)
-    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
-    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
-    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
-    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
-    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
-    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
-    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
-    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
-    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
-    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
-    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
-    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
-    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
-    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+__constant__ double kExp2[16] = {  // 2^(n / 16)
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
+    0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0, 0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0,
+    0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0,
 };
 
-__device__ __forceinline__ float logit(uint16_t b) {  // NaN counts as -inf
-  return fmaxf((float)as_half(b), -__builtin_inff());
-}
-
-// exp((x - top) / T).  The table lies in LDS.
+// exp((x - top) / T), 0 for a NaN.  The table lies in LDS.
 struct Exp {
   const double* table;
-  double top, unit;  // 64 log2(e) / T
-  bool far;          // top is +inf: it alone has weight
-  __device__ __forceinline__ Exp(const double* table, float top, float heat)
-      : table(table), top((double)top), unit(92.332482616893656877 / (double)heat),
-        far(top == __builtin_inff()) {}
+  double top, unit;
+  bool far;  // top is +inf: it alone has weight
+  // unit: unit_of(T)
+  __device__ __forceinline__ Exp(const double* table, float top, double unit)
+      : table(table), top((double)top), unit(unit), far(top == __builtin_inff()) {}
   __device__ __forceinline__ double operator()(float x) const {
     if (far) return x == __builtin_inff() ? 1.0 : 0.0;
-    const double z = fmax(((double)x - top) * unit, -70000.0);  // 2^-1093 is 0
+    const double z = fmax(((double)x - top) * unit, -17500.0);  // 2^-1093 is 0; a NaN too
     const double n = rint(z), r = z - n;
     const int i = (int)n;
-    double p = 0x1.3b2ab6fba4e77p-31;
-    p = fma(p, r, 0x1.c6b08d704a0c0p-23);
-    p = fma(p, r, 0x1.ebfbdff82c58fp-15);
-    p = fma(p, r, 0x1.62e42fefa39efp-7);
+    double p = 0x1.5d87fe78a6731p-30;
+    p = fma(p, r, 0x1.3b2ab6fba4e77p-23);
+    p = fma(p, r, 0x1.c6b08d704a0c0p-17);
+    p = fma(p, r, 0x1.ebfbdff82c58fp-11);
+    p = fma(p, r, 0x1.62e42fefa39efp-5);
     p = fma(p, r, 1.0);
-    return ldexp(p * table[i & 63], i >> 6);
+    return ldexp(p * table[i & 15], i >> 4);
   }
 };
+// 16 log2(e) / T; 0 where the maximum takes all
+__device__ __forceinline__ double unit_of(float heat) {
+  return heat > 0.0f ? 23.083120654223414519 / (double)heat : 0.0;
+}
 
+// The maximum over 16 lanes, and over the wave.
+__device__ __forceinline__ float row_max16(float v) {
+  v = fmaxf(v, dpp<0xb1>(v));
+  v = fmaxf(v, dpp<0x4e>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  return fmaxf(v, dpp<0x140>(v));
+}
+__device__ __forceinline__ float wave_max(float v) { return max_col4(row_max16(v)); }
+
+// The sum over the wave, in every lane: 16 lanes by DPP, then the four rows.
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  v = over_head<128>(v, [](double a, double b) { return a + b; });
+  auto halves = [](double v, auto&& swap) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    auto lo = swap((uint32_t)b), hi = swap((uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+           __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+  };
+  v = halves(v, [](uint32_t w) { return __builtin_amdgcn_permlane16_swap(w, w, false, false); });
+  return halves(v, [](uint32_t w) { return __builtin_amdgcn_permlane32_swap(w, w, false, false); });
+}
+
+// Running sums over the wave: rows of 16 by shifts, then the rows before.
+__device__ __forceinline__ double wave_scan64(double v) {
+  auto add = [&](auto ctrl, auto rows) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)b, decltype(ctrl)::value,
+                                                    decltype(rows)::value, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(b >> 32), decltype(ctrl)::value,
+                                                    decltype(rows)::value, 0xf, false);
+    v += __builtin_bit_cast(double, lo | (uint64_t)hi << 32);
+  };
+  add(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());
+  add(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+  add(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+  add(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+  add(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // row 0 to 1, 2 to 3
+  add(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // rows 0, 1 to 2, 3
   return v;
 }
 
@@ -900,8 +991,7 @@ __device__ __forceinline__ float heat_of(const VerifyArgs& A, int s) {
 
 // 8 values from p on, the first `count` of them; rows start on any 2 (or 4) bytes.
 __device__ __forceinline__ u32x4 logits8(const uint16_t* p, int count) {
-  typedef u32x4 __attribute__((aligned(2))) Any;
-  if (count >= 8) return *(const GLOBAL_AS Any*)p;
+  if (count >= 8) return load_words4(p);
   u32x4 v = {0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};  // -inf
 #pragma unroll
   for (int e = 0; e < 7; ++e)
@@ -922,13 +1012,17 @@ __device__ __forceinline__ void probs8(const float* p, int count, float (&v)[8])
     for (int e = 0; e < 8; ++e) v[e] = e < count ? p[e] : 0.0f;
   }
 }
-__device__ __forceinline__ float value_of(u32x4 v, int e) {
-  return logit((uint16_t)(v[e >> 1] >> (16 * (e & 1))));
+// the largest of 8, no NaN
+__device__ __forceinline__ float top8(u32x4 v) {
+  f16x2 a = as_f16x2(v[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) a = __builtin_elementwise_max(a, as_f16x2(v[i]));
+  return fmaxf(fmaxf((float)a.x, (float)a.y), -__builtin_inff());
 }
 
 template <int V>
 __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
-  __shared__ double table[64], sums[4];
+  __shared__ double table[16], sums[4];
   __shared__ float tops[4];
   __shared__ int firsts[4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -938,41 +1032,42 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   u32x4 v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8);
+  if (chunk == 0)  // the next launch counts its workgroups from 0
+    for (int i = row + t * A.b.rows; i < A.b.seqs; i += 256 * A.b.rows) A.count[i] = 0;
   int lo, m;
   const int s = seq_of_row(A.b, row, lo, m);
   if (s < 0) return;
   const float heat = heat_of(A, s);
-  if (t < 64) table[t] = kExp2[t];
+  const double unit = unit_of(heat);
+  if (t < 16) table[t] = kExp2[t];
   float top = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, value_of(v[i], e));
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  for (int i = 0; i < V; ++i) top = fmaxf(top, top8(v[i]));
+  top = wave_max(top);
   if (lane == 0) tops[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   int first = 0x7fffffff;
-#pragma unroll
-  for (int i = V - 1; i >= 0; --i)
-#pragma unroll
-    for (int e = 7; e >= 0; --e)
-      if (value_of(v[i], e) == top) first = begin + (i * 256 + t) * 8 + e;
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const int f = __shfl_xor(first, d);
-    first = f < first ? f : first;
-  }
   double sum = 0.0;
-  if (heat > 0.0f && top > -__builtin_inff()) {
-    const Exp weight(table, top, heat);
+  if (!(heat > 0.0f)) {
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i)
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (half_at(v[i], e) == top) first = begin + (i * 256 + t) * 8 + e;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      const int f = __shfl_xor(first, d);
+      first = f < first ? f : first;
+    }
+  } else if (top > -__builtin_inff()) {
+    const Exp weight(table, top, unit);
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += weight(value_of(v[i], e));
+      for (int e = 0; e < 8; ++e) sum += weight(half_at(v[i], e));
+    sum = wave_sum64(sum);
   }
-  sum = wave_sum64(sum);
   if (lane == 0) {
     sums[wave] = sum;
     firsts[wave] = first;
@@ -985,55 +1080,73 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   }
 }
 
-// The rows of sequence s joined from their chunks into st, and how many drafted tokens
-// stand; every thread of the 256 gets that number.
-__device__ __forceinline__ int verify_join(const VerifyArgs& A, int s, int lo, int m, float heat,
-                                           const double* table, VerifyStat* st, int* stop) {
-  const int t = threadIdx.x, lane = t & 63;
-  if (t == 0) *stop = m - 1;
-  __syncthreads();
-  for (int i = t >> 6; i < m; i += 4) {
-    const VerifyStat* stats = A.stats + (int64_t)(lo + i) * A.chunks;
-    float top = -__builtin_inff();
-    for (int c = lane; c < A.chunks; c += 64) top = fmaxf(top, stats[c].top);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    double total = 0.0;
-    int first = 0x7fffffff;
-    const Exp weight(table, top, heat > 0.0f ? heat : 1.0f);
-    for (int c = lane; c < A.chunks; c += 64) {
-      const VerifyStat x = stats[c];
-      if (x.top == -__builtin_inff()) continue;
-      if (x.top == top && x.first < first) first = x.first;
-      if (heat > 0.0f) total += x.sum * weight(x.top);
-    }
-    total = wave_sum64(total);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const int other = __shfl_xor(first, d);
-      first = other < first ? other : first;
-    }
-    if (lane == 0) st[i] = {heat > 0.0f ? total : 1.0, top, first};
-  }
-  __syncthreads();
+// What thread t < m - 1 knows of the token drafted behind row t: the token (-1: none
+// of the vocabulary's) and its logit.
+struct Told {
+  int token;
+  float logit;
+};
+
+// The rows of a sequence joined from their chunks into st, 16 lanes a row, and how many
+// drafted tokens stand; every thread of the 256 gets that number.
+__device__ __forceinline__ int verify_join(const VerifyArgs& A, int lo, int m, float heat,
+                                           double unit, const double* table, VerifyStat* st,
+                                           uint64_t* stops, Told& told) {
+  const int t = threadIdx.x, c16 = t & 15;
+  // what the test of token t needs is requested ahead of the chunks
+  told = {-1, 0.0f};
+  float u = 0.0f, d = 1.0f;
   if (t < m - 1) {
     const int x = A.tokens[lo + t + 1];
-    bool yes = false;
-    if (x >= 0 && x < A.vocab && st[t].top > -__builtin_inff()) {
-      const float v = logit(A.logits[(int64_t)(lo + t) * A.logits_stride + x]);
-      const double p = heat > 0.0f ? Exp(table, st[t].top, heat)(v) / st[t].sum
-                                   : (x == st[t].first ? 1.0 : 0.0);
-      double q = 1.0;
-      if (A.draft) {
-        const float d = A.draft[(int64_t)(lo + t) * A.draft_stride + x];
-        q = d > 0.0f ? (double)d : 0.0;
-      }
-      yes = (double)A.uniform[lo + t] * q < p;
+    u = A.uniform[lo + t];
+    if (x >= 0 && x < A.vocab) {
+      told = {x, (float)as_half(A.logits[(int64_t)(lo + t) * A.logits_stride + x])};
+      if (A.draft) d = A.draft[(int64_t)(lo + t) * A.draft_stride + x];
     }
-    if (!yes) atomicMin(stop, t);
   }
   __syncthreads();
-  return *stop;
+  for (int i = t >> 4; i < m; i += 16) {
+    const VerifyStat* stats = A.stats + (int64_t)(lo + i) * A.chunks;
+    float top = -__builtin_inff();
+    for (int c = c16; c < A.chunks; c += 16) top = fmaxf(top, stats[c].top);
+    top = row_max16(top);
+    double total = 0.0;
+    int first = 0x7fffffff;
+    const Exp weight(table, top, unit);
+    for (int c = c16; c < A.chunks; c += 16) {
+      const VerifyStat v = stats[c];
+      if (v.top == -__builtin_inff()) continue;
+      if (v.top == top && v.first < first) first = v.first;
+      total += v.sum * weight(v.top);
+    }
+    total = over_head<128>(total, [](double a, double b) { return a + b; });
+    if (!(heat > 0.0f)) {
+      total = 1.0;
+#pragma unroll
+      for (int k = 8; k > 0; k >>= 1) {
+        const int other = __shfl_xor(first, k);
+        first = other < first ? other : first;
+      }
+    }
+    if (c16 == 0) st[i] = {total, top, first};
+  }
+  __syncthreads();
+  bool no = t >= m - 1;
+  if (!no) {
+    const VerifyStat row = st[t];
+    const double e = heat > 0.0f ? Exp(table, row.top, unit)(told.logit)
+                                 : (told.token == row.first ? 1.0 : 0.0);
+    no = !(told.token >= 0 && row.top > -__builtin_inff() &&
+           (double)u * (d > 0.0f ? (double)d : 0.0) * row.sum < e);
+  }
+  const uint64_t mask = __builtin_amdgcn_ballot_w64(no);
+  if ((t & 63) == 0) stops[t >> 6] = mask;
+  __syncthreads();
+  int n = 0;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (n == 64 * g) n += stops[g] ? __builtin_ctzll(stops[g]) : 64;
+  return n < m - 1 ? n : m - 1;
 }
 
 // What an entry of the deciding row weighs: max(p - q, 0) and p.
@@ -1042,193 +1155,223 @@ struct Decide {
   double inv_total;
   bool greedy, refused, drafted;
   int first, told;  // the maximum's lowest index, the refused token
-  __device__ __forceinline__ Decide(const VerifyArgs& A, const double* table, int lo, int m, int n,
-                                    float heat, const VerifyStat& st)
-      : weight(table, st.top, heat > 0.0f ? heat : 1.0f), inv_total(1.0 / st.sum),
-        greedy(!(heat > 0.0f)), refused(n < m - 1), drafted(A.draft != nullptr), first(st.first),
-        told(refused ? A.tokens[lo + n + 1] : -1) {}
   __device__ __forceinline__ void operator()(int j, float x, float d, double& rest, double& p) const {
     p = greedy ? (j == first ? 1.0 : 0.0) : weight(x) * inv_total;
     rest = !refused ? 0.0 : drafted ? (d > 0.0f ? fmax(p - (double)d, 0.0) : p) : j == told ? 0.0 : p;
   }
 };
 
+__device__ __forceinline__ void put_sum(double* p, double v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get_sum(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 template <int V>
 __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
-  __shared__ double table[64], sums[4][2];
+  __shared__ double table[16], sum[4][2], base, hit_x;
   __shared__ VerifyStat st[256];
-  __shared__ int stop;
-  const int t = threadIdx.x, chunk = blockIdx.x, s = blockIdx.y;
+  __shared__ uint64_t stops[4], over[4], some_over[4];
+  __shared__ int refused_token, hit, arrived;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.y;
   const int lo = A.b.start ? A.b.start[s] : s;
   const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
-  if (m == 0) return;
-  const float heat = heat_of(A, s);
-  if (t < 64) table[t] = kExp2[t];
-  const int n = verify_join(A, s, lo, m, heat, table, st, &stop);
-  if (chunk == 0) {
-    for (int i = t; i < m; i += 256) A.rows[lo + i] = st[i];
-    if (t == 0) A.accepted[s] = n;
-  }
-  double rest = 0.0, all = 0.0;
-  if (st[n].top > -__builtin_inff()) {
-    const Decide w(A, table, lo, m, n, heat, st[n]);
-    const int begin = chunk * 2048 * V;
-    const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride + begin;
-    const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride + begin : nullptr;
-    u32x4 v[V];
-    float d[V][8] = {};
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int j = (i * 256 + t) * 8;
-      v[i] = logits8(x + j, A.vocab - begin - j);
-      if (q) probs8(q + j, A.vocab - begin - j, d[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        double r, p;
-        w(begin + (i * 256 + t) * 8 + e, value_of(v[i], e), d[i][e], r, p);
-        rest += r;
-        all += p;
-      }
-  }
-  rest = wave_sum64(rest);
-  all = wave_sum64(all);
-  if ((t & 63) == 0) {
-    sums[t >> 6][0] = rest;
-    sums[t >> 6][1] = all;
-  }
-  __syncthreads();
-  if (t < 2)
-    A.rest[((int64_t)s * A.chunks + chunk) * 2 + t] =
-        (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
-}
-
-// The sum of v over the threads before this one, and over all 256 (two barriers).
-__device__ __forceinline__ double block_before(double v, double* waves, double& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double c = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double other = __shfl_up(c, d);
-    if (lane >= d) c += other;
-  }
-  if (lane == 63) waves[wave] = c;
-  __syncthreads();
-  double before = 0.0;
-  total = 0.0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += waves[w];
-    total += waves[w];
-  }
-  __syncthreads();
-  return before + (c - v);
-}
-
-template <int V>
-__device__ __forceinline__ void verify_take(const VerifyArgs& A) {
-  __shared__ double table[64], waves[4], base;
-  __shared__ int found, last;
-  const int t = threadIdx.x, s = blockIdx.x;
-  const int lo = A.b.start ? A.b.start[s] : s;
-  const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
-  const float heat = heat_of(A, s);
-  int n = 0, token = -1;
+  int32_t* const out = A.out + s * A.out_stride;
+  float* const logprob = A.logprob ? A.logprob + s * A.out_stride : nullptr;
   if (m == 0) {
+    if (blockIdx.x > 0) return;
     if (t == 0) A.accepted[s] = 0;
-  } else {
-    if (t < 64) table[t] = kExp2[t];
-    n = A.accepted[s];
-    const VerifyStat st = A.rows[lo + n];
-    const double* sums = A.rest + (int64_t)s * A.chunks * 2;
-    if (st.top > -__builtin_inff()) {
-      const Decide w(A, table, lo, m, n, heat, st);
-      double total[2] = {0.0, 0.0};
-      for (int c = t; c < A.chunks; c += 256) {
-        total[0] += sums[2 * c];
-        total[1] += sums[2 * c + 1];
-      }
+    if (t < A.b.max_rows) {
+      out[t] = -1;
+      if (logprob) logprob[t] = 0.0f;
+    }
+    return;
+  }
+  const float heat = heat_of(A, s), u = A.uniform[lo + m - 1];
+  const double unit = unit_of(heat);
+  if (t < 16) table[t] = kExp2[t];
+  Told told;
+  const int n = verify_join(A, lo, m, heat, unit, table, st, stops, told);
+  const bool refused = n < m - 1;
+  if (t == n) refused_token = told.token;
+  __syncthreads();
+  const VerifyStat row = st[n];
+  const Decide w = {Exp(table, row.top, unit), 1.0 / row.sum, !(heat > 0.0f), refused,
+                    A.draft != nullptr, row.first, refused_token};
+  const bool some = row.top > -__builtin_inff();
+  const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
+  const float* q = w.drafted && refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
+  // entries j .. j + 7
+  auto sum8 = [&](int j, u32x4 v, const float (&d)[8], double& rest, double& all) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) (void)block_before(total[k], waves, total[k]);
-      const int k = w.refused && total[0] > 0.0 ? 0 : 1;
-      const double goal = (double)A.uniform[lo + m - 1] * total[k];
-      // the chunk whose running sum passes the goal, else the last that weighs anything
-      if (t == 0) {
-        found = 0x7fffffff;
-        last = -1;
+    for (int e = 0; e < 8; ++e) {
+      double r, p;
+      w(j + e, half_at(v, e), d[e], r, p);
+      rest += r;
+      all += p;
+    }
+  };
+  auto request8 = [&](int j, u32x4& v, float (&d)[8]) {
+    v = logits8(x + j, A.vocab - j);
+    if (q) probs8(q + j, A.vocab - j, d);
+  };
+  // Pairs of sums, one pair a thread: those of the threads before, and of all.
+  auto running = [&](const double (&v)[2], double (&before)[2], double (&total)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const double c = wave_scan64(v[k]);
+      if (lane == 63) sum[wave][k] = c;
+      before[k] = c - v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      total[k] = 0.0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (g == wave) before[k] += total[k];
+        total[k] += sum[g][k];
       }
-      double sum = 0.0;
-      for (int c0 = 0; c0 < A.chunks; c0 += 256) {
-        const int c = c0 + t;
-        const double here = c < A.chunks ? sums[2 * c + k] : 0.0;
-        double all;
-        const double before = sum + block_before(here, waves, all);
-        if (here > 0.0) {
-          if (before + here > goal) atomicMin(&found, c);
-          atomicMax(&last, c);
-        }
-        __syncthreads();
-        // (a chunk found in an earlier round stays)
-        if (c == (found != 0x7fffffff ? found : last)) base = before;
-        sum += all;
-        __syncthreads();
-        if (found != 0x7fffffff) break;
+    }
+    __syncthreads();
+  };
+  double* const sums = A.rest + (int64_t)s * A.chunks * 2;
+  {
+    double here[2] = {0.0, 0.0}, before[2], total[2];
+    if (some) {
+      const int j0 = blockIdx.x * 2048 * V + t * 8;
+      u32x4 v;
+      float d[8] = {};
+      request8(j0, v, d);
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        u32x4 v_next;
+        float d_next[8] = {};
+        if (i + 1 < V) request8(j0 + 2048 * (i + 1), v_next, d_next);
+        sum8(j0 + 2048 * i, v, d, here[0], here[1]);
+        v = v_next;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = d_next[e];
       }
-      const int chunk = found != 0x7fffffff ? found : last;
+    }
+    running(here, before, total);
+    if (t < 2) put_sum(sums + 2 * blockIdx.x + t, total[t]);
+  }
+  wait_vm<0>();
+  __syncthreads();
+  if (t == 0)
+    arrived = __hip_atomic_fetch_add(A.count + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived != A.chunks - 1) return;
+  // The last workgroup of the sequence takes the token.
+  int token = -1;
+  if (some) {
+    auto request = [&](int c0, double (&v)[2]) {
+      const bool is = c0 + t < A.chunks;
+      v[0] = is ? get_sum(sums + 2 * (c0 + t)) : 0.0;
+      v[1] = is ? get_sum(sums + 2 * (c0 + t) + 1) : 0.0;
+    };
+    double here[2], before[2], total[2], all[2];
+    request(0, here);
+    running(here, before, total);
+    for (int c0 = 256; c0 < A.chunks; c0 += 256) {
+      request(c0, here);
+      running(here, before, all);
+      total[0] += all[0];
+      total[1] += all[1];
+    }
+    const int k = refused && total[0] > 0.0 ? 0 : 1;
+    const double goal = (double)u * total[k];
+    // The first thread whose sum takes the running sum past the goal (then passed), else
+    // the last one that weighs anything, -1 where none does.
+    bool passed = false;
+    auto look = [&](double here, double before) {
+      const uint64_t a = __builtin_amdgcn_ballot_w64(here > 0.0 && before + here > goal);
+      const uint64_t b = __builtin_amdgcn_ballot_w64(here > 0.0);
+      if (lane == 0) {
+        over[wave] = a;
+        some_over[wave] = b;
+      }
       __syncthreads();
-      if (t == 0) {
-        found = 0x7fffffff;
-        last = -1;
+      int place = -1;
+      passed = false;
+#pragma unroll
+      for (int g = 3; g >= 0; --g) {
+        if (over[g]) {
+          place = 64 * g + __builtin_ctzll(over[g]);
+          passed = true;
+        } else if (!passed && place < 0 && some_over[g]) {
+          place = 64 * g + 63 - __builtin_clzll(some_over[g]);
+        }
       }
-      if (chunk >= 0) {
-        // 8 V values in a row a thread
-        const int begin = chunk * 2048 * V + t * 8 * V;
-        const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride + begin;
-        const float* q = w.drafted && w.refused ? A.draft + (int64_t)(lo + n) * A.draft_stride + begin : nullptr;
-        double c[8 * V], mine = 0.0;
-        int some = -1;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const u32x4 v = logits8(x + 8 * i, A.vocab - begin - 8 * i);
-          float d[8] = {};
-          if (q) probs8(q + 8 * i, A.vocab - begin - 8 * i, d);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            double r, p;
-            w(begin + 8 * i + e, value_of(v, e), d[e], r, p);
-            c[8 * i + e] = k ? p : r;
-            mine += c[8 * i + e];
-            if (c[8 * i + e] > 0.0) some = begin + 8 * i + e;
-          }
+      __syncthreads();
+      return place;
+    };
+    int chunk = -1;
+    double past = 0.0;
+    for (int c0 = 0; c0 < A.chunks && !passed; c0 += 256) {
+      if (A.chunks > 256) {
+        request(c0, here);
+        running(here, before, all);
+      }
+      const int place = look(here[k], past + before[k]);
+      if (place >= 0) chunk = c0 + place;
+      if (t == place) base = past + before[k];
+      if (A.chunks > 256) past += all[k];
+      __syncthreads();
+    }
+    if (chunk >= 0) {
+      // 8 V entries in a row a thread, then the one thread's, one entry a lane
+      const int j0 = chunk * 2048 * V + t * 8 * V;
+      double mine[2] = {0.0, 0.0}, run[2];
+#pragma unroll 1
+      for (int i = 0; i < V; ++i) {
+        u32x4 v;
+        float d[8] = {};
+        request8(j0 + 8 * i, v, d);
+        sum8(j0 + 8 * i, v, d, mine[0], mine[1]);
+      }
+      running(mine, run, all);
+      const double from = base + run[k];
+      const int place = look(mine[k], from);
+      if (t == place) base = from;
+      __syncthreads();
+      if (wave == 0 && place >= 0) {
+        const int j = chunk * 2048 * V + place * 8 * V + lane;
+        double f[2] = {0.0, 0.0};
+        float v = 0.0f;
+        if (lane < 8 * V && j < A.vocab) {
+          v = (float)as_half(x[j]);
+          w(j, v, q ? q[j] : 0.0f, f[0], f[1]);
         }
-        double all;
-        double run = base + block_before(mine, waves, all);
-        int hit = 0x7fffffff;
-#pragma unroll
-        for (int e = 0; e < 8 * V; ++e) {
-          run += c[e];
-          if (c[e] > 0.0 && run > goal && hit == 0x7fffffff) hit = begin + e;
+        const double c = base + wave_scan64(f[k]);  // (every lane takes part)
+        const uint64_t b = __builtin_amdgcn_ballot_w64(f[k] > 0.0);
+        const uint64_t a = __builtin_amdgcn_ballot_w64(f[k] > 0.0 && c > goal);
+        if (lane == (a ? __builtin_ctzll(a) : 63 - __builtin_clzll(b))) {
+          hit = j;
+          hit_x = v;
         }
-        if (hit != 0x7fffffff) atomicMin(&found, hit);
-        if (some >= 0) atomicMax(&last, some);
-        __syncthreads();
-        token = found != 0x7fffffff ? found : last;
+      }
+      __syncthreads();
+      if (place >= 0) {
+        token = hit;
+        if (t == n) told.logit = (float)hit_x;
       }
     }
   }
-  for (int i = t; i < A.b.max_rows; i += 256) {
-    const int x = m == 0 ? -1 : i < n ? A.tokens[lo + i + 1] : i == n ? token : -1;
-    A.out[s * A.out_stride + i] = x;
-    if (A.logprob) {
+  if (t == n) told.token = token;
+  if (t == 0) A.accepted[s] = n;
+  if (t < A.b.max_rows) {
+    const int y = t <= n ? told.token : -1;
+    out[t] = y;
+    if (logprob) {
       float lp = 0.0f;
-      if (x >= 0 && heat > 0.0f) {
-        const VerifyStat st = A.rows[lo + i];
-        const float v = logit(A.logits[(int64_t)(lo + i) * A.logits_stride + x]);
-        lp = (float)((v == st.top ? 0.0 : ((double)v - (double)st.top) / (double)heat) - log(st.sum));
+      if (y >= 0 && heat > 0.0f) {
+        const float v = told.logit, top = st[t].top;
+        lp = (float)((v == top ? 0.0 : ((double)v - (double)top) / (double)heat) - log(st[t].sum));
       }
-      A.logprob[s * A.out_stride + i] = lp;
+      logprob[t] = lp;
     }
   }
 }
@@ -1241,9 +1384,6 @@ __device__ __forceinline__ void verify_take(const VerifyArgs& A) {
   }                                                                                            \
   extern "C" __global__ __launch_bounds__(256) void verify_rest_##V(VerifyArgs A) {            \
     verify_rest<V>(A);                                                                         \
-  }                                                                                            \
-  extern "C" __global__ __launch_bounds__(256) void verify_take_##V(VerifyArgs A) {            \
-    verify_take<V>(A);                                                                         \
   }
 VERIFY(1)
 VERIFY(4)

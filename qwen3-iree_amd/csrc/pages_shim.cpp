@@ -19,7 +19,7 @@ struct {
   hipModule_t module = nullptr;
   // [head_dim 64, 128][f16, q8]
   hipFunction_t append[2][2] = {}, attn[2][2][3] = {}, read[2][2] = {};
-  hipFunction_t sums[2] = {}, rest[2] = {}, take[2] = {};  // chunks of 2048, 8192
+  hipFunction_t sums[2] = {}, rest[2] = {};  // chunks of 2048, 8192
 } c;
 
 int fail(int code, const char* fmt, ...) {
@@ -211,7 +211,6 @@ void pages_load(const char* path) {
   for (int i = 0; i < 2; ++i) {
     get(&c.sums[i], i ? "verify_sums_4" : "verify_sums_1");
     get(&c.rest[i], i ? "verify_rest_4" : "verify_rest_1");
-    get(&c.take[i], i ? "verify_take_4" : "verify_take_1");
   }
   if (!ok) {
     (void)hipModuleUnload(m);
@@ -384,7 +383,7 @@ size_t kv_verify_workspace_bytes(int32_t rows, int32_t seqs, int32_t vocab) {
       vocab > (1 << 24))
     return 0;
   const size_t chunks = (size_t)(vocab + 2047) / 2048;
-  return 16 * (chunks * ((size_t)rows + seqs) + rows);
+  return 16 * chunks * ((size_t)rows + seqs) + 4 * (size_t)seqs;
 }
 
 int kv_verify(const kv_drafts* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -429,14 +428,13 @@ int kv_verify(const kv_drafts* d, void* workspace, size_t workspace_bytes, void*
   const int chunk = verify_chunk(d->rows, d->vocab), i = chunk == 8192 ? 1 : 0;
   args.chunks = (d->vocab + chunk - 1) / chunk;
   args.stats = static_cast<VerifyStat*>(workspace);
-  args.rows = args.stats + (size_t)d->rows * args.chunks;
-  args.rest = reinterpret_cast<double*>(args.rows + d->rows);
+  args.rest = reinterpret_cast<double*>(args.stats + (size_t)d->rows * args.chunks);
+  args.count = reinterpret_cast<int32_t*>(args.rest + 2 * (size_t)d->seqs * args.chunks);
   void* p[] = {&args};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t chunks = (uint32_t)args.chunks;
   if ((rc = q8_shim::launch3(c.sums[i], chunks, (uint32_t)d->rows, 1, 256, p, st))) return rc;
-  if ((rc = q8_shim::launch3(c.rest[i], chunks, (uint32_t)d->seqs, 1, 256, p, st))) return rc;
-  return q8_shim::launch(c.take[i], (uint32_t)d->seqs, 256, p, st);
+  return q8_shim::launch3(c.rest[i], chunks, (uint32_t)d->seqs, 1, 256, p, st);
 }
 
 }  // extern "C"
