@@ -168,8 +168,9 @@ int kv_pages_read(const kv_pages* pages, int32_t layer, int32_t layers, const kv
  * rows in [1, 65535], seqs in [1, 1024], max_rows in [1, 256], out_stride >=
  * max_rows, vocab in [1, 2^24]; strides >= vocab; logits 2-byte, the others
  * 4-byte aligned.  workspace: kv_verify_workspace_bytes (256-byte aligned), needed
- * only during the call, nothing to initialise; calls that may overlap need one
- * each. */
+ * only during the call; fill it with zeros once before its first use.  That of the
+ * largest rows, seqs and vocab of a session serves all its calls; calls that may
+ * overlap need one each. */
 typedef struct kv_drafts {
   const void* logits;
   const int32_t* tokens;

@@ -85,11 +85,22 @@ struct PagesReadArgs {
 };
 
 constexpr int kSeqsMax = 1024;
-// A chunk's (or row's) maximum, its lowest index, and the sum of exp((x - top) / T).
+// Counters lie this many words apart: those of one cache line take their turns, 4 ns each.
+constexpr int kCountStep = 32;
+// A row's maximum, its lowest index, and the sum of exp((x - top) / T).
 struct VerifyStat {
   double sum;
   float top;
   int32_t first;
+};
+
+// What decides a sequence's last token: its row, 16 log2(e) / T and T, the accepted
+// tokens, the random number, and the token that was refused.
+struct VerifyPick {
+  VerifyStat row;
+  double unit;
+  float heat, u;
+  int32_t n, told;
 };
 
 struct VerifyArgs {
@@ -100,10 +111,12 @@ struct VerifyArgs {
   int32_t *out, *accepted;
   float* logprob;
   int64_t logits_stride, draft_stride, out_stride;
-  int32_t vocab, chunks;
-  VerifyStat* stats;  // [rows, chunks]
-  double* rest;       // [seqs, chunks, 2] sums of max(p - q, 0) and of p in the deciding row
-  int32_t* count;     // [seqs] workgroups that have left theirs
+  int32_t vocab, chunks, parts;  // chunks of a row in the first launch, parts in the second
+  int32_t* count;     // [2, kSeqsMax, kCountStep] workgroups of a sequence that have come to a launch's end
+  VerifyPick* picks;  // [seqs]
+  double* sums;       // [rows, chunks] of exp((x - top) / T)
+  double* tops;       // [rows, chunks] the maximum and its lowest index
+  double* rest;       // [seqs, parts, 2] sums of max(p - q, 0) and of p in the deciding row
 };
 
 #endif

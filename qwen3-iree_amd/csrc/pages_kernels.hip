@@ -10,21 +10,39 @@ namespace {
 constexpr float kLn2 = 0.693147180559945309f;
 
 // The sequence of row `row` (the wave's): the last whose start is not behind it, found
-// by counting, 64 starts a load.  lo: its first row, m: how many; -1: none's.
-__device__ __forceinline__ int seq_of_row(const PagesBatch& b, int row, int& lo, int& m) {
+// by counting, 64 sequences at a time.  lo: its first row, m: how many; -1: none's.  of: the
+// sequence's entry of `values` (null: left alone), requested with the starts.
+template <class V>
+__device__ __forceinline__ int seq_of_row(const PagesBatch& b, int row, int& lo, int& m,
+                                          const V* values, V& of) {
   if (!b.start) {
     lo = row;
     m = 1;
+    if (values) of = values[row];
     return row;
   }
   const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int i = lane; i - lane <= b.seqs; i += 64)
-    n += __popcll(__builtin_amdgcn_ballot_w64(i <= b.seqs && b.start[i <= b.seqs ? i : 0] <= row));
+  int n = 0, begin = 0, end = 0;
+  V value = V();
+  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+    const int s = s0 + lane < b.seqs ? s0 + lane : b.seqs - 1;
+    const int first = b.start[s], next = b.start[s + 1];
+    const V mine = values ? values[s] : V();
+    const int here =
+        __popcll(__builtin_amdgcn_ballot_w64(s0 + lane < b.seqs && first <= row));
+    if (here == 0) break;
+    n = s0 + here;
+    begin = first;
+    end = next;
+    value = mine;
+    if (here < 64) break;
+  }
   const int s = __builtin_amdgcn_readfirstlane(n) - 1;
-  if (s < 0 || s >= b.seqs) return -1;
-  lo = b.start[s];
-  m = rows_of(b, lo, b.start[s + 1]);
+  if (s < 0) return -1;
+  auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, s & 63); };
+  lo = pick(begin);
+  m = rows_of(b, lo, pick(end));
+  of = __builtin_bit_cast(V, pick(__builtin_bit_cast(int, value)));
   return row >= lo && row < lo + m ? s : -1;
 }
 
@@ -173,20 +191,22 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
   int h = t / G;
   u32x4 x = {};
   if (h < heads) x = request(h);
-  int lo, m;
-  const int s = seq_of_row(A.b, row, lo, m);
+  const int position = A.positions ? A.positions[row] : 0;
+  const double step = t < D / 2 ? A.turns[t] : 0.0;
+  int lo, m, length = 0;
+  const int s = seq_of_row(A.b, row, lo, m, A.b.length, length);
   if (s < 0) return;
-  const int64_t slot = (int64_t)A.b.length[s] - m + (row - lo);
+  const int64_t slot = (int64_t)length - m + (row - lo);
+  const int64_t to = pool_row(A.b, s, slot, A.kv_heads, 0);  // of head 0
   if (A.rotate) {
     if (t < D / 2) {
-      const double by = (double)(A.positions ? (int64_t)A.positions[row] : slot) * A.turns[t];
+      const double by = (double)(A.positions ? (int64_t)position : slot) * step;
       double2 a;
       sincospi(2.0 * (by - rint(by)), &a.y, &a.x);
       turn[t] = a;
     }
     __syncthreads();
   }
-  const int64_t to = pool_row(A.b, s, slot, A.kv_heads, 0);  // of head 0
   for (; h < heads; h += 256 / G) {
     const u32x4 here = x;
     if (h + 256 / G < heads) x = request(h + 256 / G);
@@ -852,10 +872,10 @@ __device__ __forceinline__ void pages_read(const PagesReadArgs& A) {
   const int lane = threadIdx.x & 63, layer = blockIdx.y;
   const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (row >= A.b.rows) return;
-  int lo, m;
-  const int s = seq_of_row(A.b, row, lo, m);
+  int lo, m, length = 0;
+  const int s = seq_of_row(A.b, row, lo, m, A.b.length, length);
   if (s < 0) return;
-  const int64_t slot = (int64_t)A.b.length[s] - m + (row - lo);
+  const int64_t slot = (int64_t)length - m + (row - lo);
   const int64_t rows = (int64_t)layer * A.b.pages * A.kv_heads * A.b.page_size;
   const int64_t to = layer * A.layer_stride + row * A.row_stride;
   for (int c = lane; c < A.kv_heads * (D / 8); c += 64) {
@@ -901,13 +921,14 @@ PAGES_READ(128, q8, true)
 // ---------------------------------------------------------------- verify ----
 //
 // verify_sums: a chunk of one row, its maximum, the maximum's lowest index and the
-// sum of exp((x - maximum) / T).  verify_rest: every workgroup of a sequence joins its
-// rows' chunks, finds the row that decides and sums max(p - q, 0) and p over its
-// chunk of it; the last of them finds the chunk and the index whose running sum passes
-// the random number, and writes the outputs.  All in f64: next to a border of the running sums, one
-// in 151936, f32 sums would give other tokens.  exp is 2^(n / 16) from a table (16
-// doubles: no two in one LDS bank) times a polynomial of degree 5 in the rest, |rest| <=
-// ln 2 / 32: 1.5e-13 of it is left out, for a third of the instructions of a full f64 exp.
+// sum of exp((x - maximum) / T); the last workgroup of a sequence joins the chunks of its
+// rows and finds the accepted tokens and the row that decides.  verify_rest: a part of that
+// row, the sums of max(p - q, 0) and of p; the last workgroup of a sequence finds the part
+// and the index whose running sum passes the random number.  All in f64: next to a
+// border of the running sums, one in 151936, f32 sums would give other tokens.  exp is
+// 2^(n / 16) from a table (16 doubles: no two in one LDS bank) times a polynomial of
+// degree 5 in the rest, |rest| <= ln 2 / 32: 1.5e-13 of it is left out, for a third of the
+// instructions of a full f64 exp.
 namespace {
 
 __constant__ double kExp2[16] = {  // 2^(n / 16)
@@ -917,31 +938,64 @@ __constant__ double kExp2[16] = {  // 2^(n / 16)
     0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0,
 };
 
-// exp((x - top) / T), 0 for a NaN.  The table lies in LDS.
+// exp((x - top) / T), 0 below 2^-1000 and for a NaN.  The table lies in LDS, the
+// polynomial's coefficients in scalar registers; n comes out of the low bits of a sum with
+// 1.5 2^52 and goes into the exponent by an addition (f64 roundings, conversions and
+// ldexp have a fraction of the rate).  Where top is +inf, which alone has weight then,
+// values go through near() first.
 struct Exp {
   const double* table;
   double top, unit;
-  bool far;  // top is +inf: it alone has weight
+  double c1, c2, c3, c4, c5, magic;
+  float least;  // x of 2^-1000, or less
+  bool far;
   // unit: unit_of(T)
-  __device__ __forceinline__ Exp(const double* table, float top, double unit)
-      : table(table), top((double)top), unit(unit), far(top == __builtin_inff()) {}
+  __device__ __forceinline__ Exp(const double* table, float top_of, double unit_of_heat)
+      : table(table), far(top_of == __builtin_inff()) {
+    const float at = far ? 0.0f : top_of;
+    top = (double)at;
+    // An f16 below `top` is further from it than |top| 2^-12 and 2^-24: a larger unit only
+    // takes 2^-1000 to something smaller.
+    unit = fmin(far ? 1.0 : unit_of_heat, (double)(16000.0f / fmaxf(fabsf(at) * 0x1p-12f, 0x1p-24f)));
+    c1 = 0x1.62e42fefa39efp-5;
+    c2 = 0x1.ebfbdff82c58fp-11;
+    c3 = 0x1.c6b08d704a0c0p-17;
+    c4 = 0x1.3b2ab6fba4e77p-23;
+    c5 = 0x1.5d87fe78a6731p-30;
+    magic = 6755399441055744.0;
+    asm("" : "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4), "+s"(c5), "+s"(magic));
+    least = at - 16000.0f / (float)unit;
+  }
+  __device__ __forceinline__ float near(float x) const {
+    return !far ? x : x == __builtin_inff() ? 0.0f : -__builtin_inff();
+  }
+  __device__ __forceinline__ u32x4 near(u32x4 v) const {
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = ((v[i] & 0xffffu) == 0x7c00u ? 0u : 0xfc00u) |
+               ((v[i] >> 16) == 0x7c00u ? 0u : 0xfc000000u);
+    }
+    return v;
+  }
+  // the same with 2^-1000, about, in the place of 0
+  __device__ __forceinline__ double some(float x) const {
+    const double z = ((double)fmaxf(x, least) - top) * unit;
+    const double y = z + magic, r = z - (y - magic);
+    const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, y);
+    const double p = fma(fma(fma(fma(fma(c5, r, c4), r, c3), r, c2), r, c1), r, 1.0) * table[i & 15];
+    const uint64_t b = __builtin_bit_cast(uint64_t, p);
+    const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(i >> 4) << 20);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
+  }
   __device__ __forceinline__ double operator()(float x) const {
-    if (far) return x == __builtin_inff() ? 1.0 : 0.0;
-    const double z = fmax(((double)x - top) * unit, -17500.0);  // 2^-1093 is 0; a NaN too
-    const double n = rint(z), r = z - n;
-    const int i = (int)n;
-    double p = 0x1.5d87fe78a6731p-30;
-    p = fma(p, r, 0x1.3b2ab6fba4e77p-23);
-    p = fma(p, r, 0x1.c6b08d704a0c0p-17);
-    p = fma(p, r, 0x1.ebfbdff82c58fp-11);
-    p = fma(p, r, 0x1.62e42fefa39efp-5);
-    p = fma(p, r, 1.0);
-    return ldexp(p * table[i & 15], i >> 4);
+    const double w = some(x);
+    return x > least ? w : 0.0;
   }
 };
 // 16 log2(e) / T; 0 where the maximum takes all
 __device__ __forceinline__ double unit_of(float heat) {
-  return heat > 0.0f ? 23.083120654223414519 / (double)heat : 0.0;
+  return heat > 0.0f ? fmax(23.083120654223414519 / (double)heat, 1e-30) : 1.0;
 }
 
 // The maximum over 16 lanes, and over the wave.
@@ -985,10 +1039,6 @@ __device__ __forceinline__ double wave_scan64(double v) {
   return v;
 }
 
-__device__ __forceinline__ float heat_of(const VerifyArgs& A, int s) {
-  return A.temperature ? A.temperature[s] : 1.0f;
-}
-
 // 8 values from p on, the first `count` of them; rows start on any 2 (or 4) bytes.
 __device__ __forceinline__ u32x4 logits8(const uint16_t* p, int count) {
   if (count >= 8) return load_words4(p);
@@ -1020,11 +1070,122 @@ __device__ __forceinline__ float top8(u32x4 v) {
   return fmaxf(fmaxf((float)a.x, (float)a.y), -__builtin_inff());
 }
 
+__device__ __forceinline__ void put_sum(double* p, double v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double get_sum(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+struct Top {  // a chunk's or row's maximum and, where it takes all, its lowest index
+  float top;
+  int first;
+};
+
+// Whether this workgroup is the last of `all` to come here with what it has left in memory
+// (past the L2s); the counter is 0 again behind it.  Every thread gets the answer.
+__device__ __forceinline__ bool last_here(int32_t* count, int all, int* arrived) {
+  wait_vm<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *arrived = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (*arrived == all - 1)
+      __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *arrived == all - 1;
+}
+
+__device__ __forceinline__ float log_of(float x, float top, double total, float heat) {
+  if (!(heat > 0.0f)) return 0.0f;
+  return (float)((x == top ? 0.0 : ((double)x - (double)top) / (double)heat) - log(total));
+}
+
+// The last workgroup of a sequence in the first launch: its rows joined from their
+// chunks, 16 lanes a row, the accepted tokens, and the row that decides.
+__device__ __forceinline__ void verify_pick(const VerifyArgs& A, int s, int lo, int m, float heat,
+                                            double unit, const double* table) {
+  __shared__ VerifyStat st[256];
+  __shared__ uint64_t stops[4];
+  const int t = threadIdx.x, c16 = t & 15;
+  // what the test of token t needs is requested ahead of the chunks
+  int told = -1;
+  float x = 0.0f, u = 0.0f, d = 1.0f;
+  if (t < m) u = A.uniform[lo + t];
+  if (t < m - 1) {
+    told = A.tokens[lo + t + 1];
+    if (told >= 0 && told < A.vocab) {
+      x = (float)as_half(A.logits[(int64_t)(lo + t) * A.logits_stride + told]);
+      if (A.draft) d = A.draft[(int64_t)(lo + t) * A.draft_stride + told];
+    } else {
+      told = -1;
+    }
+  }
+  for (int i = t >> 4; i < m; i += 16) {
+    const int64_t at = (int64_t)(lo + i) * A.chunks;
+    auto top_of = [&](int c) { return __builtin_bit_cast(Top, get_sum(A.tops + at + c)); };
+    float top = -__builtin_inff();
+    for (int c = c16; c < A.chunks; c += 16) top = fmaxf(top, top_of(c).top);
+    top = row_max16(top);
+    double total = 0.0;
+    int first = 0x7fffffff;
+    const Exp weight(table, top, unit);
+    for (int c = c16; c < A.chunks; c += 16) {
+      const double sum = get_sum(A.sums + at + c);
+      const Top v = top_of(c);
+      if (v.top == -__builtin_inff()) continue;
+      if (v.top == top && v.first < first) first = v.first;
+      total += sum * weight(weight.near(v.top));
+    }
+    total = over_head<128>(total, [](double a, double b) { return a + b; });
+    if (!(heat > 0.0f)) {
+      total = 1.0;
+#pragma unroll
+      for (int k = 8; k > 0; k >>= 1) {
+        const int other = __shfl_xor(first, k);
+        first = other < first ? other : first;
+      }
+    }
+    if (c16 == 0) st[i] = {total, top, first};
+  }
+  __syncthreads();
+  bool no = t >= m - 1;
+  if (!no) {
+    const VerifyStat row = st[t];
+    const Exp weight(table, row.top, unit);
+    const double e = heat > 0.0f ? weight(weight.near(x)) : (told == row.first ? 1.0 : 0.0);
+    no = !(told >= 0 && row.top > -__builtin_inff() &&
+           (double)u * (d > 0.0f ? (double)d : 0.0) * row.sum < e);
+  }
+  const uint64_t mask = __builtin_amdgcn_ballot_w64(no);
+  if ((t & 63) == 0) stops[t >> 6] = mask;
+  __syncthreads();
+  int n = 0;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (n == 64 * g) n += stops[g] ? __builtin_ctzll(stops[g]) : 64;
+  n = n < m - 1 ? n : m - 1;
+  if (t == 0) A.accepted[s] = n;
+  if (t == n) A.picks[s].told = told;
+  if (t == m - 1) A.picks[s].u = u;
+  if (t == 0) {
+    VerifyPick& p = A.picks[s];
+    p.row = st[n];
+    p.unit = unit;
+    p.heat = heat;
+    p.n = n;
+  }
+  if (t < A.b.max_rows && t != n) {
+    A.out[s * A.out_stride + t] = t < n ? told : -1;
+    if (A.logprob)
+      A.logprob[s * A.out_stride + t] = t < n ? log_of(x, st[t].top, st[t].sum, heat) : 0.0f;
+  }
+}
+
 template <int V>
 __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   __shared__ double table[16], sums[4];
   __shared__ float tops[4];
-  __shared__ int firsts[4];
+  __shared__ int firsts[4], arrived;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int chunk = blockIdx.x, row = blockIdx.y;
   const int begin = chunk * 2048 * V;
@@ -1032,14 +1193,13 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   u32x4 v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8);
-  if (chunk == 0)  // the next launch counts its workgroups from 0
-    for (int i = row + t * A.b.rows; i < A.b.seqs; i += 256 * A.b.rows) A.count[i] = 0;
-  int lo, m;
-  const int s = seq_of_row(A.b, row, lo, m);
-  if (s < 0) return;
-  const float heat = heat_of(A, s);
-  const double unit = unit_of(heat);
   if (t < 16) table[t] = kExp2[t];
+  int lo, m;
+  float heat = 1.0f;
+  const int s = seq_of_row(A.b, row, lo, m, A.temperature, heat);
+  if (s < 0) return;
+  if (!A.temperature) heat = 1.0f;
+  const double unit = unit_of(heat);
   float top = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < V; ++i) top = fmaxf(top, top8(v[i]));
@@ -1062,10 +1222,15 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
     }
   } else if (top > -__builtin_inff()) {
     const Exp weight(table, top, unit);
+    // (read again, from the L1: 8 at a time in one code, or registers cost occupancy)
+#pragma unroll 1
+    for (int i = 0; i < V; ++i) {
+      const u32x4 x8 = weight.near(logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8));
+      double w[8];
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += weight(half_at(v[i], e));
+      for (int e = 0; e < 8; ++e) w[e] = weight.some(half_at(x8, e));
+      sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    }
     sum = wave_sum64(sum);
   }
   if (lane == 0) {
@@ -1076,107 +1241,37 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   if (t == 0) {
 #pragma unroll
     for (int w = 1; w < 4; ++w) first = firsts[w] < first ? firsts[w] : first;
-    A.stats[(int64_t)row * A.chunks + chunk] = {(sums[0] + sums[1]) + (sums[2] + sums[3]), top, first};
+    const int64_t at = (int64_t)row * A.chunks + chunk;
+    put_sum(A.sums + at, (sums[0] + sums[1]) + (sums[2] + sums[3]));
+    put_sum(A.tops + at, __builtin_bit_cast(double, Top{top, first}));
   }
-}
-
-// What thread t < m - 1 knows of the token drafted behind row t: the token (-1: none
-// of the vocabulary's) and its logit.
-struct Told {
-  int token;
-  float logit;
-};
-
-// The rows of a sequence joined from their chunks into st, 16 lanes a row, and how many
-// drafted tokens stand; every thread of the 256 gets that number.
-__device__ __forceinline__ int verify_join(const VerifyArgs& A, int lo, int m, float heat,
-                                           double unit, const double* table, VerifyStat* st,
-                                           uint64_t* stops, Told& told) {
-  const int t = threadIdx.x, c16 = t & 15;
-  // what the test of token t needs is requested ahead of the chunks
-  told = {-1, 0.0f};
-  float u = 0.0f, d = 1.0f;
-  if (t < m - 1) {
-    const int x = A.tokens[lo + t + 1];
-    u = A.uniform[lo + t];
-    if (x >= 0 && x < A.vocab) {
-      told = {x, (float)as_half(A.logits[(int64_t)(lo + t) * A.logits_stride + x])};
-      if (A.draft) d = A.draft[(int64_t)(lo + t) * A.draft_stride + x];
-    }
-  }
-  __syncthreads();
-  for (int i = t >> 4; i < m; i += 16) {
-    const VerifyStat* stats = A.stats + (int64_t)(lo + i) * A.chunks;
-    float top = -__builtin_inff();
-    for (int c = c16; c < A.chunks; c += 16) top = fmaxf(top, stats[c].top);
-    top = row_max16(top);
-    double total = 0.0;
-    int first = 0x7fffffff;
-    const Exp weight(table, top, unit);
-    for (int c = c16; c < A.chunks; c += 16) {
-      const VerifyStat v = stats[c];
-      if (v.top == -__builtin_inff()) continue;
-      if (v.top == top && v.first < first) first = v.first;
-      total += v.sum * weight(v.top);
-    }
-    total = over_head<128>(total, [](double a, double b) { return a + b; });
-    if (!(heat > 0.0f)) {
-      total = 1.0;
-#pragma unroll
-      for (int k = 8; k > 0; k >>= 1) {
-        const int other = __shfl_xor(first, k);
-        first = other < first ? other : first;
-      }
-    }
-    if (c16 == 0) st[i] = {total, top, first};
-  }
-  __syncthreads();
-  bool no = t >= m - 1;
-  if (!no) {
-    const VerifyStat row = st[t];
-    const double e = heat > 0.0f ? Exp(table, row.top, unit)(told.logit)
-                                 : (told.token == row.first ? 1.0 : 0.0);
-    no = !(told.token >= 0 && row.top > -__builtin_inff() &&
-           (double)u * (d > 0.0f ? (double)d : 0.0) * row.sum < e);
-  }
-  const uint64_t mask = __builtin_amdgcn_ballot_w64(no);
-  if ((t & 63) == 0) stops[t >> 6] = mask;
-  __syncthreads();
-  int n = 0;
-#pragma unroll
-  for (int g = 0; g < 4; ++g)
-    if (n == 64 * g) n += stops[g] ? __builtin_ctzll(stops[g]) : 64;
-  return n < m - 1 ? n : m - 1;
+  if (last_here(A.count + s * kCountStep, m * A.chunks, &arrived)) verify_pick(A, s, lo, m, heat, unit, table);
 }
 
 // What an entry of the deciding row weighs: max(p - q, 0) and p.
 struct Decide {
   Exp weight;
   double inv_total;
-  bool greedy, refused, drafted;
+  bool greedy, drafted;
   int first, told;  // the maximum's lowest index, the refused token
   __device__ __forceinline__ void operator()(int j, float x, float d, double& rest, double& p) const {
-    p = greedy ? (j == first ? 1.0 : 0.0) : weight(x) * inv_total;
-    rest = !refused ? 0.0 : drafted ? (d > 0.0f ? fmax(p - (double)d, 0.0) : p) : j == told ? 0.0 : p;
+    p = weight(x) * inv_total;
+    if (greedy) p = j == first ? 1.0 : 0.0;
+    rest = drafted ? (d > 0.0f ? fmax(p - (double)d, 0.0) : p) : j == told ? 0.0 : p;
   }
 };
 
-__device__ __forceinline__ void put_sum(double* p, double v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ double get_sum(const double* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
+// V parts of 2048 entries a workgroup.
 template <int V>
 __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
-  __shared__ double table[16], sum[4][2], base, hit_x;
-  __shared__ VerifyStat st[256];
-  __shared__ uint64_t stops[4], over[4], some_over[4];
-  __shared__ int refused_token, hit, arrived;
+  __shared__ double table[16], sum[4][2], part_sum[4][V][2], base;
+  __shared__ uint64_t over[4], some_over[4];
+  __shared__ int arrived;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.y;
   const int lo = A.b.start ? A.b.start[s] : s;
   const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
+  const VerifyPick pick = A.picks[s];
+  if (t < 16) table[t] = kExp2[t];
   int32_t* const out = A.out + s * A.out_stride;
   float* const logprob = A.logprob ? A.logprob + s * A.out_stride : nullptr;
   if (m == 0) {
@@ -1188,32 +1283,25 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
     }
     return;
   }
-  const float heat = heat_of(A, s), u = A.uniform[lo + m - 1];
-  const double unit = unit_of(heat);
-  if (t < 16) table[t] = kExp2[t];
-  Told told;
-  const int n = verify_join(A, lo, m, heat, unit, table, st, stops, told);
+  // (starts that descend may have left a sequence without a pick)
+  if (blockIdx.x == 0 && t == 0) A.count[s * kCountStep] = 0;
+  const int n = pick.n < 0 ? 0 : pick.n < m ? pick.n : m - 1;
   const bool refused = n < m - 1;
-  if (t == n) refused_token = told.token;
-  __syncthreads();
-  const VerifyStat row = st[n];
-  const Decide w = {Exp(table, row.top, unit), 1.0 / row.sum, !(heat > 0.0f), refused,
-                    A.draft != nullptr, row.first, refused_token};
-  const bool some = row.top > -__builtin_inff();
+  const Decide w = {Exp(table, pick.row.top, pick.unit), 1.0 / pick.row.sum, !(pick.heat > 0.0f),
+                    A.draft != nullptr, pick.row.first, pick.told};
+  const bool some = pick.row.top > -__builtin_inff();
   const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
   const float* q = w.drafted && refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
   // entries j .. j + 7
   auto sum8 = [&](int j, u32x4 v, const float (&d)[8], double& rest, double& all) {
+    double r[8], p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      double r, p;
-      w(j + e, half_at(v, e), d[e], r, p);
-      rest += r;
-      all += p;
-    }
+    for (int e = 0; e < 8; ++e) w(j + e, half_at(v, e), d[e], r[e], p[e]);
+    rest += ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+    all += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
   };
   auto request8 = [&](int j, u32x4& v, float (&d)[8]) {
-    v = logits8(x + j, A.vocab - j);
+    v = w.weight.near(logits8(x + j, A.vocab - j));
     if (q) probs8(q + j, A.vocab - j, d);
   };
   // Pairs of sums, one pair a thread: those of the threads before, and of all.
@@ -1236,143 +1324,131 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
     }
     __syncthreads();
   };
-  double* const sums = A.rest + (int64_t)s * A.chunks * 2;
+  __syncthreads();  // the table
+  double* const sums = A.rest + (int64_t)s * A.parts * 2;
   {
-    double here[2] = {0.0, 0.0}, before[2], total[2];
+    const int part0 = blockIdx.x * V;
+    u32x4 v[V];
+    float d[V][8] = {};
     if (some) {
-      const int j0 = blockIdx.x * 2048 * V + t * 8;
-      u32x4 v;
-      float d[8] = {};
-      request8(j0, v, d);
-#pragma unroll 1
-      for (int i = 0; i < V; ++i) {
-        u32x4 v_next;
-        float d_next[8] = {};
-        if (i + 1 < V) request8(j0 + 2048 * (i + 1), v_next, d_next);
-        sum8(j0 + 2048 * i, v, d, here[0], here[1]);
-        v = v_next;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = d_next[e];
+      for (int i = 0; i < V; ++i) request8((part0 + i) * 2048 + t * 8, v[i], d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      double rest = 0.0, all = 0.0;
+      if (some) {
+        sum8((part0 + i) * 2048 + t * 8, v[i], d[i], rest, all);
+        rest = wave_sum64(rest);
+        all = wave_sum64(all);
+      }
+      if (lane == 0) {
+        part_sum[wave][i][0] = rest;
+        part_sum[wave][i][1] = all;
       }
     }
-    running(here, before, total);
-    if (t < 2) put_sum(sums + 2 * blockIdx.x + t, total[t]);
+    __syncthreads();
+    const double* const p = &part_sum[0][0][0];
+    if (t < 2 * V && part0 + (t >> 1) < A.parts)
+      put_sum(sums + 2 * part0 + t, (p[t] + p[2 * V + t]) + (p[4 * V + t] + p[6 * V + t]));
   }
-  wait_vm<0>();
-  __syncthreads();
-  if (t == 0)
-    arrived = __hip_atomic_fetch_add(A.count + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (arrived != A.chunks - 1) return;
+  if (!last_here(A.count + (kSeqsMax + s) * kCountStep, gridDim.x, &arrived)) return;
   // The last workgroup of the sequence takes the token.
-  int token = -1;
-  if (some) {
-    auto request = [&](int c0, double (&v)[2]) {
-      const bool is = c0 + t < A.chunks;
-      v[0] = is ? get_sum(sums + 2 * (c0 + t)) : 0.0;
-      v[1] = is ? get_sum(sums + 2 * (c0 + t) + 1) : 0.0;
-    };
-    double here[2], before[2], total[2], all[2];
-    request(0, here);
-    running(here, before, total);
-    for (int c0 = 256; c0 < A.chunks; c0 += 256) {
+  auto give = [&](int token, float of) {
+    out[n] = token;
+    if (logprob) logprob[n] = token < 0 ? 0.0f : log_of(of, pick.row.top, pick.row.sum, pick.heat);
+  };
+  if (!some) {
+    if (t == 0) give(-1, 0.0f);
+    return;
+  }
+  auto request = [&](int c0, double (&v)[2]) {
+    const bool is = c0 + t < A.parts;
+    v[0] = is ? get_sum(sums + 2 * (c0 + t)) : 0.0;
+    v[1] = is ? get_sum(sums + 2 * (c0 + t) + 1) : 0.0;
+  };
+  double here[2], before[2], total[2], all[2];
+  request(0, here);
+  running(here, before, total);
+  for (int c0 = 256; c0 < A.parts; c0 += 256) {
+    request(c0, here);
+    running(here, before, all);
+    total[0] += all[0];
+    total[1] += all[1];
+  }
+  const int k = refused && total[0] > 0.0 ? 0 : 1;
+  const double goal = (double)pick.u * total[k];
+  // The first thread whose sum takes the running sum past the goal (then passed), else
+  // the last one that weighs anything, -1 where none does.
+  bool passed = false;
+  auto look = [&](double here, double before) {
+    const uint64_t a = __builtin_amdgcn_ballot_w64(here > 0.0 && before + here > goal);
+    const uint64_t b = __builtin_amdgcn_ballot_w64(here > 0.0);
+    if (lane == 0) {
+      over[wave] = a;
+      some_over[wave] = b;
+    }
+    __syncthreads();
+    int place = -1;
+    passed = false;
+#pragma unroll
+    for (int g = 3; g >= 0; --g) {
+      if (over[g]) {
+        place = 64 * g + __builtin_ctzll(over[g]);
+        passed = true;
+      } else if (!passed && place < 0 && some_over[g]) {
+        place = 64 * g + 63 - __builtin_clzll(some_over[g]);
+      }
+    }
+    __syncthreads();
+    return place;
+  };
+  int part = -1;
+  double past = 0.0;
+  for (int c0 = 0; c0 < A.parts && !passed; c0 += 256) {
+    if (A.parts > 256) {
       request(c0, here);
       running(here, before, all);
-      total[0] += all[0];
-      total[1] += all[1];
     }
-    const int k = refused && total[0] > 0.0 ? 0 : 1;
-    const double goal = (double)u * total[k];
-    // The first thread whose sum takes the running sum past the goal (then passed), else
-    // the last one that weighs anything, -1 where none does.
-    bool passed = false;
-    auto look = [&](double here, double before) {
-      const uint64_t a = __builtin_amdgcn_ballot_w64(here > 0.0 && before + here > goal);
-      const uint64_t b = __builtin_amdgcn_ballot_w64(here > 0.0);
-      if (lane == 0) {
-        over[wave] = a;
-        some_over[wave] = b;
-      }
-      __syncthreads();
-      int place = -1;
-      passed = false;
-#pragma unroll
-      for (int g = 3; g >= 0; --g) {
-        if (over[g]) {
-          place = 64 * g + __builtin_ctzll(over[g]);
-          passed = true;
-        } else if (!passed && place < 0 && some_over[g]) {
-          place = 64 * g + 63 - __builtin_clzll(some_over[g]);
-        }
-      }
-      __syncthreads();
-      return place;
-    };
-    int chunk = -1;
-    double past = 0.0;
-    for (int c0 = 0; c0 < A.chunks && !passed; c0 += 256) {
-      if (A.chunks > 256) {
-        request(c0, here);
-        running(here, before, all);
-      }
-      const int place = look(here[k], past + before[k]);
-      if (place >= 0) chunk = c0 + place;
-      if (t == place) base = past + before[k];
-      if (A.chunks > 256) past += all[k];
-      __syncthreads();
-    }
-    if (chunk >= 0) {
-      // 8 V entries in a row a thread, then the one thread's, one entry a lane
-      const int j0 = chunk * 2048 * V + t * 8 * V;
-      double mine[2] = {0.0, 0.0}, run[2];
-#pragma unroll 1
-      for (int i = 0; i < V; ++i) {
-        u32x4 v;
-        float d[8] = {};
-        request8(j0 + 8 * i, v, d);
-        sum8(j0 + 8 * i, v, d, mine[0], mine[1]);
-      }
-      running(mine, run, all);
-      const double from = base + run[k];
-      const int place = look(mine[k], from);
-      if (t == place) base = from;
-      __syncthreads();
-      if (wave == 0 && place >= 0) {
-        const int j = chunk * 2048 * V + place * 8 * V + lane;
-        double f[2] = {0.0, 0.0};
-        float v = 0.0f;
-        if (lane < 8 * V && j < A.vocab) {
-          v = (float)as_half(x[j]);
-          w(j, v, q ? q[j] : 0.0f, f[0], f[1]);
-        }
-        const double c = base + wave_scan64(f[k]);  // (every lane takes part)
-        const uint64_t b = __builtin_amdgcn_ballot_w64(f[k] > 0.0);
-        const uint64_t a = __builtin_amdgcn_ballot_w64(f[k] > 0.0 && c > goal);
-        if (lane == (a ? __builtin_ctzll(a) : 63 - __builtin_clzll(b))) {
-          hit = j;
-          hit_x = v;
-        }
-      }
-      __syncthreads();
-      if (place >= 0) {
-        token = hit;
-        if (t == n) told.logit = (float)hit_x;
-      }
-    }
+    const int place = look(here[k], past + before[k]);
+    if (place >= 0) part = c0 + place;
+    if (t == place) base = past + before[k];
+    if (A.parts > 256) past += all[k];
+    __syncthreads();
   }
-  if (t == n) told.token = token;
-  if (t == 0) A.accepted[s] = n;
-  if (t < A.b.max_rows) {
-    const int y = t <= n ? told.token : -1;
-    out[t] = y;
-    if (logprob) {
-      float lp = 0.0f;
-      if (y >= 0 && heat > 0.0f) {
-        const float v = told.logit, top = st[t].top;
-        lp = (float)((v == top ? 0.0 : ((double)v - (double)top) / (double)heat) - log(st[t].sum));
-      }
-      logprob[t] = lp;
-    }
+  if (part < 0) {  // a sum that is no number: there is no such index
+    if (t == 0) give(-1, 0.0f);
+    return;
+  }
+  // 8 entries in a row a thread, then the one thread's, one entry a lane
+  const int j0 = part * 2048 + t * 8;
+  double mine[2] = {0.0, 0.0}, run[2];
+  {
+    u32x4 v;
+    float d[8] = {};
+    request8(j0, v, d);
+    sum8(j0, v, d, mine[0], mine[1]);
+  }
+  running(mine, run, all);
+  const double from = base + run[k];
+  const int place = look(mine[k], from);
+  if (t == place) base = from;
+  __syncthreads();
+  if (wave > 0) return;
+  const int j = part * 2048 + place * 8 + lane;
+  double f[2] = {0.0, 0.0};
+  float v = 0.0f;
+  if (place >= 0 && lane < 8 && j < A.vocab) {
+    v = (float)as_half(x[j]);
+    w(j, w.weight.near(v), q ? q[j] : 0.0f, f[0], f[1]);
+  }
+  const double c = base + wave_scan64(f[k]);  // (every lane takes part)
+  const uint64_t b = __builtin_amdgcn_ballot_w64(f[k] > 0.0);
+  const uint64_t a = __builtin_amdgcn_ballot_w64(f[k] > 0.0 && c > goal);
+  if (b == 0) {
+    if (lane == 0) give(-1, 0.0f);
+  } else if (lane == (a ? __builtin_ctzll(a) : 63 - __builtin_clzll(b))) {
+    give(j, v);
   }
 }
 

@@ -179,6 +179,9 @@ size_t attn_workspace(const kv_pages* a, const AttnPlan& p) {
   return kCountBytes + wgs * p.parts() * (a->head_dim + 2) * 4;
 }
 
+// The counters, in front where no layout of the rest reaches.
+constexpr size_t kVerifyCounts = 2 * kSeqsMax * kCountStep * sizeof(int32_t);
+
 // Logits of a workgroup: 8192, or 2048 where that leaves CUs without a workgroup.
 int verify_chunk(int32_t rows, int32_t vocab) {
   return (int64_t)rows * ((vocab + 8191) / 8192) >= q8_shim::compute_units() ? 8192 : 2048;
@@ -383,7 +386,7 @@ size_t kv_verify_workspace_bytes(int32_t rows, int32_t seqs, int32_t vocab) {
       vocab > (1 << 24))
     return 0;
   const size_t chunks = (size_t)(vocab + 2047) / 2048;
-  return 16 * chunks * ((size_t)rows + seqs) + 4 * (size_t)seqs;
+  return kVerifyCounts + 16 * chunks * ((size_t)rows + seqs) + sizeof(VerifyPick) * (size_t)seqs;
 }
 
 int kv_verify(const kv_drafts* d, void* workspace, size_t workspace_bytes, void* stream) {
@@ -425,16 +428,21 @@ int kv_verify(const kv_drafts* d, void* workspace, size_t workspace_bytes, void*
   args.draft_stride = d->draft_stride;
   args.out_stride = d->out_stride;
   args.vocab = d->vocab;
-  const int chunk = verify_chunk(d->rows, d->vocab), i = chunk == 8192 ? 1 : 0;
+  const int chunk = verify_chunk(d->rows, d->vocab), part = verify_chunk(d->seqs, d->vocab);
   args.chunks = (d->vocab + chunk - 1) / chunk;
-  args.stats = static_cast<VerifyStat*>(workspace);
-  args.rest = reinterpret_cast<double*>(args.stats + (size_t)d->rows * args.chunks);
-  args.count = reinterpret_cast<int32_t*>(args.rest + 2 * (size_t)d->seqs * args.chunks);
+  args.parts = (d->vocab + 2047) / 2048;
+  args.count = static_cast<int32_t*>(workspace);
+  args.picks = reinterpret_cast<VerifyPick*>(static_cast<char*>(workspace) + kVerifyCounts);
+  args.sums = reinterpret_cast<double*>(args.picks + d->seqs);
+  args.tops = args.sums + (size_t)d->rows * args.chunks;
+  args.rest = args.tops + (size_t)d->rows * args.chunks;
   void* p[] = {&args};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const uint32_t chunks = (uint32_t)args.chunks;
-  if ((rc = q8_shim::launch3(c.sums[i], chunks, (uint32_t)d->rows, 1, 256, p, st))) return rc;
-  return q8_shim::launch3(c.rest[i], chunks, (uint32_t)d->seqs, 1, 256, p, st);
+  if ((rc = q8_shim::launch3(c.sums[chunk == 8192], (uint32_t)args.chunks, (uint32_t)d->rows, 1, 256,
+                             p, st)))
+    return rc;
+  return q8_shim::launch3(c.rest[part == 8192], (uint32_t)((d->vocab + part - 1) / part),
+                          (uint32_t)d->seqs, 1, 256, p, st);
 }
 
 }  // extern "C"

@@ -542,7 +542,7 @@ def verify_case(Q, P, seed, vocab, counts, max_rows=None, heat="mixed", drafted=
     lb, tb, ub, hb, db, sb = map(up, (logits, tokens, u, temperature, draft, start))
     ostride = max_rows + 3
     out, acc, lp = Guarded(Q, 4 * seqs * ostride), Guarded(Q, 4 * seqs), Guarded(Q, 4 * seqs * ostride)
-    ws = Guarded(Q, P.verify_workspace_bytes(rows, seqs, vocab))
+    ws = Guarded(Q, P.verify_workspace_bytes(rows, seqs, vocab), 0)
     print(f"verify rows={rows} seqs={seqs} vocab={vocab} drafted={drafted}", flush=True)
     for _ in range(2):
         P.verify(lb, vocab + pad, vocab, rows, tb, seqs, max_rows, ub, out.ptr, ostride, acc.ptr,
@@ -638,6 +638,7 @@ def test_verify_keeps_the_models_distribution(gpu, P):
         b = [gpu.DeviceBuffer.from_array(a) for a in (logits, tokens, u, start, draft)]
         out, acc = gpu.DeviceBuffer(8 * seqs), gpu.DeviceBuffer(4 * seqs)
         ws = gpu.DeviceBuffer(P.verify_workspace_bytes(2 * seqs, seqs, vocab))
+        ws.fill(0)
         P.verify(b[0], vocab, vocab, 2 * seqs, b[1], seqs, 2, b[2], out, 2, acc, start=b[3],
                  draft=b[4], draft_stride=vocab, workspace=ws, workspace_bytes=ws.nbytes)
         gpu.synchronize()
