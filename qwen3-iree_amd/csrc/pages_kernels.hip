@@ -1245,7 +1245,34 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
     put_sum(A.sums + at, (sums[0] + sums[1]) + (sums[2] + sums[3]));
     put_sum(A.tops + at, __builtin_bit_cast(double, Top{top, first}));
   }
-  if (last_here(A.count + s * kCountStep, m * A.chunks, &arrived)) verify_pick(A, s, lo, m, heat, unit, table);
+  // (a sequence of one row has nothing to decide: the second launch joins its chunks)
+  if (A.b.max_rows > 1 && last_here(A.count + s * kCountStep, m * A.chunks, &arrived)) verify_pick(A, s, lo, m, heat, unit, table);
+}
+
+// A row joined from its chunks by a wave, every lane getting it.
+__device__ __forceinline__ VerifyStat join_row(const VerifyArgs& A, int row, int lane, double unit,
+                                               float heat, const double* table) {
+  const double *sums = A.sums + (int64_t)row * A.chunks, *tops = A.tops + (int64_t)row * A.chunks;
+  float top = -__builtin_inff();
+  for (int c = lane; c < A.chunks; c += 64) top = fmaxf(top, __builtin_bit_cast(Top, tops[c]).top);
+  top = wave_max(top);
+  double total = 0.0;
+  int first = 0x7fffffff;
+  const Exp weight(table, top, unit);
+  for (int c = lane; c < A.chunks; c += 64) {
+    const double sum = sums[c];
+    const Top v = __builtin_bit_cast(Top, tops[c]);
+    if (v.top == -__builtin_inff()) continue;
+    if (v.top == top && v.first < first) first = v.first;
+    total += sum * weight(weight.near(v.top));
+  }
+  if (heat > 0.0f) return {wave_sum64(total), top, first};
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) {
+    const int other = __shfl_xor(first, k);
+    first = other < first ? other : first;
+  }
+  return {1.0, top, first};
 }
 
 // What an entry of the deciding row weighs: max(p - q, 0) and p.
@@ -1270,7 +1297,9 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.y;
   const int lo = A.b.start ? A.b.start[s] : s;
   const int m = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
-  const VerifyPick pick = A.picks[s];
+  const bool single = A.b.max_rows == 1;
+  VerifyPick pick = {};
+  if (!single) pick = A.picks[s];
   if (t < 16) table[t] = kExp2[t];
   int32_t* const out = A.out + s * A.out_stride;
   float* const logprob = A.logprob ? A.logprob + s * A.out_stride : nullptr;
@@ -1282,6 +1311,15 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
       if (logprob) logprob[t] = 0.0f;
     }
     return;
+  }
+  __syncthreads();  // the table
+  if (single) {
+    pick.heat = A.temperature ? A.temperature[s] : 1.0f;
+    pick.u = A.uniform[lo];
+    pick.unit = unit_of(pick.heat);
+    pick.told = -1;
+    pick.row = join_row(A, lo, lane, pick.unit, pick.heat, table);
+    if (blockIdx.x == 0 && t == 0) A.accepted[s] = 0;
   }
   // (starts that descend may have left a sequence without a pick)
   if (blockIdx.x == 0 && t == 0) A.count[s * kCountStep] = 0;
@@ -1324,7 +1362,6 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
     }
     __syncthreads();
   };
-  __syncthreads();  // the table
   double* const sums = A.rest + (int64_t)s * A.parts * 2;
   {
     const int part0 = blockIdx.x * V;
