@@ -605,13 +605,22 @@ __device__ __forceinline__ float2 get_pair(const float* p) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int other = __shfl_up(v, d);
-    if ((int)(threadIdx.x & 63) >= d) v += other;
-  }
-  return v;
+// The maximum over 16 lanes, and over the wave.
+__device__ __forceinline__ float row_max16(float v) {
+  v = fmaxf(v, dpp<0xb1>(v));
+  v = fmaxf(v, dpp<0x4e>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  return fmaxf(v, dpp<0x140>(v));
+}
+__device__ __forceinline__ float wave_max(float v) { return max_col4(row_max16(v)); }
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive: rows of 16, then the rows before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
 // The work of a kv head and row block is the sequences' slots, in rounds of 128 (a block for
@@ -624,13 +633,12 @@ __device__ __forceinline__ void pages_attn(const PagesAttnArgs& A) {
   constexpr int kRows = 16 * T, kDims = D / 16, kStride = D + 4;
   __shared__ float so[4][16][kStride];
   __shared__ float sm[4][kRows], sl[4][kRows];
-  __shared__ int ends[kSeqsMax], totals[4], arrived;
+  __shared__ int ends[kSeqsMax], totals[4], longest[4], arrived;
+  __shared__ int3 seqs[kSeqsMax];  // first row, rows, length
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int kvh = blockIdx.x, rb = blockIdx.y, me = blockIdx.z;
   const int row0 = kRows * rb;
   auto node = [&A](int r) { return A.group == 1 ? r : (int)__umulhi((uint32_t)r, A.group_inv); };
-  auto first_row = [&](int s) { return A.b.start ? A.b.start[s] : s; };
-  auto row_count = [&](int s, int lo) { return A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1; };
   auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   auto blocks = [&](int rows, int length) {  // of 32 slots that this row block sees
     const int R = rows * A.group;
@@ -639,30 +647,46 @@ __device__ __forceinline__ void pages_attn(const PagesAttnArgs& A) {
   };
 
   // the sequences' running sums of rounds; one round at least where there are rows
-  int sum = 0;
+  int sum = 0, most = 0;
   for (int s0 = 0; s0 < A.b.seqs; s0 += 256) {
     const int s = s0 + t;
     int n = 0;
     if (s < A.b.seqs) {
-      const int rows = row_count(s, first_row(s));
+      const int length = A.b.length[s], lo = A.b.start ? A.b.start[s] : s;
+      const int rows = A.b.start ? rows_of(A.b, lo, A.b.start[s + 1]) : 1;
       if (row0 < rows * A.group) {
-        n = (blocks(rows, A.b.length[s]) + 3) >> 2;
+        n = (blocks(rows, length) + 3) >> 2;
         n = n > 0 ? n : 1;
       }
+      seqs[s] = {lo, rows, length};
     }
+    const float wave_most = wave_max((float)n);
     n = wave_scan(n);
-    if (lane == 63) totals[wave] = n;
+    if (lane == 63) {
+      totals[wave] = n;
+      longest[wave] = (int)wave_most;
+    }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       if (w < wave) n += totals[w];
+      most = longest[w] > most ? longest[w] : most;
     }
     if (s < A.b.seqs) ends[s] = sum + n;
     sum += (totals[0] + totals[1]) + (totals[2] + totals[3]);
     __syncthreads();
   }
   sum = uniform(sum);
-  const int share = uniform((int)((uint32_t)(sum + A.workers - 1) / (uint32_t)A.workers));
+  // Equal shares; as long as the longest sequence where that is four rounds or little more
+  // than a share (a cut costs about 6 us: 48 x 1700 slots 41.7 -> 38.6 us, 1 x 300 9.1 -> 8.4);
+  // and not so short that joining the parts of a sequence, 17 ns a row and part, takes longer
+  // than the rounds, about 1 us each (1 x 8000 slots, 24 rows of a kv head 39 -> 22 us).
+  int share = uniform((int)((uint32_t)(sum + A.workers - 1) / (uint32_t)A.workers));
+  if (most <= 4 || 2 * most <= 3 * share) share = share > most ? share : most;
+  const int rows_here = A.b.max_rows * A.group < kRows ? A.b.max_rows * A.group : kRows;
+  const int least =
+      uniform((int)(__builtin_sqrtf((float)most * (float)rows_here * 0.012f) + 0.5f));
+  share = share > least ? share : least;
   const int begin = me * share, end = begin + share < sum ? begin + share : sum;
   if (begin >= end) return;
   int s = 0;
@@ -698,8 +722,9 @@ __device__ __forceinline__ void pages_attn(const PagesAttnArgs& A) {
     const int from = s ? uniform(ends[s - 1]) : 0, to = uniform(ends[s]);
     if (from == to) continue;
     const int till = to < end ? to : end;
-    const int lo = uniform(first_row(s)), rows = uniform(row_count(s, lo));
-    const int length = uniform(A.b.length[s]), R = rows * A.group;
+    const int3 seq = seqs[s];
+    const int lo = uniform(seq.x), rows = uniform(seq.y), length = uniform(seq.z);
+    const int R = rows * A.group;
     const int unmasked = uniform(slots_seen(A.b, length, rows, node(row0)));
     int nb = uniform(blocks(rows, length));
     nb = nb < 4 * (till - from) ? nb : 4 * (till - from);
@@ -997,15 +1022,6 @@ struct Exp {
 __device__ __forceinline__ double unit_of(float heat) {
   return heat > 0.0f ? fmax(23.083120654223414519 / (double)heat, 1e-30) : 1.0;
 }
-
-// The maximum over 16 lanes, and over the wave.
-__device__ __forceinline__ float row_max16(float v) {
-  v = fmaxf(v, dpp<0xb1>(v));
-  v = fmaxf(v, dpp<0x4e>(v));
-  v = fmaxf(v, dpp<0x141>(v));
-  return fmaxf(v, dpp<0x140>(v));
-}
-__device__ __forceinline__ float wave_max(float v) { return max_col4(row_max16(v)); }
 
 // The sum over the wave, in every lane: 16 lanes by DPP, then the four rows.
 __device__ __forceinline__ double wave_sum64(double v) {
