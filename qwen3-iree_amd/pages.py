@@ -9,6 +9,7 @@ which runs one sequence over a flat cache (model/qwen3_full.mlir:1431-1526).
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import q8gemv as Q
 
@@ -55,12 +56,18 @@ class Rows(ctypes.Structure):
                 ("q_heads", _I32)]
 
 
+_ROWS = struct.Struct("=7Q4q2di4x")
+
+
 class Drafts(ctypes.Structure):
     """struct kv_drafts"""
     _fields_ = [("logits", _P), ("tokens", _P), ("start", _P), ("temperature", _P), ("draft", _P),
                 ("uniform", _P), ("out", _P), ("accepted", _P), ("logprob", _P),
                 ("logits_stride", _I64), ("draft_stride", _I64), ("out_stride", _I64),
                 ("vocab", _I32), ("rows", _I32), ("seqs", _I32), ("max_rows", _I32)]
+
+
+_DRAFTS = struct.Struct("=9Q3q4i")
 
 
 def append(pages: Pages, layer: int, batch: Batch, k, k_stride: int, v, v_stride: int,
@@ -71,10 +78,12 @@ def append(pages: Pages, layer: int, batch: Batch, k, k_stride: int, v, v_stride
     [head_dim], None: none) and rotation (theta, 0: none) by its position (None: its
     slot); the queries, treated alike, go to q_out."""
     p = Q._ptr
-    rows = Rows(p(q), p(k), p(v), p(q_out), p(q_norm), p(k_norm), p(positions), q_stride, k_stride,
-                v_stride, q_out_stride, eps, theta, q_heads)
-    Q._call("kv_pages_append", ctypes.byref(pages), int(layer), ctypes.byref(batch),
-            ctypes.byref(rows), Q._stream(stream))
+    # (struct kv_rows; filling a ctypes structure takes twice as long)
+    rows = _ROWS.pack(p(q) or 0, p(k) or 0, p(v) or 0, p(q_out) or 0, p(q_norm) or 0,
+                      p(k_norm) or 0, p(positions) or 0, q_stride, k_stride, v_stride,
+                      q_out_stride, eps, theta, q_heads)
+    Q._call("kv_pages_append", ctypes.byref(pages), int(layer), ctypes.byref(batch), rows,
+            Q._stream(stream))
 
 
 def attn_workspace_bytes(pages: Pages, batch: Batch, q_heads: int) -> int:
@@ -112,8 +121,8 @@ def verify(logits, logits_stride: int, vocab: int, rows: int, tokens, seqs: int,
     one more sampled token (out int32 [seqs, out_stride], -1 behind), and their log
     probabilities."""
     p = Q._ptr
-    drafts = Drafts(p(logits), p(tokens), p(start), p(temperature), p(draft), p(uniform), p(out),
-                    p(accepted), p(logprob), logits_stride, draft_stride, out_stride, vocab, rows,
-                    seqs, max_rows)
-    Q._call("kv_verify", ctypes.byref(drafts), Q._ptr(workspace), int(workspace_bytes),
-            Q._stream(stream))
+    drafts = _DRAFTS.pack(p(logits) or 0, p(tokens) or 0, p(start) or 0, p(temperature) or 0,
+                          p(draft) or 0, p(uniform) or 0, p(out) or 0, p(accepted) or 0,
+                          p(logprob) or 0, logits_stride, draft_stride, out_stride, vocab, rows,
+                          seqs, max_rows)
+    Q._call("kv_verify", drafts, Q._ptr(workspace), int(workspace_bytes), Q._stream(stream))

@@ -49,6 +49,15 @@ def test_struct_layouts(P, tmp_path):
             assert int(out[f"{s}.{f}"]) == getattr(c, f).offset, (s, f)
 
 
+def test_packed_structs(P):
+    """The packed forms that append and verify pass, against the structures."""
+    for packed, struct in ((P._ROWS, P.Rows), (P._DRAFTS, P.Drafts)):
+        values = [0.5 * i if t is ctypes.c_double else i + 1 for i, (_, t) in enumerate(struct._fields_)]
+        assert packed.size == ctypes.sizeof(struct)
+        got = struct.from_buffer_copy(packed.pack(*values))
+        assert [getattr(got, f) for f, _ in struct._fields_] == values
+
+
 def test_code_object(Q):
     data = (REPO / "qwen3-iree_amd" / "lib" / "pages_gfx950.hsaco").read_bytes()
     assert data[:4] == b"\x7fELF" and b"amdgcn-amd-amdhsa--gfx950" in data
