@@ -105,26 +105,31 @@ __device__ __forceinline__ double other_half(double v) {
   return __builtin_bit_cast(double, lo | (uint64_t)hi << 32);
 }
 
-// Norm (w not null) and rotation (by turn[i] = (cos, sin)) of a head's lane c.
+// Where the cosine and sine of frequency i lie: lanes that read theirs together do so from
+// banks of their own.
 template <int D>
-__device__ __forceinline__ void turn_head(double (&y)[8], int c, const uint16_t* w, double eps,
+__device__ __forceinline__ int turn_at(int i) {
+  return (i & 7) * (D / 16) + (i >> 3);
+}
+
+// Norm (by weights wv) and rotation (by turn[turn_at(i)] = (cos, sin)) of a head's lane c.
+template <int D>
+__device__ __forceinline__ void turn_head(double (&y)[8], int c, bool norm, u32x4 wv, double eps,
                                           bool rotate, const double2* turn) {
-  if (w) {
+  if (norm) {
     double ss = 0.0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
     ss = over_head<D>(ss, [](double a, double b) { return a + b; });
     const double r = rsqrt(ss / D + eps);
-    const u32x4 wv = load_words4(w + 8 * c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (double)half_at(wv, j);
   }
   if (rotate) {
     const bool second = c >= D / 16;
-    const int i = (8 * c) % (D / 2);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const double2 a = turn[i + j];
+      const double2 a = turn[turn_at<D>((8 * c) % (D / 2) + j)];
       const double o = other_half<D>(y[j]);
       y[j] = y[j] * a.x + o * (second ? a.y : -a.y);
     }
@@ -158,14 +163,17 @@ __device__ __forceinline__ uint2 codes8(const double (&y)[8], float& scale) {
   uint2 code = {0, 0};
   if (!real || scale == 0.0f) return code;
   const double inv = 1.0 / (double)scale;
+  double q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = y[j] * inv;
+  if (__builtin_amdgcn_ballot_w64(scale < 1.17549435e-38f) != 0) {  // a scale of few bits
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = fmin(fmax(q[j], -127.0), 127.0);
+  }
   uint32_t low[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    double q = y[j] * inv;
-    if (scale < 1.17549435e-38f) q = fmin(fmax(q, -127.0), 127.0);  // a scale of few bits
-    q = (q + 98304.0) - 98304.0;
-    low[j] = (uint32_t)__builtin_bit_cast(uint64_t, q + 6755399441055744.0);
-  }
+  for (int j = 0; j < 8; ++j)
+    low[j] = (uint32_t)__builtin_bit_cast(uint64_t, ((q[j] + 98304.0) - 98304.0) + 6755399441055744.0);
   const uint32_t pairs[4] = {__builtin_amdgcn_perm(low[1], low[0], 0x0c0c0400),
                              __builtin_amdgcn_perm(low[3], low[2], 0x0c0c0400),
                              __builtin_amdgcn_perm(low[5], low[4], 0x0c0c0400),
@@ -191,6 +199,9 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
   int h = t / G;
   u32x4 x = {};
   if (h < heads) x = request(h);
+  u32x4 qw = {}, kw = {};
+  if (A.q_norm) qw = load_words4(A.q_norm + 8 * c);
+  if (A.k_norm) kw = load_words4(A.k_norm + 8 * c);
   const int position = A.positions ? A.positions[row] : 0;
   const double step = t < D / 2 ? A.turns[t] : 0.0;
   int lo, m, length = 0;
@@ -203,7 +214,7 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
       const double by = (double)(A.positions ? (int64_t)position : slot) * step;
       double2 a;
       sincospi(2.0 * (by - rint(by)), &a.y, &a.x);
-      turn[t] = a;
+      turn[turn_at<D>(t)] = a;
     }
     __syncthreads();
   }
@@ -216,7 +227,8 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
     double y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = (double)half_at(here, j);
-    if (!is_v) turn_head<D>(y, c, is_q ? A.q_norm : A.k_norm, A.eps, A.rotate, turn);
+    if (!is_v)
+      turn_head<D>(y, c, (is_q ? A.q_norm : A.k_norm) != nullptr, is_q ? qw : kw, A.eps, A.rotate, turn);
     if (is_q) {
       *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + h * D + 8 * c) = packed8(y);
     } else if constexpr (Q8) {
