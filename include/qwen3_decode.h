@@ -297,6 +297,29 @@ int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_
                     int32_t position, int32_t* next_tokens, void* logits, void* q_rows, float* lse,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* The new rows of several sequences through the whole model in one pass, over a paged
+ * KV cache (kv_pages.h) of 28 layers, 8 kv heads of 128.  tokens: device int32
+ * [batch->rows]; row r sits in its sequence's slot, at the RoPE position of that
+ * slot, attends to the slots up to its own, and its k and v are written into the
+ * pages.  next_tokens (device int32 [rows]): the argmax of every row's logits, what the
+ * model says follows it (of rows that belong to no sequence: unspecified; a token outside
+ * the vocabulary counts as token 0); logits f16 [rows, 151936], may be NULL.
+ * One token a sequence is a decode step, several a prompt's chunk or drafted tokens that
+ * kv_verify then judges.  The layers' matrices are read as in qwen3_prefill_batched;
+ * with f16 pages results agree with qwen3_decode_step within the step's
+ * tolerance, 8-bit pages add their rounding.  Only enqueues; rows at most 128.
+ * workspace: device memory of qwen3_pages_workspace_bytes(rows, max_rows) bytes (0 for
+ * arguments outside the ranges), 256-byte aligned, filled with zeros once before its
+ * first use; that of the largest rows and max_rows serves smaller steps too.  Steps that
+ * may overlap need one each.  No counterpart in the reference, which runs one
+ * sequence. */
+struct kv_pages;
+struct kv_batch;
+size_t qwen3_pages_workspace_bytes(int32_t rows, int32_t max_rows);
+int qwen3_pages_step(const qwen3_weights* w, const struct kv_pages* pages,
+                     const struct kv_batch* batch, const int32_t* tokens, int32_t* next_tokens,
+                     void* logits, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Scratch offsets of the intermediates the last qwen3_decode_layer (or head)
  * left behind, all f16: "xn" [1024] rms_norm(h_in, attn_norm); "q" [2048],
  * "k" [1024], "v" [1024] the projections before head norm and RoPE;

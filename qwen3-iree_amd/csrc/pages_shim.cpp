@@ -227,6 +227,26 @@ void pages_unload() {
   c.module = nullptr;
 }
 
+int pages_check(const kv_pages* a, const kv_batch* batch, int32_t q_heads) {
+  int rc = check_pages(a);
+  if (rc) return rc;
+  if ((rc = check_batch(a, batch))) return rc;
+  if ((rc = check_heads(a, q_heads))) return rc;
+  if (batch->max_rows > kAttnRowsMax)
+    return fail(Q8_ERR_BAD_SHAPE, "%d rows of a sequence outside [1, %d]", batch->max_rows,
+                kAttnRowsMax);
+  return Q8_OK;
+}
+
+int pages_ready() { return check_ready(); }
+
+size_t pages_attn_need(const kv_pages* a, int32_t max_rows, int32_t q_heads) {
+  size_t most = 0;
+  for (int32_t m = 1; m <= max_rows; ++m)
+    most = std::max(most, attn_workspace(a, attn_plan(a, m, q_heads)));
+  return most;
+}
+
 }  // namespace q8_shim
 
 extern "C" {
@@ -295,10 +315,7 @@ size_t kv_pages_attn_workspace_bytes(const kv_pages* a, const kv_batch* batch, i
   if (check_pages(a) || check_batch(a, batch) || check_heads(a, q_heads) ||
       batch->max_rows > kAttnRowsMax)
     return 0;
-  size_t most = 0;
-  for (int32_t m = 1; m <= batch->max_rows; ++m)
-    most = std::max(most, attn_workspace(a, attn_plan(a, m, q_heads)));
-  return most;
+  return q8_shim::pages_attn_need(a, batch->max_rows, q_heads);
 }
 
 int kv_pages_attn(const kv_pages* a, int32_t layer, const kv_batch* batch, const void* q,

@@ -5,6 +5,7 @@
 // include/q8gemv.h.
 #include "q8gemv.h"
 #include "f16_cache.h"
+#include "kv_pages.h"
 #include "qwen3_decode.h"
 #include "prefill_split.h"
 #include "shim_internal.h"
@@ -1957,6 +1958,14 @@ struct TreeLayer {
   size_t bytes;
 };
 
+// Paged sequences' rows in place of a flat cache's.
+struct PagesLayer {
+  const kv_pages* pages;
+  const kv_batch* batch;
+  void* workspace;
+  size_t bytes;
+};
+
 // One layer.  xn_ready: the workspace's xn already holds rms_norm(h,
 // attn_norm of this layer) (written by the previous layer's last reduce).
 // next_norm (the next layer's attn_norm, or null): if ffn_down's reduce can
@@ -1966,12 +1975,13 @@ struct TreeLayer {
 // them there: 512 tokens 62.4 us a layer over and over, 64.1 with).
 // tree: the tokens are a tree's nodes in slots p0 .. (rope_ready, positions of
 // their own).
+// paged: the rows are those of sequences in pages (n <= kPfRowsMax; k_cache, v_cache unused).
 int launch_prefill_layer(const qwen3_weights* w, int layer, void* k_cache, void* v_cache,
                          int64_t max_seq, int32_t n, int32_t p0, int chunk_local,
                          void* const (&ws)[kPfRegions], hipStream_t st, bool xn_ready = false,
                          const void* next_norm = nullptr, bool* next_xn_ready = nullptr,
                          bool rope_ready = false, bool whole_prompt = false,
-                         const TreeLayer* tree = nullptr) {
+                         const TreeLayer* tree = nullptr, const PagesLayer* paged = nullptr) {
   const int64_t bpl_q = 2048LL * 1024 / 32 * 34, bpl_kv = 1024LL * 1024 / 32 * 34;
   const int64_t bpl_o = 1024LL * 2048 / 32 * 34, bpl_gu = 6144LL * 1024 / 32 * 34;
   const int64_t bpl_dn = 1024LL * 3072 / 32 * 34;
@@ -1992,11 +2002,11 @@ int launch_prefill_layer(const qwen3_weights* w, int layer, void* k_cache, void*
   const void* wq = f16l ? (const void*)(f16l + kPfF16Qkv * 2) : cb(w->wq) + layer * bpl_q;
   const void* wk = cb(w->wk) + layer * bpl_kv;
   const void* wv = cb(w->wv) + layer * bpl_kv;
-  if (n <= 64) {
+  if (n <= 64 || paged) {
     // 16 columns a workgroup fill the CUs with one token tile; from 17 tokens
     // on 32 columns halve the times a row is normalised (24 tokens 38.5 -> 38.2
     // us a layer, 64 tokens 46.1 -> 44.1)
-    RowsNormArgs a{h, an, {wq, wk, wv}, xn, {q, k, v}, rope_ready ? nullptr : rope, n, p0};
+    RowsNormArgs a{h, an, {wq, wk, wv}, xn, {q, k, v}, rope_ready || paged ? nullptr : rope, n, p0};
     const int i = n <= 16 ? 0 : 1;
     if ((rc = launch_rows(g.pf_rows_qkv[i][q8], n, 16, 256 >> i, 512, &a, st))) return rc;
   } else if (rows) {
@@ -2036,12 +2046,22 @@ int launch_prefill_layer(const qwen3_weights* w, int layer, void* k_cache, void*
                        nullptr, 0, 0, n, st, nullptr, 1, wk, wv, &out);
     if (rc) return rc;
   }
-  if (n <= 64) {
+  if (paged) {
+    const kv_rows x{q, k, v, qr, qn, kn, nullptr, Q8_HIDDEN * 2, Q8_HIDDEN, Q8_HIDDEN,
+                    Q8_HIDDEN * 2, 9.99999997e-7, 1e6, 16};
+    if ((rc = kv_pages_append(paged->pages, layer, paged->batch, &x, st))) return rc;
+    if ((rc = kv_pages_attn(paged->pages, layer, paged->batch, qr, Q8_HIDDEN * 2, 16,
+                            0.0883883461356163f, attn, Q8_HIDDEN * 2, nullptr, paged->workspace,
+                            paged->bytes, st)))
+      return rc;
+  } else if (n <= 64) {
     int start = p0;
     void* args[] = {&q, &k, &v, &start, &qn, &kn, &rope, &qr, &kc, &vc};
     if ((rc = launch(g.pf_rope, (uint32_t)n, 256, args, st))) return rc;
   }
-  if (tree) {
+  if (paged) {
+    // done above
+  } else if (tree) {
     if ((rc = f16_attn_tree(&tree->cache, layer, p0, qr, Q8_HIDDEN * 2, 16, tree->mask, n,
                             0.0883883461356163f, attn, Q8_HIDDEN * 2, tree->lse, tree->workspace,
                             tree->bytes, st)))
@@ -2734,6 +2754,84 @@ int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_
   }
   return f16_gemm_argmax(w->output_w, Q8_VOCAB_ROWS, ws[2], n, logits, next_tokens,
                          mb(workspace) + t.keys, stream);
+}
+
+// The step's workspace over pages: the attention's in front (its counters must stay where they
+// are whatever the step's rows), a prompt's regions, the argmax keys.
+namespace {
+
+kv_pages model_pages() {
+  kv_pages p{};
+  p.layers = kLayers;
+  p.kv_heads = (int32_t)kKvHeads;
+  p.head_dim = 128;
+  return p;
+}
+
+size_t pages_attn_bytes(int32_t max_rows) {
+  const kv_pages p = model_pages();
+  return (q8_shim::pages_attn_need(&p, max_rows, 16) + 255) / 256 * 256;
+}
+
+}  // namespace
+
+size_t qwen3_pages_workspace_bytes(int32_t rows, int32_t max_rows) {
+  if (rows < 1 || rows > kPfRowsMax || max_rows < 1 || max_rows > rows) return 0;
+  return pages_attn_bytes(max_rows) + pf_workspace_bytes(rows) + f16_gemm_argmax_workspace_bytes(rows);
+}
+
+int qwen3_pages_step(const qwen3_weights* w, const kv_pages* pages, const kv_batch* batch,
+                     const int32_t* tokens, int32_t* next_tokens, void* logits, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int rc = validate_weights(w);
+  if (rc) return rc;
+  if (!tokens || !next_tokens || !workspace)
+    return fail(Q8_ERR_NULL_POINTER, "null tokens, next_tokens or workspace");
+  if (!aligned(tokens, 4) || !aligned(next_tokens, 4) || !aligned(logits, 2) ||
+      !aligned(workspace, 256))
+    return fail(Q8_ERR_MISALIGNED,
+                "tokens and next_tokens 4, logits 2, workspace 256-byte alignment");
+  if ((rc = q8_shim::pages_check(pages, batch, 16))) return rc;
+  if (pages->layers != kLayers || pages->kv_heads != (int32_t)kKvHeads || pages->head_dim != 128)
+    return fail(Q8_ERR_BAD_SHAPE, "pages of %d layers, %d kv heads of %d: not the model's",
+                pages->layers, pages->kv_heads, pages->head_dim);
+  const int32_t n = batch->rows;
+  if (n > kPfRowsMax || batch->max_rows > n)
+    return fail(Q8_ERR_BAD_SHAPE, "%d rows, %d a sequence, outside [1, %d]", n, batch->max_rows,
+                kPfRowsMax);
+  const size_t need = qwen3_pages_workspace_bytes(n, batch->max_rows);
+  if (workspace_bytes < need)
+    return fail(Q8_ERR_BAD_SHAPE, "workspace of %zu bytes < %zu needed for %d rows",
+                workspace_bytes, need, n);
+  if ((rc = check_prefill_ready())) return rc;
+  if ((rc = q8_shim::pages_ready())) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  void* ws[kPfRegions];
+  size_t off = pages_attn_bytes(batch->max_rows);
+  const PagesLayer layer{pages, batch, workspace, off};
+  for (int i = 0; i < kPfRegions; ++i) {
+    ws[i] = mb(workspace) + off;
+    off += pf_region_bytes(n, i);
+  }
+  {
+    const void *tp = tokens, *e = w->token_embd;
+    void* h = ws[0];
+    void* args[] = {&tp, &e, &h};
+    if ((rc = launch(g.pf_embed, (uint32_t)n, 128, args, st))) return rc;
+  }
+  for (int l = 0; l < kLayers; ++l)
+    if ((rc = launch_prefill_layer(w, l, nullptr, nullptr, 1, n, 0, 0, ws, st, false, nullptr,
+                                   nullptr, true, false, nullptr, &layer)))
+      return rc;
+  {
+    const void *h = ws[0], *on = w->output_norm;
+    void *xn = ws[2], *rope = nullptr;
+    int nn = n, start = 0;
+    void* args[] = {&h, &on, &xn, &nn, &start, &rope};
+    if ((rc = launch(g.pf_norm, (uint32_t)((n + 3) / 4), 64, args, st))) return rc;
+  }
+  return f16_gemm_argmax(w->output_w, Q8_VOCAB_ROWS, ws[2], n, logits, next_tokens,
+                         mb(workspace) + off, stream);
 }
 
 }  // extern "C"

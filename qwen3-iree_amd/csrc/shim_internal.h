@@ -9,6 +9,8 @@
 #include <stdint.h>
 
 struct f16_cache;
+struct kv_pages;
+struct kv_batch;
 
 namespace q8_shim {
 
@@ -31,6 +33,11 @@ void cache_unload();
 // The same of pages_shim.cpp and its code object.
 void pages_load(const char* path);
 void pages_unload();
+// Q8_OK where kv_pages_append and kv_pages_attn would take these (heads of the query
+// rows given); the attention's workspace bytes for them.
+int pages_check(const kv_pages* pages, const kv_batch* batch, int32_t q_heads);
+int pages_ready();
+size_t pages_attn_need(const kv_pages* pages, int32_t max_rows, int32_t q_heads);
 // The workspace bytes of this one call of f16_attn_tree (arguments in range), at most
 // f16_attn_tree_workspace_bytes.
 size_t attn_tree_need(const f16_cache* cache, int32_t len, int32_t n, int32_t q_heads);

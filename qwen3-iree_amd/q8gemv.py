@@ -182,6 +182,8 @@ _SIGNATURES = {
     "qwen3_tree_workspace_bytes": [ctypes.c_int32, _I64],
     "qwen3_tree_step": [_P, _P, _P, _I64, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                         _P, _P, _P, _P, _P, _SZ, _P],
+    "qwen3_pages_workspace_bytes": [ctypes.c_int32, ctypes.c_int32],
+    "qwen3_pages_step": [_P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     "qwen3_set_step_mode": [_I],
     "qwen3_set_step_spin_limit": [ctypes.c_uint32],
     "qwen3_check_status": [_P, _P, _P],
@@ -216,6 +218,7 @@ _RESTYPES = {
     "kv_pages_attn_workspace_bytes": _SZ,
     "kv_verify_workspace_bytes": _SZ,
     "qwen3_tree_workspace_bytes": _SZ,
+    "qwen3_pages_workspace_bytes": _SZ,
     "f16_attn_tree_workspace_bytes": _SZ,
     "f16_gemm_argmax_workspace_bytes": _SZ,
     "q8gemv_shutdown": None,
