@@ -115,8 +115,9 @@ int kv_pages_append(const kv_pages* pages, int32_t layer, const kv_batch* batch,
  * slots hold that a row does not see is never used, NaN and infinities included;
  * a value of out whose v holds an infinity or NaN in a slot the row sees is not
  * finite.  q, out: f16 rows as in kv_rows; lse: f32 [rows, q_heads], may be NULL.
- * q_heads a multiple of kv_heads, at most 32 times it and at most 256; scale
- * finite and positive; max_rows at most 256.  Scores, statistics and sums are
+ * out must not overlap q (workgroups that share a row read q while others
+ * write).  q_heads a multiple of kv_heads, at most 32 times it and at most 256; scale
+ * positive and below 2^118; max_rows at most 256.  Scores, statistics and sums are
  * f32; a weight enters its product with v to 2^-22 of itself.
  * workspace: device memory of kv_pages_attn_workspace_bytes (256-byte aligned),
  * needed only during the call; fill it with zeros once before its first use.
@@ -135,7 +136,7 @@ int kv_pages_attn(const kv_pages* pages, int32_t layer, const kv_batch* batch, c
  * start = the running sums of the lengths whole sequences are read, with
  * row_stride = kv_heads * head_dim and layer_stride = max_seq * row_stride into the flat
  * cache of f16_cache.h.  Strides multiples of 8, row_stride at least kv_heads *
- * head_dim; layer_stride ignored with one layer.  k_out or v_out may be NULL. */
+ * head_dim, and so layer_stride, which is ignored with one layer; rows do not overlap.  k_out or v_out may be NULL. */
 int kv_pages_read(const kv_pages* pages, int32_t layer, int32_t layers, const kv_batch* batch,
                   void* k_out, void* v_out, int64_t row_stride, int64_t layer_stride,
                   void* stream);

@@ -333,8 +333,10 @@ int kv_pages_attn(const kv_pages* a, int32_t layer, const kv_batch* batch, const
   const int64_t width = (int64_t)q_heads * a->head_dim;
   if ((rc = check_stride("q", q, q_stride, width))) return rc;
   if ((rc = check_stride("out", out, out_stride, width))) return rc;
-  if (!(scale > 0.0f) || !std::isfinite(scale))
-    return fail(Q8_ERR_BAD_ARGUMENT, "scale %g is not finite and positive", scale);
+  const float by = scale * kLog2e * (a->type == KV_PAGES_Q8 ? 512.0f : 1.0f);
+  if (!(scale > 0.0f) || !std::isfinite(by))
+    return fail(Q8_ERR_BAD_ARGUMENT, "scale %g is not positive and below 2^118", scale);
+  if (q == out) return fail(Q8_ERR_BAD_ARGUMENT, "out is q");
   if (!aligned(lse, 4)) return fail(Q8_ERR_MISALIGNED, "lse 4-byte alignment");
   const AttnPlan plan = attn_plan(a, batch->max_rows, q_heads);
   const size_t need = attn_workspace(a, plan);
@@ -360,7 +362,7 @@ int kv_pages_attn(const kv_pages* a, int32_t layer, const kv_batch* batch, const
                      a->kv_heads,
                      group,
                      (uint32_t)((0xffffffffull + group) / group),
-                     float_bits(scale * kLog2e * (a->type == KV_PAGES_Q8 ? 512.0f : 1.0f)),
+                     float_bits(by),
                      plan.workers,
                      reinterpret_cast<int32_t*>(ws),
                      reinterpret_cast<float*>(ws + kCountBytes),
@@ -381,9 +383,9 @@ int kv_pages_read(const kv_pages* a, int32_t layer, int32_t layers, const kv_bat
   const int64_t width = (int64_t)a->kv_heads * a->head_dim;
   if ((rc = check_stride("k_out", k_out, row_stride, width))) return rc;
   if ((rc = check_stride("v_out", v_out, row_stride, width))) return rc;
-  if (layers > 1 && (layer_stride % 8 || layer_stride < 0))
-    return fail(Q8_ERR_BAD_SHAPE, "layer stride %lld is no multiple of 8 of at least 0",
-                (long long)layer_stride);
+  if (layers > 1 && (layer_stride % 8 || layer_stride < width))
+    return fail(Q8_ERR_BAD_SHAPE, "layer stride %lld is no multiple of 8 of at least %lld",
+                (long long)layer_stride, (long long)width);
   if ((rc = check_ready())) return rc;
   if (!k_out && !v_out) return Q8_OK;
   PagesReadArgs args{batch_args(a, batch),

@@ -93,6 +93,17 @@ class PagedSession:
         """Offset of the step's tokens (then the next tokens)."""
         return 4 * (self.max_seqs * (self.max_pages + 2) + 1)
 
+    def _pages_for(self, seqs: list[int], counts: list[int]) -> dict[int, int]:
+        """The pages each sequence needs for more rows; refused where there are none."""
+        need = {}
+        for s, m in zip(seqs, counts):
+            if self.length[s] + m > self.max_pages * self.page_size:
+                raise ValueError(f"sequence {s}: {self.length[s]} + {m} slots")
+            need[s] = (self.length[s] + m + self.page_size - 1) // self.page_size - len(self._held[s])
+        if sum(need.values()) > len(self._free):
+            raise ValueError(f"{sum(need.values())} pages needed, {len(self._free)} free")
+        return need
+
     def step(self, rows: dict[int, object], logits: bool = False) -> dict[int, np.ndarray]:
         """Runs each sequence's new tokens (behind the slots in use; at most 128 in all) and
         keeps their k and v; the model's next token after each.  logits: also leave
@@ -102,13 +113,7 @@ class PagedSession:
         counts = [int(t.size) for t in new]
         if not seqs or not 0 < sum(counts) <= MAX_ROWS or min(counts) < 1:
             raise ValueError(f"{counts} rows: each sequence at least one, {MAX_ROWS} at most in all")
-        need = {}
-        for s, m in zip(seqs, counts):
-            if self.length[s] + m > self.max_pages * self.page_size:
-                raise ValueError(f"sequence {s}: {self.length[s]} + {m} slots")
-            need[s] = (self.length[s] + m + self.page_size - 1) // self.page_size - len(self._held[s])
-        if sum(need.values()) > len(self._free):
-            raise ValueError(f"{sum(need.values())} pages needed, {len(self._free)} free")
+        need = self._pages_for(seqs, counts)
         for s in seqs:
             self._held[s] += [self._free.pop() for _ in range(need[s])]
         total = sum(counts)
@@ -137,6 +142,7 @@ class PagedSession:
         tokens = np.ascontiguousarray(tokens, np.int32).reshape(-1)
         if tokens.size == 0:
             raise ValueError("empty prompt")
+        self._pages_for([seq], [int(tokens.size)])
         for i in range(0, tokens.size, MAX_ROWS):
             following = self.step({seq: tokens[i:i + MAX_ROWS]})[seq]
         return int(following[-1])

@@ -514,7 +514,7 @@ def test_read(gpu, P, bits):
 # ---------------------------------------------------------------- verify ----
 
 def verify_case(Q, P, seed, vocab, counts, max_rows=None, heat="mixed", drafted=True, spoil=None,
-                pad=0, rows=None, start=None, logprob=True, uniform=None):
+                pad=0, rows=None, start=None, logprob=True, uniform=None, ws=None):
     rng = np.random.default_rng(seed)
     start = np.array(start, np.int32) if start is not None else None if counts is None else \
         np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
@@ -542,7 +542,7 @@ def verify_case(Q, P, seed, vocab, counts, max_rows=None, heat="mixed", drafted=
     lb, tb, ub, hb, db, sb = map(up, (logits, tokens, u, temperature, draft, start))
     ostride = max_rows + 3
     out, acc, lp = Guarded(Q, 4 * seqs * ostride), Guarded(Q, 4 * seqs), Guarded(Q, 4 * seqs * ostride)
-    ws = Guarded(Q, P.verify_workspace_bytes(rows, seqs, vocab), 0)
+    ws = ws or Guarded(Q, P.verify_workspace_bytes(rows, seqs, vocab), 0)
     print(f"verify rows={rows} seqs={seqs} vocab={vocab} drafted={drafted}", flush=True)
     for _ in range(2):
         P.verify(lb, vocab + pad, vocab, rows, tb, seqs, max_rows, ub, out.ptr, ostride, acc.ptr,
@@ -646,3 +646,237 @@ def test_verify_keeps_the_models_distribution(gpu, P):
     p = np.exp(row.astype(np.float64))
     want = p / p.sum() * counts.sum()
     assert ((counts - want) ** 2 / want).sum() < 25.7
+
+
+# -------------------------------------------------------------- together ----
+
+class Round:
+    """A layer's step as it is used: new rows appended, attended to and read back, then
+    judged by their logits."""
+
+    def __init__(self, Q, P, seed, bits, heads=(16, 8, 128), page=32, vocab=5000, pages=60, seqs=4):
+        self.Q, self.P, self.heads, self.vocab = Q, P, heads, vocab
+        qh, kvh, d = heads
+        rng = np.random.default_rng(seed)
+        self.pool = Pool(Q, P, rng, 2, pages, page, kvh, d, bits)
+        self.pages, self.page, self.seqs, self.rows, self.max_rows = pages, page, seqs, 3 * seqs, 5
+        self.wide = pages // seqs
+        up, n = Q.DeviceBuffer, self.rows
+        cols = self.cols = (qh + 2 * kvh) * d
+        self.table, self.length, self.start = up(4 * seqs * self.wide), up(4 * seqs), up(4 * seqs + 4)
+        self.x, self.logits, self.draft = up(2 * n * cols), up(2 * n * vocab), up(4 * n * vocab)
+        self.norms = up(4 * d)
+        self.tokens, self.u, self.heat = up(4 * n), up(4 * n), up(4 * seqs)
+        self.outs = [up(s) for s in (2 * n * qh * d, 2 * n * qh * d, 4 * n * qh, 2 * n * kvh * d,
+                                     2 * n * kvh * d, 4 * seqs * 5, 4 * seqs, 4 * seqs * 5)]
+        self.b = P.Batch(self.table, self.length, seqs, self.wide, n, self.max_rows, start=self.start)
+        self.ws = [up(P.attn_workspace_bytes(self.pool.c, self.b, qh)),
+                   up(P.verify_workspace_bytes(n, seqs, vocab))]
+        for w in self.ws:
+            w.fill(0)
+        self.put(seed)
+
+    def put(self, seed):
+        """Other inputs, tables, lengths and starts in the same buffers."""
+        rng = np.random.default_rng(seed)
+        counts = rng.integers(0, self.max_rows + 1, self.seqs)
+        while counts.sum() > self.rows:
+            counts[counts.argmax()] -= 1
+        self.table.upload(rng.permutation(self.pages)[:self.seqs * self.wide].astype(np.int32))
+        self.length.upload(rng.integers(6, self.wide * self.page + 1, self.seqs).astype(np.int32))
+        self.start.upload(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+        self.x.upload(normal(rng, (self.rows, self.cols)))
+        self.norms.upload(normal(rng, (2, self.heads[2])))
+        self.logits.upload(normal(rng, (self.rows, self.vocab), 3.0))
+        draft = rng.random((self.rows, self.vocab), dtype=np.float32)
+        self.draft.upload(draft / draft.sum(1, keepdims=True))
+        self.tokens.upload(rng.integers(0, self.vocab, self.rows).astype(np.int32))
+        self.u.upload(rng.random(self.rows, dtype=np.float32))
+        self.heat.upload(rng.integers(0, 3, self.seqs).astype(np.float32))
+        for o in self.outs:
+            o.fill(0xA5)
+
+    def run(self, stream=None):
+        qh, kvh, d = self.heads
+        P, x, n, o = self.P, self.x.ptr, self.rows, self.outs
+        P.append(self.pool.c, 1, self.b, x + 2 * qh * d, self.cols, x + 2 * (qh + kvh) * d, self.cols,
+                 k_norm=self.norms.ptr, q=x, q_stride=self.cols, q_heads=qh,
+                 q_norm=self.norms.ptr + 2 * d, q_out=o[0], q_out_stride=qh * d, theta=1e4,
+                 stream=stream)
+        P.attn(self.pool.c, 1, self.b, o[0], qh * d, qh, d ** -0.5, o[1], qh * d, o[2], self.ws[0],
+               self.ws[0].nbytes, stream)
+        P.read(self.pool.c, 1, 1, self.b, o[3], o[4], kvh * d, stream=stream)
+        P.verify(self.logits, self.vocab, self.vocab, n, self.tokens, self.seqs, self.max_rows, self.u,
+                 o[5], self.max_rows, o[6], start=self.start, temperature=self.heat, draft=self.draft,
+                 draft_stride=self.vocab, logprob=o[7], workspace=self.ws[1],
+                 workspace_bytes=self.ws[1].nbytes, stream=stream)
+
+    def got(self):
+        return [o.download(np.uint8) for o in self.outs]
+
+    def check(self):
+        """Attention, codes read back and tokens against the plain forms."""
+        qh, kvh, d = self.heads
+        data, scales = self.pool.get()
+        table = self.table.download(np.int32).reshape(self.seqs, self.wide)
+        length, start = self.length.download(np.int32), self.start.download(np.int32)
+        q = self.outs[0].download(np.float16).reshape(self.rows, qh, d)
+        layer = (data[0][1], data[1][1], *(None if s is None else s[1] for s in scales))
+        mine = np.zeros(self.rows, bool)
+        mine[:start[-1]] = True
+        ref = R.attention(np.where(mine[:, None, None], q, 0), layer, table, length, start, self.max_rows,
+                          float(np.float32(d ** -0.5)))
+        check_attn(self.outs[1].download(np.float16).reshape(self.rows, qh, d),
+                   self.outs[2].download(np.float32).reshape(self.rows, qh), ref)
+        want, accepted, _, margin = R.verify(
+            self.logits.download(np.float16).reshape(self.rows, -1), self.tokens.download(np.int32), start,
+            self.seqs, self.max_rows, self.u.download(np.float32), self.heat.download(np.float32),
+            self.draft.download(np.float32).reshape(self.rows, -1))
+        assert margin > 2.0 ** -40
+        assert np.array_equal(self.outs[5].download(np.int32).reshape(self.seqs, -1), want)
+        assert np.array_equal(self.outs[6].download(np.int32), accepted)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_captured_and_replayed(gpu, P, bits):
+    """One graph of the operators together, replayed as tables, lengths, starts and inputs
+    change, with eager runs and synchronizations between: the eager run's bits each time."""
+    r = Round(gpu, P, 1, bits)
+    stream = gpu.Stream()
+    r.run(stream)
+    stream.synchronize()
+    graph = gpu.Graph(stream, lambda: r.run(stream))
+    for seed in range(2, 7):
+        r.put(seed)
+        r.run(stream)
+        stream.synchronize()
+        eager = r.got()
+        r.check()
+        for _ in range(2):
+            for o in r.outs:
+                o.fill(0xA5)
+            graph.launch(stream)
+            stream.synchronize()
+            for a, b in zip(eager, r.got()):
+                assert np.array_equal(a, b)
+    graph.destroy()
+
+
+def test_two_streams_at_once(gpu, P):
+    """Rounds with pools and workspaces of their own, in flight together."""
+    rounds = [Round(gpu, P, 11, 16), Round(gpu, P, 12, 8), Round(gpu, P, 13, 8, (4, 1, 64), 48, 20011)]
+    alone = []
+    for r in rounds:
+        r.run()
+        gpu.synchronize()
+        alone.append(r.got())
+    streams = [gpu.Stream() for _ in rounds]
+    for _ in range(5):
+        for r, s in zip(rounds, streams):
+            r.run(s)
+    for r, s, want in zip(rounds, streams, alone):
+        s.synchronize()
+        for a, b in zip(want, r.got()):
+            assert np.array_equal(a, b)
+
+
+def test_one_workspace_for_all_calls(gpu, P):
+    """A workspace of the largest calls serves other heads, lengths, rows and types in turn,
+    also when what lies behind its counters is left over from them."""
+    rng = np.random.default_rng(14)
+    cases = [((16, 8, 128), 16, 32, [900, 40], [3, 1]), ((14, 2, 64), 8, 16, [5000], [40]),
+             ((16, 1, 128), 16, 64, [3000, 0, 17], None), ((64, 2, 64), 8, 256, [700, 2000], [1, 20]),
+             ((1, 1, 128), 16, 16, [12000], [1]), ((16, 8, 128), 8, 32, [200] * 30, None)]
+    calls, most = [], 0
+    for heads, bits, page, lengths, counts in cases:
+        need = sum((n + page - 1) // page for n in lengths) + 1
+        pool = Pool(gpu, P, rng, 1, need, page, heads[1], heads[2], bits)
+        batch = Batch(gpu, P, rng, pool, lengths, counts)
+        q = normal(rng, (batch.rows, heads[0], heads[2]))
+        calls.append((pool, batch, q, run_attn(gpu, P, pool, batch, q, 0.1)))
+        most = max(most, P.attn_workspace_bytes(pool.c, batch.c, heads[0]))
+    ws = Guarded(gpu, most, 0)
+    for i in rng.integers(0, len(calls), 40):
+        pool, batch, q, want = calls[i]
+        for a, b in zip(want, run_attn(gpu, P, pool, batch, q, 0.1, ws=ws)):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    shapes = [([3, 1, 5], 40000), ([1] * 9, 151936), ([5] * 20, 1000), (None, 9000)]
+    most = max(P.verify_workspace_bytes(100, 40, v) for _, v in shapes)
+    ws = Guarded(gpu, most, 0)
+    for i in (0, 1, 2, 3, 2, 1, 0, 3, 1):
+        verify_case(gpu, P, 20 + i, shapes[i][1], shapes[i][0], rows=40 if i == 3 else None, ws=ws)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_offsets_past_32_bits(gpu, P, bits):
+    """The pages of a second layer behind 2^32 values: written, attended to, read back."""
+    rng = np.random.default_rng(15)
+    qh, kvh, d = 16, 8, 128
+    page, pages, lengths = 4096, 600, [300, 5000, 20]
+    n = 2 * pages * kvh * page
+    size = n * d * bits // 8
+    kb, vb = gpu.DeviceBuffer(size), gpu.DeviceBuffer(size)
+    sb = [gpu.DeviceBuffer(4 * n) if bits == 8 else None for _ in range(2)]
+    for b in (kb, vb, *sb):
+        if b is not None:
+            b.fill(0x7F if bits == 16 else 0)  # f16 NaN
+    c = P.Pages(kb, vb, pages, page, 2, kvh, d, *sb)
+    table = np.array([[599, 0], [598, 300], [2, 1]], np.int32)
+    tb, lb = gpu.DeviceBuffer.from_array(table), gpu.DeviceBuffer.from_array(np.array(lengths, np.int32))
+    start = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    stb = gpu.DeviceBuffer.from_array(start)
+    every = P.Batch(tb, lb, 3, 2, int(start[-1]), 5000, start=stb)
+    x = normal(rng, (int(start[-1]), 2, kvh * d))
+    xb = gpu.DeviceBuffer.from_array(x)
+    print(f"offsets bits={bits}", flush=True)
+    P.append(c, 1, every, xb, 2 * kvh * d, xb.ptr + 2 * kvh * d, 2 * kvh * d)
+    outs = [gpu.DeviceBuffer(x.nbytes // 2) for _ in range(2)]
+    P.read(c, 1, 1, every, outs[0], outs[1], kvh * d)
+    last = P.Batch(tb, lb, 3, 2, 3)
+    q = normal(rng, (3, qh, d))
+    qb, out, lse = gpu.DeviceBuffer.from_array(q), gpu.DeviceBuffer(q.nbytes), gpu.DeviceBuffer(4 * 3 * qh)
+    ws = gpu.DeviceBuffer(P.attn_workspace_bytes(c, last, qh))
+    ws.fill(0)
+    P.attn(c, 1, last, qb, qh * d, qh, 0.09, out, qh * d, lse, ws, ws.nbytes)
+    gpu.synchronize()
+    # a small pool with the same rows, under the same tables
+    held = sorted({0, 1, 2, 300, 598, 599})
+    small_table = np.searchsorted(held, table).astype(np.int32)
+    data = [np.zeros((len(held), kvh, page, d), np.float16 if bits == 16 else np.int8) for _ in range(2)]
+    scale = [np.zeros(a.shape[:3], np.float32) if bits == 8 else None for a in data]
+    for i in range(2):
+        got = outs[i].download(np.float16).reshape(-1, kvh, d)
+        want = x[:, i].reshape(-1, kvh, d)
+        if bits == 16:
+            assert np.array_equal(got, want)
+        code, sc = quantised(want)
+        if bits == 8:  # half a step and f16's rounding
+            g, y, step = got.astype(np.float64), want.astype(np.float64), sc[..., None].astype(np.float64)
+            assert (np.abs(g - y) <= step * (0.5 + 2.0 ** -16) + 2.0 ** -11 * np.abs(g) + 2.0 ** -25).all()
+            code = np.rint(g / np.where(step > 0, step, 1))
+        for s in range(3):
+            for p in range(lengths[s]):
+                at = small_table[s, p // page], slice(None), p % page
+                data[i][at] = want[start[s] + p] if bits == 16 else code[start[s] + p]
+                if bits == 8:
+                    scale[i][at] = sc[start[s] + p]
+    ref = R.attention(q, (data[0], data[1], *scale), small_table, np.array(lengths, np.int32), None, 1,
+                      float(np.float32(0.09)))
+    check_attn(out.download(np.float16).reshape(q.shape), lse.download(np.float32).reshape(3, qh), ref)
+    for b in (kb, vb, *sb):
+        if b is not None:
+            b.free()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_same_inputs_same_bits(gpu, P, bits):
+    """Sequences cut among many workgroups, which arrive in any order."""
+    rng = np.random.default_rng(16)
+    pool = Pool(gpu, P, rng, 1, 700, 32, 8, 128, bits)
+    batch = Batch(gpu, P, rng, pool, [20000, 37, 1500], [2, 1, 5])
+    q = normal(rng, (batch.rows, 16, 128), 1.5)
+    ws = workspace(gpu, P, pool, batch, 16)
+    first = run_attn(gpu, P, pool, batch, q, 0.09, ws=ws)
+    for _ in range(6):
+        for a, b in zip(first, run_attn(gpu, P, pool, batch, q, 0.09, ws=ws)):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))

@@ -74,7 +74,7 @@ PAGES = dict(k=A, v=A, pages=10, page_size=16, layers=2, kv_heads=2, head_dim=64
 BATCH = dict(table=A, length=A, seqs=3, max_pages=4, rows=3, max_rows=1)
 APPEND = dict(k=A, k_stride=128, v=A, v_stride=128, k_norm=A, q=A, q_stride=256, q_heads=4,
               q_norm=A, q_out=A * 16, q_out_stride=256, theta=1e6)
-ATTN = dict(q=A, q_stride=256, q_heads=4, scale=0.125, out=A, out_stride=256, lse=A, workspace=A,
+ATTN = dict(q=A, q_stride=256, q_heads=4, scale=0.125, out=2 * A, out_stride=256, lse=A, workspace=A,
             workspace_bytes=1 << 40)
 READ = dict(layer=0, layers=2, k_out=A, v_out=A, row_stride=128, layer_stride=1024)
 
@@ -158,7 +158,7 @@ def test_append_refusals(Q, P, kw, code):
     ({"q_heads": 0}, 6), ({"q_heads": 3}, 6), ({"q_heads": 66}, 6), ({"q_heads": 258}, 6),
     ({"q_stride": 248}, 6), ({"q_stride": 260}, 6), ({"out_stride": 255}, 6), ({"out_stride": 128}, 6),
     ({"scale": 0.0}, 9), ({"scale": -1.0}, 9), ({"scale": math.inf}, 9), ({"scale": math.nan}, 9),
-    ({"workspace": A + 16}, 5)])
+    ({"scale": 2.0 ** 127.8}, 9), ({"out": A}, 9), ({"workspace": A + 16}, 5)])
 def test_attn_refusals(Q, P, kw, code):
     refused(Q, code, P.attn, pages(P), 0, batch(P), **{**ATTN, **kw})
 
@@ -170,7 +170,7 @@ def test_attn_rows_of_a_sequence(Q, P):
 @pytest.mark.parametrize("kw,code", [
     ({"layers": 0}, 4), ({"layers": 3}, 4), ({"layer": 1}, 4), ({"k_out": A + 8}, 5), ({"v_out": A + 2}, 5),
     ({"row_stride": 120}, 6), ({"row_stride": 132}, 6), ({"row_stride": -128}, 6),
-    ({"layer_stride": 4}, 6), ({"layer_stride": -1024}, 6)])
+    ({"layer_stride": 4}, 6), ({"layer_stride": -1024}, 6), ({"layer_stride": 0}, 6)])
 def test_read_refusals(Q, P, kw, code):
     refused(Q, code, P.read, pages(P), batch=batch(P), **{**READ, **kw})
 

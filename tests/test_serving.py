@@ -108,6 +108,10 @@ def test_refused_steps_change_nothing(make):
         with pytest.raises(ValueError):
             s.step(bad)
         assert held(s) == before and s.length == lengths
+    for n in (0, 25, 200):  # a prompt that does not fit is not begun
+        with pytest.raises(ValueError):
+            s.prompt(a, np.zeros(n))
+        assert held(s) == before and s.length == lengths
     with pytest.raises(KeyError):
         s.step({9: [1]})
     assert s.add() == 2
