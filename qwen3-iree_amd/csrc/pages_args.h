@@ -94,7 +94,7 @@ struct VerifyStat {
   int32_t first;
 };
 
-// What decides a sequence's last token: its row, 16 log2(e) / T and T, the accepted
+// What decides a sequence's last token: its row, 256 log2(e) / T and T, the accepted
 // tokens, the random number, and the token that was refused.
 struct VerifyPick {
   VerifyStat row;

@@ -963,9 +963,8 @@ PAGES_READ(128, q8, true)
 // row, the sums of max(p - q, 0) and of p; the last workgroup of a sequence finds the part
 // and the index whose running sum passes the random number.  All in f64: next to a
 // border of the running sums, one in 151936, f32 sums would give other tokens.  exp is
-// 2^(n / 16) from a table (16 doubles: no two in one LDS bank) times a polynomial of
-// degree 5 in the rest, |rest| <= ln 2 / 32: 1.5e-13 of it is left out, for a third of the
-// instructions of a full f64 exp.
+// 2^(n / 256) from a table in LDS times a polynomial of degree 3 in the rest, |rest| <= ln 2 /
+// 512: 1.4e-13 of it is left out, for a fourth of the instructions of a full f64 exp.
 namespace {
 
 __constant__ double kExp2[16] = {  // 2^(n / 16)
@@ -975,33 +974,52 @@ __constant__ double kExp2[16] = {  // 2^(n / 16)
     0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0,
 };
 
-// exp((x - top) / T), 0 below 2^-1000 and for a NaN.  The table lies in LDS, the
-// polynomial's coefficients in scalar registers; n comes out of the low bits of a sum with
-// 1.5 2^52 and goes into the exponent by an addition (f64 roundings, conversions and
-// ldexp have a fraction of the rate).  Where top is +inf, which alone has weight then,
-// values go through near() first.
+__constant__ double kFine2[16] = {  // 2^(n / 256)
+    0x1.0000000000000p+0, 0x1.00b1afa5abcbfp+0, 0x1.0163da9fb3335p+0, 0x1.02168143b0281p+0,
+    0x1.02c9a3e778061p+0, 0x1.037d42e11bbccp+0, 0x1.04315e86e7f85p+0, 0x1.04e5f72f654b1p+0,
+    0x1.059b0d3158574p+0, 0x1.0650a0e3c1f89p+0, 0x1.0706b29ddf6dep+0, 0x1.07bd42b72a836p+0,
+    0x1.0874518759bc8p+0, 0x1.092bdf66607e0p+0, 0x1.09e3ecac6f383p+0, 0x1.0a9c79b1f3919p+0,
+};
+
+// table[n] = 2^(n / 256), by 256 threads
+__device__ __forceinline__ void fill_table(double* table) {
+  const int t = threadIdx.x;
+  table[t] = kExp2[t >> 4] * kFine2[t & 15];
+}
+
+// exp((x - top) / T), 0 below 2^-1000 and for a NaN, with unit = 256 log2(e) / T: 2^(1/256)
+// to the power x unit - C, C = rint(top unit), times norm, which makes up for C.  y = x unit +
+// (1.5 2^52 - C) holds the nearest integer's n = rint(x unit) - C in its low bits, y less
+// that constant is rint(x unit), both exact, so that the rest has the rounding of one fma; n goes
+// into the exponent by an addition (f64 roundings, conversions and ldexp have a fraction
+// of the rate).  x becomes an f64 by a shift, 2^896 too small, which the unit makes up
+// for.  Where top is +inf, which alone has weight then, values go through near() first.
 struct Exp {
   const double* table;
-  double top, unit;
-  double c1, c2, c3, c4, c5, magic;
+  double unit, base, norm;
+  double c1, c2, c3;
   float least;  // x of 2^-1000, or less
   bool far;
   // unit: unit_of(T)
   __device__ __forceinline__ Exp(const double* table, float top_of, double unit_of_heat)
       : table(table), far(top_of == __builtin_inff()) {
     const float at = far ? 0.0f : top_of;
-    top = (double)at;
     // An f16 below `top` is further from it than |top| 2^-12 and 2^-24: a larger unit only
     // takes 2^-1000 to something smaller.
-    unit = fmin(far ? 1.0 : unit_of_heat, (double)(16000.0f / fmaxf(fabsf(at) * 0x1p-12f, 0x1p-24f)));
-    c1 = 0x1.62e42fefa39efp-5;
-    c2 = 0x1.ebfbdff82c58fp-11;
-    c3 = 0x1.c6b08d704a0c0p-17;
-    c4 = 0x1.3b2ab6fba4e77p-23;
-    c5 = 0x1.5d87fe78a6731p-30;
-    magic = 6755399441055744.0;
-    asm("" : "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4), "+s"(c5), "+s"(magic));
-    least = at - 16000.0f / (float)unit;
+    unit = fmin(far ? 1.0 : unit_of_heat, (double)(256000.0f / fmaxf(fabsf(at) * 0x1p-12f, 0x1p-24f)));
+    // (of 11 bits as the others are)
+    least = __uint_as_float(__float_as_uint(at - 256000.0f / (float)unit) & ~0x1fffu);
+    c1 = 0x1.62e42fefa39efp-9;
+    c2 = 0x1.ebfbdff82c58fp-19;
+    c3 = 0x1.c6b08d704a0c0p-29;
+    asm("" : "+s"(c1), "+s"(c2), "+s"(c3));
+    const double magic = 6755399441055744.0, z = (double)at * unit, c = (z + magic) - magic;
+    base = magic - c;
+    norm = poly(-fma((double)at, unit, -c));
+    unit *= 0x1p896;
+  }
+  __device__ __forceinline__ double poly(double r) const {
+    return fma(fma(fma(c3, r, c2), r, c1), r, 1.0);
   }
   __device__ __forceinline__ float near(float x) const {
     return !far ? x : x == __builtin_inff() ? 0.0f : -__builtin_inff();
@@ -1015,24 +1033,27 @@ struct Exp {
     }
     return v;
   }
-  // the same with 2^-1000, about, in the place of 0
-  __device__ __forceinline__ double some(float x) const {
-    const double z = ((double)fmaxf(x, least) - top) * unit;
-    const double y = z + magic, r = z - (y - magic);
-    const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, y);
-    const double p = fma(fma(fma(fma(fma(c5, r, c4), r, c3), r, c2), r, c1), r, 1.0) * table[i & 15];
-    const uint64_t b = __builtin_bit_cast(uint64_t, p);
-    const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(i >> 4) << 20);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
+  // The same without norm and with 2^-1000, about, in the place of 0: a product, of which
+  // `to` is the second factor.  x: an f16's value.
+  __device__ __forceinline__ double some(float x, double& to) const {
+    const uint32_t bits = (uint32_t)((int32_t)__float_as_uint(fmaxf(x, least)) >> 3) & 0x8fffffffu;
+    const double v = __builtin_bit_cast(double, (uint64_t)bits << 32);
+    const double y = fma(v, unit, base);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, y);
+    const uint64_t b = __builtin_bit_cast(uint64_t, table[n & 255]);
+    to = __builtin_bit_cast(double, (uint64_t)((uint32_t)(b >> 32) + ((n & ~255u) << 12)) << 32 | (uint32_t)b);
+    return poly(fma(v, unit, -(y - base)));
   }
-  __device__ __forceinline__ double operator()(float x) const {
-    const double w = some(x);
+  __device__ __forceinline__ double raw(float x) const {  // without norm
+    double to;
+    const double w = some(x, to) * to;
     return x > least ? w : 0.0;
   }
+  __device__ __forceinline__ double operator()(float x) const { return raw(x) * norm; }
 };
-// 16 log2(e) / T; 0 where the maximum takes all
+// 256 log2(e) / T; 0 where the maximum takes all
 __device__ __forceinline__ double unit_of(float heat) {
-  return heat > 0.0f ? fmax(23.083120654223414519 / (double)heat, 1e-30) : 1.0;
+  return heat > 0.0f ? fmax(369.3299304675746 / (double)heat, 1e-30) : 1.0;
 }
 
 // The sum over the wave, in every lane: 16 lanes by DPP, then the four rows.
@@ -1211,7 +1232,7 @@ __device__ __forceinline__ void verify_pick(const VerifyArgs& A, int s, int lo, 
 
 template <int V>
 __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
-  __shared__ double table[16], sums[4];
+  __shared__ double table[256], sums[4];
   __shared__ float tops[4];
   __shared__ int firsts[4], arrived;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -1221,7 +1242,7 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   u32x4 v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8);
-  if (t < 16) table[t] = kExp2[t];
+  fill_table(table);
   int lo, m;
   float heat = 1.0f;
   const int s = seq_of_row(A.b, row, lo, m, A.temperature, heat);
@@ -1254,12 +1275,15 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
 #pragma unroll 1
     for (int i = 0; i < V; ++i) {
       const u32x4 x8 = weight.near(logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8));
-      double w[8];
+      double w[2] = {0.0, 0.0}, to;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = weight.some(half_at(x8, e));
-      sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      for (int e = 0; e < 8; ++e) {
+        const double one = weight.some(half_at(x8, e), to);
+        w[e & 1] = fma(one, to, w[e & 1]);
+      }
+      sum += w[0] + w[1];
     }
-    sum = wave_sum64(sum);
+    sum = wave_sum64(sum) * weight.norm;
   }
   if (lane == 0) {
     sums[wave] = sum;
@@ -1306,11 +1330,11 @@ __device__ __forceinline__ VerifyStat join_row(const VerifyArgs& A, int row, int
 // What an entry of the deciding row weighs: max(p - q, 0) and p.
 struct Decide {
   Exp weight;
-  double inv_total;
+  double inv_total;  // with weight's norm
   bool greedy, drafted;
   int first, told;  // the maximum's lowest index, the refused token
   __device__ __forceinline__ void operator()(int j, float x, float d, double& rest, double& p) const {
-    p = weight(x) * inv_total;
+    p = weight.raw(x) * inv_total;
     if (greedy) p = j == first ? 1.0 : 0.0;
     rest = drafted ? (d > 0.0f ? fmax(p - (double)d, 0.0) : p) : j == told ? 0.0 : p;
   }
@@ -1319,7 +1343,7 @@ struct Decide {
 // V parts of 2048 entries a workgroup.
 template <int V>
 __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
-  __shared__ double table[16], sum[4][2], part_sum[4][V][2], base;
+  __shared__ double table[256], sum[4][2], part_sum[4][V][2], base;
   __shared__ uint64_t over[4], some_over[4];
   __shared__ int arrived;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.y;
@@ -1328,7 +1352,7 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   const bool single = A.b.max_rows == 1;
   VerifyPick pick = {};
   if (!single) pick = A.picks[s];
-  if (t < 16) table[t] = kExp2[t];
+  fill_table(table);
   int32_t* const out = A.out + s * A.out_stride;
   float* const logprob = A.logprob ? A.logprob + s * A.out_stride : nullptr;
   if (m == 0) {
@@ -1353,7 +1377,8 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   if (blockIdx.x == 0 && t == 0) A.count[s * kCountStep] = 0;
   const int n = pick.n < 0 ? 0 : pick.n < m ? pick.n : m - 1;
   const bool refused = n < m - 1;
-  const Decide w = {Exp(table, pick.row.top, pick.unit), 1.0 / pick.row.sum, !(pick.heat > 0.0f),
+  const Exp weight(table, pick.row.top, pick.unit);
+  const Decide w = {weight, weight.norm / pick.row.sum, !(pick.heat > 0.0f),
                     A.draft != nullptr, pick.row.first, pick.told};
   const bool some = pick.row.top > -__builtin_inff();
   const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
