@@ -1006,9 +1006,10 @@ struct Exp {
     const float at = far ? 0.0f : top_of;
     // An f16 below `top` is further from it than |top| 2^-12 and 2^-24: a larger unit only
     // takes 2^-1000 to something smaller.
-    unit = fmin(far ? 1.0 : unit_of_heat, (double)(256000.0f / fmaxf(fabsf(at) * 0x1p-12f, 0x1p-24f)));
+    unit = fmin(far ? 1.0 : unit_of_heat,
+                (double)(255000.0f * __builtin_amdgcn_rcpf(fmaxf(fabsf(at) * 0x1p-12f, 0x1p-24f))));
     // (of 11 bits as the others are)
-    least = __uint_as_float(__float_as_uint(at - 256000.0f / (float)unit) & ~0x1fffu);
+    least = __uint_as_float(__float_as_uint(at - 255000.0f * __builtin_amdgcn_rcpf((float)unit)) & ~0x1fffu);
     c1 = 0x1.62e42fefa39efp-9;
     c2 = 0x1.ebfbdff82c58fp-19;
     c3 = 0x1.c6b08d704a0c0p-29;
@@ -1041,7 +1042,9 @@ struct Exp {
     const double y = fma(v, unit, base);
     const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, y);
     const uint64_t b = __builtin_bit_cast(uint64_t, table[n & 255]);
-    to = __builtin_bit_cast(double, (uint64_t)((uint32_t)(b >> 32) + ((n & ~255u) << 12)) << 32 | (uint32_t)b);
+    uint32_t hi = (uint32_t)(b >> 32) + ((n & ~255u) << 12);
+    asm("" : "+v"(hi));  // (or the compiler adds in 64 bits)
+    to = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
     return poly(fma(v, unit, -(y - base)));
   }
   __device__ __forceinline__ double raw(float x) const {  // without norm
@@ -1333,10 +1336,11 @@ struct Decide {
   double inv_total;  // with weight's norm
   bool greedy, drafted;
   int first, told;  // the maximum's lowest index, the refused token
-  __device__ __forceinline__ void operator()(int j, float x, float d, double& rest, double& p) const {
-    p = weight.raw(x) * inv_total;
-    if (greedy) p = j == first ? 1.0 : 0.0;
-    rest = drafted ? (d > 0.0f ? fmax(p - (double)d, 0.0) : p) : j == told ? 0.0 : p;
+  __device__ __forceinline__ double p(int j, float x) const {
+    return greedy ? (j == first ? 1.0 : 0.0) : weight.raw(x) * inv_total;
+  }
+  __device__ __forceinline__ double rest(int j, double p, float d) const {
+    return drafted ? fmax(p - (double)fmaxf(d, 0.0f), 0.0) : j == told ? 0.0 : p;
   }
 };
 
@@ -1386,8 +1390,15 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   // entries j .. j + 7
   auto sum8 = [&](int j, u32x4 v, const float (&d)[8], double& rest, double& all) {
     double r[8], p[8];
+    if (w.greedy) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w(j + e, half_at(v, e), d[e], r[e], p[e]);
+      for (int e = 0; e < 8; ++e) p[e] = j + e == w.first ? 1.0 : 0.0;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = w.weight.raw(half_at(v, e)) * w.inv_total;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = w.rest(j + e, p[e], d[e]);
     rest += ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
     all += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
   };
@@ -1530,7 +1541,8 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   float v = 0.0f;
   if (place >= 0 && lane < 8 && j < A.vocab) {
     v = (float)as_half(x[j]);
-    w(j, w.weight.near(v), q ? q[j] : 0.0f, f[0], f[1]);
+    f[1] = w.p(j, w.weight.near(v));
+    f[0] = w.rest(j, f[1], q ? q[j] : 0.0f);
   }
   const double c = base + wave_scan64(f[k]);  // (every lane takes part)
   const uint64_t b = __builtin_amdgcn_ballot_w64(f[k] > 0.0);
