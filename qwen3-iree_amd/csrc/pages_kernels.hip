@@ -112,27 +112,27 @@ __device__ __forceinline__ int turn_at(int i) {
   return (i & 7) * (D / 16) + (i >> 3);
 }
 
-// Norm (by weights wv) and rotation (by turn[turn_at(i)] = (cos, sin)) of a head's lane c.
+// Norm of a head's lane, by weights wv.
 template <int D>
-__device__ __forceinline__ void turn_head(double (&y)[8], int c, bool norm, u32x4 wv, double eps,
-                                          bool rotate, const double2* turn) {
-  if (norm) {
-    double ss = 0.0;
+__device__ __forceinline__ void norm_head(double (&y)[8], u32x4 wv, double eps) {
+  double ss = 0.0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
-    ss = over_head<D>(ss, [](double a, double b) { return a + b; });
-    const double r = rsqrt(ss / D + eps);
+  for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
+  ss = over_head<D>(ss, [](double a, double b) { return a + b; });
+  const double r = rsqrt(ss / D + eps);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (double)half_at(wv, j);
-  }
-  if (rotate) {
-    const bool second = c >= D / 16;
+  for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (double)half_at(wv, j);
+}
+
+// Rotation of a head's lane c by turn[turn_at(i)] = (cos, sin).
+template <int D>
+__device__ __forceinline__ void turn_head(double (&y)[8], int c, const double2* turn) {
+  const bool second = c >= D / 16;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double2 a = turn[turn_at<D>((8 * c) % (D / 2) + j)];
-      const double o = other_half<D>(y[j]);
-      y[j] = y[j] * a.x + o * (second ? a.y : -a.y);
-    }
+  for (int j = 0; j < 8; ++j) {
+    const double2 a = turn[turn_at<D>((8 * c) % (D / 2) + j)];
+    const double o = other_half<D>(y[j]);
+    y[j] = y[j] * a.x + o * (second ? a.y : -a.y);
   }
 }
 
@@ -183,9 +183,9 @@ __device__ __forceinline__ uint2 codes8(const double (&y)[8], float& scale) {
   return code;
 }
 
-template <int D, bool Q8>
+template <int D, bool Q8, int kThreads>
 __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
-  constexpr int G = D / 8;
+  constexpr int G = D / 8, kHeads = kThreads / G;
   __shared__ double2 turn[D / 2];
   const int t = threadIdx.x, c = t % G, row = blockIdx.x;
   const int heads = A.q_heads + 2 * A.kv_heads;
@@ -209,26 +209,29 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
   if (s < 0) return;
   const int64_t slot = (int64_t)length - m + (row - lo);
   const int64_t to = pool_row(A.b, s, slot, A.kv_heads, 0);  // of head 0
-  if (A.rotate) {
-    if (t < D / 2) {
-      const double by = (double)(A.positions ? (int64_t)position : slot) * step;
-      double2 a;
-      sincospi(2.0 * (by - rint(by)), &a.y, &a.x);
-      turn[turn_at<D>(t)] = a;
-    }
-    __syncthreads();
+  double y[8];
+  auto normed = [&](int h, u32x4 x) {  // into y
+    const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = (double)half_at(x, j);
+    if (!is_v && (is_q ? A.q_norm : A.k_norm)) norm_head<D>(y, is_q ? qw : kw, A.eps);
+  };
+  if (A.rotate && t < D / 2) {
+    const double by = (double)(A.positions ? (int64_t)position : slot) * step;
+    double2 a;
+    sincospi(2.0 * (by - rint(by)), &a.y, &a.x);
+    turn[turn_at<D>(t)] = a;
   }
-  for (; h < heads; h += 256 / G) {
+  if (h < heads) normed(h, x);  // while the angles' waves are busy
+  if (A.rotate) __syncthreads();
+  while (h < heads) {
     const u32x4 here = x;
-    if (h + 256 / G < heads) x = request(h + 256 / G);
+    const int next = h + kHeads;
+    if (next < heads) x = request(next);
     const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
     const int64_t at = to + (int64_t)(h - A.q_heads - (is_v ? A.kv_heads : 0)) * A.b.page_size;
     void* pool = is_v ? A.v_to : A.k_to;
-    double y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = (double)half_at(here, j);
-    if (!is_v)
-      turn_head<D>(y, c, (is_q ? A.q_norm : A.k_norm) != nullptr, is_q ? qw : kw, A.eps, A.rotate, turn);
+    if (!is_v && A.rotate) turn_head<D>(y, c, turn);
     if (is_q) {
       *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + h * D + 8 * c) = packed8(y);
     } else if constexpr (Q8) {
@@ -242,6 +245,8 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
       *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(pool) + at * D + 8 * c) =
           is_v ? here : packed8(y);
     }
+    h = next;
+    if (h < heads) normed(h, x);
   }
 }
 
@@ -249,7 +254,10 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
 
 #define PAGES_APPEND(D, N, Q8)                                                                    \
   extern "C" __global__ __launch_bounds__(256) void pages_append_##D##_##N(PagesAppendArgs A) {   \
-    pages_append<D, Q8>(A);                                                                       \
+    pages_append<D, Q8, 256>(A);                                                                  \
+  }                                                                                               \
+  extern "C" __global__ __launch_bounds__(512) void pages_append_wide_##D##_##N(PagesAppendArgs A) { \
+    pages_append<D, Q8, 512>(A);                                                                  \
   }
 PAGES_APPEND(64, f16, false)
 PAGES_APPEND(64, q8, true)

@@ -18,7 +18,7 @@ namespace {
 struct {
   hipModule_t module = nullptr;
   // [head_dim 64, 128][f16, q8]
-  hipFunction_t append[2][2] = {}, attn[2][2][3] = {}, read[2][2] = {};
+  hipFunction_t append[2][2][2] = {}, attn[2][2][3] = {}, read[2][2] = {};
   hipFunction_t sums[2] = {}, rest[2] = {};  // chunks of 2048, 8192
 } c;
 
@@ -151,6 +151,10 @@ uint32_t float_bits(float f) {
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int32_t kAttnRowsMax = 256;
 constexpr int kVerifyRowsMax = 65535;
+// Up to this many rows a CU, kv_pages_append gives a row 512 threads, all its heads at once,
+// where 256 take two turns: 1 row of 32 heads 4.5 -> 4.0 us, 256 rows 5.1 -> 4.5, 512 rows 6.0 ->
+// 5.9, but 1024 rows 7.7 -> 8.1 and 8192 rows 32.5 -> 42.3 (8-bit pages, replayed in a graph).
+constexpr int kAppendWide = 2;
 
 // How kv_pages_attn divides its work.
 struct AttnPlan {
@@ -202,8 +206,10 @@ void pages_load(const char* path) {
     for (int q = 0; q < 2; ++q) {
       char name[64];
       const char* type = q ? "q8" : "f16";
-      snprintf(name, sizeof(name), "pages_append_%d_%s", 64 << d, type);
-      get(&c.append[d][q], name);
+      for (int wide = 0; wide < 2; ++wide) {
+        snprintf(name, sizeof(name), "pages_append_%s%d_%s", wide ? "wide_" : "", 64 << d, type);
+        get(&c.append[d][q][wide], name);
+      }
       snprintf(name, sizeof(name), "pages_read_%d_%s", 64 << d, type);
       get(&c.read[d][q], name);
       for (int t = 0; t < 3; ++t) {
@@ -307,8 +313,9 @@ int kv_pages_append(const kv_pages* a, int32_t layer, const kv_batch* batch, con
     for (int i = 0; i < a->head_dim / 2; ++i, turn *= step) args.turns[i] = (double)turn;
   }
   void* p[] = {&args};
-  return q8_shim::launch(c.append[dim_of(a)][a->type], (uint32_t)batch->rows, 256, p,
-                         static_cast<hipStream_t>(stream));
+  const bool wide = batch->rows <= kAppendWide * q8_shim::compute_units();
+  return q8_shim::launch(c.append[dim_of(a)][a->type][wide], (uint32_t)batch->rows,
+                         wide ? 512 : 256, p, static_cast<hipStream_t>(stream));
 }
 
 size_t kv_pages_attn_workspace_bytes(const kv_pages* a, const kv_batch* batch, int32_t q_heads) {
