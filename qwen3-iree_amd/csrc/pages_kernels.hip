@@ -70,10 +70,15 @@ __device__ __forceinline__ float half_at(u32x4 v, int j) {
 
 // --------------------------------------------------------------- append ----
 //
-// One workgroup a row; D / 8 lanes a head, 8 values each, all of the row's q, k
-// and v heads in turn.  The rotation's partners, dims i and i + D/2, are lanes half a
-// head apart.  The angles' cosines and sines are worked out once a row.  In f64: the rounding
-// to codes must not depend on an order of sums.
+// One workgroup a row; D / 8 lanes a head, 8 values each, the row's q, k and v heads
+// side by side (and in turn where there are more than the threads hold).  The rotation's
+// partners, dims i and i + D/2, are lanes half a head apart.  The angles' cosines and sines are
+// worked out once a row, by one wave while the others norm their heads.  In f64: the
+// rounding to codes must not depend on an order of sums.
+// Few rows are bound by latency (the starts, the page's entry, the angles, the store: 1 row
+// 3.3 us, 256 rows 5.3 us of 32 heads), many by the f64 operations: 8997 rows with 8-bit
+// pages 45.5 us, where their 129 MB would take 25.  A wave a row and heads in f32 were slower
+// or moved codes.
 namespace {
 
 template <int kCtrl>
@@ -278,6 +283,12 @@ PAGES_APPEND(128, q8, true)
 //     slots mean slots 4 grp + e, 16 + 4 grp + e.  A lane reads those 8 slots' dims
 //     (D/16) c16 .. + D/16 - 1 and pairs them up by byte permutes; MFMA n of the
 //     D / 16 makes the dims (D/16) i + n.
+// K and V come from memory once and are used by one wave alone: LDS would only add a stop.
+// A block's registers are requested again for the wave's next block as soon as they have
+// been used (a second set of them spilled), two waves a SIMD cover the rest.  Bound by
+// memory where sequences are long: 4 x 131072 slots of 8 kv heads in 8 bits, 1.1 GB, 193 us, 5.7 TB/s
+// (a copy 5.1); 16 x 8000 slots in f16, five rows each, 35 us, 4.0 TB/s, of which cut
+// sequences and ramps take 8; 1 x 300 slots 8 us, all latency.
 // A weight goes into the product as the sum of two f16 values (2^-22 of itself).
 // 8-bit codes become f16 multiples of 2^-9, exact; a row's k scale multiplies its
 // score and its v scale its weight, so that the reference is that of s + log2 v_scale.
@@ -909,7 +920,8 @@ PAGES_ATTN_T(128, q8, true)
 // ------------------------------------------------------------------ read ----
 //
 // A wave a row and layer, 8 values a lane at a time: bound by memory, one read of the
-// pages and one write.
+// pages and one write.  28 layers of 4096 rows from 8-bit pages, 713 MB, 136 us, 5.25 TB/s; one
+// layer of 333 rows 4 us, the latency of starts, table, page and store.
 namespace {
 
 template <int D, bool Q8>
@@ -973,6 +985,10 @@ PAGES_READ(128, q8, true)
 // border of the running sums, one in 151936, f32 sums would give other tokens.  exp is
 // 2^(n / 256) from a table in LDS times a polynomial of degree 3 in the rest, |rest| <= ln 2 /
 // 512: 1.4e-13 of it is left out, for a fourth of the instructions of a full f64 exp.
+// Bound by the f64 operations beside the memory: 185 rows of 151936 logits (56 MB) 30 us, of
+// which 16 are VALU; the deciding rows of 64 sequences with the drafter's (58 MB) 23 us; one
+// row 3 and 10 us, the last being a chain of loads and joins in one workgroup.  A wave that
+// keeps its own chunk, without the workgroup's joins, was no faster (30 us).
 namespace {
 
 __constant__ double kExp2[16] = {  // 2^(n / 16)
@@ -1155,9 +1171,9 @@ __device__ __forceinline__ bool last_here(int32_t* count, int all, int* arrived)
   return *arrived == all - 1;
 }
 
-__device__ __forceinline__ float log_of(float x, float top, double total, float heat) {
+__device__ __forceinline__ float log_of(float x, float top, double log_total, float heat) {
   if (!(heat > 0.0f)) return 0.0f;
-  return (float)((x == top ? 0.0 : ((double)x - (double)top) / (double)heat) - log(total));
+  return (float)((x == top ? 0.0 : ((double)x - (double)top) / (double)heat) - log_total);
 }
 
 // The last workgroup of a sequence in the first launch: its rows joined from their
@@ -1237,7 +1253,7 @@ __device__ __forceinline__ void verify_pick(const VerifyArgs& A, int s, int lo, 
   if (t < A.b.max_rows && t != n) {
     A.out[s * A.out_stride + t] = t < n ? told : -1;
     if (A.logprob)
-      A.logprob[s * A.out_stride + t] = t < n ? log_of(x, st[t].top, st[t].sum, heat) : 0.0f;
+      A.logprob[s * A.out_stride + t] = t < n ? log_of(x, st[t].top, log(st[t].sum), heat) : 0.0f;
   }
 }
 
@@ -1357,6 +1373,8 @@ template <int V>
 __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   __shared__ double table[256], sum[4][2], part_sum[4][V][2], base;
   __shared__ uint64_t over[4], some_over[4];
+  __shared__ __attribute__((aligned(16))) uint16_t few[8];
+  __shared__ float few_q[8];
   __shared__ int arrived;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = blockIdx.y;
   const int lo = A.b.start ? A.b.start[s] : s;
@@ -1376,28 +1394,40 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
     }
     return;
   }
-  __syncthreads();  // the table
   if (single) {
     pick.heat = A.temperature ? A.temperature[s] : 1.0f;
     pick.u = A.uniform[lo];
-    pick.unit = unit_of(pick.heat);
     pick.told = -1;
+  }
+  // (starts that descend may have left a sequence without a pick)
+  const int n = pick.n < 0 ? 0 : pick.n < m ? pick.n : m - 1;
+  const bool refused = n < m - 1;
+  const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
+  const float* q = A.draft && refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
+  // entries j .. j + 7
+  auto request8 = [&](int j, u32x4& v, float (&d)[8]) {
+    v = logits8(x + j, A.vocab - j);
+    if (q) probs8(q + j, A.vocab - j, d);
+  };
+  const int part0 = blockIdx.x * V;
+  u32x4 v[V];
+  float d[V][8] = {};
+#pragma unroll
+  for (int i = 0; i < V; ++i) request8((part0 + i) * 2048 + t * 8, v[i], d[i]);
+  __syncthreads();  // the table
+  if (single) {
+    pick.unit = unit_of(pick.heat);
     pick.row = join_row(A, lo, lane, pick.unit, pick.heat, table);
     if (blockIdx.x == 0 && t == 0) A.accepted[s] = 0;
   }
-  // (starts that descend may have left a sequence without a pick)
   if (blockIdx.x == 0 && t == 0) A.count[s * kCountStep] = 0;
-  const int n = pick.n < 0 ? 0 : pick.n < m ? pick.n : m - 1;
-  const bool refused = n < m - 1;
   const Exp weight(table, pick.row.top, pick.unit);
   const Decide w = {weight, weight.norm / pick.row.sum, !(pick.heat > 0.0f),
                     A.draft != nullptr, pick.row.first, pick.told};
   const bool some = pick.row.top > -__builtin_inff();
-  const uint16_t* x = A.logits + (int64_t)(lo + n) * A.logits_stride;
-  const float* q = w.drafted && refused ? A.draft + (int64_t)(lo + n) * A.draft_stride : nullptr;
-  // entries j .. j + 7
   auto sum8 = [&](int j, u32x4 v, const float (&d)[8], double& rest, double& all) {
     double r[8], p[8];
+    v = w.weight.near(v);
     if (w.greedy) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = j + e == w.first ? 1.0 : 0.0;
@@ -1409,10 +1439,6 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
     for (int e = 0; e < 8; ++e) r[e] = w.rest(j + e, p[e], d[e]);
     rest += ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
     all += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-  };
-  auto request8 = [&](int j, u32x4& v, float (&d)[8]) {
-    v = w.weight.near(logits8(x + j, A.vocab - j));
-    if (q) probs8(q + j, A.vocab - j, d);
   };
   // Pairs of sums, one pair a thread: those of the threads before, and of all.
   auto running = [&](const double (&v)[2], double (&before)[2], double (&total)[2]) {
@@ -1436,13 +1462,6 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   };
   double* const sums = A.rest + (int64_t)s * A.parts * 2;
   {
-    const int part0 = blockIdx.x * V;
-    u32x4 v[V];
-    float d[V][8] = {};
-    if (some) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) request8((part0 + i) * 2048 + t * 8, v[i], d[i]);
-    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       double rest = 0.0, all = 0.0;
@@ -1463,9 +1482,10 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   }
   if (!last_here(A.count + (kSeqsMax + s) * kCountStep, gridDim.x, &arrived)) return;
   // The last workgroup of the sequence takes the token.
+  double log_total = 0.0;
   auto give = [&](int token, float of) {
     out[n] = token;
-    if (logprob) logprob[n] = token < 0 ? 0.0f : log_of(of, pick.row.top, pick.row.sum, pick.heat);
+    if (logprob) logprob[n] = token < 0 ? 0.0f : log_of(of, pick.row.top, log_total, pick.heat);
   };
   if (!some) {
     if (t == 0) give(-1, 0.0f);
@@ -1478,6 +1498,8 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   };
   double here[2], before[2], total[2], all[2];
   request(0, here);
+  log_total = log(pick.row.sum);
+  asm volatile("" : "+v"(log_total));  // while the sums are on their way
   running(here, before, total);
   for (int c0 = 256; c0 < A.parts; c0 += 256) {
     request(c0, here);
@@ -1532,25 +1554,26 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   // 8 entries in a row a thread, then the one thread's, one entry a lane
   const int j0 = part * 2048 + t * 8;
   double mine[2] = {0.0, 0.0}, run[2];
-  {
-    u32x4 v;
-    float d[8] = {};
-    request8(j0, v, d);
-    sum8(j0, v, d, mine[0], mine[1]);
-  }
+  request8(j0, v[0], d[0]);
+  sum8(j0, v[0], d[0], mine[0], mine[1]);
   running(mine, run, all);
   const double from = base + run[k];
   const int place = look(mine[k], from);
-  if (t == place) base = from;
+  if (t == place) {
+    base = from;
+    *reinterpret_cast<u32x4*>(few) = v[0];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) few_q[e] = d[0][e];
+  }
   __syncthreads();
   if (wave > 0) return;
   const int j = part * 2048 + place * 8 + lane;
   double f[2] = {0.0, 0.0};
-  float v = 0.0f;
+  float of = 0.0f;
   if (place >= 0 && lane < 8 && j < A.vocab) {
-    v = (float)as_half(x[j]);
-    f[1] = w.p(j, w.weight.near(v));
-    f[0] = w.rest(j, f[1], q ? q[j] : 0.0f);
+    of = (float)as_half(few[lane]);
+    f[1] = w.p(j, w.weight.near(of));
+    f[0] = w.rest(j, f[1], few_q[lane]);
   }
   const double c = base + wave_scan64(f[k]);  // (every lane takes part)
   const uint64_t b = __builtin_amdgcn_ballot_w64(f[k] > 0.0);
@@ -1558,7 +1581,7 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   if (b == 0) {
     if (lane == 0) give(-1, 0.0f);
   } else if (lane == (a ? __builtin_ctzll(a) : 63 - __builtin_clzll(b))) {
-    give(j, v);
+    give(j, of);
   }
 }
 
