@@ -102,7 +102,7 @@ typedef struct kv_rows {
  * nearest, ties to even, at most 127 in magnitude; all zeros: scale and codes 0; a
  * row with an infinity or NaN: scale NaN, so that it reads as NaN.
  * k is computed in 64 bits up to its rounding (a sum in another order must
- * not move a value over a code's border), f16 values rounded to f32 first.
+ * not move a value over a code's border), f16 values rounded to f32 first; q in 32.
  * The table may name a page twice only where no slot is written through both. */
 int kv_pages_append(const kv_pages* pages, int32_t layer, const kv_batch* batch,
                     const kv_rows* rows, void* stream);

@@ -73,12 +73,13 @@ __device__ __forceinline__ float half_at(u32x4 v, int j) {
 // One workgroup a row; D / 8 lanes a head, 8 values each, the row's q, k and v heads
 // side by side (and in turn where there are more than the threads hold).  The rotation's
 // partners, dims i and i + D/2, are lanes half a head apart.  The angles' cosines and sines are
-// worked out once a row, by one wave while the others norm their heads.  In f64: the
-// rounding to codes must not depend on an order of sums.
+// worked out once a row, by one wave while the others norm their heads.  k and v in f64: the
+// rounding to codes must not depend on an order of sums; q, which only rounds to f16, in
+// f32 (8997 rows 45.5 -> 40.9 us).
 // Few rows are bound by latency (the starts, the page's entry, the angles, the store: 1 row
-// 3.3 us, 256 rows 5.3 us of 32 heads), many by the f64 operations: 8997 rows with 8-bit
-// pages 45.5 us, where their 129 MB would take 25.  A wave a row and heads in f32 were slower
-// or moved codes.
+// 2.9 us, 256 rows 4.9 us of 32 heads), many by the f64 operations: 8997 rows with 8-bit
+// pages 40.9 us, where their 129 MB would take 25 and the operations take 26.  A wave a row was
+// slower, and so were 64 registers for an eighth wave a SIMD, which spill (44.6 us).
 namespace {
 
 template <int kCtrl>
@@ -141,6 +142,42 @@ __device__ __forceinline__ void turn_head(double (&y)[8], int c, const double2* 
   }
 }
 
+// The queries' norm and rotation, which no code depends on, in f32: off by at most 2^-20 of
+// |y[i]| + |y[i + D/2]| before the rounding to f16.
+template <int D>
+__device__ __forceinline__ void norm_head(float (&y)[8], u32x4 wv, float eps) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
+  ss += dpp<0xb1>(ss);
+  ss += dpp<0x4e>(ss);
+  ss += dpp<0x141>(ss);
+  if constexpr (D == 128) ss += dpp<0x140>(ss);
+  const float r = __builtin_amdgcn_rsqf(ss * (1.0f / D) + eps);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = y[j] * r * half_at(wv, j);
+}
+template <int D>
+__device__ __forceinline__ void turn_head(float (&y)[8], int c, const float2* turn) {
+  const bool second = c >= D / 16;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 a = turn[turn_at<D>((8 * c) % (D / 2) + j)];
+    float o;
+    if constexpr (D == 128)
+      o = dpp<0x128>(y[j]);
+    else
+      o = __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(y[j]), 0x101f));
+    y[j] = fmaf(o, second ? a.y : -a.y, y[j] * a.x);
+  }
+}
+
+__device__ __forceinline__ u32x4 packed8(const float (&y)[8]) {
+  u32x4 o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = pack_f16x2(y[2 * j], y[2 * j + 1]);
+  return o;
+}
 __device__ __forceinline__ u32x4 packed8(const double (&y)[8]) {
   u32x4 o;
 #pragma unroll
@@ -192,6 +229,7 @@ template <int D, bool Q8, int kThreads>
 __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
   constexpr int G = D / 8, kHeads = kThreads / G;
   __shared__ double2 turn[D / 2];
+  __shared__ float2 turn_f[D / 2];
   const int t = threadIdx.x, c = t % G, row = blockIdx.x;
   const int heads = A.q_heads + 2 * A.kv_heads;
   auto request = [&](int h) {
@@ -215,31 +253,41 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
   const int64_t slot = (int64_t)length - m + (row - lo);
   const int64_t to = pool_row(A.b, s, slot, A.kv_heads, 0);  // of head 0
   double y[8];
-  auto normed = [&](int h, u32x4 x) {  // into y
-    const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
+  auto normed = [&](u32x4 x) {  // a k or v into y
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = (double)half_at(x, j);
-    if (!is_v && (is_q ? A.q_norm : A.k_norm)) norm_head<D>(y, is_q ? qw : kw, A.eps);
+    if (h < A.q_heads + A.kv_heads && A.k_norm) norm_head<D>(y, kw, A.eps);
   };
   if (A.rotate && t < D / 2) {
     const double by = (double)(A.positions ? (int64_t)position : slot) * step;
     double2 a;
     sincospi(2.0 * (by - rint(by)), &a.y, &a.x);
     turn[turn_at<D>(t)] = a;
+    turn_f[turn_at<D>(t)] = make_float2((float)a.x, (float)a.y);
   }
-  if (h < heads) normed(h, x);  // while the angles' waves are busy
+  if (h >= A.q_heads && h < heads) normed(x);  // while the angles' wave is busy
   if (A.rotate) __syncthreads();
-  while (h < heads) {
+  // (an eps that f32 does not hold: a head of zeros stays one)
+  const float eps = A.eps > 0.0 ? fmaxf((float)A.eps, 1.2e-38f) : 0.0f;
+  bool more = false;
+  for (; h < A.q_heads; h += kHeads, more = true) {
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = half_at(x, j);
+    if (h + kHeads < heads) x = request(h + kHeads);
+    if (A.q_norm) norm_head<D>(q, qw, eps);
+    if (A.rotate) turn_head<D>(q, c, turn_f);
+    *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + h * D + 8 * c) = packed8(q);
+  }
+  for (; h < heads; h += kHeads, more = true) {
+    if (more) normed(x);
     const u32x4 here = x;
-    const int next = h + kHeads;
-    if (next < heads) x = request(next);
-    const bool is_q = h < A.q_heads, is_v = h >= A.q_heads + A.kv_heads;
+    if (h + kHeads < heads) x = request(h + kHeads);
+    const bool is_v = h >= A.q_heads + A.kv_heads;
     const int64_t at = to + (int64_t)(h - A.q_heads - (is_v ? A.kv_heads : 0)) * A.b.page_size;
     void* pool = is_v ? A.v_to : A.k_to;
     if (!is_v && A.rotate) turn_head<D>(y, c, turn);
-    if (is_q) {
-      *reinterpret_cast<u32x4*>(A.q_out + row * A.q_out_stride + h * D + 8 * c) = packed8(y);
-    } else if constexpr (Q8) {
+    if constexpr (Q8) {
       float scale;
       const uint2 code = codes8<D>(y, scale);
       if (to >= 0) {
@@ -250,15 +298,13 @@ __device__ __forceinline__ void pages_append(const PagesAppendArgs& A) {
       *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(pool) + at * D + 8 * c) =
           is_v ? here : packed8(y);
     }
-    h = next;
-    if (h < heads) normed(h, x);
   }
 }
 
 }  // namespace
 
 #define PAGES_APPEND(D, N, Q8)                                                                    \
-  extern "C" __global__ __launch_bounds__(256) void pages_append_##D##_##N(PagesAppendArgs A) {   \
+  extern "C" __global__ __launch_bounds__(256) void pages_append_##D##_##N(PagesAppendArgs A) {    \
     pages_append<D, Q8, 256>(A);                                                                  \
   }                                                                                               \
   extern "C" __global__ __launch_bounds__(512) void pages_append_wide_##D##_##N(PagesAppendArgs A) { \

@@ -380,7 +380,11 @@ def append_case(Q, P, seed, heads, bits, page, lengths, counts=None, norm=True, 
             q = np.where(fine, q, 0)
             g = got_q[r].astype(np.float64)
             assert np.array_equal(np.isfinite(g), fine)
-            assert (np.abs(g - q)[fine] <= (2.0 ** -11 + 2.0 ** -23) * np.abs(q[fine]) + 2.0 ** -25).all()
+            # in f32, 2^-24 each: half of the squares' 12 sums and of eps' one, 2 for the root,
+            # 2 products; cosine, product and sum: under 16 of the two values that are turned
+            y = np.abs(np.nan_to_num(R.turned(heads_of[:qh], qn if norm else None, 1e-6, 0.0, p)))
+            turned = y + np.roll(y, d // 2, -1)
+            assert (np.abs(g - q) <= 2.0 ** -11 * np.abs(q) + 2.0 ** -20 * turned + 2.0 ** -25)[fine].all()
         if at is None:
             continue
         written[at] = True
