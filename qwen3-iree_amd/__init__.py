@@ -9,6 +9,8 @@ Modules
            trees, attention weights, eviction.
   pages    a paged KV cache of several sequences, f16 or 8-bit, and the verification of
            drafted tokens (include/kv_pages.h).
+  drafts   drafted trees through the whole model over one cache.
+  serving  several sequences through the whole model over a paged cache.
   gguf     GGUF v2/v3 reader / writer and Qwen3-0.6B checkpoint ingestion into
            the device layout (no IREE).
   weights  Q8_0 quantisation / stacking (the reference's offline weight prep)
