@@ -256,3 +256,71 @@ def test_two_sessions_on_two_streams(S, model, gpu):
     for x, want in zip(sess, alone):
         assert np.array_equal(x.read_logits(9), want)
         x.free()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_padding_rows_and_used_workspaces(S, model, gpu, bits):
+    """A step of 12 rows of which the sequences have 7: tokens outside the vocabulary in the
+    rows behind them, NaN left behind the workspace's counters, and no other row, page or
+    scale changes."""
+    from qwen3_iree_amd import pages as P
+
+    rng = np.random.default_rng(21)
+    x = S.PagedSession(model, pages=20, max_seqs=3, max_len=96, page_size=16, bits=bits)
+    seqs = [x.add() for _ in range(3)]
+    for s in seqs:
+        x.prompt(s, rng.integers(0, VOCAB, 20 + 11 * s))
+    x.step({s: rng.integers(0, VOCAB, 1 + 2 * (s % 2) + s // 2) for s in seqs}, logits=True)
+    counts = [1, 3, 2]
+    batch = x._batch(seqs, counts, [x.length[s] for s in seqs])
+    tokens = np.concatenate([x._words.download(np.int32, 6, x._tokens), [-5, 1 << 30, 7, 0, -1, 9]])
+    tb, nb = gpu.DeviceBuffer.from_array(tokens.astype(np.int32)), gpu.DeviceBuffer(4 * 12)
+    logits = gpu.DeviceBuffer(12 * VOCAB * 2)
+    n = int(gpu.load_library().qwen3_pages_workspace_bytes(12, 12))
+    counters = 1 << 16
+    ws = gpu.DeviceBuffer(n)
+
+    def pool():
+        return [b.download(np.uint8) for b in (*x._pool, *x._scales) if b is not None]
+
+    results, before = [], pool()
+    for behind in (0, 0xFF, 0x7E):
+        ws.fill(behind)
+        ws.upload(np.zeros(counters, np.uint8))
+        wide = P.Batch(batch.table, batch.length, 3, x.max_pages, 12, 12, start=batch.start)
+        gpu._call("qwen3_pages_step", model.ref(), ctypes.byref(x.pages), ctypes.byref(wide), tb.ptr, nb.ptr,
+                  logits.ptr, ws.ptr, n, None)
+        gpu.synchronize()
+        results.append((logits.download(np.uint16, 6 * VOCAB), nb.download(np.int32, 6)))
+        assert (ws.download(np.uint8, counters) == 0).all()
+    for r in results[1:]:
+        assert np.array_equal(r[0], results[0][0]) and np.array_equal(r[1], results[0][1])
+    # the same rows as before were written again, with the same values
+    for a, b in zip(before, pool()):
+        assert np.array_equal(a, b)
+    assert np.array_equal(results[0][0].view(np.float16).reshape(6, VOCAB).view(np.uint16),
+                          x.read_logits(6).view(np.uint16))
+    x.free()
+
+
+def test_sessions_of_all_sizes_share_a_workspace(S, model, gpu):
+    """One workspace of the largest step for steps of few and many rows, one and many a
+    sequence, in turn: what a fresh one gives."""
+    rng = np.random.default_rng(22)
+    x = S.PagedSession(model, pages=60, max_seqs=8, max_len=256, page_size=32, bits=8)
+    fresh = []
+    shapes = [[1], [128], [1] * 8, [16] * 8, [40, 1, 60], [7, 9], [65]]
+    for turn in range(2):
+        for i, counts in enumerate(shapes):
+            seqs = [x.add() for _ in counts]
+            r = np.random.default_rng(100 + i)
+            x.step({s: r.integers(0, VOCAB, m) for s, m in zip(seqs, counts)}, logits=True)
+            got = x.read_logits(sum(counts)).view(np.uint16).copy()
+            for s in seqs:
+                x.remove(s)
+            if turn == 0:
+                x._ws.fill(0)
+                fresh.append(got)
+            else:
+                assert np.array_equal(got, fresh[i])
+    x.free()
