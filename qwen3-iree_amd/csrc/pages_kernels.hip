@@ -77,7 +77,7 @@ __device__ __forceinline__ float half_at(u32x4 v, int j) {
 // rounding to codes must not depend on an order of sums; q, which only rounds to f16, in
 // f32 (8997 rows 45.5 -> 40.9 us).
 // Few rows are bound by latency (the starts, the page's entry, the angles, the store: 1 row
-// 2.9 us, 256 rows 4.9 us of 32 heads), many by the f64 operations: 8997 rows with 8-bit
+// 2.9 us, 171 rows 4.9 us of 32 heads), many by the f64 operations: 8997 rows with 8-bit
 // pages 40.9 us, where their 129 MB would take 25 and the operations take 26.  A wave a row was
 // slower, and so were 64 registers for an eighth wave a SIMD, which spill (44.6 us).
 namespace {
@@ -333,8 +333,8 @@ PAGES_APPEND(128, q8, true)
 // A block's registers are requested again for the wave's next block as soon as they have
 // been used (a second set of them spilled), two waves a SIMD cover the rest.  Bound by
 // memory where sequences are long: 4 x 131072 slots of 8 kv heads in 8 bits, 1.1 GB, 193 us, 5.7 TB/s
-// (a copy 5.1); 16 x 8000 slots in f16, five rows each, 35 us, 4.0 TB/s, of which cut
-// sequences and ramps take 8; 1 x 300 slots 8 us, all latency.
+// (a copy 5.1); 16 sequences of 44000 slots in f16, 45 rows, 140 MB, 35 us, 4.0 TB/s, of which
+// cut sequences and ramps take 8; 1 x 300 slots 8 us, all latency.
 // A weight goes into the product as the sum of two f16 values (2^-22 of itself).
 // 8-bit codes become f16 multiples of 2^-9, exact; a row's k scale multiplies its
 // score and its v scale its weight, so that the reference is that of s + log2 v_scale.

@@ -191,7 +191,7 @@ constexpr size_t kVerifyCounts = 2 * kSeqsMax * kCountStep * sizeof(int32_t);
 
 // Logits of a workgroup: 8192, or 2048 where that leaves CUs without a workgroup.  Of
 // 151936 logits, by 2048 and 8192: both launches of 1 row 12.1 and 15.8 us, the first of 185 rows
-// 45.2 and 29.6, of 42 rows 16.4 and 11.0, the second of 7 sequences 9.2 and 10.7, of 64
+// 45.2 and 29.6, of 27 rows 16.4 and 11.0, the second of 7 sequences 9.2 and 10.7, of 64
 // 25.3 and 23.0.
 int verify_chunk(int32_t rows, int32_t vocab) {
   return (int64_t)rows * ((vocab + 8191) / 8192) >= q8_shim::compute_units() ? 8192 : 2048;
