@@ -119,8 +119,9 @@ int kv_pages_append(const kv_pages* pages, int32_t layer, const kv_batch* batch,
  * write).  q_heads a multiple of kv_heads, at most 32 times it and at most 256; scale
  * positive and below 2^118; max_rows at most 256.  Scores, statistics and sums are
  * f32; a weight enters its product with v to 2^-22 of itself.
- * workspace: device memory of kv_pages_attn_workspace_bytes (256-byte aligned),
- * needed only during the call; fill it with zeros once before its first use.
+ * workspace: device memory of kv_pages_attn_workspace_bytes (256-byte aligned);
+ * fill it with zeros once before its first use.  Its first 64 KiB are counters, zeros again
+ * behind every call, that nothing else may write; the rest is needed only during the call.
  * The size depends on the heads and on max_rows alone, and that of the largest
  * max_rows of a session serves all its calls.  Calls that may overlap (streams,
  * graphs) need one each. */
@@ -168,8 +169,9 @@ int kv_pages_read(const kv_pages* pages, int32_t layer, int32_t layers, const kv
  * rounding is computed in 64 bits and fixed order.
  * rows in [1, 65535], seqs in [1, 1024], max_rows in [1, 256], out_stride >=
  * max_rows, vocab in [1, 2^24]; strides >= vocab; logits 2-byte, the others
- * 4-byte aligned.  workspace: kv_verify_workspace_bytes (256-byte aligned), needed
- * only during the call; fill it with zeros once before its first use.  That of the
+ * 4-byte aligned.  workspace: kv_verify_workspace_bytes (256-byte aligned); fill it
+ * with zeros once before its first use.  Its first 256 KiB are counters, zeros again behind every
+ * call, that nothing else may write; the rest is needed only during the call.  That of the
  * largest rows, seqs and vocab of a session serves all its calls; calls that may
  * overlap need one each. */
 typedef struct kv_drafts {

@@ -310,7 +310,8 @@ int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_
  * tolerance, 8-bit pages add their rounding.  Only enqueues; rows at most 128.
  * workspace: device memory of qwen3_pages_workspace_bytes(rows, max_rows) bytes (0 for
  * arguments outside the ranges), 256-byte aligned, filled with zeros once before its
- * first use; that of the largest rows and max_rows serves smaller steps too.  Steps that
+ * first use (its first 64 KiB stay zeros between steps, nothing else may write them); that of
+ * the largest rows and max_rows serves smaller steps too.  Steps that
  * may overlap need one each.  No counterpart in the reference, which runs one
  * sequence. */
 struct kv_pages;
