@@ -123,8 +123,8 @@ OBJECT_SOURCES = {
                 "step_roles.h", "q8_device.h"),
     "cache": ("cache_kernels.hip", "cache_args.h", "decode_device.h", "step_roles.h",
               "q8_device.h"),
-    "pages": ("pages_kernels.hip", "pages_args.h", "decode_device.h", "step_roles.h",
-              "q8_device.h"),
+    "pages": ("pages_kernels.hip", "pages_args.h", "verify_exp.h", "decode_device.h",
+              "step_roles.h", "q8_device.h"),
 }
 
 

@@ -2,6 +2,7 @@
 // it, rows read back, and the verification of drafted tokens.
 #include "decode_device.h"
 #include "pages_args.h"
+#include "verify_exp.h"
 
 #include <type_traits>
 
@@ -1066,41 +1067,10 @@ __device__ __forceinline__ void fill_table(double* table) {
   table[t] = kExp2[t >> 4] * kFine2[t & 15];
 }
 
-// exp((x - top) / T), 0 below 2^-1000 and for a NaN, with unit = 256 log2(e) / T: 2^(1/256)
-// to the power x unit - C, C = rint(top unit), times norm, which makes up for C.  y = x unit +
-// (1.5 2^52 - C) holds the nearest integer's n = rint(x unit) - C in its low bits, y less
-// that constant is rint(x unit), both exact, so that the rest has the rounding of one fma; n goes
-// into the exponent by an addition (f64 roundings, conversions and ldexp have a fraction
-// of the rate).  x becomes an f64 by a shift, 2^896 too small, which the unit makes up
-// for.  Where top is +inf, which alone has weight then, values go through near() first.
-struct Exp {
-  const double* table;
-  double unit, base, norm;
-  double c1, c2, c3;
-  float least;  // x of 2^-1000, or less
-  bool far;
-  // unit: unit_of(T)
-  __device__ __forceinline__ Exp(const double* table, float top_of, double unit_of_heat)
-      : table(table), far(top_of == __builtin_inff()) {
-    const float at = far ? 0.0f : top_of;
-    // An f16 below `top` is further from it than |top| 2^-12 and 2^-24: a larger unit only
-    // takes 2^-1000 to something smaller.
-    unit = fmin(far ? 1.0 : unit_of_heat,
-                (double)(255000.0f * __builtin_amdgcn_rcpf(fmaxf(fabsf(at) * 0x1p-12f, 0x1p-24f))));
-    // (of 11 bits as the others are)
-    least = __uint_as_float(__float_as_uint(at - 255000.0f * __builtin_amdgcn_rcpf((float)unit)) & ~0x1fffu);
-    c1 = 0x1.62e42fefa39efp-9;
-    c2 = 0x1.ebfbdff82c58fp-19;
-    c3 = 0x1.c6b08d704a0c0p-29;
-    asm("" : "+s"(c1), "+s"(c2), "+s"(c3));
-    const double magic = 6755399441055744.0, z = (double)at * unit, c = (z + magic) - magic;
-    base = magic - c;
-    norm = poly(-fma((double)at, unit, -c));
-    unit *= 0x1p896;
-  }
-  __device__ __forceinline__ double poly(double r) const {
-    return fma(fma(fma(c3, r, c2), r, c1), r, 1.0);
-  }
+// VerifyExp of values that may be infinite, over the table in LDS.  Where top is +inf, which
+// alone has weight then, values go through near() first.
+struct Exp : VerifyExp {
+  using VerifyExp::VerifyExp;
   __device__ __forceinline__ float near(float x) const {
     return !far ? x : x == __builtin_inff() ? 0.0f : -__builtin_inff();
   }
@@ -1113,30 +1083,7 @@ struct Exp {
     }
     return v;
   }
-  // The same without norm and with 2^-1000, about, in the place of 0: a product, of which
-  // `to` is the second factor.  x: an f16's value.
-  __device__ __forceinline__ double some(float x, double& to) const {
-    const uint32_t bits = (uint32_t)((int32_t)__float_as_uint(fmaxf(x, least)) >> 3) & 0x8fffffffu;
-    const double v = __builtin_bit_cast(double, (uint64_t)bits << 32);
-    const double y = fma(v, unit, base);
-    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, y);
-    const uint64_t b = __builtin_bit_cast(uint64_t, table[n & 255]);
-    uint32_t hi = (uint32_t)(b >> 32) + ((n & ~255u) << 12);
-    asm("" : "+v"(hi));  // (or the compiler adds in 64 bits)
-    to = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b);
-    return poly(fma(v, unit, -(y - base)));
-  }
-  __device__ __forceinline__ double raw(float x) const {  // without norm
-    double to;
-    const double w = some(x, to) * to;
-    return x > least ? w : 0.0;
-  }
-  __device__ __forceinline__ double operator()(float x) const { return raw(x) * norm; }
 };
-// 256 log2(e) / T; 0 where the maximum takes all
-__device__ __forceinline__ double unit_of(float heat) {
-  return heat > 0.0f ? fmax(369.3299304675746 / (double)heat, 1e-30) : 1.0;
-}
 
 // The sum over the wave, in every lane: 16 lanes by DPP, then the four rows.
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -1330,7 +1277,7 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
   const int s = seq_of_row(A.b, row, lo, m, A.temperature, heat);
   if (s < 0) return;
   if (!A.temperature) heat = 1.0f;
-  const double unit = unit_of(heat);
+  const double unit = verify_unit(heat);
   float top = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < V; ++i) top = fmaxf(top, top8(v[i]));
@@ -1471,7 +1418,7 @@ __device__ __forceinline__ void verify_rest(const VerifyArgs& A) {
   for (int i = 0; i < V; ++i) request8((part0 + i) * 2048 + t * 8, v[i], d[i]);
   __syncthreads();  // the table
   if (single) {
-    pick.unit = unit_of(pick.heat);
+    pick.unit = verify_unit(pick.heat);
     pick.row = join_row(A, lo, lane, pick.unit, pick.heat, table);
     if (blockIdx.x == 0 && t == 0) A.accepted[s] = 0;
   }
