@@ -79,7 +79,8 @@ int main() {
   for (int n = 0; n < 256; ++n) table[n] = std::exp2(n / 256.0);
   std::vector<float> heats;
   for (double t = 1e-6; t <= 2e4; t *= 1.37) heats.push_back((float)t);
-  for (double t : {1e-45, 1e-38, 1e-30, 1e-20, 1e-12, 1e6, 1e12, 1e20}) heats.push_back((float)t);
+  for (double t : {1e-45, 1e-38, 1e-30, 1e-20, 1e-12, 1e6, 1e12, 1e20, 1e25, 1e30, 1e35, 1e36, 3.4e38,
+                   (double)INFINITY}) heats.push_back((float)t);
   for (rcp_ulps = -1; rcp_ulps <= 1; ++rcp_ulps)
     for (float heat : heats)
       for (int sign = 0; sign < 2; ++sign)

@@ -42,3 +42,12 @@ def test_verify_temperatures(gpu, P, heat, drafted):
         T.verify_case(gpu, P, 50, 9001, [5] * 26, drafted=drafted, heat="warm", spoil=shifted(heat, top, True))
         T.verify_case(gpu, P, 51, 9001, None, rows=9, drafted=drafted, heat="warm",
                       spoil=shifted(heat, top, True))
+
+
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("heat", [1e25, 1e36, 3e38, np.inf])
+def test_verify_hottest_rows(gpu, P, heat, drafted):
+    """All finite logits alike, and -inf and NaN among them without any probability."""
+    for i, top in enumerate((-1000.0, 0.0, 40.0)):
+        T.verify_case(gpu, P, 60 + i, 9001, [3, 2, 1, 5], drafted=drafted, heat="warm",
+                      spoil=shifted(heat, top, heat < np.inf))

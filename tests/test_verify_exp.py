@@ -1,5 +1,5 @@
 """Builds and runs tests/native/verify_exp_check.cpp: the exp of the drafts' verification
-on the host, over temperatures from 1e-45 on and row maxima of every size and sign."""
+on the host, over temperatures from 1e-45 to infinity and row maxima of every size and sign."""
 from __future__ import annotations
 
 import subprocess
