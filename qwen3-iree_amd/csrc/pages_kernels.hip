@@ -346,6 +346,10 @@ namespace {
 constexpr float kRefRoom = 6.0f, kRefMax = 10.0f, kSumMax = 16384.0f;
 constexpr float kCodeUnit = 512.0f;    // codes stand in the products as code / 512
 constexpr float kLeastLogScale = -64.0f;  // values below 2^-57 leave no trace in an f16
+// A weight whose v scale is next to nothing adds to the sum of weights alone, which would
+// pass what an f32 holds: the reference moves for these too, which then are 2^74 at most
+// (kRefMax - kLeastLogScale), 2^98 the sum of 2^24.
+constexpr float kPlainMax = 0x1p64f;
 
 // 0x00b200b1 for two bytes, as f16 numbers u 2^-24, times 2^15 less 128 2^-9
 __device__ __forceinline__ f16x2 code_pair(uint32_t bytes) {
@@ -564,17 +568,19 @@ struct AttnWave {
           }
       }
       // p: weights; pv: times the v scales, what goes into the product
-      float p[8], pv[8];
+      float p[8], pv[8], plain = 0.0f;
       auto weigh = [&](float ref) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           p[e] = __builtin_amdgcn_exp2f(sv[e] - ref);
           pv[e] = Q8 ? p[e] * vs[e] : p[e];
         }
+        if constexpr (Q8)
+          plain = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         return ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
       };
       float sum = weigh(m[j]);
-      if (__builtin_amdgcn_ballot_w64(!(sum <= kSumMax)) != 0) {
+      if (__builtin_amdgcn_ballot_w64(!(sum <= kSumMax) || !(plain <= kPlainMax)) != 0) {
         float mx = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -590,10 +596,7 @@ struct AttnWave {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) o[j][d] *= alpha;
       }
-      if constexpr (Q8)
-        l[j] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-      else
-        l[j] += sum;
+      l[j] += Q8 ? plain : sum;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         typedef float f32x2_t __attribute__((ext_vector_type(2)));

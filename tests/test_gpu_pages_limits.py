@@ -51,3 +51,50 @@ def test_verify_hottest_rows(gpu, P, heat, drafted):
     for i, top in enumerate((-1000.0, 0.0, 40.0)):
         T.verify_case(gpu, P, 60 + i, 9001, [3, 2, 1, 5], drafted=drafted, heat="warm",
                       spoil=shifted(heat, top, heat < np.inf))
+
+
+def far_case(Q, P, heads, counts, gap, scale_far, other):
+    """8-bit pages whose slots have scores 0 but for some whose v is nothing (codes or scale 0,
+    or a scale of 2^-120) `gap` above in units of log 2, and, with other, a few ordinary ones as
+    far up, in the same blocks of 32 slots and in others."""
+    rng = np.random.default_rng(70)
+    qh, kvh, d = heads
+    lengths = [900, 70, 3000]
+    need = sum((n + 15) // 16 for n in lengths) + 1
+    pool = T.Pool(Q, P, rng, 1, need, 16, kvh, d, 8)
+    batch = T.Batch(Q, P, rng, pool, lengths, counts)
+    (k, v), (ks, vs) = pool.host, pool.scales
+    q = T.normal(rng, (batch.rows, qh, d))
+    q[..., 0] = 1
+    k[..., 0] = 0  # scores within about 1 of 0, by the other dims; dim 0 says how far up
+    ks[:] *= np.float32(0.1)
+    for s, n in enumerate(lengths):
+        for j in range(n):
+            page, entry = T.R.place(batch.table, s, j, need, 16)
+            up = 130 <= j < 155 or 400 <= j < 640 or j == 20
+            if not (up or (other and j in (35, 68, 140, 500, 700, 2900))):
+                continue
+            k[0, page, :, entry] = 0
+            k[0, page, :, entry, 0] = 127
+            ks[0, page, :, entry] = np.float32(gap * np.log(2.0) / 127 / 0.125)
+            if up and j != 140:
+                if scale_far is None:
+                    v[0, page, :, entry] = 0
+                    vs[0, page, :, entry] = 0
+                else:
+                    vs[0, page, :, entry] = scale_far
+    pool.upload(P)
+    got = T.run_attn(Q, P, pool, batch, q, 0.125)
+    T.check_attn(*got, T.R.attention(q, pool.layer(0), batch.table, batch.length, batch.start,
+                                     batch.max_rows, 0.125))
+
+
+@pytest.mark.parametrize("heads", [(2, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("gap", [50, 65, 75, 100, 108, 112, 115, 118, 121, 124, 126, 128, 131, 140, 300])
+def test_attn_weights_far_above_that_add_nothing(gpu, P, heads, gap):
+    """The sum of the weights stays finite where slots of no v have scores far above the
+    others': one row a sequence, and the tiles of 20 and 40 rows of a kv head."""
+    for counts in (None, [10, 1, 2], [1, 1, 20]):
+        for scale_far in (None, np.float32(2.0 ** -120)):
+            for other in (False, True):
+                far_case(gpu, P, heads, counts, gap, scale_far, other)
