@@ -13,6 +13,7 @@ import ctypes
 import numpy as np
 
 from . import decode as D
+from . import drafts
 from . import pages as P
 from . import q8gemv as Q
 
@@ -213,7 +214,10 @@ class PagedSession:
 
     def to_session(self, seq: int, session: D.DecodeSession) -> None:
         """Reads a sequence's slots into a DecodeSession's cache and puts its position behind
-        them (its token word stays)."""
+        them (its token word stays).  A session of drafted trees, which counts its own slots, is
+        refused."""
+        if isinstance(session, drafts.DraftSession):
+            raise TypeError("a session of drafted trees takes no sequence over")
         n = self.length[seq]
         if not 1 <= n < session.max_seq:
             raise ValueError(f"{n} slots into a cache of {session.max_seq}")
