@@ -53,6 +53,17 @@ def test_verify_hottest_rows(gpu, P, heat, drafted):
                       spoil=shifted(heat, top, heat < np.inf))
 
 
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("vocab", [524288, 524289, 1100003])
+def test_verify_large_vocabularies(gpu, P, vocab, drafted):
+    """More parts of a row than a workgroup has threads, the token in the first of them, in the
+    last and between."""
+    for i, uniform in enumerate((None, 0.0, 1.0 - 2.0 ** -24)):
+        T.verify_case(gpu, P, 80 + i, vocab, [2, 1, 3], drafted=drafted, uniform=uniform, heat="warm",
+                      spoil=shifted(10.0, 5.0, False))
+        T.verify_case(gpu, P, 90 + i, vocab, None, rows=2, drafted=drafted, uniform=uniform)
+
+
 def far_case(Q, P, heads, counts, gap, scale_far, other):
     """8-bit pages whose slots have scores 0 but for some whose v is nothing (codes or scale 0,
     or a scale of 2^-120) `gap` above in units of log 2, and, with other, a few ordinary ones as
