@@ -1042,10 +1042,11 @@ PAGES_READ(128, q8, true)
 // row, the sums of max(p - q, 0) and of p; the last workgroup of a sequence finds the part
 // and the index whose running sum passes the random number.  All in f64: next to a
 // border of the running sums, one in 151936, f32 sums would give other tokens.  exp is
-// 2^(n / 256) from a table in LDS times a polynomial of degree 3 in the rest, |rest| <= ln 2 /
-// 512: 1.4e-13 of it is left out, for a fourth of the instructions of a full f64 exp.
-// Bound by the f64 operations beside the memory: 185 rows of 151936 logits (56 MB) 30 us, of
-// which 16 are VALU; the deciding rows of 64 sequences with the drafter's (58 MB) 23 us; one
+// 2^(n / 256) from a table in LDS times a polynomial of degree 4 in the rest, |rest| <= ln 2 /
+// 512: 4e-17 of it is left out, for a fourth of the instructions of a full f64 exp (degree 3
+// leaves out 1.4e-13 and took 0.8 us less of 49.6 for 185 rows).
+// Bound by the f64 operations beside the memory: 185 rows of 151936 logits (56 MB) 31 us, of
+// which 17 are VALU; the deciding rows of 64 sequences with the drafter's (58 MB) 23 us; one
 // row 3 and 10 us, the last being a chain of loads and joins in one workgroup.  A wave that
 // keeps its own chunk, without the workgroup's joins, was no faster (30 us).
 namespace {
@@ -1303,7 +1304,7 @@ __device__ __forceinline__ void verify_sums(const VerifyArgs& A) {
     }
   } else if (top > -__builtin_inff()) {
     const Exp weight(table, top, unit);
-    // (read again, from the L1: 8 at a time in one code, or registers cost occupancy)
+    // (read again, from the caches: 8 at a time in one code, or registers cost occupancy)
 #pragma unroll 1
     for (int i = 0; i < V; ++i) {
       const u32x4 x8 = weight.near(logits8(x + (i * 256 + t) * 8, A.vocab - begin - (i * 256 + t) * 8));

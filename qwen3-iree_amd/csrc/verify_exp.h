@@ -31,7 +31,7 @@ VERIFY_FN float verify_rcp(float v) {
 struct VerifyExp {
   const double* table;
   double unit, base, norm;
-  double c1, c2, c3;
+  double c1, c2, c3, c4;
   float least;  // x of 2^-996, about
   bool far;
   // unit_of_heat: verify_unit(T)
@@ -50,8 +50,9 @@ struct VerifyExp {
     c1 = 0x1.62e42fefa39efp-9;
     c2 = 0x1.ebfbdff82c58fp-19;
     c3 = 0x1.c6b08d704a0c0p-29;
+    c4 = 0x1.3b2ab6fba4e77p-39;
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm("" : "+s"(c1), "+s"(c2), "+s"(c3));
+    asm("" : "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4));
 #endif
     const double magic = 6755399441055744.0, z = (double)at * unit, c = (z + magic) - magic;
     base = magic - c;
@@ -59,7 +60,8 @@ struct VerifyExp {
     unit *= 0x1p896;
   }
   VERIFY_FN double poly(double r) const {
-    return __builtin_fma(__builtin_fma(__builtin_fma(c3, r, c2), r, c1), r, 1.0);
+    return __builtin_fma(
+        __builtin_fma(__builtin_fma(__builtin_fma(c4, r, c3), r, c2), r, c1), r, 1.0);
   }
   // The same without norm and with 2^-996, about, in the place of 0: a product, of which
   // `to` is the second factor.  x: an f16's value.

@@ -39,9 +39,9 @@ static void wrong(const char* what, float top, float heat, float x, double got, 
     std::printf("%s: top %.9g T %.9g x %.9g: %.17g, exact %.17g\n", what, top, heat, x, got, want);
 }
 
-// The cubic leaves out 1.4e-13 in a weight and in norm; T's unit and (x - top) / T, of 700 at
-// most, have a rounding each, 2^-53 of themselves, and the unit's constant one more.
-static constexpr double kTol = 2 * 1.4e-13 + 4 * 700 * 1.12e-16;
+// Full 64 bits, 2^-53 each: the unit, its constant and the C library's (x - top) / T round their
+// share of an exponent d, with one spare; 16 for table, norm, polynomials and products.
+static double tolerance(double d) { return (4 * std::fabs(d) + 16) * 0x1p-53; }
 
 static void check(uint16_t top_bits, float heat) {
   const float top = half(top_bits);
@@ -53,7 +53,7 @@ static void check(uint16_t top_bits, float heat) {
     const double d = ((double)x - (double)top) / (double)heat;
     const double exact = std::isnan(x) || x == -INFINITY ? 0.0 : std::exp(d);
     if (exact > 0x1p-990) {
-      if (!(std::fabs(got - exact) <= kTol * exact) || got != all) wrong("weight", top, heat, x, got, exact);
+      if (!(std::fabs(got - exact) <= tolerance(d) * exact) || got != all) wrong("weight", top, heat, x, got, exact);
     } else {
       if (!(got >= 0.0 && got <= 0x1p-985)) wrong("small", top, heat, x, got, exact);
       if (!(all >= 0.0 && all <= 0x1p-985)) wrong("sum's", top, heat, x, all, exact);
