@@ -63,7 +63,7 @@ typedef struct kv_pages {
  * The starts do not descend (where they do it is open which rows are run).
  * A sequence whose rows are not 0 <= start[s] <= start[s + 1] <= rows or more
  * than max_rows is left out; so are rows that belong to no sequence (behind
- * start[seqs]).  What is left out is neither read nor written.  A table entry outside
+ * start[seqs]).  What is left out has no effect and its outputs are not written.  A table entry outside
  * [0, pages) and a slot outside [0, max_pages * page_size) stand for nothing: such a
  * slot is not written, reads as zeros and is not attended to. */
 typedef struct kv_batch {
@@ -102,7 +102,8 @@ typedef struct kv_rows {
  * nearest, ties to even, at most 127 in magnitude; all zeros: scale and codes 0; a
  * row with an infinity or NaN: scale NaN, so that it reads as NaN.
  * k is computed in 64 bits up to its rounding (a sum in another order must
- * not move a value over a code's border), f16 values rounded to f32 first; q in 32.
+ * not move a value over a code's border), f16 values rounded to f32 first; q in 32 but
+ * for its angles, off by at most 2^-20 of |y[i]| + |y[i + D/2]| before it is rounded.
  * The table may name a page twice only where no slot is written through both. */
 int kv_pages_append(const kv_pages* pages, int32_t layer, const kv_batch* batch,
                     const kv_rows* rows, void* stream);
@@ -118,7 +119,9 @@ int kv_pages_append(const kv_pages* pages, int32_t layer, const kv_batch* batch,
  * out must not overlap q (workgroups that share a row read q while others
  * write).  q_heads a multiple of kv_heads, at most 32 times it and at most 256; scale
  * positive and below 2^118; max_rows at most 256.  Scores, statistics and sums are
- * f32; a weight enters its product with v to 2^-22 of itself.
+ * f32; a weight (with v's scale) enters its product with v to 2^-22 of itself or 2^-31 of the
+ * row's largest, whichever is more, so that N slots add at most N 2^-31 of the largest
+ * weight times the largest |v| to the error of a value of out.
  * workspace: device memory of kv_pages_attn_workspace_bytes (256-byte aligned);
  * fill it with zeros once before its first use.  Its first 64 KiB are counters, zeros again
  * behind every call, that nothing else may write; the rest is needed only during the call.
@@ -166,7 +169,8 @@ int kv_pages_read(const kv_pages* pages, int32_t layer, int32_t layers, const kv
  * (logprob 0).  A drafted token outside [0, vocab) is refused (draft NULL: w = p).
  * A sequence without rows, or left out as in kv_batch, gives accepted 0 and -1s.
  * uniform: f32 [rows], values in [0, 1).  Everything but the logprobs' last
- * rounding is computed in 64 bits and fixed order.
+ * rounding is computed in 64 bits and fixed order; a p[r,j] below 2^-990 of the row's
+ * largest may count as 0.
  * rows in [1, 65535], seqs in [1, 1024], max_rows in [1, 256], out_stride >=
  * max_rows, vocab in [1, 2^24]; strides >= vocab; logits 2-byte, the others
  * 4-byte aligned.  workspace: kv_verify_workspace_bytes (256-byte aligned); fill it

@@ -307,7 +307,8 @@ int qwen3_tree_step(const qwen3_weights* w, void* k_cache, void* v_cache, int64_
  * One token a sequence is a decode step, several a prompt's chunk or drafted tokens that
  * kv_verify then judges.  The layers' matrices are read as in qwen3_prefill_batched;
  * with f16 pages results agree with qwen3_decode_step within the step's
- * tolerance, 8-bit pages add their rounding.  Only enqueues; rows at most 128.
+ * tolerance, 8-bit pages add their rounding.  Only enqueues; rows at most 128, max_rows at
+ * most rows.
  * workspace: device memory of qwen3_pages_workspace_bytes(rows, max_rows) bytes (0 for
  * arguments outside the ranges), 256-byte aligned, filled with zeros once before its
  * first use (its first 64 KiB stay zeros between steps, nothing else may write them); that of

@@ -332,11 +332,14 @@ PAGES_APPEND(128, q8, true)
 //     D / 16 makes the dims (D/16) i + n.
 // K and V come from memory once and are used by one wave alone: LDS would only add a stop.
 // A block's registers are requested again for the wave's next block as soon as they have
-// been used (a second set of them spilled), two waves a SIMD cover the rest.  Bound by
+// been used (a second set of them spilled), two waves a SIMD cover the rest.  Four tiles of
+// head_dim 128 leave room for one wave; two tiles spill, 2 registers in f16 and 4 in 8 bits, and
+// four tiles in 8 bits 5, which go to accumulators.  Bound by
 // memory where sequences are long: 4 x 131072 slots of 8 kv heads in 8 bits, 1.1 GB, 193 us, 5.7 TB/s
-// (a copy 5.1); 16 sequences of 44000 slots in f16, 45 rows, 140 MB, 35 us, 4.0 TB/s, of which
+// (a copy 5.1); 16 sequences, 45 rows over 34052 slots in all, f16, 140 MB, 35 us, 4.0 TB/s, of which
 // cut sequences and ramps take 8; 1 x 300 slots 8 us, all latency.
-// A weight goes into the product as the sum of two f16 values (2^-22 of itself).
+// A weight goes into the product as the sum of two f16 values: 2^-22 of itself, 2^-25 where
+// the second is subnormal, which is 2^-31 of a row's largest weight, 2^6 at least.
 // 8-bit codes become f16 multiples of 2^-9, exact; a row's k scale multiplies its
 // score and its v scale its weight, so that the reference is that of s + log2 v_scale.
 namespace {
