@@ -115,11 +115,11 @@ class PagedSession:
         if not seqs or not 0 < sum(counts) <= MAX_ROWS or min(counts) < 1:
             raise ValueError(f"{counts} rows: each sequence at least one, {MAX_ROWS} at most in all")
         need = self._pages_for(seqs, counts)
+        if logits and self._logits is None:
+            self._logits = Q.DeviceBuffer(MAX_ROWS * D.VOCAB * 2)
         for s in seqs:
             self._held[s] += [self._free.pop() for _ in range(need[s])]
         total = sum(counts)
-        if logits and self._logits is None:
-            self._logits = Q.DeviceBuffer(MAX_ROWS * D.VOCAB * 2)
         try:
             batch = self._batch(seqs, counts, [self.length[s] + m for s, m in zip(seqs, counts)])
             self._words.upload(np.concatenate(new), self._tokens)

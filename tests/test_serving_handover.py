@@ -1,5 +1,5 @@
-"""Which sessions PagedSession.to_session hands a sequence over to, on the CPU: the library's
-calls are recorded in place of being made."""
+"""Sequences handed over to flat sessions, and steps that fail before their launch, on the CPU: the
+library's calls are recorded in place of being made."""
 from __future__ import annotations
 
 import numpy as np
@@ -49,3 +49,20 @@ def test_a_session_of_drafted_trees_is_refused(make):
     with pytest.raises(TypeError, match="drafted trees"):
         s.to_session(a, flat)
     assert len(s.calls) == calls and flat.state == (11, 3) and flat.length == flat.position == 7
+
+
+def test_a_step_without_room_for_its_logits_takes_no_pages(make, Q, monkeypatch):
+    """Pages that a refused step kept would be counted as room for others' rows."""
+    s = make()
+    a, b = s.add(), s.add()
+    s.step({a: np.zeros(10)})
+
+    def full(nbytes):
+        raise Q.Q8GemvError(8, "out of memory")
+
+    monkeypatch.setattr(Q, "DeviceBuffer", full)
+    with pytest.raises(Q.Q8GemvError):
+        s.step({a: np.zeros(50)}, logits=True)
+    assert len(s._held[a]) == 1 and len(s._free) == 5 and s.length[a] == 10
+    s.step({a: [1], b: np.zeros(64)})
+    assert len(s._held[a]) == 1 and len(s._held[b]) == 4
